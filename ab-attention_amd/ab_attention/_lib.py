@@ -51,6 +51,36 @@ class PlanArgs(ctypes.Structure):
                 ("workspace_bytes", _SZ)]
 
 
+class RotaryArgs(ctypes.Structure):
+    """ab_rotary_args of include/ab_attention.h."""
+
+    _fields_ = [("q", _P), ("k", _P), ("q_out", _P), ("k_out", _P), ("positions", _P), ("batch", _I64), ("heads", _I64),
+                ("kv_heads", _I64), ("tokens", _I64), ("dim", _I64), ("dtype", _I64), ("q_stride", _I64 * 3),
+                ("k_stride", _I64 * 3), ("q_out_stride", _I64 * 3), ("k_out_stride", _I64 * 3), ("axes", _I64),
+                ("axis_dims", _I64 * 4), ("theta", ctypes.c_double), ("joint", _I64), ("halves", _I64),
+                ("position_type", _I64), ("per_batch", _I64), ("inverse", _I64)]
+
+
+class WindowArgs(ctypes.Structure):
+    """ab_window_args of include/ab_attention.h."""
+
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("out", _P), ("lse", _P), ("lengths", _P), ("offsets", _P),
+                ("page_table", _P), ("batch", _I64), ("heads", _I64), ("kv_heads", _I64), ("tokens", _I64), ("dim", _I64),
+                ("dtype", _I64), ("pages", _I64), ("page_tokens", _I64), ("table_width", _I64), ("window", _I64),
+                ("sinks", _I64), ("frame", _I64), ("scale", ctypes.c_double), ("q_stride", _I64 * 3),
+                ("k_stride", _I64 * 3), ("v_stride", _I64 * 3), ("out_stride", _I64 * 3), ("workspace", _P),
+                ("workspace_bytes", _SZ)]
+
+
+class AppendArgs(ctypes.Structure):
+    """ab_append_args of include/ab_attention.h."""
+
+    _fields_ = [("k", _P), ("v", _P), ("k_cache", _P), ("v_cache", _P), ("lengths", _P), ("offsets", _P),
+                ("page_table", _P), ("batch", _I64), ("kv_heads", _I64), ("tokens", _I64), ("dim", _I64), ("pages", _I64),
+                ("page_tokens", _I64), ("table_width", _I64), ("k_stride", _I64 * 3), ("v_stride", _I64 * 3),
+                ("k_cache_stride", _I64 * 3), ("v_cache_stride", _I64 * 3)]
+
+
 # name -> (restype, argtypes); mirrors include/ab_attention.h
 SIGNATURES = {
     "ab_last_error": (ctypes.c_char_p, []),
@@ -76,6 +106,11 @@ SIGNATURES = {
     "ab_prefill_launch_slots": (_I64, [_I64, _I64]),
     "ab_prefill_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64]),
     "ab_prefill": (ctypes.c_int, [ctypes.POINTER(PrefillArgs), _P]),
+    "ab_rotary": (ctypes.c_int, [ctypes.POINTER(RotaryArgs), _P]),
+    "ab_window_workspace_bytes": (_SZ, [ctypes.POINTER(WindowArgs)]),
+    "ab_window_attention": (ctypes.c_int, [ctypes.POINTER(WindowArgs), _P]),
+    "ab_chunk_attention": (ctypes.c_int, [ctypes.POINTER(WindowArgs), _P]),
+    "ab_append_cache": (ctypes.c_int, [ctypes.POINTER(AppendArgs), _P]),
 }
 
 # name -> (restype, argtypes); mirrors include/ab_attention_static.h
@@ -83,7 +118,7 @@ STATIC_SIGNATURES = {
     "ab_ibcs_sip_static": (ctypes.c_int, [_P, _P, _P, _I64, _I64, _P, _I64, _P, _P, _P]),
 }
 
-ABI_VERSION = 7
+ABI_VERSION = 8
 _lib = None
 _static = None
 

@@ -1,0 +1,337 @@
+"""Attention of video that is made (or trained) frame by frame: rotary positions
+over (time, height, width), attention that is causal over frames with a sliding
+window and first frames that stay visible, and the same attention of new tokens
+over a paged cache.
+
+The mask of all of them: tokens are grouped into frames of ``frame`` tokens
+(``frame=1``: plain causal attention), and the query at position p sees the key
+at position t where
+
+    t // frame <= p // frame  and
+    (p // frame - t // frame < window  or  t // frame < sinks)
+
+so ``window`` and ``sinks`` count frames; ``window=None`` is no limit. A query
+that sees nothing gets o = 0 and lse = -inf.
+
+Serving: ``rotary`` of the new tokens' Q and K, ``append_cache``, then
+``chunk_attention``, or ``StreamingAttention``, which makes the three calls and
+keeps the page table. Training: ``rotary`` and ``window_attention``. The
+reference has no counterpart: its attention sees a whole clip at once.
+
+Everything runs on the current stream of the tensors' device and synchronises
+nothing; sizes that are on the device (lengths, offsets, page tables) are
+bounded by the kernels and never read on the host.
+"""
+from __future__ import annotations
+
+import math
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_MOST = 1 << 30
+
+
+def _strided(t: torch.Tensor, align: int = 8) -> torch.Tensor:
+    """t itself where its rows (last dim contiguous, starting on 16 bytes) can be
+    read where they lie, else a contiguous copy."""
+    strides = t.stride()
+    if t.data_ptr() % 16 == 0 and strides[-1] == 1:
+        for size, stride in zip(t.shape[:-1], strides):
+            if size > 1 and (stride % align or stride < 0):
+                break
+        else:
+            return t
+    return t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+
+
+def _gpu(name: str, *tensors):
+    device = tensors[0].device
+    if device.type != "cuda" or any(t is not None and t.device != device for t in tensors):
+        raise ValueError(f"{name} requires tensors on one CUDA device")
+    return device
+
+
+# ---- rotary positions ---------------------------------------------------------
+
+
+def _rotate(q, k, positions, axes, theta, halves, joint, inverse):
+    align = 4 if q.dtype == torch.float32 else 8
+    q = _strided(q, align)
+    q_out = torch.empty_like(q)
+    k_out = None
+    if k is not None:
+        k = _strided(k, align)
+        k_out = torch.empty_like(k)
+    batch, heads, tokens, dim = q.shape
+    lib, address = _lib.load(), _lib.address
+    args = _lib.RotaryArgs(address(q), address(k), address(q_out), address(k_out), address(positions), batch, heads,
+                           0 if k is None else k.shape[1], tokens, dim, _DTYPES[q.dtype], q.stride()[:3],
+                           (0, 0, 0) if k is None else k.stride()[:3], q_out.stride()[:3],
+                           (0, 0, 0) if k is None else k_out.stride()[:3], len(axes), axes, theta, joint, halves,
+                           _POSITIONS[positions.dtype], positions.ndim == 3, inverse)
+    with _lib.on(q.device):
+        _lib.check(lib.ab_rotary(args, _lib.stream(q.device)))
+    return q_out, k_out
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, *how):
+        ctx.save_for_backward(positions)
+        ctx.how = how
+        ctx.set_materialize_grads(False)
+        return _rotate(q, k, positions, *how, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        (positions,) = ctx.saved_tensors
+        if dq is None:  # only K's result was used
+            dq, dk = dk, None
+            flipped = True
+        else:
+            flipped = False
+        grads = (None, None) if dq is None else _rotate(dq, dk, positions, *ctx.how, True)
+        if flipped:
+            grads = grads[::-1]
+        return (*grads, *[None] * (len(ctx.how) + 1))
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axes, *, theta: float = 10000.0,
+           pairing: str = "adjacent", joint: bool = False):
+    """q [B, H, N, D] and k [B, Hk, N, D] (or None) with rotary positions over several axes.
+
+    ``positions`` [N, A] or [B, N, A] (int32, int64 or float32) gives every token's
+    place on A <= 4 axes, for example (time, height, width); ``axes`` gives the
+    dims that each axis turns, even numbers that add up to at most D (Wan2.1:
+    (44, 42, 42), HunyuanVideo: (16, 56, 56)). The j-th pair of an axis of d dims
+    turns by position * theta^(-2j/d); with ``joint`` the i-th pair of all axes by
+    position * theta^(-2i/sum(axes)). ``pairing`` "adjacent" pairs values 2i and
+    2i + 1, "halves" values i and i + sum(axes)/2 (a sum divisible by 16). Dims
+    behind the axes' stay as they are. D is a multiple of 8; bf16, fp16 or float32.
+
+    Returns (q, k) as new tensors (k None if it was), in the memory order of the
+    inputs. Differentiable in q and k (the gradient is the opposite rotation).
+    """
+    if q.ndim != 4 or (k is not None and (k.ndim != 4 or k.shape[::2] != q.shape[::2] or k.shape[3] != q.shape[3])):
+        raise ValueError("rotary requires Q [B,H,N,D] and K [B,Hk,N,D] of the same batch, tokens and dim")
+    if q.dtype not in _DTYPES or (k is not None and k.dtype != q.dtype):
+        raise ValueError("rotary requires BF16, FP16 or FP32 Q/K of one type")
+    batch, _, tokens, dim = q.shape
+    if dim % 8 or dim > 1024:
+        raise ValueError("rotary requires a head dim that is a multiple of 8, at most 1024")
+    axes = tuple(int(a) for a in axes)
+    if not 1 <= len(axes) <= 4 or any(a <= 0 or a % 2 for a in axes) or sum(axes) > dim:
+        raise ValueError("axes must be 1 to 4 positive even numbers of dims that add up to at most D")
+    if pairing not in ("adjacent", "halves"):
+        raise ValueError("pairing must be 'adjacent' or 'halves'")
+    if pairing == "halves" and sum(axes) % 16:
+        raise ValueError("pairing 'halves' requires a multiple of 16 turned dims")
+    theta = float(theta)
+    if not math.isfinite(theta) or theta <= 0:
+        raise ValueError("theta must be positive and finite")
+    if positions.dtype not in _POSITIONS:
+        raise ValueError("positions must be int32, int64 or float32")
+    if positions.shape != (tokens, len(axes)) and positions.shape != (batch, tokens, len(axes)):
+        raise ValueError(f"positions must be [{tokens}, {len(axes)}] or [{batch}, {tokens}, {len(axes)}]")
+    _gpu("rotary", q, k, positions)
+    if q.shape[1] == 0 or (k is not None and k.shape[1] == 0):
+        raise ValueError("rotary requires at least one head")
+    how = (axes, theta, pairing == "halves", bool(joint))
+    positions = positions.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rotary.apply(q, k, positions, *how)
+    return _rotate(q, k, positions, *how, False)
+
+
+# ---- windowed attention -------------------------------------------------------
+
+
+def _mask(window, sinks, frame):
+    """(window, 0 for no limit, sinks, frame) as checked numbers."""
+    window = 0 if window is None else int(window)
+    sinks, frame = int(sinks), int(frame)
+    if frame < 1:
+        raise ValueError("frame must be at least one token")
+    if sinks < 0:
+        raise ValueError("sinks must not be negative")
+    return window, min(sinks, _MOST), min(frame, _MOST)
+
+
+def _check_window(window, scale, dim):
+    if window is not None and int(window) < 1:
+        raise ValueError("window must be at least one frame, or None")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    return scale
+
+
+def _run(args, entry, device):
+    """One call with the workspace that it asks for, which lives for the call only."""
+    lib = _lib.load()
+    with _lib.on(device):
+        size = lib.ab_window_workspace_bytes(args)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        args.workspace, args.workspace_bytes = _lib.address(workspace), size
+        _lib.check(getattr(lib, entry)(args, _lib.stream(device)))
+
+
+def _window_forward(q, k, v, lengths, window, sinks, frame, scale, return_lse):
+    q, k, v = _strided(q), _strided(k), _strided(v)
+    batch, heads, tokens, dim = q.shape
+    out = torch.empty_like(q)
+    lse = torch.empty((batch, heads, tokens), dtype=torch.float32, device=q.device) if return_lse else None
+    if tokens:
+        address = _lib.address
+        args = _lib.WindowArgs(address(q), address(k), address(v), address(out), address(lse), address(lengths), None, None,
+                               batch, heads, k.shape[1], tokens, dim, _DTYPES[q.dtype], 0, 0, 0, window, sinks, frame, scale,
+                               q.stride()[:3], k.stride()[:3], v.stride()[:3], out.stride()[:3], None, 0)
+        _run(args, "ab_window_attention", q.device)
+    return out, lse
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int | None = None, sinks: int = 0,
+                     frame: int = 1, lengths: torch.Tensor | None = None, scale: float | None = None,
+                     return_lse: bool = False):
+    """Attention of q [B, H, N, D] over k, v [B, Hk, N, D] that is causal over
+    frames with a sliding window and sinks (the mask above; token t is at position
+    t). D is 64 or 128, bf16 or fp16; H is a multiple of Hk, and query head h reads
+    key head h // (H // Hk). ``lengths`` int32 [B] are the batch items' tokens: the
+    ones behind them are padding that nothing reads, with o = 0 and lse = -inf.
+    ``scale`` defaults to D ** -0.5.
+
+    Returns o in q's type and memory order, and with ``return_lse`` the base-2
+    softmax normaliser as float32 [B, H, N].
+    """
+    if q.ndim != 4 or k.ndim != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
+        raise ValueError("Q [B,H,N,D] and K/V [B,Hk,N,D] must share batch, tokens and dim")
+    if q.shape[-1] not in (64, 128):
+        raise ValueError("window attention requires head_dim 64 or 128")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("window attention requires BF16 or FP16 Q/K/V of one type")
+    if k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError("the query heads must be a positive multiple of the key heads")
+    scale = _check_window(window, scale, q.shape[-1])
+    window, sinks, frame = _mask(window, sinks, frame)
+    if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != q.shape[:1] or not lengths.is_contiguous()):
+        raise ValueError("lengths must be int32 [B]")
+    _gpu("window attention", q, k, v, lengths)
+    with torch.no_grad():
+        out, lse = _window_forward(q, k, v, lengths, window, sinks, frame, scale, return_lse)
+    return (out, lse) if return_lse else out
+
+
+# ---- paged cache --------------------------------------------------------------
+
+
+class PagedCache(NamedTuple):
+    """Keys and values of many sequences in pages: two tensors [pages, heads, page
+    tokens, D] (or views of that shape of any memory order with rows of D), page
+    tokens a multiple of 8. Which page holds which tokens of which sequence is the
+    page table's: int32 [sequences, width], entry (b, i) the page of the positions
+    i * page tokens .. + page tokens - 1, or any number outside [0, pages) for
+    none, as of pages that have been given back."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+
+
+def _check_cache(name, x, heads, cache, page_table, lengths, offsets):
+    if x.ndim != 3:
+        raise ValueError(f"{name} requires packed tokens [T,H,D]")
+    if cache.k.ndim != 4 or cache.k.shape != cache.v.shape or cache.k.shape[3] != x.shape[2]:
+        raise ValueError("the cache must be two [pages,heads,page tokens,D] tensors with the tokens' D")
+    if x.shape[2] not in (64, 128):
+        raise ValueError(f"{name} requires head_dim 64 or 128")
+    if x.dtype not in (torch.bfloat16, torch.float16) or cache.k.dtype != x.dtype or cache.v.dtype != x.dtype:
+        raise ValueError(f"{name} requires BF16 or FP16 tokens and a cache of the same type")
+    if cache.k.shape[2] == 0 or cache.k.shape[2] % 8:
+        raise ValueError("pages must hold a positive multiple of 8 tokens")
+    for t in cache:
+        if t.data_ptr() % 16 or t.stride(3) != 1 or any(n > 1 and s % 8 for n, s in zip(t.shape[:3], t.stride())):
+            raise ValueError("the cache's rows must be contiguous and start on 16 bytes")
+    if heads == 0 or cache.k.shape[1] == 0 or heads % cache.k.shape[1]:
+        raise ValueError("the query heads must be a positive multiple of the cache's heads")
+    batch = page_table.shape[0]
+    if page_table.ndim != 2 or lengths.shape != (batch,) or offsets.shape != (batch + 1,):
+        raise ValueError("page_table [B,width], lengths [B] and offsets [B+1] must be of one batch")
+    for t in (page_table, lengths, offsets):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError("page_table, lengths and offsets must be contiguous int32")
+    return _gpu(name, x, *cache, page_table, lengths, offsets)
+
+
+@torch.no_grad()
+def append_cache(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                 offsets: torch.Tensor) -> PagedCache:
+    """Writes the new keys and values k, v [T, heads, D] into the cache, in place.
+
+    Sequence b's new tokens are the rows offsets[b] .. offsets[b + 1] - 1 (int32
+    [B + 1], ascending); ``lengths`` int32 [B] are the tokens of each sequence with
+    the new ones, so that its last row goes to position lengths[b] - 1. Rows whose
+    entry in the page table is no page are dropped. Returns the cache.
+    """
+    if k.shape != v.shape or v.dtype != k.dtype:
+        raise ValueError("K and V must be packed tokens [T,H,D] of one shape and type")
+    device = _check_cache("append_cache", k, k.shape[1] if k.ndim == 3 else 0, cache, page_table, lengths, offsets)
+    _gpu("append_cache", k, v)
+    if k.shape[1] != cache.k.shape[1]:
+        raise ValueError("K and V must have the cache's heads")
+    k, v = _strided(k), _strided(v)
+    lib, address = _lib.load(), _lib.address
+    pages, heads, page, dim = cache.k.shape
+
+    def rows(t):
+        return 0, t.stride(1), t.stride(0)
+
+    args = _lib.AppendArgs(address(k), address(v), address(cache.k), address(cache.v), address(lengths), address(offsets),
+                           address(page_table), page_table.shape[0], heads, k.shape[0], dim, pages, page,
+                           page_table.shape[1], rows(k), rows(v), cache.k.stride()[:3], cache.v.stride()[:3])
+    with _lib.on(device):
+        _lib.check(lib.ab_append_cache(args, _lib.stream(device)))
+    return cache
+
+
+@torch.no_grad()
+def chunk_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tensor,
+                    offsets: torch.Tensor, *, window: int | None = None, sinks: int = 0, frame: int = 1,
+                    scale: float | None = None, return_lse: bool = False, out: torch.Tensor | None = None):
+    """Attention of the sequences' new tokens q [T, H, D] over their cached keys
+    and values, the new ones among them (``append_cache`` first; ``lengths`` and
+    ``offsets`` as there). A sequence may bring one token or a whole prompt; query i
+    of n is at position lengths[b] - n + i of the mask above. Keys in places that
+    the page table gives no page are not seen, and nothing outside of the pages'
+    visible tokens is read. D is 64 or 128, bf16 or fp16; H is a multiple of the
+    cache's heads.
+
+    Returns o [T, H, D] and with ``return_lse`` the base-2 normaliser float32
+    [T, H]. Rows outside of offsets[0] .. offsets[B] - 1 are not written (with
+    ``out``, a tensor of q's shape and type to write to, they stay as they are).
+    """
+    device = _check_cache("chunk attention", q, q.shape[1] if q.ndim == 3 else 0, cache, page_table, lengths, offsets)
+    scale = _check_window(window, scale, q.shape[-1])
+    window, sinks, frame = _mask(window, sinks, frame)
+    q = _strided(q)
+    tokens, heads, dim = q.shape
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=device)
+    elif (out.shape != q.shape or out.dtype != q.dtype or out.device != device or out.data_ptr() % 8 or out.stride(2) != 1
+          or any(n > 1 and s % 4 for n, s in zip(out.shape[:2], out.stride()))):
+        raise ValueError("out must be of Q's shape, type and device, with contiguous rows that start on 8 bytes")
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
+    if tokens and page_table.shape[0]:
+        address = _lib.address
+        pages, kv_heads, page, _ = cache.k.shape
+        args = _lib.WindowArgs(address(q), address(cache.k), address(cache.v), address(out), address(lse),
+                               address(lengths), address(offsets), address(page_table), page_table.shape[0], heads, kv_heads,
+                               tokens, dim, _DTYPES[q.dtype], pages, page, page_table.shape[1], window, sinks, frame, scale,
+                               (0, q.stride(1), q.stride(0)), cache.k.stride()[:3], cache.v.stride()[:3],
+                               (0, out.stride(1), out.stride(0)), None, 0)
+        _run(args, "ab_chunk_attention", device)
+    return (out, lse) if return_lse else out

@@ -1,0 +1,160 @@
+// Windowed causal attention: the mask, the element types and the LDS tiles that
+// its forward and backward kernels share.
+#pragma once
+
+#include "common.hpp"
+#include "layout.hpp"
+
+namespace ab {
+
+// The mask. Tokens are grouped into frames of `frame` tokens (1: plain causal
+// attention). The query at position p sees the keys of its own frame and of
+// earlier ones down to `back` tokens before its frame's first, and the first
+// `sinks` tokens, as far as they are not later than its frame:
+//   [0, min(sinks, high)) and [low, high),  low = max(0, start - back),
+//   high = min(start + frame, length),      start = p - p % frame.
+// All three bounds grow with p. Positions, back, sinks and frame are at most
+// 2^30, so the sums stay inside 32 bits.
+struct WindowMask {
+    Divisor frame;
+    int32_t back, sinks;
+    __device__ __forceinline__ int start(int p) const {
+        uint32_t q = __umulhi(static_cast<uint32_t>(p), frame.m);
+        uint32_t rest = static_cast<uint32_t>(p) - q * frame.d;
+        if (rest >= frame.d) rest -= frame.d;
+        return p - static_cast<int>(rest);
+    }
+    __device__ __forceinline__ int low(int p) const { return max(0, start(p) - back); }
+    __device__ __forceinline__ int high(int p, int length) const {
+        return min(start(p) + static_cast<int>(frame.d), length);
+    }
+};
+
+// The bf16 and fp16 forms of what the kernels do with 16-bit elements.
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) unsigned char lds_u8;
+
+struct Bf16 {
+    // D = A B + C of 16x16x32 (A: 16 x 32, lane l row l % 16, k 8(l / 16) .. + 7;
+    // B: 32 x 16, lane l column l % 16, the same k; C and D: lane l column
+    // l % 16, rows 4(l / 16) .. + 3).
+    static __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    // 32x32x16 (A: lane l row l % 32, k 8(l / 32) .. + 7; D: lane l column
+    // l % 32, element e row e % 4 + 8(e / 4) + 4(l / 32)).
+    static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16(lo, hi); }
+    static __device__ __forceinline__ float lo(uint32_t w) { return bf16_lo(w); }
+    static __device__ __forceinline__ float hi(uint32_t w) { return bf16_hi(w); }
+    // Exponent bits of both halves, and what turns an exponent of all ones into
+    // the half's sign bit when added.
+    static constexpr uint32_t kExponent = 0x7f807f80u, kOverflow = 0x00800080u, kOne = 0x3f80u;
+};
+
+struct F16 {
+    static __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        const f32x2 v = {lo, hi};
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+    }
+    static __device__ __forceinline__ float lo(uint32_t w) {
+        return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w)));
+    }
+    static __device__ __forceinline__ float hi(uint32_t w) {
+        return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w >> 16)));
+    }
+    static constexpr uint32_t kExponent = 0x7c007c00u, kOverflow = 0x04000400u, kOne = 0x3c00u;
+};
+
+// Transposing LDS read: within each 16-lane group, lane i receives element
+// i % 4 of the 8 bytes read by lanes 4r + i / 4, for r = 0..3.
+__device__ __forceinline__ i16x4 lds_read_transposed(uint32_t lds) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_i16x4*>(static_cast<uintptr_t>(lds)));
+}
+
+__device__ __forceinline__ u32x4 lds_read16(uint32_t lds) {
+    return *reinterpret_cast<const lds_u32x4*>(static_cast<uintptr_t>(lds));
+}
+
+// A buffer of `bytes` bytes from `base` on: reads past its end give zeros.
+__device__ __forceinline__ u32x4 buffer_of(const void* base, uint32_t bytes) {
+    const uint64_t a = reinterpret_cast<uint64_t>(base);
+    u32x4 r = {static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32) & 0xffffu, bytes, 0x00020000u};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_readfirstlane(r[i]);
+    return r;
+}
+
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// 16 bytes per lane from the buffer, at an offset of its own in each lane,
+// straight into LDS: lane j writes bytes [lds + 16j, lds + 16j + 16); a lane
+// past the buffer's end writes zeros. Counted by vmcnt. The wait states are
+// those between scalar writes of m0 or the descriptor and their use.
+__device__ __forceinline__ void buffer_to_lds(u32x4 buffer, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// At most N of this wave's vector memory operations still in flight, none of
+// its LDS ones; then a workgroup barrier that the compiler moves no memory
+// access across.
+template <int N>
+__device__ __forceinline__ void landed_and_barrier() {
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4));
+    asm volatile("s_barrier" ::: "memory");
+}
+
+// A tensor of rows of `dim` 16-bit elements; strides in elements.
+struct Rows {
+    int64_t batch, head, token;
+};
+
+// One call of the forward pass. Rows of Q are read at q + b q.batch + h q.head +
+// t q.token; `paged`, over a cache, K and V at k.batch * page + h k.head +
+// (token in the page) k.token, and batch item b's queries are the packed rows
+// offsets[b] .. offsets[b + 1]. `row` gives the place of a query's normaliser.
+struct WindowCall {
+    const void *q, *k, *v;
+    void* out;
+    float* lse;
+    Rows q_rows, k_rows, v_rows, out_rows, row;
+    int32_t batch, heads, kv_heads, tokens;  // tokens: of a batch item, or packed rows in all
+    int32_t dim, half;                       // half: 0 bf16, 1 fp16
+    bool paged;
+    const int32_t *lengths, *offsets, *table;
+    int32_t table_width, pages;
+    Divisor page, group;                     // tokens of a page; query heads of a K/V head
+    WindowMask mask;
+    float scale_log2;
+    int32_t parts;                           // parts that every tile's keys are split into
+    float* partial_o;                        // [parts][rows][dim] with workspace
+    float2* partial_stat;                    // [parts][rows]: reference and sum
+    int64_t rows;                            // queries times heads
+};
+
+constexpr int kWindowThreads = 256;
+constexpr int kWindowRows = 128;  // query rows of a workgroup
+constexpr int kWindowKeys = 32;   // keys of a tile
+
+int launch_window(const WindowCall& call, hipStream_t stream);
+int window_parts(const WindowCall& call, int64_t most_keys);
+int64_t window_tiles(const WindowCall& call);
+
+}  // namespace ab

@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define AB_ABI_VERSION 7
+#define AB_ABI_VERSION 8
 
 enum ab_status {
     AB_OK = 0,
@@ -236,6 +236,89 @@ int ab_remap_ids(const int32_t *ids, int64_t count, const int32_t *map, int64_t 
 int ab_paged_prefill_ordered(const void *q, const void *k, const void *v, const int32_t *order,
                              int64_t batch_heads, int64_t tokens, const int32_t *ids, const float *log_weights,
                              int64_t samples, void *out, float *lse, void *stream);
+
+/* ---- Streaming video: rotary positions, windowed attention, paged cache ----
+ * No counterpart in the reference (its attention sees a whole clip). Element
+ * types of these entry points; the attention takes the 16-bit ones. */
+enum ab_dtype { AB_BF16 = 0, AB_F16 = 1, AB_F32 = 2 };
+
+/* Rotary positions over up to 4 axes. Q and K [batch, heads, tokens, dim]
+ * (k NULL or kv_heads 0: Q alone) with strides of their own (batch, head, token; in
+ * elements), rows of dim contiguous, a multiple of 8, that start on 16 bytes. Axis a
+ * turns axis_dims[a] dims (even): its j-th pair by position * theta^(-2j /
+ * axis_dims[a]), or with `joint` the i-th pair of all axes by position *
+ * theta^(-2i / sum of axis_dims). Pairs are neighbours, or with `halves` value i
+ * and i + sum / 2 (sum a multiple of 16); dims behind the axes' are copied.
+ * positions: [tokens, axes] or with per_batch [batch, tokens, axes] of
+ * position_type 0 int32, 1 int64, 2 float32. inverse: by the opposite angles
+ * (the gradient). Outputs must not overlap inputs, except at the very same places. */
+typedef struct ab_rotary_args {
+    const void *q, *k;
+    void *q_out, *k_out;
+    const void *positions;
+    int64_t batch, heads, kv_heads, tokens, dim, dtype;
+    int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3];
+    int64_t axes, axis_dims[4];
+    double theta;
+    int64_t joint, halves, position_type, per_batch, inverse;
+} ab_rotary_args;
+int ab_rotary(const ab_rotary_args *args, void *stream);
+
+/* Attention that is causal over frames of `frame` tokens, with a sliding window
+ * of `window` frames (0: no limit) and the first `sinks` frames always visible:
+ * the query at position p sees key t iff t / frame <= p / frame and (p / frame -
+ * t / frame < window or t / frame < sinks). dim 64 or 128; dtype AB_BF16 or
+ * AB_F16; heads a multiple of kv_heads; sums and the softmax in float32. A query
+ * that sees nothing gets o = 0 and lse = -inf. lse (base 2) may be NULL.
+ *
+ * ab_window_attention: q [batch, heads, tokens, dim], k, v [batch, kv_heads,
+ *   tokens, dim], query t at position t. With `lengths` int32 [batch] a batch
+ *   item has so many tokens: later ones are not read as keys, and see nothing as
+ *   queries. lse f32 [batch, heads, tokens].
+ * ab_chunk_attention: the packed new tokens of `batch` sequences over a paged
+ *   cache. q and out [tokens, heads, dim] (their batch stride is not used);
+ *   sequence b has the rows offsets[b] .. offsets[b + 1] - 1 (int32
+ *   [batch + 1], ascending), the last of which is at position lengths[b] - 1. k, v
+ *   [pages, kv_heads, page_tokens, dim] (strides page, head, token), page_tokens a
+ *   multiple of 8; page_table int32 [batch, table_width]. An entry outside
+ *   [0, pages) is no page: its keys are not seen. Rows before offsets[0] and from
+ *   offsets[batch] on are left as they are. lse f32 [tokens, heads].
+ *
+ * Strides in elements, multiples of 8 (out: of 4); q, k, v 16-byte aligned, out 8.
+ * Limits: tokens and positions under 2^30, a head of k or v (of a page) under 4 GiB.
+ * Calls that leave CUs idle split their keys over workgroups with a workspace of
+ * ab_window_workspace_bytes(args) (0: none needed; NULL: never split). */
+typedef struct ab_window_args {
+    const void *q, *k, *v;
+    void *out;
+    float *lse;
+    const int32_t *lengths, *offsets, *page_table;
+    int64_t batch, heads, kv_heads, tokens, dim, dtype;
+    int64_t pages, page_tokens, table_width;
+    int64_t window, sinks, frame;
+    double scale;
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
+    void *workspace;
+    size_t workspace_bytes;
+} ab_window_args;
+size_t ab_window_workspace_bytes(const ab_window_args *args);
+int ab_window_attention(const ab_window_args *args, void *stream);
+int ab_chunk_attention(const ab_window_args *args, void *stream);
+
+/* New keys and values k, v [tokens, kv_heads, dim] (16-bit elements) of `batch`
+ * sequences into a paged cache (offsets, lengths, page_table and the cache as in
+ * ab_chunk_attention; lengths count the new tokens). Rows whose entry is no page
+ * are dropped. Strides in elements, multiples of 8 (token, head of k and v in
+ * k_stride[2], [1]; page, head, token of the cache). */
+typedef struct ab_append_args {
+    const void *k, *v;
+    void *k_cache, *v_cache;
+    const int32_t *lengths, *offsets, *page_table;
+    int64_t batch, kv_heads, tokens, dim;
+    int64_t pages, page_tokens, table_width;
+    int64_t k_stride[3], v_stride[3], k_cache_stride[3], v_cache_stride[3];
+} ab_append_args;
+int ab_append_cache(const ab_append_args *args, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,394 @@
+"""Rotary positions, windowed attention and the paged cache on the GPU against
+their plain forms in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from ab_attention.streaming import PagedCache, append_cache, chunk_attention, rotary, window_attention
+from streaming_reference import (HALF_STEP, attend, check_lse, check_output, logit_size, seen_mask, turned)
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _rand(shape, dtype, seed, scale=1.0, token_major=False):
+    gen = torch.Generator("cuda").manual_seed(seed)
+    if token_major:
+        b, h, n, d = shape
+        return (torch.randn((b, n, h, d), generator=gen, device="cuda") * scale).to(dtype).transpose(1, 2)
+    return (torch.randn(shape, generator=gen, device="cuda") * scale).to(dtype)
+
+
+# ---- rotary -------------------------------------------------------------------
+
+
+def _check_turned(got, x, ref):
+    """One rounding of the result, and float32 sines (2^-22), products and sum of a pair of values."""
+    u = HALF_STEP[x.dtype]
+    size = x.double().abs().amax(-1, keepdim=True)
+    assert ((got.double() - ref).abs() <= u * ref.abs() + 2.0 ** -20 * size + 1e-30).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("axes,dim,halves,joint", [((44, 42, 42), 128, False, False), ((32, 48, 48), 128, True, True),
+                                                   ((16, 56, 56), 128, True, False), ((64,), 128, True, False),
+                                                   ((10, 2, 4, 6), 24, False, False), ((2,), 8, False, True)])
+@pytest.mark.parametrize("batch,heads,kv_heads,tokens", [(1, 1, 1, 1), (2, 5, 1, 37), (3, 12, 4, 260)])
+def test_rotary(dtype, axes, dim, halves, joint, batch, heads, kv_heads, tokens):
+    q = _rand((batch, heads, tokens, dim), dtype, 1)
+    k = _rand((batch, kv_heads, tokens, dim), dtype, 2, token_major=True)
+    gen = torch.Generator("cuda").manual_seed(3)
+    pos = torch.randint(0, 200000, (batch, tokens, len(axes)), generator=gen, device="cuda")
+    pairing = "halves" if halves else "adjacent"
+    for p in (pos, pos[0].to(torch.int32), pos[0].float() / 8):
+        a, b = rotary(q, k, p, axes, theta=1e4, pairing=pairing, joint=joint)
+        assert b.stride() == k.stride()
+        _check_turned(a, q, turned(q, p, axes, 1e4, halves, joint))
+        _check_turned(b, k, turned(k, p, axes, 1e4, halves, joint))
+    a, none = rotary(q, None, pos, axes, pairing=pairing, joint=joint)
+    assert none is None
+    _check_turned(a, q, turned(q, pos, axes, 1e4, halves, joint))
+
+
+def test_rotary_reads_slices_and_leaves_the_rest():
+    """Q and K as slices of one projection, and dims behind the axes bit for bit (infinities too)."""
+    packed = _rand((2, 50, 3 * 4 * 128), BF16, 5)
+    q, k, _ = (t.reshape(2, 50, 4, 128).transpose(1, 2) for t in packed.chunk(3, -1))
+    q[..., 96:] = math.inf
+    pos = torch.arange(50, device="cuda")[:, None].expand(50, 3)
+    for pairing in ("adjacent", "halves"):
+        a, b = rotary(q, k, pos, (32, 32, 32), pairing=pairing)
+        assert torch.equal(a[..., 96:], q[..., 96:]) and torch.equal(b[..., 96:], k[..., 96:])
+        _check_turned(a[..., :96], q[..., :96], turned(q[..., :96], pos, (32, 32, 32), halves=pairing == "halves"))
+    q = _rand((1, 1, 3, 16), BF16, 6)
+    q[..., 6:] = math.inf  # inside the unit of the last turned pair
+    assert torch.equal(rotary(q, None, pos[:3, :1], (6,))[0][..., 6:], q[..., 6:])
+
+
+def test_rotary_of_odd_places():
+    """A tensor whose rows do not start on 16 bytes, one with its dims strided, none at all."""
+    flat = _rand((2 * 3 * 40 + 1,), BF16, 7)
+    q = flat[1:].reshape(1, 2, 3, 40)
+    pos = torch.arange(3, device="cuda")[:, None]
+    _check_turned(rotary(q, None, pos, (40,))[0], q, turned(q, pos, (40,)))
+    q = _rand((1, 2, 40, 3), BF16, 8).transpose(2, 3)
+    _check_turned(rotary(q, None, pos, (40,))[0], q, turned(q, pos, (40,)))
+    empty = torch.empty((2, 3, 0, 64), dtype=BF16, device="cuda")
+    assert rotary(empty, empty, torch.empty((0, 1), dtype=torch.int32, device="cuda"), (64,))[0].shape == empty.shape
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rotary_gradient(dtype):
+    """The gradient is the opposite rotation; and the rotation of it gives it back."""
+    q, k = _rand((2, 6, 45, 128), dtype, 1).requires_grad_(), _rand((2, 2, 45, 128), dtype, 2).requires_grad_()
+    dq, dk = _rand((2, 6, 45, 128), dtype, 3, token_major=True), _rand((2, 2, 45, 128), dtype, 4)
+    pos = torch.randint(0, 1000, (45, 3), device="cuda")
+    axes = (44, 42, 42)
+    a, b = rotary(q, k, pos, axes)
+    gq, gk = torch.autograd.grad((a, b), (q, k), (dq, dk), retain_graph=True)
+    _check_turned(gq, dq, turned(dq, pos, axes, inverse=True))
+    _check_turned(gk, dk, turned(dk, pos, axes, inverse=True))
+    assert torch.equal(torch.autograd.grad(b, k, dk, retain_graph=True)[0], gk)
+    assert torch.equal(torch.autograd.grad(a, q, dq)[0], gq)
+    assert torch.equal(torch.autograd.grad(rotary(q, None, pos, axes)[0], q, dq)[0], gq)
+
+
+# ---- window attention ---------------------------------------------------------
+
+
+def _window_case(batch, heads, kv_heads, tokens, dim, dtype, window, sinks, frame, lengths=None, token_major=False, seed=0,
+                 junk=None, scale=None):
+    q = _rand((batch, heads, tokens, dim), dtype, seed + 1, 2.0, token_major)
+    k = _rand((batch, kv_heads, tokens, dim), dtype, seed + 2, 1.0, token_major)
+    v = _rand((batch, kv_heads, tokens, dim), dtype, seed + 3, 1.0, token_major)
+    if junk is not None:  # what lies in the padding is nobody's business
+        for b, length in enumerate(lengths):
+            for t in (q, k, v):
+                t[b, :, length:] = junk
+    dev_lengths = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    out, lse = window_attention(q, k, v, window=window, sinks=sinks, frame=frame, lengths=dev_lengths, scale=scale,
+                                return_lse=True)
+    assert out.stride() == q.stride() and out.dtype == dtype
+    at = torch.arange(tokens, device="cuda")
+    for b in range(batch):
+        n = tokens if lengths is None else max(0, min(lengths[b], tokens))
+        mask = seen_mask(at, at, window, sinks, frame) & (at[:, None] < n) & (at[None] < n)
+        o, l, spread = attend(torch.nan_to_num(q[b], 0, 0, 0), k[b], v[b], mask, scale)
+        check_output(out[b], o, spread, dtype)
+        check_lse(lse[b], l, dim, logit_size(q[b, :, :n], k[b, :, :n], scale))
+        assert (out[b, :, n:] == 0).all() and (lse[b, :, n:] == -math.inf).all()
+    same = window_attention(q, k, v, window=window, sinks=sinks, frame=frame, lengths=dev_lengths, scale=scale)
+    assert torch.equal(same, out)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("tokens", [1, 2, 7, 31, 32, 33, 63, 65, 127, 128, 129, 300])
+def test_window_lengths(tokens, dim, dtype):
+    _window_case(1, 2, 1, tokens, dim, dtype, 40, 3, 1, seed=tokens)
+
+
+@pytest.mark.parametrize("window,sinks,frame", [(None, 0, 1), (1, 0, 1), (1, 1, 1), (2, 5, 1), (33, 0, 1), (64, 40, 1),
+                                                (200, 150, 1), (10000, 3, 1), (100, 10000, 1), (None, 0, 7), (1, 0, 100),
+                                                (2, 1, 31), (3, 2, 37), (1, 3, 130), (2, 1, 260), (1, 0, 5000),
+                                                (2 ** 40, 2 ** 40, 1), (1, 0, 2 ** 40), (2 ** 31, 7, 3)])
+def test_window_masks(window, sinks, frame):
+    _window_case(2, 3, 3, 517, 128, BF16, window, sinks, frame)
+
+
+@pytest.mark.parametrize("heads,kv_heads,token_major", [(8, 2, False), (6, 1, True), (4, 4, True)])
+def test_window_heads_and_strides(heads, kv_heads, token_major):
+    _window_case(2, heads, kv_heads, 333, 128, BF16, 100, 4, 1, token_major=token_major)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("junk", [math.nan, math.inf])
+def test_window_padded_batch(dim, junk):
+    _window_case(5, 4, 2, 200, dim, BF16, 50, 2, 1, lengths=[200, 0, 1, 77, 129], junk=junk)
+    _window_case(2, 2, 2, 200, dim, F16, 2, 1, 48, lengths=[31, 150], junk=junk)
+
+
+def test_window_lengths_outside():
+    """Lengths below zero are zero, those above the tokens are the tokens."""
+    _window_case(3, 2, 2, 70, 64, BF16, 20, 0, 1, lengths=[-5, 1000, 70])
+
+
+def test_window_scale():
+    _window_case(1, 2, 2, 150, 128, BF16, None, 0, 1, scale=0.02)
+    _window_case(1, 2, 2, 150, 128, BF16, None, 0, 1, scale=-0.05)
+    _window_case(1, 2, 2, 150, 128, BF16, 30, 0, 1, scale=0.0)
+
+
+def test_window_many_tiles():
+    """More than 64 tiles of rows: the order of the XCDs' shares."""
+    _window_case(1, 3, 1, 8500, 64, BF16, 300, 5, 1)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_window_values_that_are_not_finite_reach_only_who_sees_them(value):
+    """Token 100's value row: queries before it, and those whose window has passed it, do not change."""
+    shape = (1, 2, 300, 128)
+    q, k, v = (_rand(shape, BF16, s) for s in (1, 2, 3))
+    how = dict(window=40, sinks=2)
+    clean = window_attention(q, k, v, **how)
+    v[:, :, 100, 5] = value
+    got = window_attention(q, k, v, **how)
+    hit = torch.zeros(300, dtype=torch.bool, device="cuda")
+    hit[100:140] = True
+    assert torch.equal(got[:, :, ~hit], clean[:, :, ~hit])
+    assert torch.equal(got[:, :, hit][..., :5], clean[:, :, hit][..., :5])
+    bad = got[:, :, hit][..., 5]
+    assert bad.isnan().all() if math.isnan(value) else (bad == value).all()
+    # A key row: nobody before it, nobody behind its window.
+    v[:, :, 100, 5] = 0
+    k[:, :, 100] = value if not math.isinf(value) else math.nan
+    got = window_attention(q, k, v, **how)
+    v_clean = window_attention(q, torch.nan_to_num(k), v, **how)
+    assert torch.equal(got[:, :, ~hit], v_clean[:, :, ~hit])
+
+
+def test_window_large_logits():
+    """The reference moves with the maximum: logits of hundreds, rising and falling along the keys."""
+    n = 400
+    q, k, v = (_rand((1, 1, n, 128), BF16, s) for s in (1, 2, 3))
+    for ramp in (torch.linspace(0, 60, n), torch.linspace(60, 0, n)):
+        big = (k.float() + q.float().mean(2, keepdim=True) + ramp.cuda()[None, None, :, None] * 0.2).to(BF16)
+        out, lse = window_attention(q, big, v, return_lse=True)
+        at = torch.arange(n, device="cuda")
+        o, l, spread = attend(q[0], big[0], v[0], seen_mask(at, at, None, 0, 1))
+        check_lse(lse[0], l, 128, logit_size(q, big))
+        # Logits are off by up to their size times 2^-24 * 128; the weights by as much.
+        u = HALF_STEP[BF16]
+        room = (u * (1 + u) + logit_size(q, big) * 128 * 2.0 ** -24 * 2) * (spread + o.abs()) + 1e-4
+        assert ((out[0].double() - o).abs() <= room).all()
+
+
+def test_window_of_no_tokens():
+    empty = torch.empty((2, 3, 0, 64), dtype=BF16, device="cuda")
+    out, lse = window_attention(empty, empty, empty, window=3, return_lse=True)
+    assert out.shape == empty.shape and lse.shape == (2, 3, 0)
+    none = torch.empty((0, 3, 5, 64), dtype=BF16, device="cuda")
+    assert window_attention(none, none, none).shape == none.shape
+
+
+# ---- paged cache and chunks ---------------------------------------------------
+
+
+def _cache(new, total, heads, dim, page, dtype, seed=0, spare=2, token_major=False):
+    """(cache, table on the host, lengths, offsets) with all pages filled at random."""
+    gen = torch.Generator().manual_seed(seed)
+    needed = [-(-t // page) for t in total]
+    pages = sum(needed) + spare
+    shape = (pages, heads, page, dim)
+    cache = PagedCache(*(_rand(shape, dtype, seed + s, 1.0, token_major) for s in (11, 12)))
+    table = torch.full((len(total), max(needed + [1])), -1, dtype=torch.int32)
+    order, at = torch.randperm(pages, generator=gen), 0
+    for b, n in enumerate(needed):
+        table[b, :n] = order[at:at + n]
+        at += n
+    offsets = torch.tensor([0] + new).cumsum(0).to(torch.int32)
+    return cache, table, torch.tensor(total, dtype=torch.int32), offsets
+
+
+def _check_chunk(out, lse, q, cache, table, total, offsets, window, sinks, frame, dtype):
+    page, pages = cache.k.shape[2], cache.k.shape[0]
+    for b, length in enumerate(total.tolist()):
+        start, stop = offsets[b].item(), offsets[b + 1].item()
+        if stop == start:
+            continue
+        keys = torch.arange(max(0, min(length, table.shape[1] * page)), device="cuda")
+        at = table[b].cuda().long()[keys // page]
+        there = (at >= 0) & (at < pages)
+        mask = seen_mask(length - (stop - start) + torch.arange(stop - start, device="cuda"), keys, window, sinks, frame)
+        at = at.clamp(0, pages - 1)
+        k, v = (t[at, :, keys % page].transpose(0, 1) for t in cache)
+        qb = q[start:stop].transpose(0, 1)
+        o, l, spread = attend(qb, k, v, mask & there)
+        check_output(out[start:stop].transpose(0, 1), o, spread, dtype)
+        check_lse(lse[start:stop].transpose(0, 1), l, q.shape[-1], logit_size(qb, k))
+
+
+def _chunk_case(new, total, heads, kv_heads, dim, page, dtype=BF16, window=None, sinks=0, frame=1, evict=False, seed=0,
+                token_major=False):
+    cache, table, lengths, offsets = _cache(new, total, kv_heads, dim, page, dtype, seed, token_major=token_major)
+    tokens = int(offsets[-1])
+    q = _rand((tokens + 5, heads, dim), dtype, seed + 1, 2.0)
+    for b, (n, length) in enumerate(zip(new, total)):
+        # Behind the last token a page holds whatever was there.
+        if length % page:
+            for t in cache:
+                t[table[b, length // page].long(), :, length % page:] = math.nan
+        if evict and window is not None:
+            low = max(0, (length - n) // frame - window + 1) * frame
+            gone = slice(-(-min(sinks * frame, low) // page), low // page)
+            for t in cache:
+                t[table[b, gone].long()] = math.nan
+            table[b, gone] = -1 if b % 2 else 2 ** 31 - 1
+    out = torch.full((tokens + 5, heads, dim), 7.0, dtype=dtype, device="cuda")
+    dev = [t.cuda() for t in (table, lengths, offsets)]
+    got, lse = chunk_attention(q, cache, *dev, window=window, sinks=sinks, frame=frame, return_lse=True, out=out)
+    assert got is out and (out[tokens:] == 7).all()
+    _check_chunk(out, lse, q, cache, table, lengths, offsets, window, sinks, frame, dtype)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, F16), (128, BF16)])
+@pytest.mark.parametrize("page", [8, 24, 32, 64, 1560])
+def test_chunk_pages(dim, dtype, page):
+    _chunk_case([1, 5, 64, 1, 200], [1, 5, 300, 1000, 333], 4, 2, dim, page, dtype)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (8, 1), (12, 4), (40, 8)])
+def test_chunk_single_tokens(heads, kv_heads):
+    """One token in each sequence, from the first one to long caches: split over workgroups."""
+    _chunk_case([1] * 6, [1, 2, 33, 700, 4097, 20000], heads, kv_heads, 128, 64)
+
+
+@pytest.mark.parametrize("window,sinks,frame", [(1, 0, 1), (50, 0, 1), (64, 4, 1), (300, 100, 1), (2, 1, 48), (1, 1, 100),
+                                                (3, 0, 7)])
+@pytest.mark.parametrize("new,total", [([1, 3, 150, 96], [900, 700, 150, 530]), ([1, 1], [5000, 130])])
+def test_chunk_windows(window, sinks, frame, new, total):
+    """Pages that nobody sees any more are given back, and hold NaN."""
+    _chunk_case(new, total, 6, 2, 128, 32, window=window, sinks=sinks, frame=frame, evict=True)
+
+
+def test_chunk_empty_sequences():
+    _chunk_case([0, 3, 0, 0, 1, 0], [10, 40, 0, 70, 1, 5], 4, 4, 64, 16)
+    _chunk_case([0], [100], 2, 1, 64, 16)
+
+
+def test_chunk_token_major_cache():
+    _chunk_case([5, 1, 140], [100, 64, 777], 8, 4, 128, 16, token_major=True)
+
+
+def test_chunk_many_sequences():
+    """More sequences than lanes of a wave."""
+    new = [(7 * b) % 4 for b in range(150)]
+    _chunk_case(new, [n + (13 * b) % 90 for b, n in enumerate(new)], 2, 1, 64, 16)
+
+
+def test_chunk_holes():
+    """Pages missing in the middle, all of a sequence's pages missing, more new tokens than the length says."""
+    cache, table, lengths, offsets = _cache([4, 2, 9, 1], [300, 100, 64, 2000], 2, 128, 16, BF16)
+    table[0, 3:7] = -1
+    table[0, 18] = 10 ** 6
+    table[1] = -1
+    table[3, 20:100] = -7
+    lengths[2] = 5  # positions -4 .. 4: the first four queries see nothing
+    q = _rand((16, 4, 128), BF16, 3, 2.0)
+    for window, sinks in ((None, 0), (40, 8)):
+        out, lse = chunk_attention(q, cache, table.cuda(), lengths.cuda(), offsets.cuda(), window=window, sinks=sinks, return_lse=True)
+        _check_chunk(out, lse, q, cache, table, lengths, offsets, window, sinks, 1, BF16)
+        assert (out[4:6] == 0).all() and (lse[4:6] == -math.inf).all() and (out[6:10] == 0).all()
+
+
+def test_chunk_bounds_of_device_sizes():
+    """Lengths beyond the table, offsets beyond the tokens: what is there is done, nothing else is touched."""
+    cache, table, lengths, offsets = _cache([2, 2], [64, 64], 1, 64, 16, BF16)
+    q = _rand((4, 1, 64), BF16, 3)
+    many = torch.tensor([10 ** 6, 64], dtype=torch.int32)
+    out, lse = chunk_attention(q, cache, table.cuda(), many.cuda(), offsets.cuda(), return_lse=True)
+    _check_chunk(out, lse, q, cache, table, torch.tensor([64, 64]), offsets, None, 0, 1, BF16)
+    far = torch.tensor([0, 2, 1000], dtype=torch.int32)
+    chunk_attention(q, cache, table.cuda(), lengths.cuda(), far.cuda(), out=out)
+    back = torch.tensor([3, 1, -5], dtype=torch.int32)
+    out.fill_(3)
+    chunk_attention(q, cache, table.cuda(), lengths.cuda(), back.cuda(), out=out)
+    assert (out == 3).all()
+
+
+def test_chunk_of_nothing():
+    cache, table, lengths, offsets = (t.cuda() if torch.is_tensor(t) else t for t in _cache([1], [9], 2, 64, 16, BF16))
+    q = torch.empty((0, 2, 64), dtype=BF16, device="cuda")
+    assert chunk_attention(q, cache, table, lengths, offsets).shape == q.shape
+    bare = PagedCache(*(t[:0] for t in cache))
+    out, lse = chunk_attention(_rand((1, 2, 64), BF16, 1), bare, table, lengths, offsets, return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    out, lse = chunk_attention(_rand((1, 2, 64), BF16, 1), cache, table[:, :0], lengths, offsets, return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+
+
+def test_append_and_the_far_end_of_a_cache():
+    """Pages past 2^32 bytes of a cache, written and read."""
+    pages, page, heads, dim = 4400, 64, 64, 128  # 4.6 GB each
+    cache = PagedCache(*(torch.empty((pages, heads, page, dim), dtype=BF16, device="cuda") for _ in range(2)))
+    table = torch.tensor([[4399, 7, 4398]], dtype=torch.int32)
+    lengths, offsets = torch.tensor([150], dtype=torch.int32), torch.tensor([0, 150], dtype=torch.int32)
+    k, v, q = (_rand((150, heads, dim), BF16, s) for s in (1, 2, 3))
+    dev = [t.cuda() for t in (table, lengths, offsets)]
+    append_cache(cache, k, v, *dev)
+    assert torch.equal(cache.k[4398, :, :22], k[128:].transpose(0, 1)) and torch.equal(cache.v[4399], v[:64].transpose(0, 1))
+    out, lse = chunk_attention(q, cache, *dev, return_lse=True)
+    _check_chunk(out, lse, q, cache, table, lengths, offsets, None, 0, 1, BF16)
+
+
+@pytest.mark.parametrize("dim,heads,page", [(64, 1, 8), (128, 5, 64), (64, 8, 1560)])
+@pytest.mark.parametrize("token_major", [False, True])
+def test_append(dim, heads, page, token_major):
+    new, total = [1, 0, 70, 3, 9], [1, 50, 200, 1600, 9]
+    cache, table, lengths, offsets = _cache(new, total, heads, dim, page, F16, token_major=token_major)
+    table[3, 0] = -1  # not written to: its new tokens lie behind
+    k = _rand((90, heads, dim), F16, 5)
+    v = _rand((90, 3, heads, dim), F16, 6)[:, 1]  # a slice of a projection
+    want = PagedCache(cache.k.clone(), cache.v.clone())
+    for b, (n, length) in enumerate(zip(new, total)):
+        for i in range(n):
+            at = length - n + i
+            for dst, src in zip(want, (k, v)):
+                dst[table[b, at // page].long(), :, at % page] = src[offsets[b] + i]
+    assert append_cache(cache, k, v, table.cuda(), lengths.cuda(), offsets.cuda()) is cache
+    assert torch.equal(cache.k, want.k) and torch.equal(cache.v, want.v)
+
+
+def test_append_drops_what_has_no_place():
+    cache, table, lengths, offsets = _cache([4, 4, 4], [4, 40, 4], 2, 64, 16, BF16)
+    before = PagedCache(cache.k.clone(), cache.v.clone())
+    table[0, 0] = -1
+    lengths[1] = 1000  # past the table
+    lengths[2] = 2     # two of four rows lie before position 0
+    k, v = _rand((12, 2, 64), BF16, 1), _rand((12, 2, 64), BF16, 2)
+    append_cache(cache, k, v, table.cuda(), lengths.cuda(), offsets.cuda())
+    before.k[table[2, 0].long(), :, :2] = k[10:].transpose(0, 1)
+    before.v[table[2, 0].long(), :, :2] = v[10:].transpose(0, 1)
+    assert torch.equal(cache.k, before.k) and torch.equal(cache.v, before.v)

@@ -1,0 +1,156 @@
+"""What the streaming operators refuse, before any launch (CPU only)."""
+import ctypes
+
+import pytest
+import torch
+
+from ab_attention import _lib
+from ab_attention.streaming import PagedCache, append_cache, chunk_attention, rotary, window_attention
+
+BF16 = torch.bfloat16
+
+
+def _z(*shape, dtype=BF16):
+    return torch.zeros(shape, dtype=dtype)
+
+
+_POS = torch.zeros((5, 3), dtype=torch.int32)
+
+
+@pytest.mark.parametrize("args,kw,msg", [
+    ((_z(2, 5, 128), None, _POS, (44, 42, 42)), {}, "B,H,N,D"),
+    ((_z(1, 2, 5, 128), _z(1, 2, 6, 128), _POS, (44, 42, 42)), {}, "same batch"),
+    ((_z(1, 2, 5, 128), _z(1, 2, 5, 128, dtype=torch.float16), _POS, (44, 42, 42)), {}, "one type"),
+    ((_z(1, 2, 5, 128, dtype=torch.float64), None, _POS, (44, 42, 42)), {}, "BF16"),
+    ((_z(1, 2, 5, 12), None, _POS, (4, 4, 4)), {}, "multiple of 8"),
+    ((_z(1, 2, 5, 128), None, _POS, (44, 42, 44)), {}, "add up"),
+    ((_z(1, 2, 5, 128), None, _POS, (43, 42, 42)), {}, "even"),
+    ((_z(1, 2, 5, 128), None, _POS, ()), {}, "1 to 4"),
+    ((_z(1, 2, 5, 128), None, _POS, (44, 42, 42)), {"pairing": "other"}, "pairing"),
+    ((_z(1, 2, 5, 128), None, _POS, (44, 42, 40)), {"pairing": "halves"}, "multiple of 16"),
+    ((_z(1, 2, 5, 128), None, _POS, (44, 42, 42)), {"theta": 0.0}, "theta"),
+    ((_z(1, 2, 5, 128), None, _POS, (44, 42, 42)), {"theta": float("inf")}, "theta"),
+    ((_z(1, 2, 5, 128), None, _POS.double(), (44, 42, 42)), {}, "int32"),
+    ((_z(1, 2, 5, 128), None, _POS[:4], (44, 42, 42)), {}, "positions must be"),
+    ((_z(2, 2, 5, 128), None, _POS[None].expand(3, 5, 3), (44, 42, 42)), {}, "positions must be"),
+    ((_z(1, 2, 5, 128), None, _POS, (44, 42, 42)), {}, "CUDA"),
+])
+def test_rotary_refuses(args, kw, msg):
+    with pytest.raises(ValueError, match=msg):
+        rotary(*args, **kw)
+
+
+@pytest.mark.parametrize("q,k,kw,msg", [
+    (_z(2, 8, 64), _z(2, 8, 64), {}, "B,H,N,D"),
+    (_z(1, 2, 8, 64), _z(1, 2, 9, 64), {}, "share"),
+    (_z(1, 2, 8, 96), _z(1, 2, 8, 96), {}, "64 or 128"),
+    (_z(1, 2, 8, 64, dtype=torch.float32), _z(1, 2, 8, 64, dtype=torch.float32), {}, "BF16"),
+    (_z(1, 3, 8, 64), _z(1, 2, 8, 64), {}, "multiple"),
+    (_z(1, 2, 8, 64), _z(1, 0, 8, 64), {}, "multiple"),
+    (_z(1, 2, 8, 64), _z(1, 2, 8, 64), {"window": 0}, "window"),
+    (_z(1, 2, 8, 64), _z(1, 2, 8, 64), {"window": -3}, "window"),
+    (_z(1, 2, 8, 64), _z(1, 2, 8, 64), {"sinks": -1}, "sinks"),
+    (_z(1, 2, 8, 64), _z(1, 2, 8, 64), {"frame": 0}, "frame"),
+    (_z(1, 2, 8, 64), _z(1, 2, 8, 64), {"scale": float("nan")}, "scale"),
+    (_z(1, 2, 8, 64), _z(1, 2, 8, 64), {"lengths": torch.zeros(2, dtype=torch.int32)}, "lengths"),
+    (_z(1, 2, 8, 64), _z(1, 2, 8, 64), {"lengths": torch.zeros(1, dtype=torch.int64)}, "lengths"),
+    (_z(1, 2, 8, 64), _z(1, 2, 8, 64), {}, "CUDA"),
+])
+def test_window_attention_refuses(q, k, kw, msg):
+    with pytest.raises(ValueError, match=msg):
+        window_attention(q, k, k, **kw)
+
+
+def _cache(pages=4, heads=2, page=16, dim=64, dtype=BF16):
+    return PagedCache(_z(pages, heads, page, dim, dtype=dtype), _z(pages, heads, page, dim, dtype=dtype))
+
+
+_TABLE, _LENGTHS, _OFFSETS = (torch.zeros(s, dtype=torch.int32) for s in ((2, 3), (2,), (3,)))
+
+
+@pytest.mark.parametrize("change,msg", [
+    (dict(q=_z(1, 5, 2, 64)), r"T,H,D"),
+    (dict(cache=_cache(dim=128)), "cache must be"),
+    (dict(cache=PagedCache(_z(4, 2, 16, 64), _z(4, 2, 8, 64))), "cache must be"),
+    (dict(cache=_cache(dtype=torch.float16)), "same type"),
+    (dict(cache=_cache(page=12)), "multiple of 8"),
+    (dict(cache=_cache(page=0)), "multiple of 8"),
+    (dict(cache=PagedCache(_z(4, 2, 64, 16).transpose(2, 3), _z(4, 2, 16, 64))), "rows must be"),
+    (dict(cache=_cache(heads=3)), "multiple"),
+    (dict(page_table=torch.zeros((3, 3), dtype=torch.int32)), "one batch"),
+    (dict(offsets=torch.zeros(2, dtype=torch.int32)), "one batch"),
+    (dict(lengths=torch.zeros(2, dtype=torch.int64)), "int32"),
+    (dict(page_table=torch.zeros((3, 2), dtype=torch.int32).T), "contiguous int32"),
+    (dict(), "CUDA"),
+])
+def test_cache_operators_refuse(change, msg):
+    how = dict(q=_z(5, 2, 64), cache=_cache(), page_table=_TABLE, lengths=_LENGTHS, offsets=_OFFSETS)
+    how.update(change)
+    q = how.pop("q")
+    with pytest.raises(ValueError, match=msg):
+        chunk_attention(q, **how)
+    with pytest.raises(ValueError, match=msg):
+        append_cache(how["cache"], q, q, how["page_table"], how["lengths"], how["offsets"])
+
+
+def test_append_refuses_other_shapes():
+    with pytest.raises(ValueError, match="one shape"):
+        append_cache(_cache(), _z(5, 2, 64), _z(4, 2, 64), _TABLE, _LENGTHS, _OFFSETS)
+
+
+_A = 4096  # a 16-byte aligned stand-in address: every case is refused before any runtime call
+
+
+def _window_args(**change):
+    a = _lib.WindowArgs(q=_A, k=_A, v=_A, out=_A, batch=1, heads=2, kv_heads=1, tokens=8, dim=64, dtype=0, window=0, sinks=0,
+                        frame=1, scale=0.1, pages=4, page_tokens=16, table_width=2)
+    for name in ("q_stride", "k_stride", "v_stride", "out_stride"):
+        setattr(a, name, (ctypes.c_int64 * 3)(1024, 512, 64))
+    for name, value in change.items():
+        setattr(a, name, (ctypes.c_int64 * 3)(*value) if name.endswith("stride") else value)
+    return a
+
+
+@pytest.mark.parametrize("change,msg", [
+    (dict(heads=3, kv_heads=2), b"multiple of kv_heads"), (dict(dim=96), b"64 or 128"), (dict(dtype=2), b"bf16 or fp16"),
+    (dict(frame=0), b"frame"), (dict(window=-1), b"negative"), (dict(scale=float("inf")), b"finite"),
+    (dict(tokens=1 << 30), b"too many"), (dict(batch=70000), b"too many"), (dict(k_stride=(1024, 512, 12)), b"strides"),
+    (dict(q_stride=(1024, -8, 64)), b"strides"), (dict(tokens=1 << 25, k_stride=(1 << 31, 1 << 31, 64)), b"4 GiB"),
+    (dict(q=0), b"null"), (dict(out=0), b"null"), (dict(k=_A + 8), b"aligned"), (dict(out=_A + 4), b"aligned"),
+])
+def test_window_entry_refuses(change, msg):
+    lib = _lib.load()
+    assert lib.ab_window_attention(_window_args(**change), None) == 1
+    assert msg in lib.ab_last_error() and lib.ab_last_error().startswith(b"window_attention:")
+
+
+@pytest.mark.parametrize("change,msg", [
+    (dict(page_tokens=12), b"multiple of 8"), (dict(page_tokens=0), b"multiple of 8"), (dict(lengths=0), b"null"),
+    (dict(table_width=1 << 28), b"fewer than 2^30"), (dict(pages=-1), b"pages"), (dict(k=0), b"null"),
+    (dict(page_tokens=1 << 22, k_stride=(0, 0, 1024)), b"4 GiB"),
+])
+def test_chunk_entry_refuses(change, msg):
+    lib = _lib.load()
+    args = _window_args(**{**dict(lengths=_A, offsets=_A, page_table=_A), **change})
+    assert lib.ab_chunk_attention(args, None) == 1
+    assert msg in lib.ab_last_error()
+
+
+def test_entries_of_nothing_launch_nothing():
+    lib = _lib.load()
+    assert lib.ab_window_attention(_window_args(tokens=0), None) == 0
+    assert lib.ab_window_attention(_window_args(batch=0), None) == 0
+    assert lib.ab_window_workspace_bytes(_window_args(tokens=0)) == 0
+    assert lib.ab_window_workspace_bytes(None) == 0
+    assert lib.ab_window_attention(None, None) == 1 and b"null" in lib.ab_last_error()
+    assert lib.ab_rotary(None, None) == 1 and lib.ab_append_cache(None, None) == 1
+
+
+def test_workspace_of_a_split_call():
+    """Few rows over many keys are split; the workspace holds each part's float32 rows, sums and references."""
+    lib = _lib.load()
+    args = _window_args(lengths=_A, offsets=_A, page_table=_A, tokens=1, batch=1, table_width=2048)
+    size = lib.ab_window_workspace_bytes(args)
+    row = 2 * (64 * 4 + 8)
+    assert size > 0 and size % row == 0 and size // row <= 2048 * 16 // 32
+    assert lib.ab_window_workspace_bytes(_window_args(tokens=100000, q_stride=(0, 0, 64), heads=64)) == 0
