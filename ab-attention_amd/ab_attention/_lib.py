@@ -72,6 +72,13 @@ class WindowArgs(ctypes.Structure):
                 ("workspace_bytes", _SZ)]
 
 
+class WindowGradArgs(ctypes.Structure):
+    """ab_window_grad_args of include/ab_attention.h."""
+
+    _fields_ = [("forward", WindowArgs), ("dout", _P), ("dlse", _P), ("dq", _P), ("dk", _P), ("dv", _P),
+                ("dout_stride", _I64 * 3), ("dq_stride", _I64 * 3), ("dk_stride", _I64 * 3), ("dv_stride", _I64 * 3)]
+
+
 class AppendArgs(ctypes.Structure):
     """ab_append_args of include/ab_attention.h."""
 
@@ -110,6 +117,8 @@ SIGNATURES = {
     "ab_window_workspace_bytes": (_SZ, [ctypes.POINTER(WindowArgs)]),
     "ab_window_attention": (ctypes.c_int, [ctypes.POINTER(WindowArgs), _P]),
     "ab_chunk_attention": (ctypes.c_int, [ctypes.POINTER(WindowArgs), _P]),
+    "ab_window_grad_workspace_bytes": (_SZ, [ctypes.POINTER(WindowGradArgs)]),
+    "ab_window_attention_grad": (ctypes.c_int, [ctypes.POINTER(WindowGradArgs), _P]),
     "ab_append_cache": (ctypes.c_int, [ctypes.POINTER(AppendArgs), _P]),
 }
 

@@ -182,18 +182,52 @@ def _run(args, entry, device):
         _lib.check(getattr(lib, entry)(args, _lib.stream(device)))
 
 
-def _window_forward(q, k, v, lengths, window, sinks, frame, scale, return_lse):
-    q, k, v = _strided(q), _strided(k), _strided(v)
+def _window_args(q, k, v, out, lse, lengths, window, sinks, frame, scale):
+    """The call's ab_window_args of [B, H, N, D] tensors that _strided has seen."""
     batch, heads, tokens, dim = q.shape
+    address = _lib.address
+    return _lib.WindowArgs(address(q), address(k), address(v), address(out), address(lse), address(lengths), None, None, batch,
+                           heads, k.shape[1], tokens, dim, _DTYPES[q.dtype], 0, 0, 0, window, sinks, frame, scale,
+                           q.stride()[:3], k.stride()[:3], v.stride()[:3], out.stride()[:3], None, 0)
+
+
+def _window_forward(q, k, v, lengths, window, sinks, frame, scale, return_lse):
     out = torch.empty_like(q)
-    lse = torch.empty((batch, heads, tokens), dtype=torch.float32, device=q.device) if return_lse else None
-    if tokens:
-        address = _lib.address
-        args = _lib.WindowArgs(address(q), address(k), address(v), address(out), address(lse), address(lengths), None, None,
-                               batch, heads, k.shape[1], tokens, dim, _DTYPES[q.dtype], 0, 0, 0, window, sinks, frame, scale,
-                               q.stride()[:3], k.stride()[:3], v.stride()[:3], out.stride()[:3], None, 0)
-        _run(args, "ab_window_attention", q.device)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if return_lse else None
+    if out.numel():
+        _run(_window_args(q, k, v, out, lse, lengths, window, sinks, frame, scale), "ab_window_attention", q.device)
     return out, lse
+
+
+class _Window(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, *how):
+        q, k, v = _strided(q), _strided(k), _strided(v)
+        out, lse = _window_forward(q, k, v, lengths, *how, True)
+        ctx.save_for_backward(q, k, v, out, lse, lengths)
+        ctx.how = how
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dlse):
+        q, k, v, out, lse, lengths = ctx.saved_tensors
+        if dout is None and dlse is None:
+            return (None,) * (4 + len(ctx.how))
+        dout = torch.zeros_like(out) if dout is None else _strided(dout)
+        dlse = None if dlse is None else dlse.contiguous()
+        grads = tuple(torch.empty_like(t) for t in (q, k, v))
+        if q.numel():
+            address, lib = _lib.address, _lib.load()
+            args = _lib.WindowGradArgs(_window_args(q, k, v, out, lse, lengths, *ctx.how), address(dout), address(dlse),
+                                       *map(address, grads), dout.stride()[:3], *(g.stride()[:3] for g in grads))
+            with _lib.on(q.device):
+                size = lib.ab_window_grad_workspace_bytes(args)
+                workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+                args.forward.workspace, args.forward.workspace_bytes = _lib.address(workspace), size
+                _lib.check(lib.ab_window_attention_grad(args, _lib.stream(q.device)))
+        return (*grads, *[None] * (1 + len(ctx.how)))
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int | None = None, sinks: int = 0,
@@ -207,7 +241,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     ``scale`` defaults to D ** -0.5.
 
     Returns o in q's type and memory order, and with ``return_lse`` the base-2
-    softmax normaliser as float32 [B, H, N].
+    softmax normaliser as float32 [B, H, N]. Differentiable in q, k and v, through
+    both; the same inputs give the same gradients bit for bit. Values that are not
+    finite reach the results of the queries that see them only, but may reach any
+    gradient of their batch item.
     """
     if q.ndim != 4 or k.ndim != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
         raise ValueError("Q [B,H,N,D] and K/V [B,Hk,N,D] must share batch, tokens and dim")
@@ -222,8 +259,11 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != q.shape[:1] or not lengths.is_contiguous()):
         raise ValueError("lengths must be int32 [B]")
     _gpu("window attention", q, k, v, lengths)
-    with torch.no_grad():
-        out, lse = _window_forward(q, k, v, lengths, window, sinks, frame, scale, return_lse)
+    how = (window, sinks, frame, scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _Window.apply(q, k, v, lengths, *how)
+    else:
+        out, lse = _window_forward(_strided(q), _strided(k), _strided(v), lengths, *how, return_lse)
     return (out, lse) if return_lse else out
 
 

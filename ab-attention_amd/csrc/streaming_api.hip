@@ -31,6 +31,10 @@ int rows_of(const char* what, const int64_t (&stride)[3], int64_t batch, int64_t
     return AB_OK;
 }
 
+// Whether the kernels' 32-bit offsets reach the rows of a head and 64 behind them
+// (which they ask for and get zeros).
+bool head_fits(const Rows& r, int64_t tokens) { return (r.token * (tokens + 64) + 128) * 2 <= int64_t(0xffffffff); }
+
 int check_heads(const char* what, int64_t batch, int64_t heads, int64_t kv_heads, int64_t tokens, int64_t dim) {
     if (batch < 0 || tokens < 0 || heads <= 0 || kv_heads <= 0)
         return set_error(AB_ERR_INVALID, "%s: sizes must be positive", what);
@@ -51,7 +55,7 @@ int check_cache(const char* what, int64_t batch, int64_t kv_heads, int64_t pages
         return set_error(AB_ERR_INVALID, "%s: too many pages", what);
     if (int rc = rows_of(what, k_stride, pages, kv_heads, page_tokens, 8, k)) return rc;
     if (int rc = rows_of(what, v_stride, pages, kv_heads, page_tokens, 8, v)) return rc;
-    if (std::max(k.token, v.token) * 2 * page_tokens > int64_t(0xffffffff) || std::max(k.token, v.token) >= (int64_t(1) << 28))
+    if (!head_fits(k, page_tokens) || !head_fits(v, page_tokens))
         return set_error(AB_ERR_INVALID, "%s: one head of a page must be under 4 GiB", what);
     if (batch > 0 && (!lengths || !offsets || (width > 0 && !table)))
         return set_error(AB_ERR_INVALID, "%s: null pointer", what);
@@ -113,7 +117,7 @@ int window_call(const char* what, const ab_window_args& a, bool paged, WindowCal
     } else {
         if (int rc = rows_of(what, a.k_stride, a.batch, a.kv_heads, a.tokens, 8, c.k_rows)) return rc;
         if (int rc = rows_of(what, a.v_stride, a.batch, a.kv_heads, a.tokens, 8, c.v_rows)) return rc;
-        if ((std::max(c.k_rows.token, c.v_rows.token) * a.tokens + a.dim) * 2 > int64_t(0xffffffff))
+        if (!head_fits(c.k_rows, a.tokens) || !head_fits(c.v_rows, a.tokens))
             return set_error(AB_ERR_INVALID, "%s: one head of K/V must be under 4 GiB", what);
         c.row = {a.heads * a.tokens, a.tokens, 1};
     }
@@ -219,6 +223,84 @@ int ab_window_attention(const ab_window_args* args, void* stream) {
 
 int ab_chunk_attention(const ab_window_args* args, void* stream) {
     return window_launch("chunk_attention", args, true, stream);
+}
+
+}  // extern "C"
+
+namespace {
+// The checked form of a backward call, with the floats of its workspace.
+int grad_call(const ab_window_grad_args& a, WindowGradCall& g, int64_t& stat, int64_t& partial) {
+    const char* what = "window_attention_grad";
+    const ab_window_args& f = a.forward;
+    WindowCall c;
+    if (int rc = window_call(what, f, false, c)) return rc;
+    g = WindowGradCall{};
+    g.q = f.q;
+    g.k = f.k;
+    g.v = f.v;
+    g.out = f.out;
+    g.dout = a.dout;
+    g.lse = f.lse;
+    g.dlse = a.dlse;
+    g.dq = a.dq;
+    g.dk = a.dk;
+    g.dv = a.dv;
+    g.q_rows = c.q_rows;
+    g.k_rows = c.k_rows;
+    g.v_rows = c.v_rows;
+    if (int rc = rows_of(what, f.out_stride, f.batch, f.heads, f.tokens, 8, g.out_rows)) return rc;
+    if (int rc = rows_of(what, a.dout_stride, f.batch, f.heads, f.tokens, 8, g.dout_rows)) return rc;
+    if (int rc = rows_of(what, a.dq_stride, f.batch, f.heads, f.tokens, 8, g.dq_rows)) return rc;
+    if (int rc = rows_of(what, a.dk_stride, f.batch, f.kv_heads, f.tokens, 8, g.dk_rows)) return rc;
+    if (int rc = rows_of(what, a.dv_stride, f.batch, f.kv_heads, f.tokens, 8, g.dv_rows)) return rc;
+    if (!head_fits(g.q_rows, f.tokens) || !head_fits(g.dout_rows, f.tokens))
+        return set_error(AB_ERR_INVALID, "%s: one head of Q and of its gradient must be under 4 GiB", what);
+    g.batch = c.batch;
+    g.heads = c.heads;
+    g.kv_heads = c.kv_heads;
+    g.tokens = c.tokens;
+    g.dim = c.dim;
+    g.half = c.half;
+    g.lengths = c.lengths;
+    g.group = c.heads / c.kv_heads;
+    g.mask = c.mask;
+    g.scale = static_cast<float>(f.scale);
+    g.scale_log2 = c.scale_log2;
+    plan_window_grad(g, stat, partial);
+    return AB_OK;
+}
+}  // namespace
+
+extern "C" {
+
+size_t ab_window_grad_workspace_bytes(const ab_window_grad_args* a) {
+    WindowGradCall g;
+    int64_t stat, partial;
+    if (!a || a->forward.batch <= 0 || a->forward.tokens <= 0 || grad_call(*a, g, stat, partial)) return 0;
+    return size_t(stat + partial) * sizeof(float);
+}
+
+int ab_window_attention_grad(const ab_window_grad_args* a, void* stream) {
+    const char* what = "window_attention_grad";
+    if (!a) return set_error(AB_ERR_INVALID, "%s: null pointer", what);
+    WindowGradCall g;
+    int64_t stat, partial;
+    if (int rc = grad_call(*a, g, stat, partial)) return rc;
+    const ab_window_args& f = a->forward;
+    if (f.batch == 0 || f.tokens == 0) return AB_OK;
+    for (const void* p : {f.q, f.k, f.v, static_cast<const void*>(f.out), a->dout, static_cast<const void*>(a->dq),
+                          static_cast<const void*>(a->dk), static_cast<const void*>(a->dv),
+                          static_cast<const void*>(f.workspace)}) {
+        if (!p) return set_error(AB_ERR_INVALID, "%s: null pointer", what);
+        if (!aligned(p, 16)) return set_error(AB_ERR_INVALID, "%s: tensors must be 16-byte aligned", what);
+    }
+    if (!f.lse) return set_error(AB_ERR_INVALID, "%s: null pointer", what);
+    if (f.workspace_bytes < size_t(stat + partial) * sizeof(float))
+        return set_error(AB_ERR_INVALID, "%s: workspace of %zu bytes is smaller than the %zu required", what, f.workspace_bytes,
+                         size_t(stat + partial) * sizeof(float));
+    g.stat = static_cast<float*>(f.workspace);
+    g.partial = g.stat + stat;
+    return launch_window_grad(g, static_cast<hipStream_t>(stream));
 }
 
 int ab_append_cache(const ab_append_args* a, void* stream) {

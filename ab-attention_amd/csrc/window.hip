@@ -17,14 +17,6 @@
 namespace ab {
 namespace {
 
-// Keys of a part's tiles: the first `sink_tiles` tiles start at 0, the others at `window`.
-struct TileRange {
-    int sink_tiles, window, tiles;
-    __device__ __forceinline__ int key(int u) const {
-        return kWindowKeys * (u < sink_tiles ? u : u - sink_tiles) + (u < sink_tiles ? 0 : window);
-    }
-};
-
 // What a workgroup works on. The same in all its lanes.
 struct WindowUnit {
     int b, kv_head, head;  // head: the query head, or the first one of the group
@@ -34,22 +26,6 @@ struct WindowUnit {
     int first;             // position of its first new token
     int length;            // keys of it
 };
-
-// Workgroup index -> (head, tile). Workgroups are dealt round-robin over the 8
-// XCDs; with many tiles each XCD takes a contiguous eighth of a head's tiles,
-// whose windows overlap in its L2, and every other head in the opposite order,
-// so that the longer rows of a causal mask without a window spread evenly.
-__device__ __forceinline__ bool window_place(uint32_t id, int heads, int tiles, int& head, int& tile) {
-    if (tiles < 64) {
-        head = id / tiles;
-        tile = tiles - 1 - (id - head * tiles);
-        return head < heads;
-    }
-    const int per = (tiles + 7) >> 3, x = id & 7, s = id >> 3;
-    head = s / per;
-    tile = ((head & 1) ? 7 - x : x) * per + (per - 1 - (s - head * per));
-    return head < heads && tile < tiles;
-}
 
 template <bool kPaged>
 __device__ __forceinline__ bool window_unit(const WindowCall& c, uint32_t id, int tiles, WindowUnit& u) {
@@ -119,18 +95,9 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     const int row0 = u.tile * kWindowRows, rows = min(kWindowRows, u.n * group - row0);
     auto token_at = [&](int r) { return kPaged ? (row0 + r) / group : row0 + r; };
     const int p_first = max(u.first + token_at(0), 0), p_last = min(u.first + token_at(rows - 1), u.length - 1);
-    TileRange range{0, 0, 0};
-    int end = 0;  // keys from here on are seen by no row
-    if (p_last >= p_first) {
-        const int low = mask.low(p_first);
-        end = mask.high(p_last, u.length);
-        const int sinks = min(mask.sinks, end);
-        if (low > sinks) {
-            range.sink_tiles = (sinks + kWindowKeys - 1) / kWindowKeys;
-            range.window = max(low & ~7, range.sink_tiles * kWindowKeys);
-        }
-        range.tiles = range.sink_tiles + max(0, end - range.window + kWindowKeys - 1) / kWindowKeys;
-    }
+    TileRange range;
+    range.set(mask, p_first, p_last, u.length);
+    const int end = range.end;
     int tile0 = 0, tiles = range.tiles;
     if constexpr (kSplit) {
         const int part = blockIdx.y;
@@ -462,8 +429,7 @@ __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
 template <class T, int D, bool kPaged>
 int launch_as(const WindowCall& c, hipStream_t stream) {
     const int64_t tiles = window_tiles(c), heads = kPaged ? c.kv_heads : int64_t(c.batch) * c.heads;
-    const int64_t per_head = tiles < 64 ? tiles : (tiles + 7) / 8 * 8;
-    const dim3 grid(static_cast<unsigned>(per_head * heads), static_cast<unsigned>(c.parts));
+    const dim3 grid(window_grid(heads, tiles), static_cast<unsigned>(c.parts));
     if (c.parts == 1) {
         hipLaunchKernelGGL((window_kernel<T, D, kPaged, false>), grid, dim3(kWindowThreads), 0, stream, c, int(tiles));
         return check_launch("window_kernel");

@@ -149,12 +149,73 @@ struct WindowCall {
     int64_t rows;                            // queries times heads
 };
 
+// One call of the backward pass over strided tensors. `stat` holds, for every
+// 32 queries of a head, their 32 normalisers and 32 values of -delta.
+struct WindowGradCall {
+    const void *q, *k, *v, *out, *dout;
+    const float *lse, *dlse;  // dlse: of the normalisers, or none
+    void *dq, *dk, *dv;
+    Rows q_rows, k_rows, v_rows, out_rows, dout_rows, dq_rows, dk_rows, dv_rows;
+    int32_t batch, heads, kv_heads, tokens, dim, half;
+    const int32_t* lengths;
+    int32_t group;
+    WindowMask mask;
+    float scale, scale_log2;
+    float* stat;
+    int32_t sink_tiles, sink_parts;  // key tiles whose queries are split, and into how many parts
+    float* partial;                  // [batch][kv_heads][sink_tiles][sink_parts][2][128][dim]
+};
+
 constexpr int kWindowThreads = 256;
 constexpr int kWindowRows = 128;  // query rows of a workgroup
 constexpr int kWindowKeys = 32;   // keys of a tile
 
+// Keys of a run of tiles: the first `sink_tiles` tiles start at 0, the others at
+// `window`; together they hold every key that some position from p_first to
+// p_last sees, once.
+struct TileRange {
+    int sink_tiles, window, tiles, end;  // end: keys from here on are seen by none
+    __device__ __forceinline__ int key(int u) const {
+        return kWindowKeys * (u < sink_tiles ? u : u - sink_tiles) + (u < sink_tiles ? 0 : window);
+    }
+    __device__ __forceinline__ void set(const WindowMask& mask, int p_first, int p_last, int length) {
+        sink_tiles = window = tiles = end = 0;
+        if (p_last < p_first) return;
+        const int low = mask.low(p_first);
+        end = mask.high(p_last, length);
+        const int sinks = min(mask.sinks, end);
+        if (low > sinks) {
+            sink_tiles = (sinks + kWindowKeys - 1) / kWindowKeys;
+            window = max(low & ~7, sink_tiles * kWindowKeys);
+        }
+        tiles = sink_tiles + max(0, end - window + kWindowKeys - 1) / kWindowKeys;
+    }
+};
+
+// Workgroup index -> (head, tile). Workgroups are dealt round-robin over the 8
+// XCDs; with many tiles each XCD takes a contiguous eighth of a head's tiles,
+// whose windows overlap in its L2, and every other head in the opposite order,
+// so that the longer rows of a causal mask without a window spread evenly.
+__device__ __forceinline__ bool window_place(uint32_t id, int heads, int tiles, int& head, int& tile) {
+    if (tiles < 64) {
+        head = id / tiles;
+        tile = tiles - 1 - (id - head * tiles);
+        return head < heads;
+    }
+    const int per = (tiles + 7) >> 3, x = id & 7, s = id >> 3;
+    head = s / per;
+    tile = ((head & 1) ? 7 - x : x) * per + (per - 1 - (s - head * per));
+    return head < heads && tile < tiles;
+}
+inline unsigned window_grid(int64_t heads, int64_t tiles) {
+    return static_cast<unsigned>((tiles < 64 ? tiles : (tiles + 7) / 8 * 8) * heads);
+}
+
 int launch_window(const WindowCall& call, hipStream_t stream);
 int window_parts(const WindowCall& call, int64_t most_keys);
 int64_t window_tiles(const WindowCall& call);
+int launch_window_grad(const WindowGradCall& call, hipStream_t stream);
+// Sets sink_tiles and sink_parts; returns the floats of stat and of partial.
+void plan_window_grad(WindowGradCall& call, int64_t& stat, int64_t& partial);
 
 }  // namespace ab

@@ -1,0 +1,447 @@
+// Windowed causal attention, backward.
+//
+// With P = 2^(S scale log2(e) - lse) recomputed from the forward pass'
+// normalisers, S = Q K^T, and delta = rowsum(dO o O) - dlse / ln 2,
+//   dV = P^T dO,  dS = P o (dO V^T - delta),  dQ = scale dS K,  dK = scale dS^T Q.
+// Two kernels of one shape, so that every sum has one owner and one order (no
+// atomics): a workgroup owns 128 rows, 32 a wave, kept in registers, and streams
+// tiles of 32 rows of the other side through LDS:
+//   queries: X = (Q, dO) owned, Y = (K, V) streamed, dQ += Y1^T dS,
+//   keys:    X = (K, V) owned, Y = (Q, dO) streamed (of all query heads that
+//            share them, one after the other), dK += Y1^T dS, dV += Y2^T P,
+// each with S^T = Y1 X1^T and dP^T = Y2 X2^T on 16x16x32 MFMAs whose lanes hold
+// one owned row and four streamed ones, which is the form the second products
+// take P and dS in. P and dS are rounded to 16 bits there (the matrix cores'
+// input type); all sums are float32.
+// The first keys (sinks) are seen by every later query. Their tiles would run
+// many times longer than the others, so their queries are split into parts whose
+// float32 sums a third kernel adds up, always in the same order.
+#include <algorithm>
+
+#include "window.hpp"
+
+namespace ab {
+namespace {
+
+constexpr int kTileRows = kWindowKeys;  // streamed rows of a tile
+static_assert(kTileRows == 32, "stat blocks are 32 queries");
+
+__device__ __forceinline__ int length_of(const WindowGradCall& c, int b) {
+    return c.lengths ? min(max(c.lengths[b], 0), c.tokens) : c.tokens;
+}
+
+// stat of 32 queries of a head per workgroup of D / 2 lanes... : row r's
+// normaliser and -delta. Rows past the batch item's length get zeros: nothing
+// of theirs is read.
+template <class T, int D>
+__global__ __launch_bounds__(256) void window_delta_kernel(WindowGradCall c, int blocks) {
+    constexpr int kLanes = D / 8, kRowsEach = 256 / kLanes;  // lanes of a row, rows at once
+    const int bh = blockIdx.y + gridDim.y * blockIdx.z, b = bh / c.heads, h = bh - b * c.heads;
+    if (b >= c.batch) return;
+    const int length = length_of(c, b), lane = threadIdx.x % kLanes;
+    float* stat = c.stat + (int64_t(bh) * blocks + blockIdx.x) * 64;
+#pragma unroll
+    for (int r = threadIdx.x / kLanes; r < 32; r += kRowsEach) {
+        const int t = blockIdx.x * 32 + r;
+        float sum = 0.f, lse = 0.f;
+        if (t < length) {
+            const uint16_t* o = static_cast<const uint16_t*>(c.out) + b * c.out_rows.batch + h * c.out_rows.head + t * c.out_rows.token;
+            const uint16_t* d = static_cast<const uint16_t*>(c.dout) + b * c.dout_rows.batch + h * c.dout_rows.head + t * c.dout_rows.token;
+            const u32x4 ow = *reinterpret_cast<const u32x4*>(o + 8 * lane), dw = *reinterpret_cast<const u32x4*>(d + 8 * lane);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sum = __builtin_fmaf(T::lo(ow[i]), T::lo(dw[i]), sum);
+                sum = __builtin_fmaf(T::hi(ow[i]), T::hi(dw[i]), sum);
+            }
+        }
+#pragma unroll
+        for (int s = 1; s < kLanes; s *= 2) sum += __shfl_xor(sum, s);
+        if (t < length && lane == 0) {
+            const int64_t at = int64_t(bh) * c.tokens + t;
+            lse = c.lse[at];
+            if (c.dlse) sum -= c.dlse[at] * 1.4426950408889634f;
+        }
+        if (lane == 0) {
+            stat[r] = lse;
+            stat[32 + r] = -sum;
+        }
+    }
+}
+
+// 4 bytes per lane from the buffer straight into LDS: lane j writes [lds + 4j, + 4).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void buffer_to_lds4(u32x4 buffer, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// A tensor's rows of one head, up to `rows` of them: reads past them give zeros.
+template <int D>
+__device__ __forceinline__ u32x4 head_buffer(const void* base, const Rows& r, int64_t b, int64_t h, int rows) {
+    const char* at = static_cast<const char*>(base) + (b * r.batch + h * r.head) * 2;
+    return buffer_of(at, rows > 0 ? static_cast<uint32_t>(rows - 1) * static_cast<uint32_t>(r.token * 2) + 2 * D : 0);
+}
+
+template <class T, int D, bool kKeys>
+__global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGradCall c, int tiles_per_head) {
+    constexpr int kSteps = D / 32, kBlocks = D / 16, kQuad = 4 * D * 2, kBytes = kTileRows * D * 2, kOps = D / 64;
+    constexpr int kOpRows = 1024 / (2 * D);
+    constexpr int kStat = 4 * kBytes;
+    // Two stages of Y1, two of Y2, and each wave's copy of the streamed rows' stat.
+    __shared__ __align__(16) unsigned char smem[4 * kBytes + (kKeys ? 8 * 256 : 0)];
+
+    // Owned rows. Sink tiles come first, part by part, then the tiles behind them.
+    int head, tile, part = 0, parts = 1;
+    if constexpr (kKeys) {
+        const int extra = c.sink_tiles * c.sink_parts;
+        const int per_head = tiles_per_head - c.sink_tiles + extra;
+        head = blockIdx.x / per_head;
+        tile = blockIdx.x - head * per_head;
+        if (tile < extra) {
+            parts = c.sink_parts;
+            part = tile % parts;
+            tile /= parts;
+        } else {
+            tile -= extra - c.sink_tiles;
+        }
+    } else {
+        if (!window_place(blockIdx.x, c.batch * c.heads, tiles_per_head, head, tile)) return;
+    }
+    const int heads = kKeys ? c.kv_heads : c.heads;
+    const int b = head / heads, h = head - b * heads;  // own head
+    const int length = length_of(c, b);
+    const WindowMask mask = c.mask;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int li = lane & 15, lg = lane >> 4;
+    const int own0 = tile * kWindowRows, own_last = min(own0 + kWindowRows, length) - 1;
+
+    // Queries that see a key at position p: start(p) .. until(p) - 1.
+    auto until = [&](int p) {
+        if (p < mask.sinks) return length;
+        const uint32_t far = static_cast<uint32_t>(mask.start(p)) + mask.frame.d;
+        return static_cast<int>(min(static_cast<uint32_t>(length), far + static_cast<uint32_t>(mask.back)));
+    };
+
+    // Streamed tiles: `rounds` heads times `tiles` tiles.
+    TileRange range;
+    int rounds = 1;
+    if constexpr (kKeys) {
+        range.sink_tiles = range.window = range.tiles = range.end = 0;
+        if (own_last >= own0) {
+            range.window = mask.start(own0) & ~(kTileRows - 1);
+            range.end = own0 < mask.sinks ? length : until(own_last);
+            range.tiles = (range.end - range.window + kTileRows - 1) / kTileRows;
+        }
+        rounds = c.group;
+    } else {
+        range.set(mask, own0, own_last, length);
+    }
+    const int64_t all = int64_t(rounds) * range.tiles;
+    const int first = static_cast<int>(all * part / parts), last = static_cast<int>(all * (part + 1) / parts);
+
+    // X as the B operand: owned row 16j + li of the wave's 32, dims 32s + 8lg .. + 7.
+    u32x4 x1[2][kSteps], x2[2][kSteps];
+    int from[2], to[2], sink[2];  // streamed rows seen: from .. to - 1, and those before sink
+    float lse[2] = {0.f, 0.f}, neg_delta[2] = {0.f, 0.f};
+    int own[2];
+    const int stat_blocks = (c.tokens + 31) / 32;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int p = own0 + wave * 32 + 16 * j + li;
+        own[j] = p;
+        const bool there = p < length;
+        const int64_t at = min(p, c.tokens - 1);
+        const Rows &r1 = kKeys ? c.k_rows : c.q_rows, &r2 = kKeys ? c.v_rows : c.dout_rows;
+        const uint16_t* a = static_cast<const uint16_t*>(kKeys ? c.k : c.q) + b * r1.batch + h * r1.head + at * r1.token + 8 * lg;
+        const uint16_t* d = static_cast<const uint16_t*>(kKeys ? c.v : c.dout) + b * r2.batch + h * r2.head + at * r2.token + 8 * lg;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            x1[j][s] = x2[j][s] = u32x4{0, 0, 0, 0};
+            if (there) {
+                x1[j][s] = *reinterpret_cast<const u32x4*>(a + 32 * s);
+                x2[j][s] = *reinterpret_cast<const u32x4*>(d + 32 * s);
+            }
+        }
+        from[j] = to[j] = sink[j] = 0;
+        if (there) {
+            if constexpr (kKeys) {
+                from[j] = mask.start(p);
+                to[j] = until(p);
+            } else {
+                from[j] = mask.low(p);
+                to[j] = mask.high(p, length);
+                sink[j] = min(mask.sinks, to[j]);
+                const float* stat = c.stat + (int64_t(head) * stat_blocks + (p >> 5)) * 64 + (p & 31);
+                lse[j] = stat[0];
+                neg_delta[j] = stat[32];
+            }
+        }
+    }
+    // Tiles that all rows of this wave see whole need no mask.
+    int full_from = 1, full_to = 0, full_sink = 0;
+    const int w0 = own0 + wave * 32, w1 = min(w0 + 31, length - 1);
+    const bool active = w1 >= w0;
+    if (active) {
+        if constexpr (kKeys) {
+            full_from = mask.start(w1);
+            full_to = w1 < mask.sinks ? length : until(max(w0, mask.sinks));
+        } else {
+            full_from = mask.low(w1);
+            full_to = mask.high(w0, length);
+            full_sink = min(mask.sinks, full_to);
+        }
+    }
+
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)smem));
+    const Rows &y1_rows = kKeys ? c.q_rows : c.k_rows, &y2_rows = kKeys ? c.dout_rows : c.v_rows;
+    const uint32_t y1_token = static_cast<uint32_t>(y1_rows.token * 2), y2_token = static_cast<uint32_t>(y2_rows.token * 2);
+    // Transfers of this wave: rows 8w .. 8w + 7 of a tile. Every four rows lie as
+    // blocks of 4 rows x 16 dims, block m at position m ^ (quad & 1): row reads and
+    // transposing reads both spread over the banks.
+    uint32_t src1[kOps], src2[kOps];
+#pragma unroll
+    for (int e = 0; e < kOps; ++e) {
+        const int quad = D == 128 ? e : lane >> 5, block = (lane >> 3) % kBlocks, r = (lane >> 1) & 3, half = lane & 1;
+        const uint32_t row = 8 * wave + (D == 128 ? 0 : 4 * quad) + r, at = uint32_t(2 * (block ^ (quad & 1)) + half) * 16u;
+        src1[e] = row * y1_token + at;
+        src2[e] = row * y2_token + at;
+    }
+    // The round and the tile of the next transfer.
+    int next = first, next_round = range.tiles ? first / range.tiles : 0, next_tile = first - next_round * range.tiles;
+    u32x4 y1_buf, y2_buf, stat_buf;
+    auto enter_round = [&](int round) {
+        const int hy = kKeys ? h * c.group + round : h / c.group;
+        y1_buf = head_buffer<D>(kKeys ? c.q : c.k, y1_rows, b, hy, range.end);
+        y2_buf = head_buffer<D>(kKeys ? c.dout : c.v, y2_rows, b, hy, range.end);
+        if constexpr (kKeys)
+            stat_buf = buffer_of(c.stat + (int64_t(b) * c.heads + hy) * stat_blocks * 64, stat_blocks * 256);
+    };
+    enter_round(next_round);
+    auto transfer = [&]() {
+        if (next >= last) return;
+        const uint32_t row = range.key(next_tile), stage = (next & 1) * kBytes + wave * (8 * D * 2);
+#pragma unroll
+        for (int e = 0; e < kOps; ++e) {
+            buffer_to_lds(y1_buf, src1[e] + (row + kOpRows * e) * y1_token, lds0 + stage + 1024 * e);
+            buffer_to_lds(y2_buf, src2[e] + (row + kOpRows * e) * y2_token, lds0 + 2 * kBytes + stage + 1024 * e);
+        }
+        if constexpr (kKeys) buffer_to_lds4(stat_buf, row * 8 + 4 * lane, lds0 + kStat + ((next & 1) * 4 + wave) * 256);
+        ++next;
+        if (++next_tile == range.tiles) {
+            next_tile = 0;
+            if (next < last) enter_round(++next_round);
+        }
+    };
+
+    // Row reads (A of S and dP): row 16h + li, dims 32s + 8lg .. + 7: quad li / 4,
+    // block 2s + lg / 2. Transposing reads as in the forward pass.
+    uint32_t row_abs[2], tr_abs[2];
+    {
+        const int quad = li >> 2, par = quad & 1, base = quad * kQuad + (li & 3) * 32 + (lg & 1) * 16;
+        // block m = 2s + lg / 2 at position m ^ par
+        row_abs[0] = lds0 + base + (((lg >> 1) ^ par)) * 128;
+        row_abs[1] = row_abs[0] + 2 * kBytes;
+        const int tpar = lg & 1, tbase = lg * kQuad + 32 * (li >> 2) + 8 * (li & 3);
+        tr_abs[0] = lds0 + tbase + tpar * 128;
+        tr_abs[1] = lds0 + tbase - tpar * 128;
+    }
+
+    f32x4 acc1[kBlocks][2], acc2[kKeys ? kBlocks : 1][2];
+#pragma unroll
+    for (int m = 0; m < kBlocks; ++m)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            acc1[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (kKeys) acc2[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+
+    int tile_now = next_tile;
+    transfer();
+    for (int t = first; t < last; ++t) {
+        landed_and_barrier<0>();
+        transfer();
+        const int row0 = range.key(tile_now), stage = (t & 1) * kBytes;
+        if (++tile_now == range.tiles) tile_now = 0;
+        if (!active) continue;
+        const bool masked = !((row0 >= full_from && row0 + kTileRows <= full_to) || row0 + kTileRows <= full_sink);
+
+        f32x4 sc[4], dp[4];  // [2h + j]: streamed rows 16h + 4lg + r, owned row 16j + li
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+        f32x4 row_lse[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            if constexpr (kKeys) {
+                const uint32_t at = lds0 + kStat + ((t & 1) * 4 + wave) * 256 + (16 * half + 4 * lg) * 4;
+                row_lse[half] = __builtin_bit_cast(f32x4, lds_read16(at));
+                dp[2 * half] = dp[2 * half + 1] = __builtin_bit_cast(f32x4, lds_read16(at + 128));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) dp[2 * half + j] = f32x4{neg_delta[j], neg_delta[j], neg_delta[j], neg_delta[j]};
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const u32x4 a1 = lds_read16(row_abs[0] + stage + half * 4 * kQuad + s * 256);
+                const u32x4 a2 = lds_read16(row_abs[1] + stage + half * 4 * kQuad + s * 256);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    sc[2 * half + j] = T::mfma16(a1, x1[j][s], sc[2 * half + j]);
+                    dp[2 * half + j] = T::mfma16(a2, x2[j][s], dp[2 * half + j]);
+                }
+            }
+        u32x4 pw[2], dw[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                    float p[2], ds[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float z = __builtin_fmaf(sc[2 * half + j][r + i], c.scale_log2, kKeys ? -row_lse[half][r + i] : -lse[j]);
+                        p[i] = fast_exp2(z);
+                        ds[i] = p[i] * dp[2 * half + j][r + i];
+                        if (masked) {
+                            const int row = row0 + 16 * half + 4 * lg + r + i;
+                            const bool sees = (row >= from[j] && row < to[j]) || (!kKeys && row < sink[j]);
+                            p[i] = sees ? p[i] : 0.f;
+                            ds[i] = sees ? ds[i] : 0.f;
+                        }
+                    }
+                    pw[j][2 * half + r / 2] = T::pack(p[0], p[1]);
+                    dw[j][2 * half + r / 2] = T::pack(ds[0], ds[1]);
+                }
+#pragma unroll
+        for (int m = 0; m < kBlocks; ++m) {
+            const uint32_t at = tr_abs[m & 1] + stage + m * 128;
+            const u32x4 a1 = __builtin_bit_cast(u32x4, __builtin_shufflevector(lds_read_transposed(at), lds_read_transposed(at + 4 * kQuad), 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc1[m][j] = T::mfma16(a1, dw[j], acc1[m][j]);
+            if constexpr (kKeys) {
+                const u32x4 a2 = __builtin_bit_cast(u32x4, __builtin_shufflevector(lds_read_transposed(at + 2 * kBytes), lds_read_transposed(at + 2 * kBytes + 4 * kQuad), 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc2[m][j] = T::mfma16(a2, pw[j], acc2[m][j]);
+            }
+        }
+    }
+
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int p = own[j];
+        if constexpr (kKeys) {
+            if (parts > 1) {
+                float* dst = c.partial + ((int64_t(head) * c.sink_tiles + tile) * parts + part) * (2 * kWindowRows * D) +
+                             (p - own0) * D + 4 * lg;
+#pragma unroll
+                for (int m = 0; m < kBlocks; ++m) {
+                    *reinterpret_cast<f32x4*>(dst + 16 * m) = acc1[m][j];
+                    *reinterpret_cast<f32x4*>(dst + kWindowRows * D + 16 * m) = acc2[m][j];
+                }
+                continue;
+            }
+        }
+        if (p >= c.tokens) continue;
+        const float live = p < length ? 1.f : 0.f;
+        const Rows& r1 = kKeys ? c.dk_rows : c.dq_rows;
+        uint16_t* d1 = static_cast<uint16_t*>(kKeys ? c.dk : c.dq) + b * r1.batch + h * r1.head + p * r1.token + 4 * lg;
+        const float scale = c.scale;
+#pragma unroll
+        for (int m = 0; m < kBlocks; ++m) {
+            f32x4 g = acc1[m][j] * scale;
+            if (live == 0.f) g = f32x4{0.f, 0.f, 0.f, 0.f};
+            *reinterpret_cast<u32x2*>(d1 + 16 * m) = u32x2{T::pack(g[0], g[1]), T::pack(g[2], g[3])};
+        }
+        if constexpr (kKeys) {
+            uint16_t* d2 = static_cast<uint16_t*>(c.dv) + b * c.dv_rows.batch + h * c.dv_rows.head + p * c.dv_rows.token + 4 * lg;
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m) {
+                f32x4 g = acc2[m][j];
+                if (live == 0.f) g = f32x4{0.f, 0.f, 0.f, 0.f};
+                *reinterpret_cast<u32x2*>(d2 + 16 * m) = u32x2{T::pack(g[0], g[1]), T::pack(g[2], g[3])};
+            }
+        }
+    }
+}
+
+// The parts of the sinks' tiles added up, in order: eight values of a row per thread.
+template <class T, int D>
+__global__ __launch_bounds__(256) void window_sinks_kernel(WindowGradCall c) {
+    constexpr int kLanes = D / 8, kTileValues = kWindowRows * D;
+    const int at = blockIdx.x * 256 + threadIdx.x;  // of a tile's rows times lanes, dK's then dV's
+    const int which = at / (kWindowRows * kLanes), row = at / kLanes % kWindowRows, lane = at % kLanes;
+    const int tile = blockIdx.y, head = blockIdx.z, b = head / c.kv_heads, h = head - b * c.kv_heads;
+    const int p = tile * kWindowRows + row;
+    if (which > 1 || p >= c.tokens) return;
+    float sum[8] = {};
+    if (p < length_of(c, b)) {
+        const float* src = c.partial + ((int64_t(head) * c.sink_tiles + tile) * c.sink_parts) * (2 * kTileValues) +
+                           which * kTileValues + row * D + lane * 8;
+        for (int i = 0; i < c.sink_parts; ++i, src += 2 * kTileValues) {
+            const f32x4 x = reinterpret_cast<const f32x4*>(src)[0], y = reinterpret_cast<const f32x4*>(src)[1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                sum[e] += x[e];
+                sum[4 + e] += y[e];
+            }
+        }
+    }
+    const float scale = which ? 1.f : c.scale;
+    const Rows& r = which ? c.dv_rows : c.dk_rows;
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = T::pack(sum[2 * i] * scale, sum[2 * i + 1] * scale);
+    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(which ? c.dv : c.dk) + b * r.batch + h * r.head + p * r.token + lane * 8) = w;
+}
+
+template <class T, int D>
+int launch_as(const WindowGradCall& c, hipStream_t stream) {
+    const int blocks = (c.tokens + 31) / 32, tiles = (c.tokens + kWindowRows - 1) / kWindowRows;
+    const unsigned bh = static_cast<unsigned>(c.batch * c.heads), kv = static_cast<unsigned>(c.batch * c.kv_heads);
+    const unsigned y = std::min(bh, 32768u);
+    hipLaunchKernelGGL((window_delta_kernel<T, D>), dim3(blocks, y, (bh + y - 1) / y), dim3(256), 0, stream, c, blocks);
+    if (int rc = check_launch("window_delta_kernel")) return rc;
+    const unsigned items = static_cast<unsigned>(tiles - c.sink_tiles + c.sink_tiles * c.sink_parts);
+    hipLaunchKernelGGL((window_grad_kernel<T, D, true>), dim3(items * kv), dim3(kWindowThreads), 0, stream, c, tiles);
+    if (int rc = check_launch("window_grad_kernel")) return rc;
+    if (c.sink_tiles) {
+        // In launches of at most 65,535 heads.
+        hipLaunchKernelGGL((window_sinks_kernel<T, D>), dim3(2 * kWindowRows * (D / 8) / 256, c.sink_tiles, kv), dim3(256), 0,
+                           stream, c);
+        if (int rc = check_launch("window_sinks_kernel")) return rc;
+    }
+    hipLaunchKernelGGL((window_grad_kernel<T, D, false>), dim3(window_grid(int64_t(bh), tiles)), dim3(kWindowThreads), 0, stream, c,
+                       tiles);
+    return check_launch("window_grad_kernel");
+}
+}  // namespace
+
+// Tiles with sinks are split into parts of about as many queries as a tile
+// behind them has (its window), at most 64 of them.
+void plan_window_grad(WindowGradCall& c, int64_t& stat, int64_t& partial) {
+    const int64_t blocks = (int64_t(c.tokens) + 31) / 32, tiles = (int64_t(c.tokens) + kWindowRows - 1) / kWindowRows;
+    stat = int64_t(c.batch) * c.heads * blocks * 64;
+    partial = 0;
+    c.sink_tiles = c.sink_parts = 0;
+    const int64_t window = int64_t(c.mask.back) + c.mask.frame.d + kWindowRows;
+    const int64_t sinks = std::min<int64_t>((int64_t(c.mask.sinks) + kWindowRows - 1) / kWindowRows, tiles);
+    const int64_t parts = std::min<int64_t>((c.tokens + window - 1) / window, 64);
+    if (sinks > 0 && parts > 1 && sinks <= 65535 && int64_t(c.batch) * c.kv_heads <= 65535) {
+        c.sink_tiles = static_cast<int32_t>(sinks);
+        c.sink_parts = static_cast<int32_t>(parts);
+        partial = int64_t(c.batch) * c.kv_heads * sinks * parts * 2 * kWindowRows * c.dim;
+    }
+}
+
+int launch_window_grad(const WindowGradCall& c, hipStream_t stream) {
+    if (c.dim == 128) return c.half ? launch_as<F16, 128>(c, stream) : launch_as<Bf16, 128>(c, stream);
+    return c.half ? launch_as<F16, 64>(c, stream) : launch_as<Bf16, 64>(c, stream);
+}
+
+}  // namespace ab

@@ -305,6 +305,25 @@ size_t ab_window_workspace_bytes(const ab_window_args *args);
 int ab_window_attention(const ab_window_args *args, void *stream);
 int ab_chunk_attention(const ab_window_args *args, void *stream);
 
+/* The gradient of ab_window_attention. forward: that call's arguments with its out
+ * and lse (not NULL); its workspace fields are this call's, of
+ * ab_window_grad_workspace_bytes(args) bytes, 16-byte aligned, never 0 where there
+ * are tokens. dout is out's gradient, dlse (or NULL) lse's. Writes all of dq, dk and dv, of
+ * q's, k's and v's shapes and type (0 for the tokens behind a length); gradients of
+ * shared key heads are summed over their query heads in float32. The same inputs
+ * give the same bits. A value that is not finite may spread to any gradient of
+ * its batch item. Alignment as for q; out too must be 16-byte aligned, its
+ * strides multiples of 8. */
+typedef struct ab_window_grad_args {
+    ab_window_args forward;
+    const void *dout;
+    const float *dlse;
+    void *dq, *dk, *dv;
+    int64_t dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+} ab_window_grad_args;
+size_t ab_window_grad_workspace_bytes(const ab_window_grad_args *args);
+int ab_window_attention_grad(const ab_window_grad_args *args, void *stream);
+
 /* New keys and values k, v [tokens, kv_heads, dim] (16-bit elements) of `batch`
  * sequences into a paged cache (offsets, lengths, page_table and the cache as in
  * ab_chunk_attention; lengths count the new tokens). Rows whose entry is no page

@@ -73,3 +73,42 @@ def turned(x, positions, axes, theta=10000.0, halves=False, joint=False, inverse
             x[..., b] = xa * angle.sin() + xb * angle.cos()
         base += dims // 2
     return x
+
+
+def attend_grad(q, k, v, do, mask, dlse=None, scale=None):
+    """(dq, dk, dv) of ``attend`` in 64 bits, and how far a kernel may be that rounds P, dS, the output (which delta is
+    made of) and each gradient once, by at most half a step, relative to u."""
+    group = q.shape[0] // k.shape[0]
+    heads, n, dim = k.shape
+    scale = dim ** -0.5 if scale is None else scale
+    q, do = q.double(), do.double()
+    k, v = k.double().repeat_interleave(group, 0), v.double().repeat_interleave(group, 0)
+    z = (q @ k.transpose(1, 2) * scale).masked_fill(~mask, -math.inf)
+    lse = torch.logsumexp(z, -1, keepdim=True)
+    p = torch.where(lse > -math.inf, torch.exp(z - lse), 0.0)
+    o = p @ v
+    dp = do @ v.transpose(1, 2)
+    delta = (do * o).sum(-1, keepdim=True)
+    if dlse is not None:
+        delta = delta - dlse.double()[..., None] / math.log(2)
+    ds = p * (dp - delta)
+    off = p * (do.abs() * (p @ v.abs() + o.abs())).sum(-1, keepdim=True)  # of dS, from P's and the output's rounding
+    # float32 sums of dim products in dP, and P's own error of some 2^-17 from the logits', next to u of 2^-11 at least
+    noise = p * (do.abs() @ v.abs().transpose(1, 2)) + off + p * delta.abs()
+    size = ds.abs() + off + 2.0 ** -6 * noise
+
+    def shared(x):
+        return x.reshape(heads, group, n, dim).sum(1)
+
+    dq = scale * ds @ k
+    dk, dv = shared(scale * ds.transpose(1, 2) @ q), shared(p.transpose(1, 2) @ do)
+    rooms = (abs(scale) * size @ k.abs() + dq.abs(), shared(abs(scale) * size.transpose(1, 2) @ q.abs()) + dk.abs(),
+             shared(1.01 * p.transpose(1, 2) @ do.abs()) + dv.abs())
+    return (dq, dk, dv), rooms
+
+
+def check_gradient(got, want, room, dtype, name=""):
+    """u times the room, with 2 % for products of roundings, and the float32 arithmetic's 2^-17 of it."""
+    u = HALF_STEP[dtype]
+    worst = ((got.double() - want).abs() - (1.02 * u + 2.0 ** -17) * room - 1e-7).max().item() if want.numel() else 0.0
+    assert worst <= 0, (name, worst)

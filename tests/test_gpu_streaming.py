@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from ab_attention.streaming import PagedCache, append_cache, chunk_attention, rotary, window_attention
-from streaming_reference import (HALF_STEP, attend, check_lse, check_output, logit_size, seen_mask, turned)
+from streaming_reference import (HALF_STEP, attend, attend_grad, check_gradient, check_lse, check_output, logit_size,
+                                 seen_mask, turned)
 
 pytestmark = pytest.mark.gpu
 
@@ -211,6 +212,119 @@ def test_window_of_no_tokens():
     assert out.shape == empty.shape and lse.shape == (2, 3, 0)
     none = torch.empty((0, 3, 5, 64), dtype=BF16, device="cuda")
     assert window_attention(none, none, none).shape == none.shape
+
+
+def _grad_case(batch, heads, kv_heads, tokens, dim, dtype, window, sinks, frame, lengths=None, token_major=False, seed=0,
+               with_lse=False, scale=None, junk=None):
+    q = _rand((batch, heads, tokens, dim), dtype, seed + 1, 1.5, token_major)
+    k = _rand((batch, kv_heads, tokens, dim), dtype, seed + 2, 1.0, token_major)
+    v = _rand((batch, kv_heads, tokens, dim), dtype, seed + 3, 1.0, not token_major)
+    do = _rand((batch, heads, tokens, dim), dtype, seed + 4, 1.0, token_major)
+    dlse = _rand((batch, heads, tokens), F32, seed + 5) if with_lse else None
+    n_of = [tokens if lengths is None else max(0, min(n, tokens)) for n in (lengths or [0] * batch)]
+    if junk is not None:
+        for b, n in enumerate(n_of):
+            for t in (q, k, v, do):
+                t[b, :, n:] = junk
+    for t in (q, k, v):
+        t.requires_grad_()
+    dev_lengths = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    out, lse = window_attention(q, k, v, window=window, sinks=sinks, frame=frame, lengths=dev_lengths, scale=scale,
+                                return_lse=True)
+    if with_lse:
+        grads = torch.autograd.grad((out, lse), (q, k, v), (do, dlse), retain_graph=True)
+        again = torch.autograd.grad((out, lse), (q, k, v), (do, dlse))
+    else:
+        grads = torch.autograd.grad(out, (q, k, v), do, retain_graph=True)
+        again = torch.autograd.grad(out, (q, k, v), do)
+    at = torch.arange(tokens, device="cuda")
+    for b, n in enumerate(n_of):
+        want, room = attend_grad(q[b, :, :n], k[b, :, :n], v[b, :, :n], do[b, :, :n],
+                                 seen_mask(at[:n], at[:n], window, sinks, frame), None if dlse is None else dlse[b, :, :n], scale)
+        for name, got, w, r in zip("qkv", grads, want, room):
+            check_gradient(got[b, :, :n], w, r, dtype, name)
+            assert (got[b, :, n:] == 0).all(), name
+    for t, g, a in zip((q, k, v), grads, again):
+        assert g.shape == t.shape and g.dtype == t.dtype and g.stride() == t.stride()
+        assert torch.equal(g, a)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("tokens", [1, 2, 31, 33, 64, 127, 129, 300])
+def test_window_gradient_lengths(tokens, dim, dtype):
+    _grad_case(1, 2, 1, tokens, dim, dtype, 40, 3, 1, seed=tokens)
+
+
+@pytest.mark.parametrize("window,sinks,frame", [(None, 0, 1), (1, 0, 1), (2, 5, 1), (33, 0, 1), (64, 40, 1), (20, 300, 1),
+                                                (10000, 3, 1), (None, 0, 7), (1, 0, 100), (2, 1, 31), (3, 2, 37), (1, 3, 130),
+                                                (2, 1, 260), (1, 0, 5000), (2 ** 40, 2 ** 40, 1), (1, 1, 129)])
+def test_window_gradient_masks(window, sinks, frame):
+    _grad_case(2, 3, 3, 517, 128, BF16, window, sinks, frame)
+
+
+@pytest.mark.parametrize("heads,kv_heads,token_major", [(8, 2, False), (6, 1, True), (4, 4, True)])
+def test_window_gradient_heads_and_strides(heads, kv_heads, token_major):
+    _grad_case(2, heads, kv_heads, 333, 128, BF16, 60, 4, 1, token_major=token_major, with_lse=True)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_window_gradient_padded_batch(dim):
+    for junk in (math.nan, math.inf):
+        _grad_case(5, 4, 2, 200, dim, BF16, 50, 2, 1, lengths=[200, 0, 1, 77, 129], junk=junk)
+        _grad_case(2, 2, 1, 400, dim, F16, 2, 1, 48, lengths=[31, 350], junk=junk, with_lse=True)
+
+
+def test_window_gradient_many_tiles_and_scale():
+    _grad_case(1, 3, 1, 8500, 64, BF16, 300, 5, 1)
+    _grad_case(1, 2, 2, 200, 128, BF16, 50, 0, 1, scale=-0.06)
+
+
+def test_window_gradient_parts_of_the_graph():
+    """Only some of q, k, v, only the normaliser, an expanded gradient, a value shared by q and k."""
+    q, k, v = (_rand((1, 2, 90, 64), BF16, s) for s in (1, 2, 3))
+    how = dict(window=30, sinks=1, return_lse=True)
+    ones = torch.ones((), dtype=BF16, device="cuda").expand(1, 2, 90, 64)
+    full = [t.clone().requires_grad_() for t in (q, k, v)]
+    want = torch.autograd.grad(window_attention(*full, **how)[0], full, ones.contiguous())
+    got = torch.autograd.grad(window_attention(*full, **how)[0], full, ones)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    one = k.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(window_attention(q, one, v, **how)[0], one, ones)[0], want[1])
+    lse = window_attention(*full, **how)[1]
+    dq, dk = torch.autograd.grad(lse.sum(), full[:2])
+    at = torch.arange(90, device="cuda")
+    (wq, wk, _), (rq, rk, _) = attend_grad(q[0], k[0], v[0], torch.zeros_like(q[0]), seen_mask(at, at, 30, 1, 1),
+                                           torch.ones_like(lse[0]))
+    check_gradient(dq[0], wq, rq, BF16)
+    check_gradient(dk[0], wk, rk, BF16)
+    same = q.clone().requires_grad_()
+    both = torch.autograd.grad(window_attention(same, same, v, **how)[0], same, ones)[0]
+    pair = [q.clone().requires_grad_() for _ in range(2)]
+    dq, dk = torch.autograd.grad(window_attention(*pair, v, **how)[0], pair, ones)
+    assert torch.equal(both, dq + dk)
+
+
+def test_window_gradient_against_differences():
+    """A directional derivative of a weighted sum of the output and the normaliser in 64 bits, by central differences of
+    the definition, against the kernels' gradients."""
+    shape, n = (1, 2, 140, 64), 140
+    q, k, v, do = (_rand(shape, F16, s).requires_grad_(s < 4) for s in (1, 2, 3, 4))
+    how = dict(window=50, sinks=3)
+    at = torch.arange(n, device="cuda")
+    mask = seen_mask(at, at, 50, 3, 1)
+    grads = torch.autograd.grad(window_attention(q, k, v, **how), (q, k, v), do)
+
+    def loss(*t):
+        return (attend(*(x.double()[0] for x in t), mask)[0] * do[0].double()).sum().item()
+
+    for i, name in enumerate("qkv"):
+        step = _rand(shape, F32, 10 + i).double()
+        sides = [[t.detach().double() + (e * step if j == i else 0) for j, t in enumerate((q, k, v))] for e in (1e-5, -1e-5)]
+        slope = (loss(*sides[0]) - loss(*sides[1])) / 2e-5
+        got = (grads[i].double() * step).sum().item()
+        # Each value of the gradient carries a few roundings of 2^-11 with signs of their own: five of their standard deviations.
+        assert abs(got - slope) <= 5 * 4 * 2.0 ** -11 * (grads[i].double() * step).norm().item() + 1e-4 * abs(slope), (name, got, slope)
 
 
 # ---- paged cache and chunks ---------------------------------------------------

@@ -154,3 +154,36 @@ def test_workspace_of_a_split_call():
     row = 2 * (64 * 4 + 8)
     assert size > 0 and size % row == 0 and size // row <= 2048 * 16 // 32
     assert lib.ab_window_workspace_bytes(_window_args(tokens=100000, q_stride=(0, 0, 64), heads=64)) == 0
+
+
+def _grad_args(**change):
+    g = _lib.WindowGradArgs(dout=_A, dq=_A, dk=_A, dv=_A)
+    g.forward = _window_args(lse=_A, workspace=_A, workspace_bytes=1 << 20)
+    for name in ("dout_stride", "dq_stride", "dk_stride", "dv_stride"):
+        setattr(g, name, (ctypes.c_int64 * 3)(1024, 512, 64))
+    for name, value in change.items():
+        target = g.forward if hasattr(g.forward, name) else g
+        setattr(target, name, (ctypes.c_int64 * 3)(*value) if name.endswith("stride") else value)
+    return g
+
+
+@pytest.mark.parametrize("change,msg", [
+    (dict(dout=0), b"null"), (dict(dk=0), b"null"), (dict(lse=0), b"null"), (dict(workspace=0), b"null"),
+    (dict(dq=_A + 8), b"aligned"), (dict(out=_A + 8), b"aligned"), (dict(workspace_bytes=64), b"smaller"),
+    (dict(dv_stride=(1024, 512, 4)), b"strides"), (dict(out_stride=(1024, 512, 68)), b"strides"), (dict(dim=32), b"64 or 128"),
+])
+def test_gradient_entry_refuses(change, msg):
+    lib = _lib.load()
+    assert lib.ab_window_attention_grad(_grad_args(**change), None) == 1
+    assert msg in lib.ab_last_error() and lib.ab_last_error().startswith(b"window_attention_grad:")
+
+
+def test_gradient_workspace():
+    """Normalisers and deltas of every 32 queries; float32 parts only where sinks are seen from far behind a window."""
+    lib = _lib.load()
+    assert lib.ab_window_grad_workspace_bytes(_grad_args(tokens=0)) == 0
+    strides = dict(q_stride=(1 << 22, 1 << 20, 64), k_stride=(1 << 22, 1 << 20, 64), v_stride=(1 << 22, 1 << 20, 64))
+    plain = lib.ab_window_grad_workspace_bytes(_grad_args(tokens=1024, window=100, **strides))
+    assert plain == 2 * 32 * 64 * 4
+    sinks = lib.ab_window_grad_workspace_bytes(_grad_args(tokens=1024, window=100, sinks=4, **strides))
+    assert (sinks - plain) % (2 * 128 * 64 * 4) == 0 and sinks > plain
