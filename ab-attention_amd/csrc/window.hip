@@ -17,6 +17,9 @@
 namespace ab {
 namespace {
 
+constexpr int kRing = 4;         // stages of K and of V in LDS
+constexpr float kSlack = 8.0f;  // largest logit (base 2) above a row's reference: P stays within 2^8
+
 // What a workgroup works on. The same in all its lanes.
 struct WindowUnit {
     int b, kv_head, head;  // head: the query head, or the first one of the group
@@ -74,13 +77,27 @@ struct WindowTile {
     static constexpr int kBytes = kWindowKeys * D * 2;     // K (or V) of one tile
     static constexpr int kOps = D / 64;                    // transfers of a wave for K (or V) of a tile
     static constexpr int kOpKeys = 1024 / (2 * D);         // keys of a transfer
+    static constexpr int kVRing = kRing * kBytes;
+    static constexpr int kVotes = 2 * kRing * kBytes;
+    static constexpr int kLdsBytes = kVotes + 16;
 };
+
+// The maxima of a and b over the four lanes l, 16 + l, 32 + l, 48 + l.
+__device__ __forceinline__ void max_over_rows(float& a, float& b) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    const float m = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+    const float m2 = fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+    const auto u = __builtin_amdgcn_permlane16_swap(__float_as_uint(m2), __float_as_uint(m2), false, false);
+    a = __uint_as_float(u[0]);
+    b = __uint_as_float(u[1]);
+}
 
 template <class T, int D, bool kPaged, bool kSplit>
 __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c, int tiles_per_head) {
     using Tile = WindowTile<T, D>;
-    constexpr int kSteps = Tile::kSteps, kBlocks = Tile::kBlocks;
-    __shared__ __align__(16) unsigned char smem[4 * Tile::kBytes];  // two stages of K, two of V
+    constexpr int kSteps = Tile::kSteps, kBlocks = Tile::kBlocks, kOps = Tile::kOps;
+    extern __shared__ __align__(16) unsigned char smem[];
 
     WindowUnit u;
     if (!window_unit<kPaged>(c, blockIdx.x, tiles_per_head, u)) return;
@@ -104,38 +121,40 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
         tile0 = static_cast<int>(int64_t(tiles) * part / c.parts);
         tiles = static_cast<int>(int64_t(tiles) * (part + 1) / c.parts) - tile0;
     }
+    // Row 16j + li of this wave's 32: its token and query head.
+    auto row_of = [&](int j, int& token, int& head) {
+        const int r = wave * 32 + 16 * j + li, packed = row0 + min(r, rows - 1);
+        token = kPaged ? packed / group : packed;
+        head = u.head + (kPaged ? packed - token * group : 0);
+        return r < rows;
+    };
 
-    // Q as the B operand of S^T = K Q^T: row 16j + li of the wave's 32, dims
-    // 32s + 8lg .. + 7. The row's own bounds; all zero for a row without keys.
+    // Q as the B operand of S^T = K Q^T: row 16j + li, dims 32s + 8lg .. + 7. The
+    // row's own bounds; all zero for a row without keys.
     u32x4 bq[2][kSteps];
     int low[2], seen[2], sink[2];  // keys low .. low + seen - 1 and 0 .. sink - 1
-    int64_t out_at[2], stat_at[2];
-    bool stored[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        const int r = wave * 32 + 16 * j + li;
-        stored[j] = r < rows;
-        const int packed = row0 + min(r, rows - 1);
-        const int token = kPaged ? packed / group : packed, head = u.head + (kPaged ? packed - token * group : 0);
+        int token, head;
+        const bool stored = row_of(j, token, head);
         const uint16_t* qrow = static_cast<const uint16_t*>(c.q) + u.b * c.q_rows.batch + head * c.q_rows.head +
                                int64_t(u.off + token) * c.q_rows.token + 8 * lg;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) bq[j][s] = *reinterpret_cast<const u32x4*>(qrow + 32 * s);
         const int p = u.first + token;
-        const bool sees = stored[j] && p >= 0 && p < u.length;
+        const bool sees = stored && p >= 0 && p < u.length;
         const int high = mask.high(max(p, 0), u.length);
         low[j] = mask.low(max(p, 0));
         seen[j] = sees ? high - low[j] : 0;
         sink[j] = sees ? min(mask.sinks, high) : 0;
-        out_at[j] = u.b * c.out_rows.batch + head * c.out_rows.head + int64_t(u.off + token) * c.out_rows.token;
-        stat_at[j] = u.b * c.row.batch + head * c.row.head + int64_t(u.off + token) * c.row.token;
     }
     // Tiles that every row of this wave sees need no mask: keys from full_low to
     // full_high, and those before full_sink. A wave with a row that exists but
     // sees nothing masks every tile.
     int full_low = 0, full_high = 0, full_sink = 0;
     const int wave_rows = min(32, rows - wave * 32);
-    if (wave_rows > 0) {
+    const bool active = wave_rows > 0;
+    if (active) {
         const int pf = u.first + token_at(wave * 32), pl = u.first + token_at(wave * 32 + wave_rows - 1);
         if (pf >= 0 && pl < u.length) {
             full_low = mask.low(pl);
@@ -150,73 +169,23 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     const uint32_t k_token = static_cast<uint32_t>(c.k_rows.token * 2), v_token = static_cast<uint32_t>(c.v_rows.token * 2);
     const int32_t* table = kPaged ? c.table + int64_t(u.b) * c.table_width : nullptr;
 
-    // The page of a key (a multiple of 8): where it starts and how many of its
-    // tokens exist; nothing for an entry that names no page.
-    auto page_of = [&](int key, int64_t& page, uint32_t& in_page, uint32_t& there) {
-        uint32_t rest;
-        const uint32_t index = c.page.quotient(static_cast<uint32_t>(key), rest);
-        page = 0;
-        in_page = rest;
-        there = 0;
-        if (key < end) {
-            const int entry = __builtin_amdgcn_readfirstlane(table[index]);
-            if (static_cast<uint32_t>(entry) < static_cast<uint32_t>(c.pages)) {
-                page = entry;
-                there = min(static_cast<int>(c.page.d), end - (key - static_cast<int>(rest)));
-            }
-        }
-    };
-
-    // Transfers of this wave: keys 8w .. 8w + 7 of the tile, kOpKeys at a time.
-    // K keeps rows of D elements whose 16-byte chunks are swizzled (position =
-    // chunk ^ key); V keeps, for every four keys, blocks of 4 keys x 16 dims,
-    // block m at position m ^ (quad & 1): both the row reads of K and the
-    // transposing reads of V then spread over the banks.
-    uint32_t k_src[Tile::kOps], v_src[Tile::kOps];
-#pragma unroll
-    for (int e = 0; e < Tile::kOps; ++e) {
-        constexpr int kChunks = D / 8;
-        const int key = lane / kChunks, pos = lane % kChunks, in_tile = 8 * wave + Tile::kOpKeys * e + key;
-        k_src[e] = uint32_t(key) * k_token + uint32_t(pos ^ (in_tile % kChunks)) * 16u;
-        const int quad = D == 128 ? e : lane >> 5, block = (lane >> 3) % kBlocks, r = (lane >> 1) & 3, h = lane & 1;
-        v_src[e] = uint32_t((D == 128 ? 0 : 4 * quad) + r) * v_token + uint32_t(2 * (block ^ (quad & 1)) + h) * 16u;
-    }
-    auto transfer = [&](int t) {
-        if (t >= tiles) return;
-        const int key = range.key(tile0 + t) + 8 * wave;
-        const uint32_t stage = (t & 1) * Tile::kBytes + wave * (8 * D * 2);
-        u32x4 kbuf, vbuf;
-        uint32_t at;
-        if constexpr (kPaged) {
-            int64_t page;
-            uint32_t there;
-            page_of(key, page, at, there);
-            kbuf = buffer_of(kbase + page * c.k_rows.batch * 2, there ? (there - 1) * k_token + 2 * D : 0);
-            vbuf = buffer_of(vbase + page * c.v_rows.batch * 2, there ? (there - 1) * v_token + 2 * D : 0);
-        } else {
-            at = key;
-            kbuf = buffer_of(kbase, uint32_t(end - 1) * k_token + 2 * D);
-            vbuf = buffer_of(vbase, uint32_t(end - 1) * v_token + 2 * D);
-        }
-#pragma unroll
-        for (int e = 0; e < Tile::kOps; ++e) {
-            buffer_to_lds(kbuf, k_src[e] + (at + Tile::kOpKeys * e) * k_token, lds0 + stage + 1024 * e);
-            buffer_to_lds(vbuf, v_src[e] + (at + Tile::kOpKeys * e) * v_token, lds0 + 2 * Tile::kBytes + stage + 1024 * e);
-        }
-    };
-
     // Whether a key that some row would see lies on no page (then every tile
     // asks the table for its keys).
     bool holes = false;
     if constexpr (kPaged) {
+        bool bad = false;
         if (tiles > 0) {
             const int first_page = range.key(tile0) / static_cast<int>(c.page.d);
             const int last_page = (min(range.key(tile0 + tiles - 1) + kWindowKeys, end) - 1) / static_cast<int>(c.page.d);
-            bool bad = false;
             for (int i = first_page + tid; i <= last_page; i += kWindowThreads)
                 bad |= static_cast<uint32_t>(table[i]) >= static_cast<uint32_t>(c.pages);
-            holes = __syncthreads_or(bad);
         }
+        uint32_t* votes = reinterpret_cast<uint32_t*>(smem + Tile::kVotes);
+        const uint32_t vote = __any(bad) ? 1u : 0u;
+        if (lane == 0) votes[wave] = vote;
+        landed_and_barrier<0>();
+        const u32x4 all = *reinterpret_cast<const u32x4*>(votes);
+        holes = __builtin_amdgcn_readfirstlane(all[0] | all[1] | all[2] | all[3]) != 0;
     }
     auto on_page = [&](int key) {
         const uint32_t q0 = __umulhi(static_cast<uint32_t>(key), c.page.m);
@@ -224,166 +193,388 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
         return key < end && static_cast<uint32_t>(table[min(index, static_cast<uint32_t>(c.table_width - 1))]) < static_cast<uint32_t>(c.pages);
     };
 
+    // Transfers of this wave: keys 8w .. 8w + 7 of a tile, kOpKeys at a time.
+    // K keeps rows of D elements whose 16-byte chunks are swizzled (position =
+    // chunk ^ key); V keeps, for every four keys, blocks of 4 keys x 16 dims,
+    // block m at position m ^ (quad & 1): both the row reads of K and the
+    // transposing reads of V then spread over the banks.
+    uint32_t k_src[kOps], v_src[kOps];
+#pragma unroll
+    for (int e = 0; e < kOps; ++e) {
+        constexpr int kChunks = D / 8;
+        const int key = lane / kChunks, pos = lane % kChunks, in_tile = 8 * wave + Tile::kOpKeys * e + key;
+        k_src[e] = uint32_t(Tile::kOpKeys * e + key) * k_token + uint32_t(pos ^ (in_tile % kChunks)) * 16u;
+        const int quad = D == 128 ? e : lane >> 5, block = (lane >> 3) % kBlocks, r = (lane >> 1) & 3, h = lane & 1;
+        v_src[e] = uint32_t(4 * quad + r) * v_token + uint32_t(2 * (block ^ (quad & 1)) + h) * 16u;
+    }
+    // Where this wave's eight keys of a tile lie: the page, the first key's place in
+    // it, and how many of the page's (or tensor's) keys exist. Nothing for tiles
+    // past the last one (their transfers only keep the count of each step) and for
+    // keys that lie on no page.
+    struct Place {
+        int32_t page;
+        uint32_t at, there;
+    };
+    auto place_of = [&](int t) {
+        const int key = range.key(tile0 + t) + 8 * wave;
+        Place p{0, static_cast<uint32_t>(key), t < tiles ? static_cast<uint32_t>(end) : 0u};
+        if constexpr (kPaged) {
+            const uint32_t index = c.page.quotient(static_cast<uint32_t>(key), p.at);
+            if (t < tiles && key < end) {
+                const auto entries = (const __attribute__((address_space(4))) int32_t*)reinterpret_cast<uintptr_t>(table);
+                const int32_t entry = entries[index];
+                const bool is_page = static_cast<uint32_t>(entry) < static_cast<uint32_t>(c.pages);
+                p.page = is_page ? entry : 0;
+                p.there = is_page ? min(c.page.d, static_cast<uint32_t>(end - key) + p.at) : 0u;
+            } else {
+                p.there = 0;
+            }
+        }
+        return p;
+    };
+    auto move = [&](const char* base, const Rows& rows_of, uint32_t token, const uint32_t (&src)[kOps], const Place& p, uint32_t lds) {
+        const u32x4 buffer = buffer_of(base + (kPaged ? int64_t(p.page) * rows_of.batch * 2 : 0),
+                                       p.there ? (p.there - 1) * token + 2 * D : 0);
+        const uint32_t at = p.at * token;
+#pragma unroll
+        for (int e = 0; e < kOps; ++e) buffer_to_lds(buffer, src[e] + at, lds + wave * (8 * D * 2) + 1024 * e);
+    };
+    auto move_k = [&](int t, const Place& p) { move(kbase, c.k_rows, k_token, k_src, p, lds0 + (t & (kRing - 1)) * Tile::kBytes); };
+    auto move_v = [&](int t, const Place& p) {
+        move(vbase, c.v_rows, v_token, v_src, p, lds0 + Tile::kVRing + (t & (kRing - 1)) * Tile::kBytes);
+    };
+
+    // Reads of operands: K's row 16h + li, chunk 4s + lg; V's quad lg + 4h, block
+    // b, of which lane li gets dim 16b + li of the four keys.
     uint32_t k_abs[kSteps], v_abs[2];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) k_abs[s] = lds0 + li * (2 * D) + 16 * ((4 * s + lg) ^ (li % (D / 8)));
     {
-        const int par = lg & 1, base = 2 * Tile::kBytes + lg * Tile::kQuadBytes + 32 * (li >> 2) + 8 * (li & 3);
+        const int par = lg & 1, base = Tile::kVRing + lg * Tile::kQuadBytes + 32 * (li >> 2) + 8 * (li & 3);
         v_abs[0] = lds0 + base + par * 128;  // even block: position block + par
         v_abs[1] = lds0 + base - par * 128;  // odd block: position block - par
     }
+    auto read_k = [&](int t, int f) {  // f = kSteps h + s
+        return lds_read16(k_abs[f % kSteps] + (t & (kRing - 1)) * Tile::kBytes + (f / kSteps) * 16 * 2 * D);
+    };
+    auto read_v = [&](int t, int b, int h) {
+        return lds_read_transposed(v_abs[b & 1] + (t & (kRing - 1)) * Tile::kBytes + b * 128 + h * 4 * Tile::kQuadBytes);
+    };
+    auto is_masked = [&](int t) {
+        const int key = range.key(tile0 + t);
+        return holes || t >= tiles ||
+               !((key >= full_low && key + kWindowKeys <= full_high) || key + kWindowKeys <= full_sink);
+    };
+    // Bit r of the result: key 16h + 4lg + r of tile t is seen by row 16j + li.
+    auto seen_keys = [&](int t, int h, int j) {
+        const int key = range.key(tile0 + t) + 16 * h + 4 * lg;
+        uint32_t bits = 0;
+        if (t < tiles && (!kPaged || !holes || on_page(key)))
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                bits |= static_cast<uint32_t>(key + r - low[j]) < static_cast<uint32_t>(seen[j]) || key + r < sink[j] ? 1u << r : 0u;
+        return bits;
+    };
 
     f32x4 o_acc[kBlocks][2];  // dims 16b + 4lg .. + 3 of row 16j + li
+    float m_run[2], l_run[2];
+    bool started[2];
+    auto reset = [&]() {
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b)
+        for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) o_acc[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
-
-    transfer(0);
-    for (int t = 0; t < tiles; ++t) {
-        landed_and_barrier<0>();
-        transfer(t + 1);
-        if (wave_rows <= 0) continue;
-        const int key0 = range.key(tile0 + t), stage = (t & 1) * Tile::kBytes;
-        const bool masked = holes || !((key0 >= full_low && key0 + kWindowKeys <= full_high) || key0 + kWindowKeys <= full_sink);
-
-        // S^T: keys 16h + 4lg + r of row 16j + li in sc[2h + j][r].
-        f32x4 sc[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) sc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const u32x4 a = lds_read16(k_abs[s] + stage + h * 16 * 2 * D);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) sc[2 * h + j] = T::mfma16(a, bq[j][s], sc[2 * h + j]);
-            }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) sc[x] *= c.scale_log2;
-        float top[2] = {-INFINITY, -INFINITY};
-        uint32_t visible[2] = {0xffu, 0xffu};  // bit 4h + r
-        if (masked) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int key = key0 + 16 * h + 4 * lg;
-                const bool there = !kPaged || !holes || on_page(key);
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const bool sees = there && (static_cast<uint32_t>(key + r - low[j]) < static_cast<uint32_t>(seen[j]) ||
-                                                    key + r < sink[j]);
-                        if (!sees) {
-                            sc[2 * h + j][r] = -INFINITY;
-                            visible[j] &= ~(1u << (4 * h + r));
-                        }
-                    }
-            }
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) top[x & 1] = fmaxf(top[x & 1], sc[x][r]);
-        uint32_t pw[2][4];
+            for (int j = 0; j < 2; ++j) o_acc[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            top[j] = fmaxf(top[j], __shfl_xor(top[j], 16));
-            top[j] = fmaxf(top[j], __shfl_xor(top[j], 32));
-            const float m = fmaxf(m_run[j], top[j]);
-            const float reference = m == -INFINITY ? 0.f : m;
-            const float alpha = fast_exp2(m_run[j] - reference);
-            m_run[j] = m;
-            float sum = 0.f;
+            m_run[j] = 0.f;
+            l_run[j] = 0.f;
+            started[j] = false;
+        }
+    };
+    auto start_s = [&](const u32x4 (&ka)[2 * kSteps], f32x4 (&s)[4]) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 4 * kSteps; ++x) {
+            const int step = x >> 2, h = (x >> 1) & 1, j = x & 1;
+            s[2 * h + j] = T::mfma16(ka[kSteps * h + step], bq[j][step], s[2 * h + j]);
+        }
+    };
+    // Logits of tile t against the rows' references, from S; mx[j] their maximum
+    // over this lane's keys.
+    auto mask_logits = [&](int t, f32x4 (&s)[4], float (&mx)[2]) {
+        mx[0] = mx[1] = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t bits = seen_keys(t, h, j);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (!(bits >> r & 1)) s[2 * h + j][r] = -INFINITY;
+                    mx[j] = fmaxf(mx[j], s[2 * h + j][r]);
+                }
+            }
+    };
+    // Moves the reference of the rows whose maximum has risen by more than kSlack
+    // above it (or that have none yet): their sums, and the logits at hand, follow.
+    auto move_reference = [&](f32x4 (&s)[4], float (&mx)[2]) {
+        max_over_rows(mx[0], mx[1]);
+        const bool grow0 = mx[0] > (started[0] ? kSlack : -INFINITY), grow1 = mx[1] > (started[1] ? kSlack : -INFINITY);
+        if (!__any(grow0 || grow1)) return;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const bool grow = j ? grow1 : grow0;
+            const float shift = grow ? mx[j] : 0.f;
+            const float alpha = started[j] ? fast_exp2(-shift) : 1.f;  // the sums are 0 before
+            started[j] |= grow;
+            m_run[j] += shift;
+            l_run[j] *= alpha;
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) o_acc[b][j] *= alpha;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int r = 0; r < 4; r += 2) {
-                    const float p0 = fast_exp2(sc[2 * h + j][r] - reference), p1 = fast_exp2(sc[2 * h + j][r + 1] - reference);
-                    sum += p0 + p1;
-                    pw[j][2 * h + r / 2] = T::pack(p0, p1);
-                }
-            l_run[j] = l_run[j] * alpha + sum;
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o_acc[b][j][r] *= alpha;
+                for (int r = 0; r < 4; ++r) s[2 * h + j][r] -= shift;
         }
-        // O^T += V^T P^T: the MFMA's k index 8lg + 4h + r is key 16h + 4lg + r
-        // on both operands, so P stays where the first product left it.
+    };
+
+    // The pass that calls take. Step t: phase A computes S(t + 1) beside p = 2^y of
+    // tile t, the reads of V(t) and the transfers of K(t + 5) and V(t + 3); phase B
+    // adds V(t)^T P(t)^T beside the logits of tile t + 1 and the reads of K(t + 2).
+    // Returns whether a tile that some rows see in part held a value that is not
+    // finite: 0 times it is no zero, so the tile cannot be computed like that.
+    auto fast_pass = [&]() -> bool {
+        uint32_t odd = 0;
+        auto step = [&](int t, f32x4 (&sc)[4], f32x4 (&sn)[4], float (&mx)[2], u32x4 (&ka)[2 * kSteps], Place& kp, Place& vp) {
+            landed_and_barrier<4 * kOps>();
+            if (!active) {
+                move_k(t + 5, kp);
+                move_v(t + 3, vp);
+                kp = place_of(t + 6);
+                vp = place_of(t + 4);
+                return;
+            }
+            move_reference(sc, mx);
+            constexpr int kEach = 16 / (4 * kSteps);  // values of P beside each MFMA
+            uint32_t pw[2][4];
+            float psum[2] = {0.f, 0.f}, p_prev = 0.f;
+            u32x4 va[kBlocks];
+            i16x4 v_lo = {0, 0, 0, 0};
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-            const uint32_t at = v_abs[b & 1] + stage + b * 128;
-            u32x4 a = __builtin_bit_cast(u32x4, __builtin_shufflevector(lds_read_transposed(at),
-                                                                         lds_read_transposed(at + 4 * Tile::kQuadBytes), 0, 1, 2, 3, 4, 5, 6, 7));
-            if (masked) {
-                // 0 times an infinity or a NaN is no zero: values that are not finite
-                // reach only the rows that see them.
-                uint32_t odd = 0;
+            for (int x = 0; x < 4; ++x) sn[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                for (int w = 0; w < 4; ++w) odd |= (a[w] & T::kExponent) + T::kOverflow;
-                if (__any((odd & 0x80008000u) != 0)) {
-                    u32x4 finite = a, up = {0, 0, 0, 0}, down = {0, 0, 0, 0};
+            for (int x = 0; x < 4 * kSteps; ++x) {
+                const int st = x >> 2, h = (x >> 1) & 1, j = x & 1;
+                sn[2 * h + j] = T::mfma16(ka[kSteps * h + st], bq[j][st], sn[2 * h + j]);
 #pragma unroll
-                    for (int w = 0; w < 4; ++w)
+                for (int i = 0; i < kEach; ++i) {
+                    const int e = x * kEach + i, n = e >> 2, r = e & 3;  // n = 2h' + j'
+                    const float p = fast_exp2(sc[n][r]);
+                    psum[n & 1] += p;
+                    if (e & 1) pw[n & 1][2 * (n >> 1) + (r >> 1)] = T::pack(p_prev, p);
+                    p_prev = p;
+                }
+                const i16x4 vh = read_v(t, x >> 1, x & 1);
+                if (x & 1) va[x >> 1] = __builtin_bit_cast(u32x4, __builtin_shufflevector(v_lo, vh, 0, 1, 2, 3, 4, 5, 6, 7));
+                else v_lo = vh;
+                if (x == 2) move_k(t + 5, kp);
+                if (x == 6) move_v(t + 3, vp);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            l_run[0] += psum[0];
+            l_run[1] += psum[1];
+            if (is_masked(t)) {
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const uint32_t bits = (a[w] >> (16 * half)) & 0xffffu, exponent = T::kExponent & 0xffffu;
-                            if ((bits & exponent) != exponent) continue;
-                            const bool nan = (bits & 0x7fffu) != exponent;
-                            finite[w] &= half ? 0xffffu : 0xffff0000u;
-                            if (nan || !(bits & 0x8000u)) up[w] |= T::kOne << (16 * half);
-                            if (nan || (bits & 0x8000u)) down[w] |= T::kOne << (16 * half);
-                        }
-                    a = finite;
+                for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) odd |= (va[b][w] & T::kExponent) + T::kOverflow;
+            }
+            mx[0] = mx[1] = -INFINITY;
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+            for (int x = 0; x < 2 * kBlocks; ++x) {
+                const int b = x >> 1, j = x & 1;
+                const u32x4 p = {pw[j][0], pw[j][1], pw[j][2], pw[j][3]};
+                o_acc[b][j] = T::mfma16(va[b], p, o_acc[b][j]);
+                if (x < 2 * kSteps) ka[x] = read_k(t + 2, x);
+                constexpr int kPairs = 8 / kBlocks;  // pairs of logits of tile t + 1 beside every second MFMA
+                if (x & 1)
+#pragma unroll
+                    for (int i = 0; i < kPairs; ++i) {
+                        const int e = 2 * ((x >> 1) * kPairs + i), n = e >> 2, r = e & 3;
+                        const float y0 = __builtin_fmaf(sn[n][r], c.scale_log2, -m_run[n & 1]);
+                        const float y1 = __builtin_fmaf(sn[n][r + 1], c.scale_log2, -m_run[n & 1]);
+                        sn[n][r] = y0;
+                        sn[n][r + 1] = y1;
+                        mx[n & 1] = fmaxf(fmaxf(mx[n & 1], y0), y1);
+                    }
+                if (x == 2 * kBlocks - 4) kp = place_of(t + 6);
+                if (x == 2 * kBlocks - 2) vp = place_of(t + 4);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (is_masked(t + 1)) mask_logits(t + 1, sn, mx);
+        };
+
+        reset();
+        // K(0 .. 3) and V(0 .. 2); S(0) and K(1) to registers once K(0) and K(1) are
+        // in; K(4) goes to K(0)'s place only after every wave has read that. The last
+        // transfers before step 0 are then K(3), V(1), V(2), K(4), as its wait expects.
+        landed_and_barrier<0>();
+        {
+            const Place p0 = place_of(0), p1 = place_of(1), p2 = place_of(2), p3 = place_of(3);
+            move_k(0, p0);
+            move_k(1, p1);
+            move_k(2, p2);
+            move_v(0, p0);
+            move_k(3, p3);
+            move_v(1, p1);
+            move_v(2, p2);
+        }
+        const Place p4 = place_of(4);
+        Place kp = place_of(5), vp = place_of(3);
+        f32x4 s0[4], s1[4];
+        u32x4 ka[2 * kSteps];
+        float mx[2] = {-INFINITY, -INFINITY};
+        landed_and_barrier<5 * kOps>();
+        if (active) {
+#pragma unroll
+            for (int f = 0; f < 2 * kSteps; ++f) ka[f] = read_k(0, f);
+            start_s(ka, s0);
+#pragma unroll
+            for (int f = 0; f < 2 * kSteps; ++f) ka[f] = read_k(1, f);
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s0[n][r] *= c.scale_log2;
+                    mx[n & 1] = fmaxf(mx[n & 1], s0[n][r]);
+                }
+            if (is_masked(0)) mask_logits(0, s0, mx);
+        }
+        landed_and_barrier<63>();  // every wave's reads of K(0) are done
+        move_k(4, p4);
+        int t = 0;
+        for (; t + 3 < tiles; t += 4) {
+            step(t, s0, s1, mx, ka, kp, vp);
+            step(t + 1, s1, s0, mx, ka, kp, vp);
+            step(t + 2, s0, s1, mx, ka, kp, vp);
+            step(t + 3, s1, s0, mx, ka, kp, vp);
+        }
+        for (; t + 1 < tiles; t += 2) {
+            step(t, s0, s1, mx, ka, kp, vp);
+            step(t + 1, s1, s0, mx, ka, kp, vp);
+        }
+        if (t < tiles) step(t, s0, s1, mx, ka, kp, vp);
+        // No transfer may still be landing when the LDS is released or filled again.
+        uint32_t* votes = reinterpret_cast<uint32_t*>(smem + Tile::kVotes);
+        const uint32_t vote = __any((odd & 0x80008000u) != 0) ? 1u : 0u;
+        landed_and_barrier<0>();
+        if (lane == 0) votes[wave] = vote;
+        landed_and_barrier<0>();
+        const u32x4 all = *reinterpret_cast<const u32x4*>(votes);
+        return __builtin_amdgcn_readfirstlane(all[0] | all[1] | all[2] | all[3]) != 0;
+    };
+
+    // The same sums, tile by tile, with values that are not finite kept from the
+    // rows that do not see them: V without them, and where a row sees one, an
+    // infinity of its sign (or, for NaN, of both).
+    auto careful_pass = [&]() {
+        reset();
+        landed_and_barrier<0>();
+        for (int t = 0; t < tiles; ++t) {
+            const Place p = place_of(t);
+            move_k(0, p);
+            move_v(0, p);
+            landed_and_barrier<0>();
+            if (active) {
+                u32x4 ka[2 * kSteps];
+                f32x4 s[4];
+                float mx[2];
+#pragma unroll
+                for (int f = 0; f < 2 * kSteps; ++f) ka[f] = read_k(0, f);
+                start_s(ka, s);
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[n][r] = __builtin_fmaf(s[n][r], c.scale_log2, -m_run[n & 1]);
+                mask_logits(t, s, mx);
+                move_reference(s, mx);
+                u32x4 pw[2], sees[2];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const uint32_t bits = seen_keys(t, n >> 1, n & 1);
+#pragma unroll
+                    for (int r = 0; r < 4; r += 2) {
+                        const float a = fast_exp2(s[n][r]), b = fast_exp2(s[n][r + 1]);
+                        l_run[n & 1] += a + b;
+                        pw[n & 1][2 * (n >> 1) + r / 2] = T::pack(a, b);
+                        sees[n & 1][2 * (n >> 1) + r / 2] = (bits >> r & 1 ? T::kOne : 0u) | (bits >> (r + 1) & 1 ? T::kOne << 16 : 0u);
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) {
+                    const u32x4 a = __builtin_bit_cast(u32x4, __builtin_shufflevector(read_v(0, b, 0), read_v(0, b, 1), 0, 1, 2, 3, 4, 5, 6, 7));
+                    u32x4 finite, up, down;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        // All ones in the halves that are no number, are NaN, are negative.
+                        const uint32_t none = ((((a[w] & T::kExponent) + T::kOverflow) & 0x80008000u) >> 15) * 0xffffu;
+                        const uint32_t nan = ((((a[w] & ~T::kExponent & 0x7fff7fffu) + 0x7fff7fffu) & 0x80008000u) >> 15) * 0xffffu;
+                        const uint32_t minus = ((a[w] & 0x80008000u) >> 15) * 0xffffu;
+                        finite[w] = a[w] & ~none;
+                        up[w] = none & (nan | ~minus) & (T::kOne * 0x10001u);
+                        down[w] = none & (nan | minus) & (T::kOne * 0x10001u);
+                    }
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        u32x4 sees;
-#pragma unroll
-                        for (int w = 0; w < 4; ++w)
-                            sees[w] = ((visible[j] >> (2 * w)) & 1 ? T::kOne : 0u) | ((visible[j] >> (2 * w + 1)) & 1 ? T::kOne << 16 : 0u);
                         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-                        const f32x4 ups = T::mfma16(up, sees, zero), downs = T::mfma16(down, sees, zero);
+                        const f32x4 ups = T::mfma16(up, sees[j], zero), downs = T::mfma16(down, sees[j], zero);
+                        o_acc[b][j] = T::mfma16(finite, pw[j], o_acc[b][j]);
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            if (ups[r] > 0.f) o_acc[b][j][r] += INFINITY;
-                            if (downs[r] > 0.f) o_acc[b][j][r] -= INFINITY;
+                            o_acc[b][j][r] += ups[r] > 0.f ? INFINITY : 0.f;
+                            o_acc[b][j][r] -= downs[r] > 0.f ? INFINITY : 0.f;
                         }
                     }
                 }
             }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const u32x4 p = {pw[j][0], pw[j][1], pw[j][2], pw[j][3]};
-                o_acc[b][j] = T::mfma16(a, p, o_acc[b][j]);
-            }
+            landed_and_barrier<0>();  // read before the next tile's transfers
         }
-    }
+    };
+    if (fast_pass()) careful_pass();
 
+    if (!active) return;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        float l = l_run[j];
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
-        if (!stored[j]) continue;
+        const auto s16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(l_run[j]), __float_as_uint(l_run[j]), false, false);
+        const float l16 = __uint_as_float(s16[0]) + __uint_as_float(s16[1]);
+        const auto s32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(l16), __float_as_uint(l16), false, false);
+        const float l = __uint_as_float(s32[0]) + __uint_as_float(s32[1]);
+        int token, head;
+        if (!row_of(j, token, head)) continue;
+        const int64_t stat_at = u.b * c.row.batch + head * c.row.head + int64_t(u.off + token) * c.row.token;
         if constexpr (kSplit) {
-            const int64_t at = blockIdx.y * c.rows + stat_at[j];
-            if (lg == 0) c.partial_stat[at] = float2{m_run[j], l};
+            const int64_t at = blockIdx.y * c.rows + stat_at;
+            if (lg == 0) c.partial_stat[at] = float2{started[j] ? m_run[j] : -INFINITY, l};
             if (l == 0.f) continue;
             float* dst = c.partial_o + at * D + 4 * lg;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) *reinterpret_cast<f32x4*>(dst + 16 * b) = o_acc[b][j];
         } else {
             const float inv = l == 0.f ? 0.f : 1.0f / l;
-            uint16_t* orow = static_cast<uint16_t*>(c.out) + out_at[j] + 4 * lg;
+            uint16_t* orow = static_cast<uint16_t*>(c.out) + u.b * c.out_rows.batch + head * c.out_rows.head +
+                             int64_t(u.off + token) * c.out_rows.token + 4 * lg;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
                 const u32x2 w = {T::pack(o_acc[b][j][0] * inv, o_acc[b][j][1] * inv),
                                  T::pack(o_acc[b][j][2] * inv, o_acc[b][j][3] * inv)};
                 *reinterpret_cast<u32x2*>(orow + 16 * b) = w;
             }
-            if (c.lse && lg == 0) c.lse[stat_at[j]] = l == 0.f ? -INFINITY : m_run[j] + log2f(l);
+            if (c.lse && lg == 0) c.lse[stat_at] = l == 0.f ? -INFINITY : m_run[j] + log2f(l);
         }
     }
 }
@@ -430,12 +621,12 @@ template <class T, int D, bool kPaged>
 int launch_as(const WindowCall& c, hipStream_t stream) {
     const int64_t tiles = window_tiles(c), heads = kPaged ? c.kv_heads : int64_t(c.batch) * c.heads;
     const dim3 grid(window_grid(heads, tiles), static_cast<unsigned>(c.parts));
-    if (c.parts == 1) {
-        hipLaunchKernelGGL((window_kernel<T, D, kPaged, false>), grid, dim3(kWindowThreads), 0, stream, c, int(tiles));
-        return check_launch("window_kernel");
-    }
-    hipLaunchKernelGGL((window_kernel<T, D, kPaged, true>), grid, dim3(kWindowThreads), 0, stream, c, int(tiles));
+    const auto kernel = c.parts == 1 ? window_kernel<T, D, kPaged, false> : window_kernel<T, D, kPaged, true>;
+    constexpr int kLds = WindowTile<T, D>::kLdsBytes;
+    if (int rc = ensure_lds_limit(reinterpret_cast<const void*>(kernel), kLds)) return rc;
+    hipLaunchKernelGGL(kernel, grid, dim3(kWindowThreads), kLds, stream, c, int(tiles));
     if (int rc = check_launch("window_kernel")) return rc;
+    if (c.parts == 1) return 0;
     hipLaunchKernelGGL((window_combine_kernel<T, D, kPaged>), dim3(static_cast<unsigned>((c.rows + 3) / 4)), dim3(256), 0, stream, c);
     return check_launch("window_combine_kernel");
 }
