@@ -82,12 +82,22 @@ struct WindowTile {
     static constexpr int kLdsBytes = kVotes + 16;
 };
 
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// v_max_f32 without the NaN quieting that the compiler adds around fmaxf.
+__device__ __forceinline__ float vmax(float a, float b) {
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+#pragma clang diagnostic pop
+
 // The maxima of a and b over the four lanes l, 16 + l, 32 + l, 48 + l.
 __device__ __forceinline__ void max_over_rows(float& a, float& b) {
     const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-    const float m = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    const float m = vmax(__uint_as_float(s[0]), __uint_as_float(s[1]));
     const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    const float m2 = fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+    const float m2 = vmax(__uint_as_float(t[0]), __uint_as_float(t[1]));
     const auto u = __builtin_amdgcn_permlane16_swap(__float_as_uint(m2), __float_as_uint(m2), false, false);
     a = __uint_as_float(u[0]);
     b = __uint_as_float(u[1]);
@@ -215,33 +225,54 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
         int32_t page;
         uint32_t at, there;
     };
-    auto place_of = [&](int t) {
-        const int key = range.key(tile0 + t) + 8 * wave;
-        Place p{0, static_cast<uint32_t>(key), t < tiles ? static_cast<uint32_t>(end) : 0u};
+    int next_tile = 0, next_key = 0;  // of the next place
+    auto first_place = [&]() {
+        next_tile = 0;
+        next_key = range.key(tile0);
+    };
+    auto next_place = [&]() {
+        const int key = next_key + 8 * wave;
+        const bool there = next_tile < tiles;
+        Place p{0, static_cast<uint32_t>(key), there ? static_cast<uint32_t>(end) : 0u};
         if constexpr (kPaged) {
-            const uint32_t index = c.page.quotient(static_cast<uint32_t>(key), p.at);
-            if (t < tiles && key < end) {
+            const uint32_t near = __umulhi(static_cast<uint32_t>(key), c.page.m);
+            const uint32_t rest = static_cast<uint32_t>(key) - near * c.page.d;
+            const uint32_t index = rest >= c.page.d ? near + 1 : near;
+            p.at = rest >= c.page.d ? rest - c.page.d : rest;
+            if (there && key < end) {
                 const auto entries = (const __attribute__((address_space(4))) int32_t*)reinterpret_cast<uintptr_t>(table);
                 const int32_t entry = entries[index];
                 const bool is_page = static_cast<uint32_t>(entry) < static_cast<uint32_t>(c.pages);
-                p.page = is_page ? entry : 0;
-                p.there = is_page ? min(c.page.d, static_cast<uint32_t>(end - key) + p.at) : 0u;
+                p.page = __builtin_amdgcn_readfirstlane(is_page ? entry : 0);
+                p.there = __builtin_amdgcn_readfirstlane(is_page ? min(c.page.d, static_cast<uint32_t>(end - key) + p.at) : 0u);
             } else {
                 p.there = 0;
             }
         }
+        ++next_tile;
+        next_key = tile0 + next_tile == range.sink_tiles ? range.window : next_key + kWindowKeys;
         return p;
     };
-    auto move = [&](const char* base, const Rows& rows_of, uint32_t token, const uint32_t (&src)[kOps], const Place& p, uint32_t lds) {
+    // n rows take n * token - less bytes (kept from the compiler, which turns the sum
+    // into a borrow in vector registers).
+    uint32_t k_less = k_token - 2 * D, v_less = v_token - 2 * D;
+    asm volatile("" : "+s"(k_less), "+s"(v_less));
+    const uint32_t k_all = end * k_token - k_less, v_all = end * v_token - v_less;
+    auto move = [&](const char* base, const Rows& rows_of, uint32_t token, uint32_t less, uint32_t all, const uint32_t (&src)[kOps],
+                    const Place& p, uint32_t lds) {
         const u32x4 buffer = buffer_of(base + (kPaged ? int64_t(p.page) * rows_of.batch * 2 : 0),
-                                       p.there ? (p.there - 1) * token + 2 * D : 0);
+                                       p.there == 0 ? 0 : kPaged ? p.there * token - less : all);
         const uint32_t at = p.at * token;
-#pragma unroll
-        for (int e = 0; e < kOps; ++e) buffer_to_lds(buffer, src[e] + at, lds + wave * (8 * D * 2) + 1024 * e);
+        if constexpr (kOps == 2)
+            buffer_to_lds(buffer, src[0] + at, src[1] + at, lds + wave * (8 * D * 2));
+        else
+            buffer_to_lds(buffer, src[0] + at, lds + wave * (8 * D * 2));
     };
-    auto move_k = [&](int t, const Place& p) { move(kbase, c.k_rows, k_token, k_src, p, lds0 + (t & (kRing - 1)) * Tile::kBytes); };
+    auto move_k = [&](int t, const Place& p) {
+        move(kbase, c.k_rows, k_token, k_less, k_all, k_src, p, lds0 + (t & (kRing - 1)) * Tile::kBytes);
+    };
     auto move_v = [&](int t, const Place& p) {
-        move(vbase, c.v_rows, v_token, v_src, p, lds0 + Tile::kVRing + (t & (kRing - 1)) * Tile::kBytes);
+        move(vbase, c.v_rows, v_token, v_less, v_all, v_src, p, lds0 + Tile::kVRing + (t & (kRing - 1)) * Tile::kBytes);
     };
 
     // Reads of operands: K's row 16h + li, chunk 4s + lg; V's quad lg + 4h, block
@@ -260,10 +291,17 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     auto read_v = [&](int t, int b, int h) {
         return lds_read_transposed(v_abs[b & 1] + (t & (kRing - 1)) * Tile::kBytes + b * 128 + h * 4 * Tile::kQuadBytes);
     };
+    // Tiles without a mask: `clear` of them from `clear_from` on, and those before
+    // clear_sink.
+    int clear_from = 0, clear = 0, clear_sink = 0;
+    if (!holes) {
+        const int skipped = range.sink_tiles - tile0;  // tiles of this part before the window's
+        clear_from = max(skipped, 0) + max(0, full_low - range.window - max(-skipped, 0) * kWindowKeys + kWindowKeys - 1) / kWindowKeys;
+        clear = max(0, min(tiles, (full_high - range.window) / kWindowKeys + skipped) - clear_from);
+        clear_sink = min(range.sink_tiles ? skipped : tiles, full_sink / kWindowKeys - tile0);
+    }
     auto is_masked = [&](int t) {
-        const int key = range.key(tile0 + t);
-        return holes || t >= tiles ||
-               !((key >= full_low && key + kWindowKeys <= full_high) || key + kWindowKeys <= full_sink);
+        return static_cast<uint32_t>(t - clear_from) >= static_cast<uint32_t>(clear) && t >= clear_sink;
     };
     // Bit r of the result: key 16h + 4lg + r of tile t is seen by row 16j + li.
     auto seen_keys = [&](int t, int h, int j) {
@@ -277,8 +315,8 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     };
 
     f32x4 o_acc[kBlocks][2];  // dims 16b + 4lg .. + 3 of row 16j + li
-    float m_run[2], l_run[2];
-    bool started[2];
+    // Reference and sum of row j; -inf until the row's first finite logit, then kSlack.
+    float m_run[2], l_run[2], slack[2];
     auto reset = [&]() {
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b)
@@ -288,7 +326,7 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
         for (int j = 0; j < 2; ++j) {
             m_run[j] = 0.f;
             l_run[j] = 0.f;
-            started[j] = false;
+            slack[j] = -INFINITY;
         }
     };
     auto start_s = [&](const u32x4 (&ka)[2 * kSteps], f32x4 (&s)[4]) {
@@ -320,14 +358,14 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     // above it (or that have none yet): their sums, and the logits at hand, follow.
     auto move_reference = [&](f32x4 (&s)[4], float (&mx)[2]) {
         max_over_rows(mx[0], mx[1]);
-        const bool grow0 = mx[0] > (started[0] ? kSlack : -INFINITY), grow1 = mx[1] > (started[1] ? kSlack : -INFINITY);
+        const bool grow0 = mx[0] > slack[0], grow1 = mx[1] > slack[1];
         if (!__any(grow0 || grow1)) return;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const bool grow = j ? grow1 : grow0;
             const float shift = grow ? mx[j] : 0.f;
-            const float alpha = started[j] ? fast_exp2(-shift) : 1.f;  // the sums are 0 before
-            started[j] |= grow;
+            const float alpha = slack[j] == kSlack ? fast_exp2(-shift) : 1.f;  // the sums are 0 before
+            slack[j] = grow ? kSlack : slack[j];
             m_run[j] += shift;
             l_run[j] *= alpha;
 #pragma unroll
@@ -346,13 +384,19 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     // finite: 0 times it is no zero, so the tile cannot be computed like that.
     auto fast_pass = [&]() -> bool {
         uint32_t odd = 0;
-        auto step = [&](int t, f32x4 (&sc)[4], f32x4 (&sn)[4], float (&mx)[2], u32x4 (&ka)[2 * kSteps], Place& kp, Place& vp) {
+        // Places of K(t + 5), of tile t + 4 and of V(t + 3) before step t.
+        Place kp, mp, vp;
+        auto next_step = [&]() {
+            vp = mp;
+            mp = kp;
+            kp = next_place();
+        };
+        auto step = [&](int t, f32x4 (&sc)[4], f32x4 (&sn)[4], float (&mx)[2], u32x4 (&ka)[2 * kSteps]) {
             landed_and_barrier<4 * kOps>();
             if (!active) {
                 move_k(t + 5, kp);
                 move_v(t + 3, vp);
-                kp = place_of(t + 6);
-                vp = place_of(t + 4);
+                next_step();
                 return;
             }
             move_reference(sc, mx);
@@ -384,6 +428,10 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
                 if (x == 6) move_v(t + 3, vp);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            // P is made here, beside the MFMAs, and not moved behind the branch.
+#pragma unroll
+            for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(pw[i >> 2][i & 3]));
+            asm volatile("" : "+v"(psum[0]), "+v"(psum[1]));
             l_run[0] += psum[0];
             l_run[1] += psum[1];
             if (is_masked(t)) {
@@ -412,10 +460,10 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
                         sn[n][r + 1] = y1;
                         mx[n & 1] = fmaxf(fmaxf(mx[n & 1], y0), y1);
                     }
-                if (x == 2 * kBlocks - 4) kp = place_of(t + 6);
-                if (x == 2 * kBlocks - 2) vp = place_of(t + 4);
+                if (x == 2 * kBlocks - 4) next_step();
                 __builtin_amdgcn_sched_barrier(0);
             }
+            asm volatile("" : "+v"(mx[0]), "+v"(mx[1]));  // made beside the MFMAs too
             if (is_masked(t + 1)) mask_logits(t + 1, sn, mx);
         };
 
@@ -425,17 +473,19 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
         // transfers before step 0 are then K(3), V(1), V(2), K(4), as its wait expects.
         landed_and_barrier<0>();
         {
-            const Place p0 = place_of(0), p1 = place_of(1), p2 = place_of(2), p3 = place_of(3);
+            first_place();
+            const Place p0 = next_place(), p1 = next_place(), p2 = next_place();
+            vp = next_place();
             move_k(0, p0);
             move_k(1, p1);
             move_k(2, p2);
             move_v(0, p0);
-            move_k(3, p3);
+            move_k(3, vp);
             move_v(1, p1);
             move_v(2, p2);
         }
-        const Place p4 = place_of(4);
-        Place kp = place_of(5), vp = place_of(3);
+        mp = next_place();
+        kp = next_place();
         f32x4 s0[4], s1[4];
         u32x4 ka[2 * kSteps];
         float mx[2] = {-INFINITY, -INFINITY};
@@ -456,19 +506,19 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
             if (is_masked(0)) mask_logits(0, s0, mx);
         }
         landed_and_barrier<63>();  // every wave's reads of K(0) are done
-        move_k(4, p4);
+        move_k(4, mp);
         int t = 0;
         for (; t + 3 < tiles; t += 4) {
-            step(t, s0, s1, mx, ka, kp, vp);
-            step(t + 1, s1, s0, mx, ka, kp, vp);
-            step(t + 2, s0, s1, mx, ka, kp, vp);
-            step(t + 3, s1, s0, mx, ka, kp, vp);
+            step(t, s0, s1, mx, ka);
+            step(t + 1, s1, s0, mx, ka);
+            step(t + 2, s0, s1, mx, ka);
+            step(t + 3, s1, s0, mx, ka);
         }
         for (; t + 1 < tiles; t += 2) {
-            step(t, s0, s1, mx, ka, kp, vp);
-            step(t + 1, s1, s0, mx, ka, kp, vp);
+            step(t, s0, s1, mx, ka);
+            step(t + 1, s1, s0, mx, ka);
         }
-        if (t < tiles) step(t, s0, s1, mx, ka, kp, vp);
+        if (t < tiles) step(t, s0, s1, mx, ka);
         // No transfer may still be landing when the LDS is released or filled again.
         uint32_t* votes = reinterpret_cast<uint32_t*>(smem + Tile::kVotes);
         const uint32_t vote = __any((odd & 0x80008000u) != 0) ? 1u : 0u;
@@ -485,8 +535,9 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     auto careful_pass = [&]() {
         reset();
         landed_and_barrier<0>();
+        first_place();
         for (int t = 0; t < tiles; ++t) {
-            const Place p = place_of(t);
+            const Place p = next_place();
             move_k(0, p);
             move_v(0, p);
             landed_and_barrier<0>();
@@ -559,7 +610,7 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
         const int64_t stat_at = u.b * c.row.batch + head * c.row.head + int64_t(u.off + token) * c.row.token;
         if constexpr (kSplit) {
             const int64_t at = blockIdx.y * c.rows + stat_at;
-            if (lg == 0) c.partial_stat[at] = float2{started[j] ? m_run[j] : -INFINITY, l};
+            if (lg == 0) c.partial_stat[at] = float2{slack[j] == kSlack ? m_run[j] : -INFINITY, l};
             if (l == 0.f) continue;
             float* dst = c.partial_o + at * D + 4 * lg;
 #pragma unroll

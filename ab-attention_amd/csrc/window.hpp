@@ -89,13 +89,11 @@ __device__ __forceinline__ u32x4 lds_read16(uint32_t lds) {
     return *reinterpret_cast<const lds_u32x4*>(static_cast<uintptr_t>(lds));
 }
 
-// A buffer of `bytes` bytes from `base` on: reads past its end give zeros.
+// A buffer of `bytes` bytes from `base` on, the same in all lanes: reads past its
+// end give zeros.
 __device__ __forceinline__ u32x4 buffer_of(const void* base, uint32_t bytes) {
     const uint64_t a = reinterpret_cast<uint64_t>(base);
-    u32x4 r = {static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32) & 0xffffu, bytes, 0x00020000u};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_readfirstlane(r[i]);
-    return r;
+    return u32x4{static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32) & 0xffffu, bytes, 0x00020000u};
 }
 
 #pragma clang diagnostic push
@@ -107,6 +105,14 @@ __device__ __forceinline__ u32x4 buffer_of(const void* base, uint32_t bytes) {
 __device__ __forceinline__ void buffer_to_lds(u32x4 buffer, uint32_t offset, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer)
                  : "memory", "m0");
+}
+// The same twice, into 1 KiB each.
+__device__ __forceinline__ void buffer_to_lds(u32x4 buffer, uint32_t offset0, uint32_t offset1, uint32_t lds) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+        "s_add_u32 m0, %0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds" ::"s"(lds),
+        "v"(offset0), "v"(offset1), "s"(buffer)
+        : "memory", "m0", "scc");
 }
 #pragma clang diagnostic pop
 
