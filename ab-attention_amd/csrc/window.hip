@@ -31,10 +31,10 @@ struct WindowUnit {
 };
 
 template <bool kPaged>
-__device__ __forceinline__ bool window_unit(const WindowCall& c, uint32_t id, int tiles, WindowUnit& u) {
+__device__ __forceinline__ bool window_unit(const WindowCall& c, const WindowGrid& grid, uint32_t id, WindowUnit& u) {
     int head;
     if constexpr (!kPaged) {
-        if (!window_place(id, c.batch * c.heads, tiles, head, u.tile)) return false;
+        grid.place(id, head, u.tile);
         u.b = head / c.heads;
         u.head = head - u.b * c.heads;
         u.kv_head = u.head / static_cast<int>(c.group.d);
@@ -47,7 +47,7 @@ __device__ __forceinline__ bool window_unit(const WindowCall& c, uint32_t id, in
         // Sequence b's tiles take the slots from offsets[b] * group / 128 + b on:
         // never fewer than it needs, so no sum over the sequences is wanted.
         int slot;
-        if (!window_place(id, c.kv_heads, tiles, head, slot)) return false;
+        grid.place(id, head, slot);
         u.kv_head = head;
         u.head = head * c.group.d;
         const int lane = threadIdx.x & 63;
@@ -104,13 +104,13 @@ __device__ __forceinline__ void max_over_rows(float& a, float& b) {
 }
 
 template <class T, int D, bool kPaged, bool kSplit>
-__global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c, int tiles_per_head) {
+__global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c, WindowGrid places) {
     using Tile = WindowTile<T, D>;
     constexpr int kSteps = Tile::kSteps, kBlocks = Tile::kBlocks, kOps = Tile::kOps;
     extern __shared__ __align__(16) unsigned char smem[];
 
     WindowUnit u;
-    if (!window_unit<kPaged>(c, blockIdx.x, tiles_per_head, u)) return;
+    if (!window_unit<kPaged>(c, places, blockIdx.x, u)) return;
     const int group = kPaged ? c.group.d : 1;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -178,6 +178,7 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     const char* vbase = static_cast<const char*>(c.v) + ((kPaged ? 0 : u.b * c.v_rows.batch) + u.kv_head * c.v_rows.head) * 2;
     const uint32_t k_token = static_cast<uint32_t>(c.k_rows.token * 2), v_token = static_cast<uint32_t>(c.v_rows.token * 2);
     const int32_t* table = kPaged ? c.table + int64_t(u.b) * c.table_width : nullptr;
+    const int last_entry = c.table_width - 1;
 
     // Whether a key that some row would see lies on no page (then every tile
     // asks the table for its keys).
@@ -225,7 +226,20 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
         int32_t page;
         uint32_t at, there;
     };
-    int next_tile = 0, next_key = 0;  // of the next place
+    // The next place: its tile, its first key, and over a cache the page table's
+    // entry, which ask() fetches well before next_place() takes it.
+    int next_tile = 0, next_key = 0, next_entry = -1;
+    uint32_t next_at = 0;
+    auto ask = [&]() {
+        if constexpr (kPaged) {
+            const uint32_t key = next_key + 8 * wave;
+            const uint32_t near = __umulhi(key, c.page.m), rest = key - near * c.page.d;
+            const uint32_t index = rest >= c.page.d ? near + 1 : near;
+            next_at = rest >= c.page.d ? rest - c.page.d : rest;
+            const auto entries = (const __attribute__((address_space(4))) int32_t*)reinterpret_cast<uintptr_t>(table);
+            next_entry = entries[min(index, static_cast<uint32_t>(last_entry))];
+        }
+    };
     auto first_place = [&]() {
         next_tile = 0;
         next_key = range.key(tile0);
@@ -235,23 +249,18 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
         const bool there = next_tile < tiles;
         Place p{0, static_cast<uint32_t>(key), there ? static_cast<uint32_t>(end) : 0u};
         if constexpr (kPaged) {
-            const uint32_t near = __umulhi(static_cast<uint32_t>(key), c.page.m);
-            const uint32_t rest = static_cast<uint32_t>(key) - near * c.page.d;
-            const uint32_t index = rest >= c.page.d ? near + 1 : near;
-            p.at = rest >= c.page.d ? rest - c.page.d : rest;
-            if (there && key < end) {
-                const auto entries = (const __attribute__((address_space(4))) int32_t*)reinterpret_cast<uintptr_t>(table);
-                const int32_t entry = entries[index];
-                const bool is_page = static_cast<uint32_t>(entry) < static_cast<uint32_t>(c.pages);
-                p.page = __builtin_amdgcn_readfirstlane(is_page ? entry : 0);
-                p.there = __builtin_amdgcn_readfirstlane(is_page ? min(c.page.d, static_cast<uint32_t>(end - key) + p.at) : 0u);
-            } else {
-                p.there = 0;
-            }
+            const bool is_page = there && key < end && static_cast<uint32_t>(next_entry) < static_cast<uint32_t>(c.pages);
+            p.page = is_page ? next_entry : 0;
+            p.at = next_at;
+            p.there = is_page ? min(c.page.d, static_cast<uint32_t>(end - key) + next_at) : 0u;
         }
         ++next_tile;
         next_key = tile0 + next_tile == range.sink_tiles ? range.window : next_key + kWindowKeys;
         return p;
+    };
+    auto ask_place = [&]() {
+        ask();
+        return next_place();
     };
     // n rows take n * token - less bytes (kept from the compiler, which turns the sum
     // into a borrow in vector registers).
@@ -393,6 +402,7 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
         };
         auto step = [&](int t, f32x4 (&sc)[4], f32x4 (&sn)[4], float (&mx)[2], u32x4 (&ka)[2 * kSteps]) {
             landed_and_barrier<4 * kOps>();
+            ask();
             if (!active) {
                 move_k(t + 5, kp);
                 move_v(t + 3, vp);
@@ -467,15 +477,14 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
             if (is_masked(t + 1)) mask_logits(t + 1, sn, mx);
         };
 
-        reset();
         // K(0 .. 3) and V(0 .. 2); S(0) and K(1) to registers once K(0) and K(1) are
         // in; K(4) goes to K(0)'s place only after every wave has read that. The last
         // transfers before step 0 are then K(3), V(1), V(2), K(4), as its wait expects.
         landed_and_barrier<0>();
         {
             first_place();
-            const Place p0 = next_place(), p1 = next_place(), p2 = next_place();
-            vp = next_place();
+            const Place p0 = ask_place(), p1 = ask_place(), p2 = ask_place();
+            vp = ask_place();
             move_k(0, p0);
             move_k(1, p1);
             move_k(2, p2);
@@ -484,8 +493,8 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
             move_v(1, p1);
             move_v(2, p2);
         }
-        mp = next_place();
-        kp = next_place();
+        mp = ask_place();
+        kp = ask_place();
         f32x4 s0[4], s1[4];
         u32x4 ka[2 * kSteps];
         float mx[2] = {-INFINITY, -INFINITY};
@@ -537,7 +546,7 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
         landed_and_barrier<0>();
         first_place();
         for (int t = 0; t < tiles; ++t) {
-            const Place p = next_place();
+            const Place p = ask_place();
             move_k(0, p);
             move_v(0, p);
             landed_and_barrier<0>();
@@ -596,7 +605,9 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
             landed_and_barrier<0>();  // read before the next tile's transfers
         }
     };
-    if (fast_pass()) careful_pass();
+    // Without a key there may be no page table either: nothing is asked for.
+    reset();
+    if (tiles > 0 && fast_pass()) careful_pass();
 
     if (!active) return;
 #pragma unroll
@@ -671,11 +682,12 @@ __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
 template <class T, int D, bool kPaged>
 int launch_as(const WindowCall& c, hipStream_t stream) {
     const int64_t tiles = window_tiles(c), heads = kPaged ? c.kv_heads : int64_t(c.batch) * c.heads;
-    const dim3 grid(window_grid(heads, tiles), static_cast<unsigned>(c.parts));
+    const WindowGrid places = window_grid(heads, tiles, kPaged && c.batch > 1);
+    const dim3 grid(places.size(), static_cast<unsigned>(c.parts));
     const auto kernel = c.parts == 1 ? window_kernel<T, D, kPaged, false> : window_kernel<T, D, kPaged, true>;
     constexpr int kLds = WindowTile<T, D>::kLdsBytes;
     if (int rc = ensure_lds_limit(reinterpret_cast<const void*>(kernel), kLds)) return rc;
-    hipLaunchKernelGGL(kernel, grid, dim3(kWindowThreads), kLds, stream, c, int(tiles));
+    hipLaunchKernelGGL(kernel, grid, dim3(kWindowThreads), kLds, stream, c, places);
     if (int rc = check_launch("window_kernel")) return rc;
     if (c.parts == 1) return 0;
     hipLaunchKernelGGL((window_combine_kernel<T, D, kPaged>), dim3(static_cast<unsigned>((c.rows + 3) / 4)), dim3(256), 0, stream, c);

@@ -85,29 +85,30 @@ __device__ __forceinline__ u32x4 head_buffer(const void* base, const Rows& r, in
 }
 
 template <class T, int D, bool kKeys>
-__global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGradCall c, int tiles_per_head) {
+__global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGradCall c, WindowGrid places) {
     constexpr int kSteps = D / 32, kBlocks = D / 16, kQuad = 4 * D * 2, kBytes = kTileRows * D * 2, kOps = D / 64;
     constexpr int kOpRows = 1024 / (2 * D);
     constexpr int kStat = 4 * kBytes;
     // Two stages of Y1, two of Y2, and each wave's copy of the streamed rows' stat.
     __shared__ __align__(16) unsigned char smem[4 * kBytes + (kKeys ? 8 * 256 : 0)];
 
-    // Owned rows. Sink tiles come first, part by part, then the tiles behind them.
+    // Owned rows. Of keys, the sinks' tiles come first, part by part: `places` are
+    // the tiles behind them.
     int head, tile, part = 0, parts = 1;
     if constexpr (kKeys) {
-        const int extra = c.sink_tiles * c.sink_parts;
-        const int per_head = tiles_per_head - c.sink_tiles + extra;
-        head = blockIdx.x / per_head;
-        tile = blockIdx.x - head * per_head;
-        if (tile < extra) {
+        const uint32_t split = c.batch * c.kv_heads * c.sink_tiles * c.sink_parts;
+        if (blockIdx.x < split) {
             parts = c.sink_parts;
-            part = tile % parts;
-            tile /= parts;
+            tile = blockIdx.x / parts;
+            part = blockIdx.x - tile * parts;
+            head = tile / c.sink_tiles;
+            tile -= head * c.sink_tiles;
         } else {
-            tile -= extra - c.sink_tiles;
+            places.place(blockIdx.x - split, head, tile);
+            tile = c.sink_tiles + (places.tiles - 1 - tile);  // the first keys are seen most
         }
     } else {
-        if (!window_place(blockIdx.x, c.batch * c.heads, tiles_per_head, head, tile)) return;
+        places.place(blockIdx.x, head, tile);
     }
     const int heads = kKeys ? c.kv_heads : c.heads;
     const int b = head / heads, h = head - b * heads;  // own head
@@ -407,8 +408,9 @@ int launch_as(const WindowGradCall& c, hipStream_t stream) {
     const unsigned y = std::min(bh, 32768u);
     hipLaunchKernelGGL((window_delta_kernel<T, D>), dim3(blocks, y, (bh + y - 1) / y), dim3(256), 0, stream, c, blocks);
     if (int rc = check_launch("window_delta_kernel")) return rc;
-    const unsigned items = static_cast<unsigned>(tiles - c.sink_tiles + c.sink_tiles * c.sink_parts);
-    hipLaunchKernelGGL((window_grad_kernel<T, D, true>), dim3(items * kv), dim3(kWindowThreads), 0, stream, c, tiles);
+    const unsigned split = kv * c.sink_tiles * c.sink_parts;
+    const WindowGrid keys = window_grid(kv, tiles - c.sink_tiles, false), queries = window_grid(bh, tiles, false);
+    hipLaunchKernelGGL((window_grad_kernel<T, D, true>), dim3(split + keys.size()), dim3(kWindowThreads), 0, stream, c, keys);
     if (int rc = check_launch("window_grad_kernel")) return rc;
     if (c.sink_tiles) {
         // In launches of at most 65,535 heads.
@@ -416,8 +418,7 @@ int launch_as(const WindowGradCall& c, hipStream_t stream) {
                            stream, c);
         if (int rc = check_launch("window_sinks_kernel")) return rc;
     }
-    hipLaunchKernelGGL((window_grad_kernel<T, D, false>), dim3(window_grid(int64_t(bh), tiles)), dim3(kWindowThreads), 0, stream, c,
-                       tiles);
+    hipLaunchKernelGGL((window_grad_kernel<T, D, false>), dim3(queries.size()), dim3(kWindowThreads), 0, stream, c, queries);
     return check_launch("window_grad_kernel");
 }
 }  // namespace
