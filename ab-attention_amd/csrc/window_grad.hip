@@ -24,6 +24,11 @@ namespace ab {
 namespace {
 
 constexpr int kTileRows = kWindowKeys;  // streamed rows of a tile
+constexpr int kStages = 4;              // of streamed tiles in LDS
+template <int D, bool kKeys>
+constexpr int grad_lds() {
+    return 2 * kStages * kTileRows * D * 2 + (kKeys ? kStages * 4 * 256 : 0);
+}
 static_assert(kTileRows == 32, "stat blocks are 32 queries");
 
 __device__ __forceinline__ int length_of(const WindowGradCall& c, int b) {
@@ -88,9 +93,9 @@ template <class T, int D, bool kKeys>
 __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGradCall c, WindowGrid places) {
     constexpr int kSteps = D / 32, kBlocks = D / 16, kQuad = 4 * D * 2, kBytes = kTileRows * D * 2, kOps = D / 64;
     constexpr int kOpRows = 1024 / (2 * D);
-    constexpr int kStat = 4 * kBytes;
-    // Two stages of Y1, two of Y2, and each wave's copy of the streamed rows' stat.
-    __shared__ __align__(16) unsigned char smem[4 * kBytes + (kKeys ? 8 * 256 : 0)];
+    // Four stages of Y1, four of Y2, and each wave's copy of the streamed rows' stat.
+    constexpr int kY2 = kStages * kBytes, kStat = 2 * kStages * kBytes;
+    extern __shared__ __align__(16) unsigned char smem[];
 
     // Owned rows. Of keys, the sinks' tiles come first, part by part: `places` are
     // the tiles behind them.
@@ -117,6 +122,13 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4;
+    // The lane, for values made anew in each tile: D = 128 leaves the loop over
+    // queries no register to keep them in (four spilled ones cost 10 %).
+    auto lane_now = [&]() {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        return l;
+    };
     const int own0 = tile * kWindowRows, own_last = min(own0 + kWindowRows, length) - 1;
 
     // Queries that see a key at position p: start(p) .. until(p) - 1.
@@ -145,14 +157,11 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
 
     // X as the B operand: owned row 16j + li of the wave's 32, dims 32s + 8lg .. + 7.
     u32x4 x1[2][kSteps], x2[2][kSteps];
-    int from[2], to[2], sink[2];  // streamed rows seen: from .. to - 1, and those before sink
     float lse[2] = {0.f, 0.f}, neg_delta[2] = {0.f, 0.f};
-    int own[2];
     const int stat_blocks = (c.tokens + 31) / 32;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int p = own0 + wave * 32 + 16 * j + li;
-        own[j] = p;
         const bool there = p < length;
         const int64_t at = min(p, c.tokens - 1);
         const Rows &r1 = kKeys ? c.k_rows : c.q_rows, &r2 = kKeys ? c.v_rows : c.dout_rows;
@@ -166,21 +175,29 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
                 x2[j][s] = *reinterpret_cast<const u32x4*>(d + 32 * s);
             }
         }
-        from[j] = to[j] = sink[j] = 0;
-        if (there) {
-            if constexpr (kKeys) {
-                from[j] = mask.start(p);
-                to[j] = until(p);
-            } else {
-                from[j] = mask.low(p);
-                to[j] = mask.high(p, length);
-                sink[j] = min(mask.sinks, to[j]);
+        if constexpr (!kKeys) {
+            if (there) {
                 const float* stat = c.stat + (int64_t(head) * stat_blocks + (p >> 5)) * 64 + (p & 31);
                 lse[j] = stat[0];
                 neg_delta[j] = stat[32];
             }
         }
     }
+    // Streamed rows that the owned row at p sees: from .. from + count - 1, and those
+    // before sink.
+    auto seen_rows = [&](int p, int& from, int& count, int& sink) {
+        const bool there = p < length;
+        if constexpr (kKeys) {
+            from = mask.start(p);
+            count = there ? until(p) - from : 0;
+            sink = 0;
+        } else {
+            const int high = mask.high(p, length);
+            from = mask.low(p);
+            count = there ? high - from : 0;
+            sink = there ? min(mask.sinks, high) : 0;
+        }
+    };
     // Tiles that all rows of this wave see whole need no mask.
     int full_from = 1, full_to = 0, full_sink = 0;
     const int w0 = own0 + wave * 32, w1 = min(w0 + 31, length - 1);
@@ -202,14 +219,11 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
     // Transfers of this wave: rows 8w .. 8w + 7 of a tile. Every four rows lie as
     // blocks of 4 rows x 16 dims, block m at position m ^ (quad & 1): row reads and
     // transposing reads both spread over the banks.
-    uint32_t src1[kOps], src2[kOps];
-#pragma unroll
-    for (int e = 0; e < kOps; ++e) {
-        const int quad = D == 128 ? e : lane >> 5, block = (lane >> 3) % kBlocks, r = (lane >> 1) & 3, half = lane & 1;
-        const uint32_t row = 8 * wave + (D == 128 ? 0 : 4 * quad) + r, at = uint32_t(2 * (block ^ (quad & 1)) + half) * 16u;
-        src1[e] = row * y1_token + at;
-        src2[e] = row * y2_token + at;
-    }
+    // With D = 128 a transfer is one quad, and the second one's blocks are swapped in
+    // pairs: 32 bytes up or down.
+    const int quad0 = D == 128 ? 0 : lane >> 5, block0 = (lane >> 3) % kBlocks;
+    const uint32_t src_row = 8 * wave + 4 * quad0 + ((lane >> 1) & 3), src_at = (2 * (block0 ^ quad0) + (lane & 1)) * 16u;
+    const uint32_t src1 = src_row * y1_token + src_at, src2 = src_row * y2_token + src_at;
     // The round and the tile of the next transfer.
     int next = first, next_round = range.tiles ? first / range.tiles : 0, next_tile = first - next_round * range.tiles;
     u32x4 y1_buf, y2_buf, stat_buf;
@@ -222,14 +236,23 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
     };
     enter_round(next_round);
     auto transfer = [&]() {
-        if (next >= last) return;
-        const uint32_t row = range.key(next_tile), stage = (next & 1) * kBytes + wave * (8 * D * 2);
-#pragma unroll
-        for (int e = 0; e < kOps; ++e) {
-            buffer_to_lds(y1_buf, src1[e] + (row + kOpRows * e) * y1_token, lds0 + stage + 1024 * e);
-            buffer_to_lds(y2_buf, src2[e] + (row + kOpRows * e) * y2_token, lds0 + 2 * kBytes + stage + 1024 * e);
+        const uint32_t row = range.key(next_tile), place = next & (kStages - 1), stage = place * kBytes + wave * (8 * D * 2);
+        // Past the last tile: nothing but the count.
+        u32x4 y1 = y1_buf, y2 = y2_buf;
+        if (next >= last) y1[2] = y2[2] = 0;
+        if constexpr (kOps == 2) {
+            const uint32_t swap = lane_now() & 8 ? -32 : 32;
+            buffer_to_lds(y1, src1 + row * y1_token, src1 + swap + (row + kOpRows) * y1_token, lds0 + stage);
+            buffer_to_lds(y2, src2 + row * y2_token, src2 + swap + (row + kOpRows) * y2_token, lds0 + kY2 + stage);
+        } else {
+            buffer_to_lds(y1, src1 + row * y1_token, lds0 + stage);
+            buffer_to_lds(y2, src2 + row * y2_token, lds0 + kY2 + stage);
         }
-        if constexpr (kKeys) buffer_to_lds4(stat_buf, row * 8 + 4 * lane, lds0 + kStat + ((next & 1) * 4 + wave) * 256);
+        if constexpr (kKeys) {
+            u32x4 stat = stat_buf;
+            if (next >= last) stat[2] = 0;
+            buffer_to_lds4(stat, row * 8 + 4 * lane_now(), lds0 + kStat + (place * 4 + wave) * 256);
+        }
         ++next;
         if (++next_tile == range.tiles) {
             next_tile = 0;
@@ -239,12 +262,11 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
 
     // Row reads (A of S and dP): row 16h + li, dims 32s + 8lg .. + 7: quad li / 4,
     // block 2s + lg / 2. Transposing reads as in the forward pass.
-    uint32_t row_abs[2], tr_abs[2];
+    uint32_t row_abs, tr_abs[2];
     {
         const int quad = li >> 2, par = quad & 1, base = quad * kQuad + (li & 3) * 32 + (lg & 1) * 16;
         // block m = 2s + lg / 2 at position m ^ par
-        row_abs[0] = lds0 + base + (((lg >> 1) ^ par)) * 128;
-        row_abs[1] = row_abs[0] + 2 * kBytes;
+        row_abs = lds0 + base + (((lg >> 1) ^ par)) * 128;
         const int tpar = lg & 1, tbase = lg * kQuad + 32 * (li >> 2) + 8 * (li & 3);
         tr_abs[0] = lds0 + tbase + tpar * 128;
         tr_abs[1] = lds0 + tbase - tpar * 128;
@@ -260,65 +282,79 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
         }
 
     int tile_now = next_tile;
-    transfer();
-    for (int t = first; t < last; ++t) {
+    if (first < last) {
         landed_and_barrier<0>();
         transfer();
-        const int row0 = range.key(tile_now), stage = (t & 1) * kBytes;
+        transfer();
+        transfer();
+    }
+    // Stage t + 3 is that of t - 1, which every wave has left at the barrier.
+    constexpr int kTileOps = 2 * kOps + (kKeys ? 1 : 0);
+    for (int t = first; t < last; ++t) {
+        landed_and_barrier<2 * kTileOps>();
+        transfer();
+        const int row0 = range.key(tile_now), place = t & (kStages - 1), stage = place * kBytes;
         if (++tile_now == range.tiles) tile_now = 0;
         if (!active) continue;
         const bool masked = !((row0 >= full_from && row0 + kTileRows <= full_to) || row0 + kTileRows <= full_sink);
 
-        f32x4 sc[4], dp[4];  // [2h + j]: streamed rows 16h + 4lg + r, owned row 16j + li
-#pragma unroll
-        for (int x = 0; x < 4; ++x) sc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-        f32x4 row_lse[2];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            if constexpr (kKeys) {
-                const uint32_t at = lds0 + kStat + ((t & 1) * 4 + wave) * 256 + (16 * half + 4 * lg) * 4;
-                row_lse[half] = __builtin_bit_cast(f32x4, lds_read16(at));
-                dp[2 * half] = dp[2 * half + 1] = __builtin_bit_cast(f32x4, lds_read16(at + 128));
-            } else {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) dp[2 * half + j] = f32x4{neg_delta[j], neg_delta[j], neg_delta[j], neg_delta[j]};
-            }
-        }
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const u32x4 a1 = lds_read16(row_abs[0] + stage + half * 4 * kQuad + s * 256);
-                const u32x4 a2 = lds_read16(row_abs[1] + stage + half * 4 * kQuad + s * 256);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    sc[2 * half + j] = T::mfma16(a1, x1[j][s], sc[2 * half + j]);
-                    dp[2 * half + j] = T::mfma16(a2, x2[j][s], dp[2 * half + j]);
-                }
-            }
+        // In halves of 16 streamed rows: S and dP of row 16 half + 4lg + r and owned
+        // row 16j + li, then P and dS as the second products take them.
         u32x4 pw[2], dw[2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+        for (int half = 0; half < 2; ++half) {
+            f32x4 sc[2], dp[2], row_lse;
+            if constexpr (kKeys) {
+                const uint32_t at = lds0 + kStat + (place * 4 + wave) * 256 + 64 * half + 16 * (lane_now() >> 4);
+                row_lse = __builtin_bit_cast(f32x4, lds_read16(at));
+                dp[0] = dp[1] = __builtin_bit_cast(f32x4, lds_read16(at + 128));
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                sc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if constexpr (!kKeys) dp[j] = f32x4{neg_delta[j], neg_delta[j], neg_delta[j], neg_delta[j]};
+            }
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                const u32x4 a1 = lds_read16(row_abs + stage + half * 4 * kQuad + s * 256);
+                const u32x4 a2 = lds_read16(row_abs + stage + kY2 + half * 4 * kQuad + s * 256);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    sc[j] = T::mfma16(a1, x1[j][s], sc[j]);
+                    dp[j] = T::mfma16(a2, x2[j][s], dp[j]);
+                }
+            }
+            // sc becomes P, dp dS.
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    sc[j][r] = fast_exp2(__builtin_fmaf(sc[j][r], c.scale_log2, kKeys ? -row_lse[r] : -lse[j]));
+                    dp[j][r] *= sc[j][r];
+                }
+            if (masked) {
+                const int l = lane_now(), row = row0 + 16 * half + 4 * (l >> 4);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    int from, count, sink;
+                    seen_rows(own0 + wave * 32 + 16 * j + (l & 15), from, count, sink);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        bool sees = static_cast<uint32_t>(row + r - from) < static_cast<uint32_t>(count);
+                        if constexpr (!kKeys) sees |= row + r < sink;
+                        sc[j][r] = sees ? sc[j][r] : 0.f;
+                        dp[j][r] = sees ? dp[j][r] : 0.f;
+                    }
+                }
+            }
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; r += 2) {
-                    float p[2], ds[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float z = __builtin_fmaf(sc[2 * half + j][r + i], c.scale_log2, kKeys ? -row_lse[half][r + i] : -lse[j]);
-                        p[i] = fast_exp2(z);
-                        ds[i] = p[i] * dp[2 * half + j][r + i];
-                        if (masked) {
-                            const int row = row0 + 16 * half + 4 * lg + r + i;
-                            const bool sees = (row >= from[j] && row < to[j]) || (!kKeys && row < sink[j]);
-                            p[i] = sees ? p[i] : 0.f;
-                            ds[i] = sees ? ds[i] : 0.f;
-                        }
-                    }
-                    pw[j][2 * half + r / 2] = T::pack(p[0], p[1]);
-                    dw[j][2 * half + r / 2] = T::pack(ds[0], ds[1]);
+                    pw[j][2 * half + r / 2] = T::pack(sc[j][r], sc[j][r + 1]);
+                    dw[j][2 * half + r / 2] = T::pack(dp[j][r], dp[j][r + 1]);
                 }
+        }
 #pragma unroll
         for (int m = 0; m < kBlocks; ++m) {
             const uint32_t at = tr_abs[m & 1] + stage + m * 128;
@@ -326,16 +362,18 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
 #pragma unroll
             for (int j = 0; j < 2; ++j) acc1[m][j] = T::mfma16(a1, dw[j], acc1[m][j]);
             if constexpr (kKeys) {
-                const u32x4 a2 = __builtin_bit_cast(u32x4, __builtin_shufflevector(lds_read_transposed(at + 2 * kBytes), lds_read_transposed(at + 2 * kBytes + 4 * kQuad), 0, 1, 2, 3, 4, 5, 6, 7));
+                const u32x4 a2 = __builtin_bit_cast(u32x4, __builtin_shufflevector(lds_read_transposed(at + kY2), lds_read_transposed(at + kY2 + 4 * kQuad), 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
                 for (int j = 0; j < 2; ++j) acc2[m][j] = T::mfma16(a2, pw[j], acc2[m][j]);
             }
         }
     }
 
+    // No transfer may still be landing when the LDS is released.
+    landed_and_barrier<0>();
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        const int p = own[j];
+        const int p = own0 + wave * 32 + 16 * j + li;
         if constexpr (kKeys) {
             if (parts > 1) {
                 float* dst = c.partial + ((int64_t(head) * c.sink_tiles + tile) * parts + part) * (2 * kWindowRows * D) +
@@ -410,7 +448,10 @@ int launch_as(const WindowGradCall& c, hipStream_t stream) {
     if (int rc = check_launch("window_delta_kernel")) return rc;
     const unsigned split = kv * c.sink_tiles * c.sink_parts;
     const WindowGrid keys = window_grid(kv, tiles - c.sink_tiles, false), queries = window_grid(bh, tiles, false);
-    hipLaunchKernelGGL((window_grad_kernel<T, D, true>), dim3(split + keys.size()), dim3(kWindowThreads), 0, stream, c, keys);
+    const auto by_keys = window_grad_kernel<T, D, true>, by_queries = window_grad_kernel<T, D, false>;
+    if (int rc = ensure_lds_limit(reinterpret_cast<const void*>(by_keys), grad_lds<D, true>())) return rc;
+    if (int rc = ensure_lds_limit(reinterpret_cast<const void*>(by_queries), grad_lds<D, false>())) return rc;
+    hipLaunchKernelGGL(by_keys, dim3(split + keys.size()), dim3(kWindowThreads), (grad_lds<D, true>()), stream, c, keys);
     if (int rc = check_launch("window_grad_kernel")) return rc;
     if (c.sink_tiles) {
         // In launches of at most 65,535 heads.
@@ -418,7 +459,7 @@ int launch_as(const WindowGradCall& c, hipStream_t stream) {
                            stream, c);
         if (int rc = check_launch("window_sinks_kernel")) return rc;
     }
-    hipLaunchKernelGGL((window_grad_kernel<T, D, false>), dim3(queries.size()), dim3(kWindowThreads), 0, stream, c, queries);
+    hipLaunchKernelGGL(by_queries, dim3(queries.size()), dim3(kWindowThreads), (grad_lds<D, false>()), stream, c, queries);
     return check_launch("window_grad_kernel");
 }
 }  // namespace
