@@ -25,6 +25,7 @@ bounded by the kernels and never read on the host.
 from __future__ import annotations
 
 import math
+import struct
 from typing import NamedTuple
 
 import torch
@@ -39,21 +40,34 @@ _MOST = 1 << 30
 def _strided(t: torch.Tensor, align: int = 8) -> torch.Tensor:
     """t itself where its rows (last dim contiguous, starting on 16 bytes) can be
     read where they lie, else a contiguous copy."""
-    strides = t.stride()
-    if t.data_ptr() % 16 == 0 and strides[-1] == 1:
-        for size, stride in zip(t.shape[:-1], strides):
-            if size > 1 and (stride % align or stride < 0):
-                break
-        else:
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
             return t
-    return t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+        strides = t.stride()
+        if strides[-1] == 1 and not any(n > 1 and s % align for n, s in zip(t.shape, strides[:-1])):
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
-def _gpu(name: str, *tensors):
-    device = tensors[0].device
-    if device.type != "cuda" or any(t is not None and t.device != device for t in tensors):
+def _gpu(name: str, first, *others):
+    device = first.device
+    if device.type != "cuda":
         raise ValueError(f"{name} requires tensors on one CUDA device")
+    for t in others:
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} requires tensors on one CUDA device")
     return device
+
+
+def _call(entry: str, device, packed: bytes):
+    with _lib.on(device):
+        _lib.check(_lib.raw(entry)(packed, _lib.raw_stream(device)))
+
+
+_ROTARY, _WINDOW, _APPEND = map(_lib.packer, (_lib.RotaryArgs, _lib.WindowArgs, _lib.AppendArgs))
+_GRAD_REST = struct.Struct("=5Q12q")  # ab_window_grad_args behind its forward part
+_WORKSPACE = struct.Struct("=2Q")     # the last fields of ab_window_args
+_ZERO = (0, 0, 0)
 
 
 # ---- rotary positions ---------------------------------------------------------
@@ -63,19 +77,17 @@ def _rotate(q, k, positions, axes, theta, halves, joint, inverse):
     align = 4 if q.dtype == torch.float32 else 8
     q = _strided(q, align)
     q_out = torch.empty_like(q)
-    k_out = None
+    batch, heads, tokens, dim = q.shape
+    k_out, k_at, k_out_at, k_heads, k_stride, k_out_stride = None, 0, 0, 0, _ZERO, _ZERO
     if k is not None:
         k = _strided(k, align)
         k_out = torch.empty_like(k)
-    batch, heads, tokens, dim = q.shape
-    lib, address = _lib.load(), _lib.address
-    args = _lib.RotaryArgs(address(q), address(k), address(q_out), address(k_out), address(positions), batch, heads,
-                           0 if k is None else k.shape[1], tokens, dim, _DTYPES[q.dtype], q.stride()[:3],
-                           (0, 0, 0) if k is None else k.stride()[:3], q_out.stride()[:3],
-                           (0, 0, 0) if k is None else k_out.stride()[:3], len(axes), axes, theta, joint, halves,
-                           _POSITIONS[positions.dtype], positions.ndim == 3, inverse)
-    with _lib.on(q.device):
-        _lib.check(lib.ab_rotary(args, _lib.stream(q.device)))
+        k_at, k_out_at, k_heads, k_stride, k_out_stride = (k.data_ptr(), k_out.data_ptr(), k.shape[1], k.stride()[:3],
+                                                           k_out.stride()[:3])
+    _call("ab_rotary", q.device, _ROTARY.pack(
+        q.data_ptr(), k_at, q_out.data_ptr(), k_out_at, positions.data_ptr(), batch, heads, k_heads, tokens, dim,
+        _DTYPES[q.dtype], *q.stride()[:3], *k_stride, *q_out.stride()[:3], *k_out_stride, len(axes), *axes,
+        *(0,) * (4 - len(axes)), theta, joint, halves, _POSITIONS[positions.dtype], positions.ndim == 3, inverse))
     return q_out, k_out
 
 
@@ -172,30 +184,30 @@ def _check_window(window, scale, dim):
     return scale
 
 
-def _run(args, entry, device):
+def _run(entry, device, packed):
     """One call with the workspace that it asks for, which lives for the call only."""
-    lib = _lib.load()
     with _lib.on(device):
-        size = lib.ab_window_workspace_bytes(args)
-        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        args.workspace, args.workspace_bytes = _lib.address(workspace), size
-        _lib.check(getattr(lib, entry)(args, _lib.stream(device)))
+        size = _lib.raw("ab_window_workspace_bytes")(packed)
+        if size:
+            workspace = torch.empty(size, dtype=torch.uint8, device=device)
+            packed = packed[:-_WORKSPACE.size] + _WORKSPACE.pack(workspace.data_ptr(), size)
+        _lib.check(_lib.raw(entry)(packed, _lib.raw_stream(device)))
 
 
-def _window_args(q, k, v, out, lse, lengths, window, sinks, frame, scale):
+def _window_args(q, k, v, out, lse, lengths, window, sinks, frame, scale, workspace=0, size=0):
     """The call's ab_window_args of [B, H, N, D] tensors that _strided has seen."""
     batch, heads, tokens, dim = q.shape
-    address = _lib.address
-    return _lib.WindowArgs(address(q), address(k), address(v), address(out), address(lse), address(lengths), None, None, batch,
-                           heads, k.shape[1], tokens, dim, _DTYPES[q.dtype], 0, 0, 0, window, sinks, frame, scale,
-                           q.stride()[:3], k.stride()[:3], v.stride()[:3], out.stride()[:3], None, 0)
+    return _WINDOW.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                        0 if lengths is None else lengths.data_ptr(), 0, 0, batch, heads, k.shape[1], tokens, dim,
+                        _DTYPES[q.dtype], 0, 0, 0, window, sinks, frame, scale, *q.stride()[:3], *k.stride()[:3],
+                        *v.stride()[:3], *out.stride()[:3], workspace, size)
 
 
 def _window_forward(q, k, v, lengths, window, sinks, frame, scale, return_lse):
     out = torch.empty_like(q)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if return_lse else None
+    lse = q.new_empty(q.shape[:3], dtype=torch.float32) if return_lse else None
     if out.numel():
-        _run(_window_args(q, k, v, out, lse, lengths, window, sinks, frame, scale), "ab_window_attention", q.device)
+        _run("ab_window_attention", q.device, _window_args(q, k, v, out, lse, lengths, window, sinks, frame, scale))
     return out, lse
 
 
@@ -219,14 +231,12 @@ class _Window(torch.autograd.Function):
         dlse = None if dlse is None else dlse.contiguous()
         grads = tuple(torch.empty_like(t) for t in (q, k, v))
         if q.numel():
-            address, lib = _lib.address, _lib.load()
-            args = _lib.WindowGradArgs(_window_args(q, k, v, out, lse, lengths, *ctx.how), address(dout), address(dlse),
-                                       *map(address, grads), dout.stride()[:3], *(g.stride()[:3] for g in grads))
-            with _lib.on(q.device):
-                size = lib.ab_window_grad_workspace_bytes(args)
-                workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-                args.forward.workspace, args.forward.workspace_bytes = _lib.address(workspace), size
-                _lib.check(lib.ab_window_attention_grad(args, _lib.stream(q.device)))
+            rest = _GRAD_REST.pack(dout.data_ptr(), 0 if dlse is None else dlse.data_ptr(), *(g.data_ptr() for g in grads),
+                                   *dout.stride()[:3], *(s for g in grads for s in g.stride()[:3]))
+            tensors = (q, k, v, out, lse, lengths, *ctx.how)
+            size = _lib.raw("ab_window_grad_workspace_bytes")(_window_args(*tensors) + rest)
+            workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+            _call("ab_window_attention_grad", q.device, _window_args(*tensors, workspace.data_ptr(), size) + rest)
         return (*grads, *[None] * (1 + len(ctx.how)))
 
 
@@ -246,15 +256,20 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     finite reach the results of the queries that see them only, but may reach any
     gradient of their batch item.
     """
-    if q.ndim != 4 or k.ndim != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
+    if q.ndim != 4 or k.ndim != 4 or k.shape != v.shape:
         raise ValueError("Q [B,H,N,D] and K/V [B,Hk,N,D] must share batch, tokens and dim")
-    if q.shape[-1] not in (64, 128):
+    batch, heads, tokens, dim = q.shape
+    kv_heads = k.shape[1]
+    if k.shape != (batch, kv_heads, tokens, dim):
+        raise ValueError("Q [B,H,N,D] and K/V [B,Hk,N,D] must share batch, tokens and dim")
+    if dim != 128 and dim != 64:
         raise ValueError("window attention requires head_dim 64 or 128")
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype = q.dtype
+    if (dtype != torch.bfloat16 and dtype != torch.float16) or k.dtype != dtype or v.dtype != dtype:
         raise ValueError("window attention requires BF16 or FP16 Q/K/V of one type")
-    if k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
+    if kv_heads == 0 or heads == 0 or heads % kv_heads:
         raise ValueError("the query heads must be a positive multiple of the key heads")
-    scale = _check_window(window, scale, q.shape[-1])
+    scale = _check_window(window, scale, dim)
     window, sinks, frame = _mask(window, sinks, frame)
     if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != q.shape[:1] or not lengths.is_contiguous()):
         raise ValueError("lengths must be int32 [B]")
@@ -282,32 +297,38 @@ class PagedCache(NamedTuple):
     v: torch.Tensor
 
 
-def _check_cache(name, x, heads, cache, page_table, lengths, offsets):
+def _check_cache(name, x, cache, page_table, lengths, offsets):
+    """The checks of packed tokens x and what belongs to a cache; the cache's heads."""
     if x.ndim != 3:
         raise ValueError(f"{name} requires packed tokens [T,H,D]")
-    if cache.k.ndim != 4 or cache.k.shape != cache.v.shape or cache.k.shape[3] != x.shape[2]:
+    heads, dim = x.shape[1], x.shape[2]
+    k, v = cache
+    if k.ndim != 4 or k.shape != v.shape or k.shape[3] != dim:
         raise ValueError("the cache must be two [pages,heads,page tokens,D] tensors with the tokens' D")
-    if x.shape[2] not in (64, 128):
+    if dim != 128 and dim != 64:
         raise ValueError(f"{name} requires head_dim 64 or 128")
-    if x.dtype not in (torch.bfloat16, torch.float16) or cache.k.dtype != x.dtype or cache.v.dtype != x.dtype:
+    dtype = x.dtype
+    if (dtype != torch.bfloat16 and dtype != torch.float16) or k.dtype != dtype or v.dtype != dtype:
         raise ValueError(f"{name} requires BF16 or FP16 tokens and a cache of the same type")
-    if cache.k.shape[2] == 0 or cache.k.shape[2] % 8:
+    _, kv_heads, page, _ = k.shape
+    if page == 0 or page % 8:
         raise ValueError("pages must hold a positive multiple of 8 tokens")
     for t in cache:
-        if t.data_ptr() % 16 or t.stride(3) != 1 or any(n > 1 and s % 8 for n, s in zip(t.shape[:3], t.stride())):
+        if t.data_ptr() % 16 or not (t.is_contiguous() or (
+                t.stride(3) == 1 and not any(n > 1 and s % 8 for n, s in zip(t.shape, t.stride()[:3])))):
             raise ValueError("the cache's rows must be contiguous and start on 16 bytes")
-    if heads == 0 or cache.k.shape[1] == 0 or heads % cache.k.shape[1]:
+    if heads == 0 or kv_heads == 0 or heads % kv_heads:
         raise ValueError("the query heads must be a positive multiple of the cache's heads")
-    batch = page_table.shape[0]
-    if page_table.ndim != 2 or lengths.shape != (batch,) or offsets.shape != (batch + 1,):
+    if page_table.ndim != 2 or lengths.ndim != 1 or offsets.ndim != 1 or not (
+            page_table.shape[0] == lengths.shape[0] == offsets.shape[0] - 1):
         raise ValueError("page_table [B,width], lengths [B] and offsets [B+1] must be of one batch")
     for t in (page_table, lengths, offsets):
         if t.dtype != torch.int32 or not t.is_contiguous():
             raise ValueError("page_table, lengths and offsets must be contiguous int32")
-    return _gpu(name, x, *cache, page_table, lengths, offsets)
+    _gpu(name, x, k, v, page_table, lengths, offsets)
+    return kv_heads
 
 
-@torch.no_grad()
 def append_cache(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
                  offsets: torch.Tensor) -> PagedCache:
     """Writes the new keys and values k, v [T, heads, D] into the cache, in place.
@@ -319,26 +340,18 @@ def append_cache(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table
     """
     if k.shape != v.shape or v.dtype != k.dtype:
         raise ValueError("K and V must be packed tokens [T,H,D] of one shape and type")
-    device = _check_cache("append_cache", k, k.shape[1] if k.ndim == 3 else 0, cache, page_table, lengths, offsets)
-    _gpu("append_cache", k, v)
-    if k.shape[1] != cache.k.shape[1]:
+    if _check_cache("append_cache", k, cache, page_table, lengths, offsets) != k.shape[1]:
         raise ValueError("K and V must have the cache's heads")
+    device = _gpu("append_cache", k, v)
     k, v = _strided(k), _strided(v)
-    lib, address = _lib.load(), _lib.address
     pages, heads, page, dim = cache.k.shape
-
-    def rows(t):
-        return 0, t.stride(1), t.stride(0)
-
-    args = _lib.AppendArgs(address(k), address(v), address(cache.k), address(cache.v), address(lengths), address(offsets),
-                           address(page_table), page_table.shape[0], heads, k.shape[0], dim, pages, page,
-                           page_table.shape[1], rows(k), rows(v), cache.k.stride()[:3], cache.v.stride()[:3])
-    with _lib.on(device):
-        _lib.check(lib.ab_append_cache(args, _lib.stream(device)))
+    _call("ab_append_cache", device, _APPEND.pack(
+        k.data_ptr(), v.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), lengths.data_ptr(), offsets.data_ptr(),
+        page_table.data_ptr(), page_table.shape[0], heads, k.shape[0], dim, pages, page, page_table.shape[1],
+        0, k.stride(1), k.stride(0), 0, v.stride(1), v.stride(0), *cache.k.stride()[:3], *cache.v.stride()[:3]))
     return cache
 
 
-@torch.no_grad()
 def chunk_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tensor,
                     offsets: torch.Tensor, *, window: int | None = None, sinks: int = 0, frame: int = 1,
                     scale: float | None = None, return_lse: bool = False, out: torch.Tensor | None = None):
@@ -354,24 +367,23 @@ def chunk_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
     [T, H]. Rows outside of offsets[0] .. offsets[B] - 1 are not written (with
     ``out``, a tensor of q's shape and type to write to, they stay as they are).
     """
-    device = _check_cache("chunk attention", q, q.shape[1] if q.ndim == 3 else 0, cache, page_table, lengths, offsets)
+    _check_cache("chunk attention", q, cache, page_table, lengths, offsets)
+    device = q.device
     scale = _check_window(window, scale, q.shape[-1])
     window, sinks, frame = _mask(window, sinks, frame)
     q = _strided(q)
     tokens, heads, dim = q.shape
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=device)
+        out = q.new_empty((tokens, heads, dim))
     elif (out.shape != q.shape or out.dtype != q.dtype or out.device != device or out.data_ptr() % 8 or out.stride(2) != 1
           or any(n > 1 and s % 4 for n, s in zip(out.shape[:2], out.stride()))):
         raise ValueError("out must be of Q's shape, type and device, with contiguous rows that start on 8 bytes")
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
+    lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
     if tokens and page_table.shape[0]:
-        address = _lib.address
         pages, kv_heads, page, _ = cache.k.shape
-        args = _lib.WindowArgs(address(q), address(cache.k), address(cache.v), address(out), address(lse),
-                               address(lengths), address(offsets), address(page_table), page_table.shape[0], heads, kv_heads,
-                               tokens, dim, _DTYPES[q.dtype], pages, page, page_table.shape[1], window, sinks, frame, scale,
-                               (0, q.stride(1), q.stride(0)), cache.k.stride()[:3], cache.v.stride()[:3],
-                               (0, out.stride(1), out.stride(0)), None, 0)
-        _run(args, "ab_chunk_attention", device)
+        _run("ab_chunk_attention", device, _WINDOW.pack(
+            q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+            lengths.data_ptr(), offsets.data_ptr(), page_table.data_ptr(), page_table.shape[0], heads, kv_heads, tokens, dim,
+            _DTYPES[q.dtype], pages, page, page_table.shape[1], window, sinks, frame, scale, 0, q.stride(1), q.stride(0),
+            *cache.k.stride()[:3], *cache.v.stride()[:3], 0, out.stride(1), out.stride(0), 0, 0))
     return (out, lse) if return_lse else out
