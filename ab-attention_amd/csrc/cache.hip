@@ -8,6 +8,7 @@ namespace ab {
 namespace {
 
 __global__ __launch_bounds__(256) void append_kernel(AppendCall c) {
+    touch(c.k, c.v, c.k_cache_rows.token, c.v_cache_rows.token, c.table, c.batch);
     const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (row >= c.tokens) return;
     // The sequence: the last one that starts at or before the row.

@@ -8,8 +8,8 @@
 // fraction of a turn in 64 bits (positions of 10^5 and more keep their last
 // bits), their sine and cosine taken in float32, and each result is rounded to
 // its type once. Every thread holds the sines of one token's few pairs and
-// walks over heads of Q, then of K, so that their cost (about 400 instructions)
-// is shared by the heads; what bounds the kernel is reading and writing the rows.
+// walks over heads of Q, then of K, so that their cost (some 250 instructions) is
+// shared by the heads; what bounds the kernel is reading and writing the rows.
 #include <algorithm>
 
 #include "rotary.hpp"
@@ -57,26 +57,44 @@ struct Values<F32> {
     static constexpr int kBytes = 4;
 };
 
-// Sine and cosine of pair `i` at a token's positions.
-__device__ __forceinline__ void turn(const RotaryCall& c, int64_t token, int i, float& s, float& co) {
-    int axis = 0, first = 0;
+// Sines and cosines of kPairs pairs from `first` on at a token's positions, those at
+// `end` and behind it left as they are. The frequency of the first one is an
+// exponential; its neighbours' follow by the axis' ratio, a rounding of 2^-53 each.
+template <int kPairs>
+__device__ __forceinline__ void turns(const RotaryCall& c, int64_t token, int first, int end, float (&s)[kPairs], float (&co)[kPairs]) {
+    int axis = 0, begin = 0;  // the first pair's axis, and that axis' first pair
 #pragma unroll
     for (int a = 0; a < kMaxAxes - 1; ++a) {
         const int pairs = c.pairs[a];
-        if (axis == a && a < c.axes - 1 && i - first >= pairs) {
+        if (axis == a && a < c.axes - 1 && first - begin >= pairs) {
             ++axis;
-            first += pairs;
+            begin += pairs;
         }
     }
-    const int64_t at = token * c.axes + axis;
-    const double p = c.position_kind == 0   ? static_cast<double>(static_cast<const int32_t*>(c.positions)[at])
-                     : c.position_kind == 1 ? static_cast<double>(static_cast<const int64_t*>(c.positions)[at])
-                                            : static_cast<double>(static_cast<const float*>(c.positions)[at]);
-    const double step = c.joint ? c.step[0] * i : c.step[axis] * (i - first);  // -log2 of the frequency
-    const double turns = p * exp2(-step) * 0.15915494309189533577;             // 1 / (2 pi)
-    const float f = static_cast<float>(2.0 * (turns - rint(turns)));
-    sincospif(f, &s, &co);
-    s *= c.sign;
+    auto position = [&](int a) {
+        const int64_t at = token * c.axes + a;
+        return c.position_kind == 0   ? static_cast<double>(static_cast<const int32_t*>(c.positions)[at])
+               : c.position_kind == 1 ? static_cast<double>(static_cast<const int64_t*>(c.positions)[at])
+                                      : static_cast<double>(static_cast<const float*>(c.positions)[at]);
+    };
+    double p = position(axis) * 0.15915494309189533577;  // 1 / (2 pi): turns at frequency 1
+    double frequency = exp2(-(c.joint ? c.step[0] * first : c.step[axis] * (first - begin)));
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+        if (first + i >= end) break;
+        if (i > 0) {
+            if (axis < c.axes - 1 && first + i - begin >= c.pairs[axis]) {
+                begin += c.pairs[axis];
+                p = position(++axis) * 0.15915494309189533577;
+                frequency = c.joint ? frequency * c.ratio[0] : 1.0;
+            } else {
+                frequency *= c.ratio[c.joint ? 0 : axis];
+            }
+        }
+        const double turns = p * frequency;
+        sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s[i], &co[i]);
+        s[i] *= c.sign;
+    }
 }
 
 // Thread: one unit of one token. Adjacent pairs: eight values, four pairs.
@@ -84,6 +102,7 @@ __device__ __forceinline__ void turn(const RotaryCall& c, int64_t token, int i, 
 template <class T, bool kHalves>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryCall c) {
     using V = Values<T>;
+    touch(c.in[0], c.out_rows[0].token, c.positions, c.heads[0], c.units, c.per_batch);
     const uint32_t g = blockIdx.x * kThreads + threadIdx.x;
     const uint32_t units = c.units;
     const uint32_t token = g / units, unit = g - token * units;  // token of all batch items
@@ -94,25 +113,16 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryCall c) {
     const bool copied = kHalves ? static_cast<int>(unit) * kUnit >= half : static_cast<int>(unit) * kUnit >= c.turned;
     const int at = kHalves && copied ? c.turned + (unit * kUnit - half) : unit * kUnit;
 
-    constexpr int kPairs = kHalves ? 8 : 4;
-    float s[kPairs], co[kPairs];
-#pragma unroll
-    for (int i = 0; i < kPairs; ++i) {
-        s[i] = 0.f;
-        co[i] = 1.f;
-        const int pair = kHalves ? at + i : at / 2 + i;
-        if (!copied && pair < half) turn(c, c.per_batch ? token : t, pair, s[i], co[i]);
-    }
-
-    // Heads of Q and K as one list; this workgroup's are from `head0` on.
+    // Heads of Q and K as one list; this workgroup's are from `head0` on. kAhead rows
+    // are read before the first is written, the first ones before the sines are made.
     const int heads = c.heads[0] + c.heads[1];
     const int head0 = blockIdx.y * c.heads_each, head1 = min(head0 + c.heads_each, heads);
     auto place = [&](const Rows& r, int tensor, int h) {
         return (b * r.batch + (h - (tensor ? c.heads[0] : 0)) * r.head + t * r.token + at) * V::kBytes;
     };
-    constexpr int kAhead = 4;  // rows read before the first is written
-    for (int h0 = head0; h0 < head1; h0 += kAhead) {
-        float x[kAhead][kUnit], y[kHalves ? kAhead : 1][kUnit];
+    constexpr int kAhead = 4;
+    float x[kAhead][kUnit], y[kHalves ? kAhead : 1][kUnit];
+    auto read = [&](int h0) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int h = min(h0 + i, head1 - 1), k = h >= c.heads[0];
@@ -121,6 +131,15 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryCall c) {
             if constexpr (kHalves)
                 if (!copied) V::load(src + half * V::kBytes, y[i]);
         }
+    };
+    read(head0);
+
+    constexpr int kPairs = kHalves ? 8 : 4;
+    float s[kPairs] = {}, co[kPairs] = {};
+    if (!copied) turns<kPairs>(c, c.per_batch ? token : t, kHalves ? at : at / 2, half, s, co);
+
+    for (int h0 = head0; h0 < head1; h0 += kAhead) {
+        if (h0 > head0) read(h0);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int h = h0 + i, k = h >= c.heads[0];

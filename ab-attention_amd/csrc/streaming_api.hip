@@ -197,8 +197,10 @@ int ab_rotary(const ab_rotary_args* a, void* stream) {
     c.out[1] = a->k_out;
     c.positions = a->positions;
     c.axes = static_cast<int32_t>(a->axes);
-    for (int i = 0; i < a->axes; ++i)
+    for (int i = 0; i < a->axes; ++i) {
         c.step[i] = std::log2(a->theta) * 2.0 / double(a->joint ? turned : a->axis_dims[i]);
+        c.ratio[i] = std::exp2(-c.step[i]);
+    }
     c.heads[0] = static_cast<int32_t>(a->heads);
     c.heads[1] = static_cast<int32_t>(kv_heads);
     c.position_kind = static_cast<int32_t>(a->position_type);

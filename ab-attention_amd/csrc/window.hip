@@ -108,6 +108,7 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     using Tile = WindowTile<T, D>;
     constexpr int kSteps = Tile::kSteps, kBlocks = Tile::kBlocks, kOps = Tile::kOps;
     extern __shared__ __align__(16) unsigned char smem[];
+    touch(c.q, c.k_rows.batch, c.row.batch, c.lengths, c.rows, places.heads);
 
     WindowUnit u;
     if (!window_unit<kPaged>(c, places, blockIdx.x, u)) return;

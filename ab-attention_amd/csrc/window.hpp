@@ -116,6 +116,14 @@ __device__ __forceinline__ void buffer_to_lds(u32x4 buffer, uint32_t offset0, ui
 }
 #pragma clang diagnostic pop
 
+// The first thing each of these kernels does: a value from every 64-byte line of
+// its arguments (in host memory) at once, so that the lines arrive together and not
+// one after the other where the compiler first needs them.
+template <class A, class B, class C, class D, class E, class F>
+__device__ __forceinline__ void touch(A a, B b, C c, D d, E e, F f) {
+    asm volatile("" ::"s"(a), "s"(b), "s"(c), "s"(d), "s"(e), "s"(f));
+}
+
 // At most N of this wave's vector memory operations still in flight, none of
 // its LDS ones; then a workgroup barrier that the compiler moves no memory
 // access across.

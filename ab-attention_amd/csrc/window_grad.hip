@@ -96,6 +96,7 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
     // Four stages of Y1, four of Y2, and each wave's copy of the streamed rows' stat.
     constexpr int kY2 = kStages * kBytes, kStat = 2 * kStages * kBytes;
     extern __shared__ __align__(16) unsigned char smem[];
+    touch(c.q, c.k_rows.batch, c.out_rows.batch, c.dq_rows.batch, c.lengths, c.partial);
 
     // Owned rows. Of keys, the sinks' tiles come first, part by part: `places` are
     // the tiles behind them.
