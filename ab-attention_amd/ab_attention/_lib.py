@@ -65,8 +65,8 @@ class RotaryArgs(ctypes.Structure):
 class WindowArgs(ctypes.Structure):
     """ab_window_args of include/ab_attention.h."""
 
-    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("out", _P), ("lse", _P), ("lengths", _P), ("offsets", _P),
-                ("page_table", _P), ("batch", _I64), ("heads", _I64), ("kv_heads", _I64), ("tokens", _I64), ("dim", _I64),
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("out", _P), ("out_rest", _P), ("lse", _P), ("lengths", _P),
+                ("offsets", _P), ("page_table", _P), ("batch", _I64), ("heads", _I64), ("kv_heads", _I64), ("tokens", _I64), ("dim", _I64),
                 ("dtype", _I64), ("pages", _I64), ("page_tokens", _I64), ("table_width", _I64), ("window", _I64),
                 ("sinks", _I64), ("frame", _I64), ("scale", ctypes.c_double), ("q_stride", _I64 * 3),
                 ("k_stride", _I64 * 3), ("v_stride", _I64 * 3), ("out_stride", _I64 * 3), ("workspace", _P),

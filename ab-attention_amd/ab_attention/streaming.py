@@ -194,20 +194,20 @@ def _run(entry, device, packed):
         _lib.check(_lib.raw(entry)(packed, _lib.raw_stream(device)))
 
 
-def _window_args(q, k, v, out, lse, lengths, window, sinks, frame, scale, workspace=0, size=0):
+def _window_args(q, k, v, out, rest, lse, lengths, window, sinks, frame, scale, workspace=0, size=0):
     """The call's ab_window_args of [B, H, N, D] tensors that _strided has seen."""
     batch, heads, tokens, dim = q.shape
-    return _WINDOW.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-                        0 if lengths is None else lengths.data_ptr(), 0, 0, batch, heads, k.shape[1], tokens, dim,
+    return _WINDOW.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if rest is None else rest.data_ptr(),
+                        0 if lse is None else lse.data_ptr(), 0 if lengths is None else lengths.data_ptr(), 0, 0, batch, heads, k.shape[1], tokens, dim,
                         _DTYPES[q.dtype], 0, 0, 0, window, sinks, frame, scale, *q.stride()[:3], *k.stride()[:3],
                         *v.stride()[:3], *out.stride()[:3], workspace, size)
 
 
-def _window_forward(q, k, v, lengths, window, sinks, frame, scale, return_lse):
+def _window_forward(q, k, v, lengths, window, sinks, frame, scale, return_lse, rest=None):
     out = torch.empty_like(q)
     lse = q.new_empty(q.shape[:3], dtype=torch.float32) if return_lse else None
     if out.numel():
-        _run("ab_window_attention", q.device, _window_args(q, k, v, out, lse, lengths, window, sinks, frame, scale))
+        _run("ab_window_attention", q.device, _window_args(q, k, v, out, rest, lse, lengths, window, sinks, frame, scale))
     return out, lse
 
 
@@ -215,8 +215,9 @@ class _Window(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, *how):
         q, k, v = _strided(q), _strided(k), _strided(v)
-        out, lse = _window_forward(q, k, v, lengths, *how, True)
-        ctx.save_for_backward(q, k, v, out, lse, lengths)
+        rest = torch.empty_like(q)  # what out's rounding takes: delta is made of both
+        out, lse = _window_forward(q, k, v, lengths, *how, True, rest)
+        ctx.save_for_backward(q, k, v, out, rest, lse, lengths)
         ctx.how = how
         ctx.set_materialize_grads(False)
         return out, lse
@@ -224,19 +225,19 @@ class _Window(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dlse):
-        q, k, v, out, lse, lengths = ctx.saved_tensors
+        q, k, v, out, rest, lse, lengths = ctx.saved_tensors
         if dout is None and dlse is None:
             return (None,) * (4 + len(ctx.how))
         dout = torch.zeros_like(out) if dout is None else _strided(dout)
         dlse = None if dlse is None else dlse.contiguous()
         grads = tuple(torch.empty_like(t) for t in (q, k, v))
         if q.numel():
-            rest = _GRAD_REST.pack(dout.data_ptr(), 0 if dlse is None else dlse.data_ptr(), *(g.data_ptr() for g in grads),
-                                   *dout.stride()[:3], *(s for g in grads for s in g.stride()[:3]))
-            tensors = (q, k, v, out, lse, lengths, *ctx.how)
-            size = _lib.raw("ab_window_grad_workspace_bytes")(_window_args(*tensors) + rest)
+            behind = _GRAD_REST.pack(dout.data_ptr(), 0 if dlse is None else dlse.data_ptr(), *(g.data_ptr() for g in grads),
+                                     *dout.stride()[:3], *(s for g in grads for s in g.stride()[:3]))
+            tensors = (q, k, v, out, rest, lse, lengths, *ctx.how)
+            size = _lib.raw("ab_window_grad_workspace_bytes")(_window_args(*tensors) + behind)
             workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-            _call("ab_window_attention_grad", q.device, _window_args(*tensors, workspace.data_ptr(), size) + rest)
+            _call("ab_window_attention_grad", q.device, _window_args(*tensors, workspace.data_ptr(), size) + behind)
         return (*grads, *[None] * (1 + len(ctx.how)))
 
 
@@ -382,7 +383,7 @@ def chunk_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
     if tokens and page_table.shape[0]:
         pages, kv_heads, page, _ = cache.k.shape
         _run("ab_chunk_attention", device, _WINDOW.pack(
-            q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+            q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), out.data_ptr(), 0, 0 if lse is None else lse.data_ptr(),
             lengths.data_ptr(), offsets.data_ptr(), page_table.data_ptr(), page_table.shape[0], heads, kv_heads, tokens, dim,
             _DTYPES[q.dtype], pages, page, page_table.shape[1], window, sinks, frame, scale, 0, q.stride(1), q.stride(0),
             *cache.k.stride()[:3], *cache.v.stride()[:3], 0, out.stride(1), out.stride(0), 0, 0))

@@ -81,6 +81,7 @@ int window_call(const char* what, const ab_window_args& a, bool paged, WindowCal
     c.k = a.k;
     c.v = a.v;
     c.out = a.out;
+    c.out_rest = a.out_rest;
     c.lse = a.lse;
     c.batch = static_cast<int32_t>(a.batch);
     c.heads = static_cast<int32_t>(a.heads);
@@ -139,7 +140,7 @@ int window_launch(const char* what, const ab_window_args* a, bool paged, void* s
     if (a->batch == 0 || a->tokens == 0) return AB_OK;
     const bool no_cache = paged && (a->pages == 0 || a->table_width == 0);
     if (!a->q || !a->out || (!no_cache && (!a->k || !a->v))) return set_error(AB_ERR_INVALID, "%s: null pointer", what);
-    if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->out, 8))
+    if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->out, 8) || !aligned(a->out_rest, 8))
         return set_error(AB_ERR_INVALID, "%s: q/k/v must be 16-byte and out 8-byte aligned", what);
     if (!a->workspace) c.parts = 1;
     if (c.parts > 1) {
@@ -241,6 +242,7 @@ int grad_call(const ab_window_grad_args& a, WindowGradCall& g, int64_t& stat, in
     g.k = f.k;
     g.v = f.v;
     g.out = f.out;
+    g.out_rest = f.out_rest;
     g.dout = a.dout;
     g.lse = f.lse;
     g.dlse = a.dlse;
@@ -297,6 +299,7 @@ int ab_window_attention_grad(const ab_window_grad_args* a, void* stream) {
         if (!aligned(p, 16)) return set_error(AB_ERR_INVALID, "%s: tensors must be 16-byte aligned", what);
     }
     if (!f.lse) return set_error(AB_ERR_INVALID, "%s: null pointer", what);
+    if (!aligned(f.out_rest, 16)) return set_error(AB_ERR_INVALID, "%s: tensors must be 16-byte aligned", what);
     if (f.workspace_bytes < size_t(stat + partial) * sizeof(float))
         return set_error(AB_ERR_INVALID, "%s: workspace of %zu bytes is smaller than the %zu required", what, f.workspace_bytes,
                          size_t(stat + partial) * sizeof(float));

@@ -82,6 +82,14 @@ struct WindowTile {
     static constexpr int kLdsBytes = kVotes + 16;
 };
 
+// What rounding two values to `rounded` took from them, rounded itself (nothing of
+// values that are not finite).
+template <class T>
+__device__ __forceinline__ uint32_t rest_of(float a, float b, uint32_t rounded) {
+    const float x = a - T::lo(rounded), y = b - T::hi(rounded);
+    return T::pack(fabsf(x) < INFINITY ? x : 0.f, fabsf(y) < INFINITY ? y : 0.f);
+}
+
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 // v_max_f32 without the NaN quieting that the compiler adds around fmaxf.
@@ -633,9 +641,12 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
                              int64_t(u.off + token) * c.out_rows.token + 4 * lg;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
-                const u32x2 w = {T::pack(o_acc[b][j][0] * inv, o_acc[b][j][1] * inv),
-                                 T::pack(o_acc[b][j][2] * inv, o_acc[b][j][3] * inv)};
+                const f32x4 o = o_acc[b][j] * inv;
+                const u32x2 w = {T::pack(o[0], o[1]), T::pack(o[2], o[3])};
                 *reinterpret_cast<u32x2*>(orow + 16 * b) = w;
+                if (c.out_rest)
+                    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(c.out_rest) + (orow - static_cast<uint16_t*>(c.out)) + 16 * b) =
+                        u32x2{rest_of<T>(o[0], o[1], w[0]), rest_of<T>(o[2], o[3], w[1])};
             }
             if (c.lse && lg == 0) c.lse[stat_at] = l == 0.f ? -INFINITY : m_run[j] + log2f(l);
         }
@@ -672,11 +683,17 @@ __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
         for (int i = 0; i < D / 64; ++i) o[i] += w * src[i];
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
-    uint16_t* dst = static_cast<uint16_t*>(c.out) + out_at + lane * (D / 64);
-    if constexpr (D == 128)
-        *reinterpret_cast<uint32_t*>(dst) = T::pack(o[0] * inv, o[1] * inv);
-    else
-        *dst = static_cast<uint16_t>(T::pack(o[0] * inv, 0.f));
+    const int64_t at = out_at + lane * (D / 64);
+    const float first = o[0] * inv, second = D == 128 ? o[D / 64 - 1] * inv : 0.f;
+    const uint32_t w = T::pack(first, second), rest = rest_of<T>(first, second, w);
+    auto store = [&](void* to, uint32_t value) {
+        if constexpr (D == 128)
+            *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(to) + at) = value;
+        else
+            static_cast<uint16_t*>(to)[at] = static_cast<uint16_t>(value);
+    };
+    store(c.out, w);
+    if (c.out_rest) store(c.out_rest, rest);
     if (c.lse && lane == 0) c.lse[row] = l == 0.f ? -INFINITY : m + log2f(l);
 }
 

@@ -146,7 +146,7 @@ struct Rows {
 // offsets[b] .. offsets[b + 1]. `row` gives the place of a query's normaliser.
 struct WindowCall {
     const void *q, *k, *v;
-    void* out;
+    void *out, *out_rest;  // out_rest: what out's rounding took, or none
     float* lse;
     Rows q_rows, k_rows, v_rows, out_rows, row;
     int32_t batch, heads, kv_heads, tokens;  // tokens: of a batch item, or packed rows in all
@@ -166,7 +166,7 @@ struct WindowCall {
 // One call of the backward pass over strided tensors. `stat` holds, for every
 // 32 queries of a head, their 32 normalisers and 32 values of -delta.
 struct WindowGradCall {
-    const void *q, *k, *v, *out, *dout;
+    const void *q, *k, *v, *out, *out_rest, *dout;  // out_rest: or none
     const float *lse, *dlse;  // dlse: of the normalisers, or none
     void *dq, *dk, *dv;
     Rows q_rows, k_rows, v_rows, out_rows, dout_rows, dq_rows, dk_rows, dv_rows;

@@ -284,13 +284,15 @@ int ab_rotary(const ab_rotary_args *args, void *stream);
  *   [0, pages) is no page: its keys are not seen. Rows before offsets[0] and from
  *   offsets[batch] on are left as they are. lse f32 [tokens, heads].
  *
+ * out_rest (NULL, or of out's strides and type) gets what out's rounding took from
+ * the result, rounded itself: ab_window_attention_grad makes its delta of the two.
  * Strides in elements, multiples of 8 (out: of 4); q, k, v 16-byte aligned, out 8.
  * Limits: tokens and positions under 2^30, a head of k or v (of a page) under 4 GiB.
  * Calls that leave CUs idle split their keys over workgroups with a workspace of
  * ab_window_workspace_bytes(args) (0: none needed; NULL: never split). */
 typedef struct ab_window_args {
     const void *q, *k, *v;
-    void *out;
+    void *out, *out_rest;
     float *lse;
     const int32_t *lengths, *offsets, *page_table;
     int64_t batch, heads, kv_heads, tokens, dim, dtype;
@@ -306,7 +308,8 @@ int ab_window_attention(const ab_window_args *args, void *stream);
 int ab_chunk_attention(const ab_window_args *args, void *stream);
 
 /* The gradient of ab_window_attention. forward: that call's arguments with its out
- * and lse (not NULL); its workspace fields are this call's, of
+ * and lse (not NULL), and out_rest if it made one (without it the gradients of q and k
+ * carry out's rounding too); its workspace fields are this call's, of
  * ab_window_grad_workspace_bytes(args) bytes, 16-byte aligned, never 0 where there
  * are tokens. dout is out's gradient, dlse (or NULL) lse's. Writes all of dq, dk and dv, of
  * q's, k's and v's shapes and type (0 for the tokens behind a length); gradients of
