@@ -388,3 +388,103 @@ def chunk_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
             _DTYPES[q.dtype], pages, page, page_table.shape[1], window, sinks, frame, scale, 0, q.stride(1), q.stride(0),
             *cache.k.stride()[:3], *cache.v.stride()[:3], 0, out.stride(1), out.stride(0), 0, 0))
     return (out, lse) if return_lse else out
+
+
+class StreamingAttention:
+    """The attention layers of a transformer that makes several videos (or texts)
+    chunk by chunk: their paged caches, and one page table for all of them.
+
+    A step is ``begin(new)``, with the new tokens of every sequence (0 for one that
+    pauses), then in every layer ``attend(layer, q, k, v, positions)``. Pages are
+    given out on the host as sequences grow, given back when no later query can see
+    any of their tokens (behind the window, not among the sinks), and by
+    ``finish(sequence)``. ``pages`` is how many there are in each layer's cache;
+    ``begin`` raises ValueError, and changes nothing, when they do not suffice.
+
+    ``axes`` (with theta, pairing and joint) turns Q and K by ``rotary``; without it
+    they are used as they come.
+    """
+
+    def __init__(self, layers: int, sequences: int, heads: int, pages: int, page_tokens: int, *, dim: int = 128,
+                 window: int | None = None, sinks: int = 0, frame: int = 1, axes=None, theta: float = 10000.0,
+                 pairing: str = "adjacent", joint: bool = False, scale: float | None = None, dtype=torch.bfloat16,
+                 device="cuda"):
+        if layers < 1 or sequences < 1 or heads < 1 or pages < 1:
+            raise ValueError("layers, sequences, heads and pages must be positive")
+        if page_tokens < 8 or page_tokens % 8:
+            raise ValueError("pages must hold a positive multiple of 8 tokens")
+        if dim not in (64, 128) or dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("streaming attention requires head_dim 64 or 128 in BF16 or FP16")
+        self.scale = _check_window(window, scale, dim)
+        _, self.sinks, self.frame = _mask(window, sinks, frame)
+        self.window = window
+        self.axes, self.turn = axes, dict(theta=theta, pairing=pairing, joint=joint)
+        self.page_tokens, self.device = page_tokens, torch.device(device)
+        shape = (pages, heads, page_tokens, dim)
+        self.caches = [PagedCache(*(torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(2)))
+                       for _ in range(layers)]
+        self.free = list(range(pages - 1, -1, -1))
+        self.tokens = [0] * sequences    # of each sequence, with those of the step that began last
+        self.held = [{} for _ in range(sequences)]  # of each sequence: place in its table -> page
+        self.page_table = self.lengths = self.offsets = None
+
+    def _behind(self, first: int) -> range:
+        """The places of a sequence's table that queries from position ``first`` on do not see."""
+        if self.window is None:
+            return range(0)
+        low = max(0, first // self.frame - int(self.window) + 1) * self.frame
+        sinks = min(self.sinks * self.frame, low)
+        return range(-(-sinks // self.page_tokens), low // self.page_tokens)
+
+    def begin(self, new) -> None:
+        """Starts a step of new[s] more tokens in sequence s."""
+        new = [int(n) for n in new]
+        if len(new) != len(self.tokens) or min(new) < 0:
+            raise ValueError(f"new must give the new tokens of {len(self.tokens)} sequences")
+        total = [t + n for t, n in zip(self.tokens, new)]
+        gone, wanted = [], []
+        for s, (n, length) in enumerate(zip(new, total)):
+            behind = self._behind(length - n)
+            if n:
+                gone += [(s, i) for i in self.held[s] if i in behind]
+                wanted += [(s, i) for i in range((length - n) // self.page_tokens, -(-length // self.page_tokens))
+                           if i not in self.held[s]]
+        if len(wanted) > len(self.free) + len(gone):
+            raise ValueError(f"{len(wanted)} more pages are needed, {len(self.free) + len(gone)} are free")
+        for s, i in gone:
+            self.free.append(self.held[s].pop(i))
+        for s, i in wanted:
+            self.held[s][i] = self.free.pop()
+        self.tokens = total
+        width = max(1, max(-(-length // self.page_tokens) for length in total))
+        table = [[-1] * width for _ in total]
+        for row, held in zip(table, self.held):
+            for i, page in held.items():
+                row[i] = page
+        offsets = [0]
+        for n in new:
+            offsets.append(offsets[-1] + n)
+        self.page_table, self.lengths, self.offsets = (
+            torch.tensor(values, dtype=torch.int32, pin_memory=True).to(self.device, non_blocking=True)
+            for values in (table, total, offsets))
+
+    def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor | None = None, *,
+               return_lse: bool = False):
+        """The layer's attention of the step's new tokens, packed one sequence behind the
+        other: q [T, H, D], k and v [T, heads, D]; positions [T, axes] where axes were
+        given. Returns o [T, H, D] (and lse [T, H])."""
+        if self.offsets is None:
+            raise ValueError("attend comes after begin")
+        if self.axes is not None:
+            if positions is None:
+                raise ValueError("positions are needed to turn Q and K")
+            q, k = (t[0].transpose(0, 1) for t in rotary(*(t.transpose(0, 1)[None] for t in (q, k)), positions, self.axes, **self.turn))
+        cache = append_cache(self.caches[layer], k, v, self.page_table, self.lengths, self.offsets)
+        return chunk_attention(q, cache, self.page_table, self.lengths, self.offsets, window=self.window, sinks=self.sinks,
+                               frame=self.frame, scale=self.scale, return_lse=return_lse)
+
+    def finish(self, sequence: int) -> None:
+        """Gives a sequence's pages back; it starts again at position 0."""
+        self.free += self.held[sequence].values()
+        self.held[sequence] = {}
+        self.tokens[sequence] = 0

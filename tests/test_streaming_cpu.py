@@ -5,7 +5,8 @@ import pytest
 import torch
 
 from ab_attention import _lib
-from ab_attention.streaming import PagedCache, append_cache, chunk_attention, rotary, window_attention
+from ab_attention.streaming import (PagedCache, StreamingAttention, append_cache, chunk_attention, rotary,
+                                    window_attention)
 
 BF16 = torch.bfloat16
 
@@ -187,3 +188,41 @@ def test_gradient_workspace():
     assert plain == 2 * 32 * 64 * 4
     sinks = lib.ab_window_grad_workspace_bytes(_grad_args(tokens=1024, window=100, sinks=4, **strides))
     assert (sinks - plain) % (2 * 128 * 64 * 4) == 0 and sinks > plain
+
+
+@pytest.mark.parametrize("change,msg", [(dict(layers=0), "positive"), (dict(pages=0), "positive"), (dict(page_tokens=12), "multiple of 8"),
+                                        (dict(dim=96), "64 or 128"), (dict(dtype=torch.float32), "BF16"), (dict(window=0), "window"),
+                                        (dict(frame=0), "frame"), (dict(sinks=-1), "sinks")])
+def test_streaming_attention_refuses(change, msg):
+    how = dict(layers=1, sequences=1, heads=1, pages=2, page_tokens=16, device="cpu")
+    how.update(change)
+    with pytest.raises(ValueError, match=msg):
+        StreamingAttention(**how)
+
+
+def test_streaming_attention_needs_a_step_and_positions():
+    stream = StreamingAttention(1, 1, 1, 2, 16, dim=64, device="cpu", axes=(64,))
+    x = _z(3, 1, 64)
+    with pytest.raises(ValueError, match="begin"):
+        stream.attend(0, x, x, x)
+    stream.offsets = _OFFSETS
+    with pytest.raises(ValueError, match="positions"):
+        stream.attend(0, x, x, x)
+
+
+def test_pages_behind_the_window():
+    """Pages go back when none of their tokens can be seen again, whatever the sizes of frames and pages."""
+    from streaming_reference import seen_mask
+
+    for window, sinks, frame, page in ((3, 1, 10, 8), (1, 0, 7, 16), (40, 5, 1, 8), (2, 2, 24, 8), (2, 1, 8, 24)):
+        stream = StreamingAttention(1, 1, 1, 2, page, dim=64, window=window, sinks=sinks, frame=frame, device="cpu")
+        keys = torch.arange(400)
+        for first in (0, 1, 39, 40, 41, 200, 399):
+            seen = seen_mask(torch.arange(first, 400), keys, window, sinks, frame).any(0)
+            behind = stream._behind(first)
+            for i in range(400 // page):
+                inside = seen[i * page:(i + 1) * page]
+                if i in behind:
+                    assert not inside.any()
+                elif (i + 1) * page <= first // frame * frame:  # a page of the past that is kept holds something to see
+                    assert inside.any(), (window, sinks, frame, page, first, i)
