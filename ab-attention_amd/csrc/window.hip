@@ -151,15 +151,22 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     // Q as the B operand of S^T = K Q^T: row 16j + li, dims 32s + 8lg .. + 7. The
     // row's own bounds; all zero for a row without keys.
     u32x4 bq[2][kSteps];
+    auto read_q = [&]() {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            int token, head;
+            row_of(j, token, head);
+            const uint16_t* qrow = static_cast<const uint16_t*>(c.q) + u.b * c.q_rows.batch + head * c.q_rows.head +
+                                   int64_t(u.off + token) * c.q_rows.token + 8 * lg;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) bq[j][s] = *reinterpret_cast<const u32x4*>(qrow + 32 * s);
+        }
+    };
     int low[2], seen[2], sink[2];  // keys low .. low + seen - 1 and 0 .. sink - 1
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         int token, head;
         const bool stored = row_of(j, token, head);
-        const uint16_t* qrow = static_cast<const uint16_t*>(c.q) + u.b * c.q_rows.batch + head * c.q_rows.head +
-                               int64_t(u.off + token) * c.q_rows.token + 8 * lg;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) bq[j][s] = *reinterpret_cast<const u32x4*>(qrow + 32 * s);
         const int p = u.first + token;
         const bool sees = stored && p >= 0 && p < u.length;
         const int high = mask.high(max(p, 0), u.length);
@@ -375,9 +382,10 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     // Moves the reference of the rows whose maximum has risen by more than kSlack
     // above it (or that have none yet): their sums, and the logits at hand, follow.
     auto move_reference = [&](f32x4 (&s)[4], float (&mx)[2]) {
+        // A lane's own keys show it: no exchange while nothing grows.
+        if (!__any(mx[0] > slack[0] || mx[1] > slack[1])) return;
         max_over_rows(mx[0], mx[1]);
         const bool grow0 = mx[0] > slack[0], grow1 = mx[1] > slack[1];
-        if (!__any(grow0 || grow1)) return;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const bool grow = j ? grow1 : grow0;
@@ -489,7 +497,6 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
         // K(0 .. 3) and V(0 .. 2); S(0) and K(1) to registers once K(0) and K(1) are
         // in; K(4) goes to K(0)'s place only after every wave has read that. The last
         // transfers before step 0 are then K(3), V(1), V(2), K(4), as its wait expects.
-        landed_and_barrier<0>();
         {
             first_place();
             const Place p0 = ask_place(), p1 = ask_place(), p2 = ask_place();
@@ -502,6 +509,7 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
             move_v(1, p1);
             move_v(2, p2);
         }
+        if (active) read_q();  // behind the transfers, not before them
         mp = ask_place();
         kp = ask_place();
         f32x4 s0[4], s1[4];
@@ -523,7 +531,9 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
                 }
             if (is_masked(0)) mask_logits(0, s0, mx);
         }
-        landed_and_barrier<63>();  // every wave's reads of K(0) are done
+        // Every wave's reads of K(0) are done. Q, asked for last, is here, and with it
+        // all transfers; said to the compiler too, which else waits for Q in the loop.
+        landed_and_barrier<0>();
         move_k(4, mp);
         int t = 0;
         for (; t + 3 < tiles; t += 4) {
