@@ -11,6 +11,7 @@
 // heads that share keys read them once. It visits only tiles of 32 keys that
 // some of its rows see: the sinks' tiles, then the window's.
 #include <algorithm>
+#include <initializer_list>
 
 #include "window.hpp"
 
@@ -44,26 +45,54 @@ __device__ __forceinline__ bool window_unit(const WindowCall& c, const WindowGri
         u.length = c.lengths ? min(max(c.lengths[u.b], 0), c.tokens) : c.tokens;
         return true;
     } else {
-        // Sequence b's tiles take the slots from offsets[b] * group / 128 + b on:
-        // never fewer than it needs, so no sum over the sequences is wanted.
-        int slot;
-        grid.place(id, head, slot);
-        u.kv_head = head;
-        u.head = head * c.group.d;
+        int head, slot;
         const int lane = threadIdx.x & 63;
-        int before = 0;
-        for (int at = 0; at < c.batch; at += 64) {
-            const int b = min(at + lane, c.batch - 1);
-            const int64_t start = int64_t(min(max(c.offsets[b], 0), c.tokens)) * c.group.d / kWindowRows + b;
-            before += __popcll(__ballot(at + lane < c.batch && start <= slot));
+        const int group = static_cast<int>(c.group.d), tokens = c.tokens;
+        if (c.batch <= 64) {
+            // Lane b looks at sequence b. The tiles of the sequences with the most
+            // visible keys come first, over all heads: each adds up the tiles of those
+            // before it (12 sequences of 1 to 1,111 new tokens over 1,668 to 9,000: 383
+            // us in the order of their rows, 303 so).
+            slot = id / c.kv_heads;
+            head = id - slot * c.kv_heads;
+            const int b = min(lane, c.batch - 1);
+            const int off = min(max(c.offsets[b], 0), tokens), n = lane < c.batch ? min(max(c.offsets[b + 1], 0), tokens) - off : 0;
+            const int tiles = n > 0 ? static_cast<int>((int64_t(n) * group + kWindowRows - 1) / kWindowRows) : 0;
+            const int length = static_cast<int>(min(int64_t(max(c.lengths[b], 0)), int64_t(c.table_width) * c.page.d));
+            const int cost = n > 0 ? static_cast<int>(min(int64_t(length), int64_t(c.mask.back) + c.mask.frame.d + c.mask.sinks)) : -1;
+            int start = 0;
+            for (int j = 0; j < c.batch; ++j) {
+                const int other = __builtin_amdgcn_readlane(cost, j), its = __builtin_amdgcn_readlane(tiles, j);
+                start += other > cost || (other == cost && j < lane) ? its : 0;
+            }
+            const uint64_t mine = __ballot(slot >= start && slot < start + tiles);
+            if (mine == 0) return false;
+            u.b = __builtin_amdgcn_readfirstlane(__builtin_ctzll(mine));
+            u.off = __builtin_amdgcn_readlane(off, u.b);
+            u.n = __builtin_amdgcn_readlane(n, u.b);
+            u.length = __builtin_amdgcn_readlane(length, u.b);
+            u.tile = __builtin_amdgcn_readlane(start + tiles - 1, u.b) - slot;
+        } else {
+            // Sequence b's tiles take the slots from offsets[b] * group / 128 + b on:
+            // never fewer than it needs, so no sum over the sequences is wanted.
+            grid.place(id, head, slot);
+            int before = 0;
+            for (int at = 0; at < c.batch; at += 64) {
+                const int b = min(at + lane, c.batch - 1);
+                const int64_t start = int64_t(min(max(c.offsets[b], 0), tokens)) * group / kWindowRows + b;
+                before += __popcll(__ballot(at + lane < c.batch && start <= slot));
+            }
+            u.b = __builtin_amdgcn_readfirstlane(before) - 1;
+            if (u.b < 0) return false;
+            u.off = min(max(c.offsets[u.b], 0), tokens);
+            u.n = min(max(c.offsets[u.b + 1], 0), tokens) - u.off;
+            u.tile = slot - static_cast<int>(int64_t(u.off) * group / kWindowRows + u.b);
+            if (int64_t(u.tile) * kWindowRows >= int64_t(u.n) * group) return false;
+            u.length = static_cast<int>(min(int64_t(max(c.lengths[u.b], 0)), int64_t(c.table_width) * c.page.d));
         }
-        u.b = __builtin_amdgcn_readfirstlane(before) - 1;
-        if (u.b < 0) return false;
-        u.off = min(max(c.offsets[u.b], 0), c.tokens);
-        u.n = min(max(c.offsets[u.b + 1], 0), c.tokens) - u.off;
-        u.tile = slot - static_cast<int>(int64_t(u.off) * c.group.d / kWindowRows + u.b);
-        if (int64_t(u.tile) * kWindowRows >= int64_t(u.n) * c.group.d) return false;
-        u.length = static_cast<int>(min(int64_t(max(c.lengths[u.b], 0)), int64_t(c.table_width) * c.page.d));
+        for (int* p : {&u.off, &u.n, &u.length, &u.tile, &head}) *p = __builtin_amdgcn_readfirstlane(*p);
+        u.kv_head = head;
+        u.head = head * group;
         u.first = u.length - u.n;
         return true;
     }
@@ -710,7 +739,7 @@ __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
 template <class T, int D, bool kPaged>
 int launch_as(const WindowCall& c, hipStream_t stream) {
     const int64_t tiles = window_tiles(c), heads = kPaged ? c.kv_heads : int64_t(c.batch) * c.heads;
-    const WindowGrid places = window_grid(heads, tiles, kPaged && c.batch > 1);
+    const WindowGrid places = window_grid(heads, tiles);
     const dim3 grid(places.size(), static_cast<unsigned>(c.parts));
     const auto kernel = c.parts == 1 ? window_kernel<T, D, kPaged, false> : window_kernel<T, D, kPaged, true>;
     constexpr int kLds = WindowTile<T, D>::kLdsBytes;

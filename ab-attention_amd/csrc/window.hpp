@@ -210,38 +210,34 @@ struct TileRange {
 // over the 8 XCDs in order, and one that has nothing to do keeps an XCD's place
 // empty until the others' turn has come (40 heads x 37 tiles with three gaps in
 // 40: 3,830 us instead of 3,285).
-// The list: the last `run` tiles (the longest) of every head, then the ones before
-// them, so that short rows end the call. With runs of eight, one for each XCD, the
-// tiles of an XCD lie 1,024 rows apart; groups of 4 to 32 neighbours, whose windows
-// overlap in its L2, fetch half as much but are slower nearly everywhere, for they
-// do not start together (12 heads of 480p, window of 4 frames: 1,508 us, in groups
-// 1,560 to 1,740; causal 16 x 16,384 1,112, in groups 1,139 to 1,707), and so are
-// whole heads one after the other (1,640; 1,235). Runs of eight deal every eighth
-// tile to the same XCD: where the tiles are sequences of a batch, of lengths of
-// their own, their few (under 64) tiles go head by head instead (32 sequences x 8
-// heads, a token each: 378 us in runs of eight, 254 head by head).
+// The list: the last eight tiles (the longest) of every head, one for each XCD, then
+// the eight before them, so that short rows end the call. Groups of 4 to 32
+// neighbouring tiles for each XCD, whose windows overlap in its L2, fetch half as
+// much but are slower nearly everywhere, for they do not start together (12 heads of
+// 480p, window of 4 frames: 1,508 us, in groups 1,560 to 1,740; causal 16 x 16,384
+// 1,112, in groups 1,139 to 1,707), and so are whole heads one after the other (1,640;
+// 1,235).
 struct WindowGrid {
-    uint32_t heads, tiles, run;
+    static constexpr uint32_t kRun = 8;
+    uint32_t heads, tiles;
     unsigned size() const { return heads * tiles; }
     __device__ __forceinline__ void place(uint32_t n, int& head, int& tile) const {
-        const uint32_t runs = tiles / run, whole = runs * run * heads;
-        uint32_t each = run, first = 0;
+        const uint32_t runs = tiles / kRun, whole = runs * kRun * heads;
+        uint32_t each = kRun, first = 0;
         if (n < whole) {
-            first = n / (run * heads);
-            n -= first * run * heads;
-            first *= run;
+            first = n / (kRun * heads);
+            n -= first * kRun * heads;
+            first *= kRun;
         } else {
             n -= whole;
-            each = tiles - runs * run;
-            first = runs * run;
+            each = tiles - runs * kRun;
+            first = runs * kRun;
         }
         head = n / each;
         tile = tiles - 1 - (first + n - head * each);
     }
 };
-inline WindowGrid window_grid(int64_t heads, int64_t tiles, bool ragged) {
-    return {static_cast<uint32_t>(heads), static_cast<uint32_t>(tiles), ragged && tiles < 64 ? static_cast<uint32_t>(tiles) : 8u};
-}
+inline WindowGrid window_grid(int64_t heads, int64_t tiles) { return {static_cast<uint32_t>(heads), static_cast<uint32_t>(tiles)}; }
 
 int launch_window(const WindowCall& call, hipStream_t stream);
 int window_parts(const WindowCall& call, int64_t most_keys);

@@ -453,7 +453,7 @@ int launch_as(const WindowGradCall& c, hipStream_t stream) {
     hipLaunchKernelGGL((window_delta_kernel<T, D>), dim3(blocks, y, (bh + y - 1) / y), dim3(256), 0, stream, c, blocks);
     if (int rc = check_launch("window_delta_kernel")) return rc;
     const unsigned split = kv * c.sink_tiles * c.sink_parts;
-    const WindowGrid keys = window_grid(kv, tiles - c.sink_tiles, false), queries = window_grid(bh, tiles, false);
+    const WindowGrid keys = window_grid(kv, tiles - c.sink_tiles), queries = window_grid(bh, tiles);
     const auto by_keys = window_grad_kernel<T, D, true>, by_queries = window_grad_kernel<T, D, false>;
     if (int rc = ensure_lds_limit(reinterpret_cast<const void*>(by_keys), grad_lds<D, true>())) return rc;
     if (int rc = ensure_lds_limit(reinterpret_cast<const void*>(by_queries), grad_lds<D, false>())) return rc;
