@@ -35,16 +35,19 @@ from . import _lib
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 _MOST = 1 << 30
+_REACH = (1 << 31) - 128  # 16-bit elements
 
 
 def _strided(t: torch.Tensor, align: int = 8) -> torch.Tensor:
     """t itself where its rows (last dim contiguous, starting on 16 bytes) can be
-    read where they lie, else a contiguous copy."""
+    read where they lie, else a contiguous copy; of [B, H, N, D] the kernels reach
+    4 GiB from a head's first row on."""
     if t.data_ptr() % 16 == 0:
         if t.is_contiguous():
             return t
         strides = t.stride()
-        if strides[-1] == 1 and not any(n > 1 and s % align for n, s in zip(t.shape, strides[:-1])):
+        if strides[-1] == 1 and not any(n > 1 and s % align for n, s in zip(t.shape, strides[:-1])) and (
+                strides[-2] * (t.shape[-2] + 64) < _REACH or t.ndim == 3):
             return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -166,7 +169,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
 
 def _mask(window, sinks, frame):
     """(window, 0 for no limit, sinks, frame) as checked numbers."""
-    window = 0 if window is None else int(window)
+    window = 0 if window is None else min(int(window), _MOST)
     sinks, frame = int(sinks), int(frame)
     if frame < 1:
         raise ValueError("frame must be at least one token")
@@ -426,6 +429,7 @@ class StreamingAttention:
         self.free = list(range(pages - 1, -1, -1))
         self.tokens = [0] * sequences    # of each sequence, with those of the step that began last
         self.held = [{} for _ in range(sequences)]  # of each sequence: place in its table -> page
+        self.step_tokens = 0
         self.page_table = self.lengths = self.offsets = None
 
     def _behind(self, first: int) -> range:
@@ -455,7 +459,7 @@ class StreamingAttention:
             self.free.append(self.held[s].pop(i))
         for s, i in wanted:
             self.held[s][i] = self.free.pop()
-        self.tokens = total
+        self.tokens, self.step_tokens = total, sum(new)
         width = max(1, max(-(-length // self.page_tokens) for length in total))
         table = [[-1] * width for _ in total]
         for row, held in zip(table, self.held):
@@ -475,6 +479,8 @@ class StreamingAttention:
         given. Returns o [T, H, D] (and lse [T, H])."""
         if self.offsets is None:
             raise ValueError("attend comes after begin")
+        if any(t.ndim != 3 or t.shape[0] != self.step_tokens for t in (q, k, v)):
+            raise ValueError(f"Q, K and V must be the step's {self.step_tokens} packed tokens [T,H,D]")
         if self.axes is not None:
             if positions is None:
                 raise ValueError("positions are needed to turn Q and K")

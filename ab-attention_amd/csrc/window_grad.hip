@@ -25,6 +25,7 @@ namespace {
 
 constexpr int kTileRows = kWindowKeys;  // streamed rows of a tile
 constexpr int kStages = 4;              // of streamed tiles in LDS
+constexpr int64_t kMostPartial = int64_t(1) << 28;  // floats
 template <int D, bool kKeys>
 constexpr int grad_lds() {
     return 2 * kStages * kTileRows * D * 2 + (kKeys ? kStages * 4 * 256 : 0);
@@ -471,7 +472,7 @@ int launch_as(const WindowGradCall& c, hipStream_t stream) {
 }  // namespace
 
 // Tiles with sinks are split into parts of about as many queries as a tile
-// behind them has (its window), at most 64 of them.
+// behind them has (its window), at most 64 of them and 1 GiB of partial sums.
 void plan_window_grad(WindowGradCall& c, int64_t& stat, int64_t& partial) {
     const int64_t blocks = (int64_t(c.tokens) + 31) / 32, tiles = (int64_t(c.tokens) + kWindowRows - 1) / kWindowRows;
     stat = int64_t(c.batch) * c.heads * blocks * 64;
@@ -479,11 +480,13 @@ void plan_window_grad(WindowGradCall& c, int64_t& stat, int64_t& partial) {
     c.sink_tiles = c.sink_parts = 0;
     const int64_t window = int64_t(c.mask.back) + c.mask.frame.d + kWindowRows;
     const int64_t sinks = std::min<int64_t>((int64_t(c.mask.sinks) + kWindowRows - 1) / kWindowRows, tiles);
-    const int64_t parts = std::min<int64_t>((c.tokens + window - 1) / window, 64);
-    if (sinks > 0 && parts > 1 && sinks <= 65535 && int64_t(c.batch) * c.kv_heads <= 65535) {
+    const int64_t kv = int64_t(c.batch) * c.kv_heads, each = 2 * kWindowRows * c.dim;  // floats of a part
+    if (sinks == 0 || sinks > 65535 || kv > 65535) return;
+    const int64_t parts = std::min<int64_t>({(c.tokens + window - 1) / window, 64, kMostPartial / (kv * sinks * each)});
+    if (parts > 1) {
         c.sink_tiles = static_cast<int32_t>(sinks);
         c.sink_parts = static_cast<int32_t>(parts);
-        partial = int64_t(c.batch) * c.kv_heads * sinks * parts * 2 * kWindowRows * c.dim;
+        partial = kv * sinks * parts * each;
     }
 }
 

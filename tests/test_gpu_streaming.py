@@ -206,6 +206,12 @@ def test_window_large_logits():
         assert ((out[0].double() - o).abs() <= room).all()
 
 
+@pytest.mark.parametrize("heads,tokens", [(3, 1), (1, 900), (700, 40)])
+def test_window_odd_grids(heads, tokens):
+    """One row in all, one head of several tiles, more heads than tiles."""
+    _window_case(1, heads, heads, tokens, 64, BF16, 100, 1, 1)
+
+
 def test_window_of_no_tokens():
     empty = torch.empty((2, 3, 0, 64), dtype=BF16, device="cuda")
     out, lse = window_attention(empty, empty, empty, window=3, return_lse=True)
@@ -303,6 +309,31 @@ def test_window_gradient_parts_of_the_graph():
     pair = [q.clone().requires_grad_() for _ in range(2)]
     dq, dk = torch.autograd.grad(window_attention(*pair, v, **how)[0], pair, ones)
     assert torch.equal(both, dq + dk)
+
+
+def test_window_gradient_without_the_rest():
+    """The C entry with out alone: within the room that the output's rounding is given, and no nearer than with both."""
+    from ab_attention import _lib
+    from ab_attention import streaming as st
+
+    shape = (1, 2, 300, 64)
+    q, k, v, do = (_rand(shape, BF16, s) for s in (1, 2, 3, 4))
+    how = (50, 3, 1, 64 ** -0.5)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    out, lse = window_attention(*leaves, window=50, sinks=3, return_lse=True)
+    with_rest = torch.autograd.grad(out, leaves, do)
+    grads = [torch.empty_like(q) for _ in range(3)]
+    behind = st._GRAD_REST.pack(do.data_ptr(), 0, *(g.data_ptr() for g in grads), *do.stride()[:3],
+                                *(s for g in grads for s in g.stride()[:3]))
+    args = (q, k, v, out.detach(), None, lse.detach(), None, *how)
+    size = _lib.raw("ab_window_grad_workspace_bytes")(st._window_args(*args) + behind)
+    workspace = torch.empty(size, dtype=torch.uint8, device="cuda")
+    st._call("ab_window_attention_grad", q.device, st._window_args(*args, workspace.data_ptr(), size) + behind)
+    at = torch.arange(300, device="cuda")
+    want, room = attend_grad(q[0], k[0], v[0], do[0], seen_mask(at, at, 50, 3, 1))
+    for g, both, w, r in zip(grads, with_rest, want, room):
+        check_gradient(g[0], w, r, BF16)
+        assert (both[0].double() - w).norm() <= 1.001 * (g[0].double() - w).norm()
 
 
 def test_window_gradient_against_differences():

@@ -170,7 +170,7 @@ def _grad_args(**change):
 
 @pytest.mark.parametrize("change,msg", [
     (dict(dout=0), b"null"), (dict(dk=0), b"null"), (dict(lse=0), b"null"), (dict(workspace=0), b"null"),
-    (dict(dq=_A + 8), b"aligned"), (dict(out=_A + 8), b"aligned"), (dict(workspace_bytes=64), b"smaller"),
+    (dict(dq=_A + 8), b"aligned"), (dict(out=_A + 8), b"aligned"), (dict(out_rest=_A + 8), b"aligned"), (dict(workspace_bytes=64), b"smaller"),
     (dict(dv_stride=(1024, 512, 4)), b"strides"), (dict(out_stride=(1024, 512, 68)), b"strides"), (dict(dim=32), b"64 or 128"),
 ])
 def test_gradient_entry_refuses(change, msg):
@@ -188,6 +188,22 @@ def test_gradient_workspace():
     assert plain == 2 * 32 * 64 * 4
     sinks = lib.ab_window_grad_workspace_bytes(_grad_args(tokens=1024, window=100, sinks=4, **strides))
     assert (sinks - plain) % (2 * 128 * 64 * 4) == 0 and sinks > plain
+    far = dict(q_stride=(0, 1 << 20, 64), k_stride=(0, 1 << 20, 64), v_stride=(0, 1 << 20, 64), batch=1)
+    big = lib.ab_window_grad_workspace_bytes(_grad_args(tokens=1 << 20, window=1, sinks=1 << 19, **far))
+    assert 0 < big <= (1 << 30) + 2 * (1 << 15) * 256
+
+
+def test_rows_out_of_reach_are_copied():
+    """Heads of which a kernel's 32-bit offsets do not reach the last row are read from a copy."""
+    from ab_attention.streaming import _strided
+
+    base = torch.zeros(64, dtype=BF16)
+    near = base.as_strided((1, 1, 1000, 64), (0, 0, 0, 1))
+    assert _strided(near) is near
+    far = torch.empty((1, 1, 70, 64), dtype=BF16, device="meta").as_strided((1, 1, 70, 64), (1 << 36, 1 << 36, 1 << 25, 1))
+    assert far.stride(2) * (70 + 64) >= (1 << 31) and _strided(far).is_contiguous()
+    packed = torch.empty((70, 2, 64), dtype=BF16, device="meta").as_strided((70, 2, 64), (1 << 27, 64, 1))
+    assert _strided(packed) is packed
 
 
 @pytest.mark.parametrize("change,msg", [(dict(layers=0), "positive"), (dict(pages=0), "positive"), (dict(page_tokens=12), "multiple of 8"),
@@ -205,9 +221,11 @@ def test_streaming_attention_needs_a_step_and_positions():
     x = _z(3, 1, 64)
     with pytest.raises(ValueError, match="begin"):
         stream.attend(0, x, x, x)
-    stream.offsets = _OFFSETS
+    stream.offsets, stream.step_tokens = _OFFSETS, 3
     with pytest.raises(ValueError, match="positions"):
         stream.attend(0, x, x, x)
+    with pytest.raises(ValueError, match="3 packed tokens"):
+        stream.attend(0, x[:2], x, x)
 
 
 def test_pages_behind_the_window():
