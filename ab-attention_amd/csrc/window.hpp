@@ -176,8 +176,12 @@ struct WindowGradCall {
     WindowMask mask;
     float scale, scale_log2;
     float* stat;
-    int32_t sink_tiles, sink_parts;  // key tiles whose queries are split, and into how many parts
-    float* partial;                  // [batch][kv_heads][sink_tiles][sink_parts][2][128][dim]
+    // Parts that the streamed rows of a tile are split into: of the first sink_tiles
+    // key tiles, of the others, of query tiles.
+    int32_t sink_tiles, sink_parts, key_parts, query_parts;
+    // Their float32 sums: [heads][tiles][parts][dK, dV][128][dim] of the sinks' tiles,
+    // then of the other key tiles, then [heads][tiles][parts][128][dim] of query tiles.
+    float* partial;
 };
 
 constexpr int kWindowThreads = 256;
@@ -243,7 +247,7 @@ int launch_window(const WindowCall& call, hipStream_t stream);
 int window_parts(const WindowCall& call, int64_t most_keys);
 int64_t window_tiles(const WindowCall& call);
 int launch_window_grad(const WindowGradCall& call, hipStream_t stream);
-// Sets sink_tiles and sink_parts; returns the floats of stat and of partial.
+// Sets the tiles and parts of a split; returns the floats of stat and of partial.
 void plan_window_grad(WindowGradCall& call, int64_t& stat, int64_t& partial);
 
 }  // namespace ab

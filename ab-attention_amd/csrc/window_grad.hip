@@ -15,8 +15,10 @@
 // input type); all sums are float32.
 // The first keys (sinks) are seen by every later query. Their tiles would run
 // many times longer than the others, so their queries are split into parts whose
-// float32 sums a third kernel adds up, always in the same order.
+// float32 sums a third kernel adds up, always in the same order; so are all tiles of
+// calls with too few of them to fill the chip.
 #include <algorithm>
+#include <initializer_list>
 
 #include "window.hpp"
 
@@ -105,8 +107,10 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
     touch(c.q, c.k_rows.batch, c.out_rows.batch, c.dq_rows.batch, c.lengths, c.partial);
 
     // Owned rows. Of keys, the sinks' tiles come first, part by part: `places` are
-    // the tiles behind them.
+    // the tiles behind them. slot: the place of a part's sums.
+    constexpr int kPartial = (kKeys ? 2 : 1) * kWindowRows * D;
     int head, tile, part = 0, parts = 1;
+    uint32_t slot = blockIdx.x;
     if constexpr (kKeys) {
         const uint32_t split = c.batch * c.kv_heads * c.sink_tiles * c.sink_parts;
         if (blockIdx.x < split) {
@@ -116,14 +120,26 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
             head = tile / c.sink_tiles;
             tile -= head * c.sink_tiles;
         } else {
-            places.place(blockIdx.x - split, head, tile);
-            tile = c.sink_tiles + (places.tiles - 1 - tile);  // the first keys are seen most
+            const uint32_t id = (blockIdx.x - split) / c.key_parts;
+            parts = c.key_parts;
+            part = blockIdx.x - split - id * parts;
+            places.place(id, head, tile);
+            tile = places.tiles - 1 - tile;  // the first keys are seen most
+            slot = split + (head * places.tiles + tile) * parts + part;
+            tile += c.sink_tiles;
         }
     } else {
-        places.place(blockIdx.x, head, tile);
+        const uint32_t id = blockIdx.x / c.query_parts;
+        parts = c.query_parts;
+        part = blockIdx.x - id * parts;
+        places.place(id, head, tile);
+        slot = (head * places.tiles + tile) * parts + part;
     }
+    // Divisions leave them in vector registers.
+    for (int* p : {&head, &tile, &part}) *p = __builtin_amdgcn_readfirstlane(*p);
+    slot = __builtin_amdgcn_readfirstlane(slot);
     const int heads = kKeys ? c.kv_heads : c.heads;
-    const int b = head / heads, h = head - b * heads;  // own head
+    const int b = __builtin_amdgcn_readfirstlane(head / heads), h = head - b * heads;  // own head
     const int length = length_of(c, b);
     const WindowMask mask = c.mask;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -361,6 +377,8 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
                     pw[j][2 * half + r / 2] = T::pack(sc[j][r], sc[j][r + 1]);
                     dw[j][2 * half + r / 2] = T::pack(dp[j][r], dp[j][r + 1]);
                 }
+            // Reads of the next half not before: with them D = 128 spills.
+            __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int m = 0; m < kBlocks; ++m) {
@@ -381,17 +399,14 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int p = own0 + wave * 32 + 16 * j + li;
-        if constexpr (kKeys) {
-            if (parts > 1) {
-                float* dst = c.partial + ((int64_t(head) * c.sink_tiles + tile) * parts + part) * (2 * kWindowRows * D) +
-                             (p - own0) * D + 4 * lg;
+        if (parts > 1) {
+            float* dst = c.partial + int64_t(slot) * kPartial + (p - own0) * D + 4 * lg;
 #pragma unroll
-                for (int m = 0; m < kBlocks; ++m) {
-                    *reinterpret_cast<f32x4*>(dst + 16 * m) = acc1[m][j];
-                    *reinterpret_cast<f32x4*>(dst + kWindowRows * D + 16 * m) = acc2[m][j];
-                }
-                continue;
+            for (int m = 0; m < kBlocks; ++m) {
+                *reinterpret_cast<f32x4*>(dst + 16 * m) = acc1[m][j];
+                if constexpr (kKeys) *reinterpret_cast<f32x4*>(dst + kWindowRows * D + 16 * m) = acc2[m][j];
             }
+            continue;
         }
         if (p >= c.tokens) continue;
         const float live = p < length ? 1.f : 0.f;
@@ -416,20 +431,28 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
     }
 }
 
-// The parts of the sinks' tiles added up, in order: eight values of a row per thread.
+// The parts of split tiles added up, in order: eight values of a row per thread.
+// Tiles first .. first + count - 1 of every head; outputs dK and dV, or dQ alone.
+struct Sums {
+    const float* partial;
+    int first, count, parts, heads, outputs;
+    void* out[2];
+    Rows rows[2];
+    float scale[2];
+};
 template <class T, int D>
-__global__ __launch_bounds__(256) void window_sinks_kernel(WindowGradCall c) {
+__global__ __launch_bounds__(256) void window_sums_kernel(WindowGradCall c, Sums s) {
     constexpr int kLanes = D / 8, kTileValues = kWindowRows * D;
-    const int at = blockIdx.x * 256 + threadIdx.x;  // of a tile's rows times lanes, dK's then dV's
+    const int at = blockIdx.x * 256 + threadIdx.x;  // of a tile's rows times lanes, of the first output, then of the second
     const int which = at / (kWindowRows * kLanes), row = at / kLanes % kWindowRows, lane = at % kLanes;
-    const int tile = blockIdx.y, head = blockIdx.z, b = head / c.kv_heads, h = head - b * c.kv_heads;
-    const int p = tile * kWindowRows + row;
-    if (which > 1 || p >= c.tokens) return;
+    const int head = blockIdx.z, b = head / s.heads, h = head - b * s.heads;
+    const int p = (s.first + static_cast<int>(blockIdx.y)) * kWindowRows + row;
+    if (which >= s.outputs || p >= c.tokens) return;
     float sum[8] = {};
     if (p < length_of(c, b)) {
-        const float* src = c.partial + ((int64_t(head) * c.sink_tiles + tile) * c.sink_parts) * (2 * kTileValues) +
-                           which * kTileValues + row * D + lane * 8;
-        for (int i = 0; i < c.sink_parts; ++i, src += 2 * kTileValues) {
+        const int64_t each = int64_t(s.outputs) * kTileValues;
+        const float* src = s.partial + (int64_t(head) * s.count + blockIdx.y) * s.parts * each + which * kTileValues + row * D + lane * 8;
+        for (int i = 0; i < s.parts; ++i, src += each) {
             const f32x4 x = reinterpret_cast<const f32x4*>(src)[0], y = reinterpret_cast<const f32x4*>(src)[1];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -438,12 +461,12 @@ __global__ __launch_bounds__(256) void window_sinks_kernel(WindowGradCall c) {
             }
         }
     }
-    const float scale = which ? 1.f : c.scale;
-    const Rows& r = which ? c.dv_rows : c.dk_rows;
+    const float scale = which ? s.scale[1] : s.scale[0];
+    const Rows r = which ? s.rows[1] : s.rows[0];
     u32x4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = T::pack(sum[2 * i] * scale, sum[2 * i + 1] * scale);
-    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(which ? c.dv : c.dk) + b * r.batch + h * r.head + p * r.token + lane * 8) = w;
+    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(which ? s.out[1] : s.out[0]) + b * r.batch + h * r.head + p * r.token + lane * 8) = w;
 }
 
 template <class T, int D>
@@ -453,41 +476,71 @@ int launch_as(const WindowGradCall& c, hipStream_t stream) {
     const unsigned y = std::min(bh, 32768u);
     hipLaunchKernelGGL((window_delta_kernel<T, D>), dim3(blocks, y, (bh + y - 1) / y), dim3(256), 0, stream, c, blocks);
     if (int rc = check_launch("window_delta_kernel")) return rc;
+    auto sums = [&](const Sums& s, unsigned all_heads) {
+        hipLaunchKernelGGL((window_sums_kernel<T, D>), dim3(s.outputs * kWindowRows * (D / 8) / 256, s.count, all_heads), dim3(256), 0,
+                           stream, c, s);
+        return check_launch("window_sums_kernel");
+    };
     const unsigned split = kv * c.sink_tiles * c.sink_parts;
     const WindowGrid keys = window_grid(kv, tiles - c.sink_tiles), queries = window_grid(bh, tiles);
     const auto by_keys = window_grad_kernel<T, D, true>, by_queries = window_grad_kernel<T, D, false>;
     if (int rc = ensure_lds_limit(reinterpret_cast<const void*>(by_keys), grad_lds<D, true>())) return rc;
     if (int rc = ensure_lds_limit(reinterpret_cast<const void*>(by_queries), grad_lds<D, false>())) return rc;
-    hipLaunchKernelGGL(by_keys, dim3(split + keys.size()), dim3(kWindowThreads), (grad_lds<D, true>()), stream, c, keys);
+    hipLaunchKernelGGL(by_keys, dim3(split + keys.size() * c.key_parts), dim3(kWindowThreads), (grad_lds<D, true>()), stream, c, keys);
     if (int rc = check_launch("window_grad_kernel")) return rc;
-    if (c.sink_tiles) {
-        // In launches of at most 65,535 heads.
-        hipLaunchKernelGGL((window_sinks_kernel<T, D>), dim3(2 * kWindowRows * (D / 8) / 256, c.sink_tiles, kv), dim3(256), 0,
-                           stream, c);
-        if (int rc = check_launch("window_sinks_kernel")) return rc;
-    }
-    hipLaunchKernelGGL(by_queries, dim3(queries.size()), dim3(kWindowThreads), (grad_lds<D, false>()), stream, c, queries);
-    return check_launch("window_grad_kernel");
+    Sums s{c.partial, 0, c.sink_tiles, c.sink_parts, c.kv_heads, 2, {c.dk, c.dv}, {c.dk_rows, c.dv_rows}, {c.scale, 1.f}};
+    if (c.sink_tiles)
+        if (int rc = sums(s, kv)) return rc;
+    const int64_t each = int64_t(kWindowRows) * D;
+    s.partial += int64_t(split) * 2 * each;
+    s.first = c.sink_tiles;
+    s.count = static_cast<int>(keys.tiles);
+    s.parts = c.key_parts;
+    if (c.key_parts > 1)
+        if (int rc = sums(s, kv)) return rc;
+    WindowGradCall q = c;
+    if (c.key_parts > 1) s.partial += int64_t(keys.size()) * c.key_parts * 2 * each;
+    q.partial = const_cast<float*>(s.partial);
+    hipLaunchKernelGGL(by_queries, dim3(queries.size() * c.query_parts), dim3(kWindowThreads), (grad_lds<D, false>()), stream, q, queries);
+    if (int rc = check_launch("window_grad_kernel")) return rc;
+    if (c.query_parts == 1) return 0;
+    return sums({q.partial, 0, tiles, c.query_parts, c.heads, 1, {c.dq, c.dq}, {c.dq_rows, c.dq_rows}, {c.scale, c.scale}}, bh);
 }
 }  // namespace
 
 // Tiles with sinks are split into parts of about as many queries as a tile
-// behind them has (its window), at most 64 of them and 1 GiB of partial sums.
+// behind them has (its window), at most 64 of them and 1 GiB of partial sums. All
+// tiles are split where that gives each CU at most two workgroups, of eight steps at
+// least: 1,560 tokens of 4 heads over 2, 4 frames of 390: 224 us forward and backward
+// with whole tiles, 95 with split ones.
 void plan_window_grad(WindowGradCall& c, int64_t& stat, int64_t& partial) {
     const int64_t blocks = (int64_t(c.tokens) + 31) / 32, tiles = (int64_t(c.tokens) + kWindowRows - 1) / kWindowRows;
     stat = int64_t(c.batch) * c.heads * blocks * 64;
     partial = 0;
     c.sink_tiles = c.sink_parts = 0;
+    c.key_parts = c.query_parts = 1;
     const int64_t window = int64_t(c.mask.back) + c.mask.frame.d + kWindowRows;
+    const int64_t kv = int64_t(c.batch) * c.kv_heads, bh = int64_t(c.batch) * c.heads;
+    const int64_t each = kWindowRows * int64_t(c.dim);  // floats of a part
+    if (tiles > 65535 || bh > 65535) return;
     const int64_t sinks = std::min<int64_t>((int64_t(c.mask.sinks) + kWindowRows - 1) / kWindowRows, tiles);
-    const int64_t kv = int64_t(c.batch) * c.kv_heads, each = 2 * kWindowRows * c.dim;  // floats of a part
-    if (sinks == 0 || sinks > 65535 || kv > 65535) return;
-    const int64_t parts = std::min<int64_t>({(c.tokens + window - 1) / window, 64, kMostPartial / (kv * sinks * each)});
-    if (parts > 1) {
-        c.sink_tiles = static_cast<int32_t>(sinks);
-        c.sink_parts = static_cast<int32_t>(parts);
-        partial = kv * sinks * parts * each;
+    if (sinks > 0) {
+        const int64_t parts = std::min<int64_t>({(c.tokens + window - 1) / window, 64, kMostPartial / (kv * sinks * 2 * each)});
+        if (parts > 1) {
+            c.sink_tiles = static_cast<int32_t>(sinks);
+            c.sink_parts = static_cast<int32_t>(parts);
+            partial = kv * sinks * parts * 2 * each;
+        }
     }
+    auto split = [&](int64_t units, int64_t steps) {
+        return static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(units, 1), steps / 8, 16})));
+    };
+    const int64_t seen = std::min<int64_t>(window, c.tokens);  // queries of a key tile, about
+    const int64_t key_units = kv * (tiles - c.sink_tiles), query_units = bh * tiles;
+    c.key_parts = split(key_units, c.group * (seen / kTileRows));
+    c.query_parts = split(query_units, std::min<int64_t>(seen + c.mask.sinks, c.tokens) / kTileRows);
+    if (c.key_parts > 1) partial += key_units * c.key_parts * 2 * each;
+    if (c.query_parts > 1) partial += query_units * c.query_parts * each;
 }
 
 int launch_window_grad(const WindowGradCall& c, hipStream_t stream) {
