@@ -9,7 +9,25 @@
 // One workgroup of four waves takes 128 rows of one K/V head of one batch item:
 // tokens, or over a cache (token, query head of the group) pairs, so that the
 // heads that share keys read them once. It visits only tiles of 32 keys that
-// some of its rows see: the sinks' tiles, then the window's.
+// some of its rows see: the sinks' tiles, then the window's; only tiles that some
+// row of a wave sees in part are masked. K and V go straight from memory into two
+// rings of four LDS stages, three to five tiles ahead, through buffers that end
+// where the visible keys of a tensor or a page do: what lies behind arrives as
+// zeros and is never read. The step is software-pipelined: the first product of the
+// next tile beside this tile's exponentials, this tile's second product beside the
+// next one's logits. The reference of a row moves only where a logit passes it by
+// more than 2^8. P is rounded to the input type for the second product, the output
+// once at the end; sums are float32.
+//
+// What bounds it: with many keys the matrix cores at the board's power limit, with
+// the LDS (16 KiB read by each wave of a step) and the vector units (118
+// instructions beside 32 MFMAs) close behind: 12 heads of 32,760 tokens that all see
+// each other 1,130 TFLOP/s, causal over frames with a window of four 946 (rows that
+// straddle frames, 16 us a workgroup to fill and empty the pipeline). The
+// straightforward form of this kernel (two stages, one tile at a time) did 605. With
+// single tokens over long caches it is memory: 4.6 TB/s of the 4.9 that a copy
+// reaches, the keys split over workgroups. 9 tiles of a short call take 14 us, half
+// of them the pipeline's filling.
 #include <algorithm>
 #include <initializer_list>
 
@@ -759,7 +777,9 @@ int64_t window_tiles(const WindowCall& c) {
 }
 
 // Parts that the keys of every tile of rows are split into: as many as give
-// each CU two workgroups, with at least 8 tiles of keys in each.
+// each CU two workgroups, with at least 8 tiles of keys in each (a part costs 512
+// bytes of partial results per row, written and read, and the call a second kernel of
+// 5 us).
 int window_parts(const WindowCall& c, int64_t most_keys) {
     int64_t units = window_tiles(c) * (c.paged ? c.kv_heads : int64_t(c.batch) * c.heads);
     const int64_t key_tiles = (most_keys + kWindowKeys - 1) / kWindowKeys;

@@ -17,6 +17,12 @@
 // many times longer than the others, so their queries are split into parts whose
 // float32 sums a third kernel adds up, always in the same order; so are all tiles of
 // calls with too few of them to fill the chip.
+// What bounds it: the matrix cores at the power limit and the LDS, whose operand
+// reads (one 1 KiB fragment for two MFMAs) take as long as they do. 12 heads of
+// 32,760 tokens, window of four frames of 1,560: keys 2,764 us (1,024 TFLOP/s over
+// four products), queries 1,861 (1,140 over three), deltas 40 to 49, sinks 28. One
+// kernel with the five products alone would have to add dQ up with atomics, in an
+// order of its own each time.
 #include <algorithm>
 #include <initializer_list>
 
