@@ -24,6 +24,7 @@ bounded by the kernels and never read on the host.
 """
 from __future__ import annotations
 
+import functools
 import math
 import struct
 from typing import NamedTuple
@@ -64,7 +65,9 @@ def _gpu(name: str, first, *others):
 
 def _call(entry: str, device, packed: bytes):
     with _lib.on(device):
-        _lib.check(_lib.raw(entry)(packed, _lib.raw_stream(device)))
+        status = _lib.raw(entry)(packed, _lib.raw_stream(device))
+    if status:
+        _lib.check(status)
 
 
 _ROTARY, _WINDOW, _APPEND = map(_lib.packer, (_lib.RotaryArgs, _lib.WindowArgs, _lib.AppendArgs))
@@ -117,6 +120,18 @@ class _Rotary(torch.autograd.Function):
         return (*grads, *[None] * (len(ctx.how) + 1))
 
 
+@functools.lru_cache(maxsize=64)
+def _axes(axes, dim, pairing):
+    """axes, checked."""
+    if not 1 <= len(axes) <= 4 or any(a <= 0 or a % 2 for a in axes) or sum(axes) > dim:
+        raise ValueError("axes must be 1 to 4 positive even numbers of dims that add up to at most D")
+    if pairing not in ("adjacent", "halves"):
+        raise ValueError("pairing must be 'adjacent' or 'halves'")
+    if pairing == "halves" and sum(axes) % 16:
+        raise ValueError("pairing 'halves' requires a multiple of 16 turned dims")
+    return axes
+
+
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axes, *, theta: float = 10000.0,
            pairing: str = "adjacent", joint: bool = False):
     """q [B, H, N, D] and k [B, Hk, N, D] (or None) with rotary positions over several axes.
@@ -140,19 +155,14 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
     batch, _, tokens, dim = q.shape
     if dim % 8 or dim > 1024:
         raise ValueError("rotary requires a head dim that is a multiple of 8, at most 1024")
-    axes = tuple(int(a) for a in axes)
-    if not 1 <= len(axes) <= 4 or any(a <= 0 or a % 2 for a in axes) or sum(axes) > dim:
-        raise ValueError("axes must be 1 to 4 positive even numbers of dims that add up to at most D")
-    if pairing not in ("adjacent", "halves"):
-        raise ValueError("pairing must be 'adjacent' or 'halves'")
-    if pairing == "halves" and sum(axes) % 16:
-        raise ValueError("pairing 'halves' requires a multiple of 16 turned dims")
+    axes = _axes(tuple(map(int, axes)), dim, pairing)
     theta = float(theta)
     if not math.isfinite(theta) or theta <= 0:
         raise ValueError("theta must be positive and finite")
     if positions.dtype not in _POSITIONS:
         raise ValueError("positions must be int32, int64 or float32")
-    if positions.shape != (tokens, len(axes)) and positions.shape != (batch, tokens, len(axes)):
+    shape = positions.shape
+    if shape != (tokens, len(axes)) and shape != (batch, tokens, len(axes)):
         raise ValueError(f"positions must be [{tokens}, {len(axes)}] or [{batch}, {tokens}, {len(axes)}]")
     _gpu("rotary", q, k, positions)
     if q.shape[1] == 0 or (k is not None and k.shape[1] == 0):
@@ -194,7 +204,9 @@ def _run(entry, device, packed):
         if size:
             workspace = torch.empty(size, dtype=torch.uint8, device=device)
             packed = packed[:-_WORKSPACE.size] + _WORKSPACE.pack(workspace.data_ptr(), size)
-        _lib.check(_lib.raw(entry)(packed, _lib.raw_stream(device)))
+        status = _lib.raw(entry)(packed, _lib.raw_stream(device))
+    if status:
+        _lib.check(status)
 
 
 def _window_args(q, k, v, out, rest, lse, lengths, window, sinks, frame, scale, workspace=0, size=0):
