@@ -244,15 +244,20 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     const int last_entry = c.table_width - 1;
 
     // Whether a key that some row would see lies on no page (then every tile
-    // asks the table for its keys).
+    // asks the table for its keys). Pages between the sinks and the window, which
+    // may have been given back, do not count.
     bool holes = false;
     if constexpr (kPaged) {
         bool bad = false;
-        if (tiles > 0) {
-            const int first_page = range.key(tile0) / static_cast<int>(c.page.d);
-            const int last_page = (min(range.key(tile0 + tiles - 1) + kWindowKeys, end) - 1) / static_cast<int>(c.page.d);
-            for (int i = first_page + tid; i <= last_page; i += kWindowThreads)
+        auto scan = [&](int from, int to) {
+            const int page = static_cast<int>(c.page.d);
+            for (int i = from / page + tid; i <= (to - 1) / page; i += kWindowThreads)
                 bad |= static_cast<uint32_t>(table[i]) >= static_cast<uint32_t>(c.pages);
+        };
+        if (tiles > 0) {
+            const int last = tile0 + tiles - 1;
+            if (tile0 < range.sink_tiles) scan(range.key(tile0), min(mask.sinks, end));
+            if (last >= range.sink_tiles) scan(range.key(max(tile0, range.sink_tiles)), min(range.key(last) + kWindowKeys, end));
         }
         uint32_t* votes = reinterpret_cast<uint32_t*>(smem + Tile::kVotes);
         const uint32_t vote = __any(bad) ? 1u : 0u;
