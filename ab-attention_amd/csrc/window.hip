@@ -716,7 +716,10 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
 }
 
 // A split row: m = max over its parts, w = 2^(m_part - m), o = sum w o_part /
-// sum w l_part. One wave per row; bound by reading the partial results.
+// sum w l_part. One wave per row: lane p looks at part p (of at most 64), then all
+// lanes add up the parts' rows, four loads ahead. Bound by reading the partial
+// results or, for few rows, by two loads after one another (part after part, 52 parts
+// took 50 us).
 template <class T, int D, bool kPaged>
 __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
     const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
@@ -732,17 +735,32 @@ __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
         const int64_t bh = row / c.tokens, token = row - bh * c.tokens, b = bh / c.heads, head = bh - b * c.heads;
         out_at = b * c.out_rows.batch + head * c.out_rows.head + token * c.out_rows.token;
     }
-    float m = -INFINITY;
-    for (int p = 0; p < c.parts; ++p) m = fmaxf(m, c.partial_stat[p * c.rows + row].x);
-    float l = 0.f, o[D / 64] = {};
-    for (int p = 0; p < c.parts; ++p) {
-        const float2 stat = c.partial_stat[p * c.rows + row];
-        if (stat.y == 0.f) continue;
-        const float w = fast_exp2(stat.x - m);
-        l += w * stat.y;
-        const float* src = c.partial_o + (p * c.rows + row) * D + lane * (D / 64);
+    float2 stat = {-INFINITY, 0.f};
+    if (lane < c.parts) stat = c.partial_stat[lane * c.rows + row];
+    const bool some = stat.y != 0.f;  // a part without a key has written no row
+    float m = some ? stat.x : -INFINITY;
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) o[i] += w * src[i];
+    for (int s = 1; s < 64; s *= 2) m = fmaxf(m, __shfl_xor(m, s));
+    const float weight = some ? fast_exp2(stat.x - m) : 0.f;
+    float l = some ? weight * stat.y : 0.f, o[D / 64] = {};
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) l += __shfl_xor(l, s);
+    constexpr int kAhead = 4;
+    for (int p0 = 0; p0 < c.parts; p0 += kAhead) {
+        float x[kAhead][D / 64];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const float* src = c.partial_o + (min(p0 + i, c.parts - 1) * c.rows + row) * D + lane * (D / 64);
+#pragma unroll
+            for (int e = 0; e < D / 64; ++e) x[i][e] = src[e];
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (p0 + i >= c.parts) break;
+            const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), p0 + i));
+#pragma unroll
+            for (int e = 0; e < D / 64; ++e) o[e] += w != 0.f ? w * x[i][e] : 0.f;
+        }
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     const int64_t at = out_at + lane * (D / 64);
@@ -781,15 +799,32 @@ int64_t window_tiles(const WindowCall& c) {
     return (int64_t(c.tokens) + kWindowRows - 1) / kWindowRows;
 }
 
-// Parts that the keys of every tile of rows are split into: as many as give
-// each CU two workgroups, with at least 8 tiles of keys in each (a part costs 512
-// bytes of partial results per row, written and read, and the call a second kernel of
-// 5 us).
+// Parts that the keys of every tile of rows are split into: those that cost least.
+// A workgroup's time is its steps and about 6 us to fill and empty its pipeline; a step
+// takes 0.80 us where each CU has a workgroup and 0.95 where it has two (D = 64: 0.6 of
+// that), and more than 512 workgroups go in rounds. Splitting adds a second kernel
+// of 6 us and the partial results' traffic. Over 150 calls of 1 to 400 GFLOP drawn from
+// the range of sizes this took 5.7 % less time than as many parts as give each CU two
+// workgroups; lone steps of 0.55 us (the dense kernel's) took 2.6 % less, of 0.90 and
+// 0.95 the same. One token of 8 heads over 16,384 keys: 38 us.
 int window_parts(const WindowCall& c, int64_t most_keys) {
-    int64_t units = window_tiles(c) * (c.paged ? c.kv_heads : int64_t(c.batch) * c.heads);
-    const int64_t key_tiles = (most_keys + kWindowKeys - 1) / kWindowKeys;
-    const int64_t parts = std::min<int64_t>({(512 + units - 1) / units, key_tiles / 8, 64});
-    return static_cast<int>(std::max<int64_t>(parts, 1));
+    const double units = double(window_tiles(c)) * (c.paged ? c.kv_heads : int64_t(c.batch) * c.heads);
+    const int64_t steps = (most_keys + kWindowKeys - 1) / kWindowKeys;
+    const double scale = c.dim == 128 ? 1.0 : 0.6;
+    auto cost = [&](int64_t parts) {
+        const double groups = units * double(parts), rounds = std::max(1.0, groups / 512);
+        const double step = scale * (groups <= 256 ? 0.80 : 0.80 + 0.15 * std::min(1.0, groups / 256 - 1));
+        const double traffic = double(c.rows) * (c.dim * 4.0 + 8) * double(parts) * 2 / 4.5e6;
+        return rounds * (double((steps + parts - 1) / parts) * step + 6) + (parts > 1 ? 6 + traffic : 0.0);
+    };
+    int best = 1;
+    double least = 0.95 * cost(1);
+    for (int64_t parts = 2; parts <= 64 && parts * 4 <= steps; ++parts)
+        if (cost(parts) < least) {
+            best = static_cast<int>(parts);
+            least = cost(parts);
+        }
+    return best;
 }
 
 int launch_window(const WindowCall& c, hipStream_t stream) {
