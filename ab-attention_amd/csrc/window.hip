@@ -15,8 +15,8 @@
 // where the visible keys of a tensor or a page do: what lies behind arrives as
 // zeros and is never read. The step is software-pipelined: the first product of the
 // next tile beside this tile's exponentials, this tile's second product beside the
-// next one's logits. The reference of a row moves only where a logit passes it by
-// more than 2^8. P is rounded to the input type for the second product, the output
+// next one's logits. The reference of a row moves only where a logit (base 2) passes
+// it by more than 8. P is rounded to the input type for the second product, the output
 // once at the end; sums are float32.
 //
 // What bounds it: with many keys the matrix cores at the board's power limit, with

@@ -44,11 +44,6 @@ struct Bf16 {
     static __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
-    // 32x32x16 (A: lane l row l % 32, k 8(l / 32) .. + 7; D: lane l column
-    // l % 32, element e row e % 4 + 8(e / 4) + 4(l / 32)).
-    static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    }
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16(lo, hi); }
     static __device__ __forceinline__ float lo(uint32_t w) { return bf16_lo(w); }
     static __device__ __forceinline__ float hi(uint32_t w) { return bf16_hi(w); }
@@ -60,9 +55,6 @@ struct Bf16 {
 struct F16 {
     static __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    }
-    static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
