@@ -286,6 +286,21 @@ def test_window_gradient_many_tiles_and_scale():
     _grad_case(1, 2, 2, 200, 128, BF16, 50, 0, 1, scale=-0.06)
 
 
+@pytest.mark.parametrize("tokens,stride", [(100000, 20480), (110000, 20480)])
+def test_window_rows_4_gib_apart(tokens, stride):
+    """A head whose rows span almost 4 GiB is read in place, a longer one from a copy: the bits of contiguous tensors."""
+    base = torch.empty(tokens * stride, dtype=BF16, device="cuda")
+    views = [base.as_strided((1, 1, tokens, 64), (0, 0, stride, 1), 64 * i) for i in range(4)]
+    for i, view in enumerate(views):
+        view.copy_(_rand((1, 1, tokens, 64), BF16, i + 1))
+    leaves = [t.detach().requires_grad_() for t in views[:3]]
+    plain = [t.detach().contiguous().requires_grad_() for t in views[:3]]
+    out, want = (window_attention(*t, window=300, sinks=3) for t in (leaves, plain))
+    assert torch.equal(out, want)
+    for g, w in zip(torch.autograd.grad(out, leaves, views[3]), torch.autograd.grad(want, plain, views[3].contiguous())):
+        assert torch.equal(g, w)
+
+
 def test_window_gradient_parts_of_the_graph():
     """Only some of q, k, v, only the normaliser, an expanded gradient, a value shared by q and k."""
     q, k, v = (_rand((1, 2, 90, 64), BF16, s) for s in (1, 2, 3))
@@ -524,6 +539,11 @@ def test_append(dim, heads, page, token_major):
                 dst[table[b, at // page].long(), :, at % page] = src[offsets[b] + i]
     assert append_cache(cache, k, v, table.cuda(), lengths.cuda(), offsets.cuda()) is cache
     assert torch.equal(cache.k, want.k) and torch.equal(cache.v, want.v)
+
+
+def test_chunk_without_a_window_over_a_long_cache():
+    """Positions past 100,000, pages in any order, a prompt and a token."""
+    _chunk_case([130, 1], [100100, 120001], 2, 1, 64, 256)
 
 
 def test_append_drops_what_has_no_place():
