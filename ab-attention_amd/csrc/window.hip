@@ -105,7 +105,8 @@ __device__ __forceinline__ bool window_unit(const WindowCall& c, const WindowGri
             u.off = min(max(c.offsets[u.b], 0), tokens);
             u.n = min(max(c.offsets[u.b + 1], 0), tokens) - u.off;
             u.tile = slot - static_cast<int>(int64_t(u.off) * group / kWindowRows + u.b);
-            if (int64_t(u.tile) * kWindowRows >= int64_t(u.n) * group) return false;
+            // A tile before the sequence's first: offsets that do not ascend.
+            if (u.tile < 0 || int64_t(u.tile) * kWindowRows >= int64_t(u.n) * group) return false;
             u.length = static_cast<int>(min(int64_t(max(c.lengths[u.b], 0)), int64_t(c.table_width) * c.page.d));
         }
         for (int* p : {&u.off, &u.n, &u.length, &u.tile, &head}) *p = __builtin_amdgcn_readfirstlane(*p);

@@ -498,6 +498,19 @@ def test_chunk_bounds_of_device_sizes():
     assert (out == 3).all()
 
 
+def test_chunk_of_many_sequences_in_no_order():
+    """Offsets that go back and forth over more sequences than lanes of a wave: rows and pages that are no sequence's
+    stay as they were."""
+    batch, tokens, heads = 70, 100, 8
+    cache, table, lengths, _ = _cache([1] * batch, [64] * batch, 1, 64, 16, BF16)
+    offsets = torch.zeros(batch + 1, dtype=torch.int32)
+    offsets[:2] = torch.tensor([50, 100])
+    guard = torch.full((tokens + 400, heads, 64), 3.0, dtype=BF16, device="cuda")
+    q = _rand((tokens + 400, heads, 64), BF16, 3)[200:200 + tokens]
+    chunk_attention(q, cache, table.cuda(), lengths.cuda(), offsets.cuda(), out=guard[200:200 + tokens])
+    assert (guard[:250] == 3).all() and (guard[200 + tokens:] == 3).all()
+
+
 def test_chunk_of_nothing():
     cache, table, lengths, offsets = (t.cuda() if torch.is_tensor(t) else t for t in _cache([1], [9], 2, 64, 16, BF16))
     q = torch.empty((0, 2, 64), dtype=BF16, device="cuda")
