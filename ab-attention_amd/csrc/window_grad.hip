@@ -539,7 +539,8 @@ void plan_window_grad(WindowGradCall& c, int64_t& stat, int64_t& partial) {
         }
     }
     auto split = [&](int64_t units, int64_t steps) {
-        return static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(units, 1), steps / 8, 16})));
+        // No units: the sinks' tiles are all there are.
+        return units == 0 ? 1 : static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>({512 / units, steps / 8, 16})));
     };
     const int64_t seen = std::min<int64_t>(window, c.tokens);  // queries of a key tile, about
     const int64_t key_units = kv * (tiles - c.sink_tiles), query_units = bh * tiles;

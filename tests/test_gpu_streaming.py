@@ -269,6 +269,12 @@ def test_window_gradient_masks(window, sinks, frame):
     _grad_case(2, 3, 3, 517, 128, BF16, window, sinks, frame)
 
 
+@pytest.mark.parametrize("heads,kv_heads,window,sinks", [(2, 2, 400, 1000), (4, 1, 90, 900), (4, 1, 90, 870)])
+def test_window_gradient_sinks_in_all_tiles(heads, kv_heads, window, sinks):
+    """The sinks reach into the last tile of keys (or the one before it), and behind it."""
+    _grad_case(1, heads, kv_heads, 1000, 64, BF16, window, sinks, 1)
+
+
 @pytest.mark.parametrize("heads,kv_heads,token_major", [(8, 2, False), (6, 1, True), (4, 4, True)])
 def test_window_gradient_heads_and_strides(heads, kv_heads, token_major):
     _grad_case(2, heads, kv_heads, 333, 128, BF16, 60, 4, 1, token_major=token_major, with_lse=True)
