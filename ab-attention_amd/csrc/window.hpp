@@ -50,6 +50,7 @@ struct Bf16 {
     // Exponent bits of both halves, and what turns an exponent of all ones into
     // the half's sign bit when added.
     static constexpr uint32_t kExponent = 0x7f807f80u, kOverflow = 0x00800080u, kOne = 0x3f80u;
+    static constexpr int kLift = 0;  // log2 of what probabilities are rounded as multiples of
 };
 
 struct F16 {
@@ -69,6 +70,7 @@ struct F16 {
         return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w >> 16)));
     }
     static constexpr uint32_t kExponent = 0x7c007c00u, kOverflow = 0x04000400u, kOne = 0x3c00u;
+    static constexpr int kLift = 10;
 };
 
 // Transposing LDS read: within each 16-lane group, lane i receives element

@@ -12,7 +12,9 @@
 // each with S^T = Y1 X1^T and dP^T = Y2 X2^T on 16x16x32 MFMAs whose lanes hold
 // one owned row and four streamed ones, which is the form the second products
 // take P and dS in. P and dS are rounded to 16 bits there (the matrix cores'
-// input type); all sums are float32.
+// input type); all sums are float32. Below 2^-14, a probability among 16,384 equal
+// ones, fp16 has fewer bits: P is 2^10 P there until dV is stored. dS is as large as
+// dO makes it and stays as it is.
 // The first keys (sinks) are seen by every later query. Their tiles would run
 // many times longer than the others, so their queries are split into parts whose
 // float32 sums a third kernel adds up, always in the same order; so are all tiles of
@@ -40,11 +42,14 @@ constexpr int grad_lds() {
 }
 static_assert(kTileRows == 32, "stat blocks are 32 queries");
 
+template <class T>
+constexpr float kLowered = 1.0f / (1 << T::kLift);
+
 __device__ __forceinline__ int length_of(const WindowGradCall& c, int b) {
     return c.lengths ? min(max(c.lengths[b], 0), c.tokens) : c.tokens;
 }
 
-// stat of 32 queries of a head per workgroup: row r's normaliser and -delta, of the
+// stat of 32 queries of a head per workgroup: row r's normaliser (less kLift) and -delta, of the
 // output before it was rounded (out + out_rest): with out alone dQ and dK of 4 x
 // 4,099 tokens were 2.6e-3 off in bf16, 1.5 times the least that rounding them
 // leaves. Rows past the batch item's length get zeros: nothing
@@ -77,7 +82,7 @@ __global__ __launch_bounds__(256) void window_delta_kernel(WindowGradCall c, int
         for (int s = 1; s < kLanes; s *= 2) sum += __shfl_xor(sum, s);
         if (t < length && lane == 0) {
             const int64_t at = int64_t(bh) * c.tokens + t;
-            lse = c.lse[at];
+            lse = c.lse[at] - T::kLift;
             if (c.dlse) sum -= c.dlse[at] * 1.4426950408889634f;
         }
         if (lane == 0) {
@@ -207,7 +212,7 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
         if constexpr (!kKeys) {
             if (there) {
                 const float* stat = c.stat + (int64_t(head) * stat_blocks + (p >> 5)) * 64 + (p & 31);
-                lse[j] = stat[0];
+                lse[j] = stat[0] + T::kLift;
                 neg_delta[j] = stat[32];
             }
         }
@@ -359,6 +364,7 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     sc[j][r] = fast_exp2(__builtin_fmaf(sc[j][r], c.scale_log2, kKeys ? -row_lse[r] : -lse[j]));
+                    if constexpr (kKeys && T::kLift > 0) dp[j][r] *= kLowered<T>;
                     dp[j][r] *= sc[j][r];
                 }
             if (masked) {
@@ -429,7 +435,7 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_grad_kernel(WindowGr
             uint16_t* d2 = static_cast<uint16_t*>(c.dv) + b * c.dv_rows.batch + h * c.dv_rows.head + p * c.dv_rows.token + 4 * lg;
 #pragma unroll
             for (int m = 0; m < kBlocks; ++m) {
-                f32x4 g = acc2[m][j];
+                f32x4 g = acc2[m][j] * kLowered<T>;
                 if (live == 0.f) g = f32x4{0.f, 0.f, 0.f, 0.f};
                 *reinterpret_cast<u32x2*>(d2 + 16 * m) = u32x2{T::pack(g[0], g[1]), T::pack(g[2], g[3])};
             }
@@ -494,7 +500,7 @@ int launch_as(const WindowGradCall& c, hipStream_t stream) {
     if (int rc = ensure_lds_limit(reinterpret_cast<const void*>(by_queries), grad_lds<D, false>())) return rc;
     hipLaunchKernelGGL(by_keys, dim3(split + keys.size() * c.key_parts), dim3(kWindowThreads), (grad_lds<D, true>()), stream, c, keys);
     if (int rc = check_launch("window_grad_kernel")) return rc;
-    Sums s{c.partial, 0, c.sink_tiles, c.sink_parts, c.kv_heads, 2, {c.dk, c.dv}, {c.dk_rows, c.dv_rows}, {c.scale, 1.f}};
+    Sums s{c.partial, 0, c.sink_tiles, c.sink_parts, c.kv_heads, 2, {c.dk, c.dv}, {c.dk_rows, c.dv_rows}, {c.scale, kLowered<T>}};
     if (c.sink_tiles)
         if (int rc = sums(s, kv)) return rc;
     const int64_t each = int64_t(kWindowRows) * D;

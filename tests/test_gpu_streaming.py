@@ -357,6 +357,27 @@ def test_window_gradient_without_the_rest():
         assert (both[0].double() - w).norm() <= 1.001 * (g[0].double() - w).norm()
 
 
+def test_window_gradient_of_small_probabilities():
+    """fp16 keys that every query gives about 2^-18, where fp16 itself has a quarter of its bits: dV rounds them
+    relative to their size all the same."""
+    n, dim = 1000, 64
+    q, k, v, do = (_rand((1, 1, n, dim), F16, s) for s in (1, 2, 3, 4))
+    q[..., 0], k[..., 0] = 4, 0
+    k[:, :, 0] = 0
+    k[:, :, 0, 0] = 25  # 25 * 4 / 8 * log2(e): 18 above the others
+    do *= 32
+    leaf = v.clone().requires_grad_()
+    dv = torch.autograd.grad(window_attention(q, k, leaf), leaf, do)[0][0].double()
+    at = torch.arange(n, device="cuda")
+    mask = seen_mask(at, at, None, 0, 1)
+    (_, _, want), _ = attend_grad(q[0], k[0], v[0], do[0], mask)
+    p = torch.softmax((q[0].double() @ k[0].double().transpose(1, 2) / 8).masked_fill(~mask, -math.inf), -1)
+    # Every P rounded once with a sign of its own (a half step bounds the deviation), and the gradient once.
+    u = HALF_STEP[F16]
+    room = u * (p.transpose(1, 2) ** 2 @ do[0].double() ** 2)[:, 1:].sum().sqrt() + u * want[:, 1:].norm() + 2.0 ** -25 * (n * dim) ** 0.5
+    assert (dv - want)[:, 1:].norm() <= room
+
+
 def test_window_gradient_against_differences():
     """A directional derivative of a weighted sum of the output and the normaliser in 64 bits, by central differences of
     the definition, against the kernels' gradients."""
