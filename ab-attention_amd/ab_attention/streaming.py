@@ -268,7 +268,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
 
     Returns o in q's type and memory order, and with ``return_lse`` the base-2
     softmax normaliser as float32 [B, H, N]. Differentiable in q, k and v, through
-    both; the same inputs give the same gradients bit for bit. Values that are not
+    both; the same inputs give the same gradients bit for bit. In fp16 the logits'
+    gradients are rounded to fp16 on their way, so the losses of small gradients
+    want the scaling that is usual in fp16. Values that are not
     finite reach the results of the queries that see them only, but may reach any
     gradient of their batch item.
     """
@@ -358,6 +360,8 @@ def append_cache(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table
         raise ValueError("K and V must be packed tokens [T,H,D] of one shape and type")
     if _check_cache("append_cache", k, cache, page_table, lengths, offsets) != k.shape[1]:
         raise ValueError("K and V must have the cache's heads")
+    if any(not t.is_contiguous() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())) for t in cache):
+        raise ValueError("append_cache cannot write to an expanded cache")
     device = _gpu("append_cache", k, v)
     k, v = _strided(k), _strided(v)
     pages, heads, page, dim = cache.k.shape
@@ -392,8 +396,8 @@ def chunk_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
     if out is None:
         out = q.new_empty((tokens, heads, dim))
     elif (out.shape != q.shape or out.dtype != q.dtype or out.device != device or out.data_ptr() % 8 or out.stride(2) != 1
-          or any(n > 1 and s % 4 for n, s in zip(out.shape[:2], out.stride()))):
-        raise ValueError("out must be of Q's shape, type and device, with contiguous rows that start on 8 bytes")
+          or any(n > 1 and (s % 4 or s == 0) for n, s in zip(out.shape[:2], out.stride()))):
+        raise ValueError("out must be of Q's shape, type and device, with contiguous rows that start on 8 bytes, each its own")
     lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
     if tokens and page_table.shape[0]:
         pages, kv_heads, page, _ = cache.k.shape
@@ -438,6 +442,7 @@ class StreamingAttention:
         shape = (pages, heads, page_tokens, dim)
         self.caches = [PagedCache(*(torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(2)))
                        for _ in range(layers)]
+        self.device = self.caches[0].k.device  # with its index: other devices may become the current one
         self.free = list(range(pages - 1, -1, -1))
         self.tokens = [0] * sequences    # of each sequence, with those of the step that began last
         self.held = [{} for _ in range(sequences)]  # of each sequence: place in its table -> page

@@ -525,6 +525,18 @@ def test_chunk_bounds_of_device_sizes():
     assert (out == 3).all()
 
 
+def test_chunk_and_append_refuse_rows_that_share_memory():
+    cache, *where = _cache([4], [40], 2, 64, 16, BF16)
+    where = [t.cuda() for t in where]
+    x = _rand((4, 2, 64), BF16, 1)
+    with pytest.raises(ValueError, match="each its own"):
+        chunk_attention(x, cache, *where, out=x[:1].expand(4, 2, 64))
+    wide = PagedCache(cache.k, cache.v[:1].expand(cache.k.shape))
+    chunk_attention(x, wide, *where)  # may be read
+    with pytest.raises(ValueError, match="expanded"):
+        append_cache(wide, x, x, *where)
+
+
 def test_chunk_of_many_sequences_in_no_order():
     """Offsets that go back and forth over more sequences than lanes of a wave: rows and pages that are no sequence's
     stay as they were."""
