@@ -130,7 +130,8 @@ int window_call(const char* what, const ab_window_args& a, bool paged, WindowCal
 }
 
 size_t workspace_bytes(const WindowCall& c) {
-    return c.parts == 1 ? 0 : size_t(c.parts) * size_t(c.rows) * (size_t(c.dim) * sizeof(float) + sizeof(float2));
+    const size_t rounded = !c.paged && c.out_rest ? sizeof(float) : 0;
+    return c.parts == 1 ? 0 : size_t(c.parts) * size_t(c.rows) * (size_t(c.dim) * sizeof(float) + sizeof(float2) + rounded);
 }
 
 int window_launch(const char* what, const ab_window_args* a, bool paged, void* stream) {
@@ -150,6 +151,7 @@ int window_launch(const char* what, const ab_window_args* a, bool paged, void* s
         if (!aligned(a->workspace, 16)) return set_error(AB_ERR_INVALID, "%s: workspace must be 16-byte aligned", what);
         c.partial_o = static_cast<float*>(a->workspace);
         c.partial_stat = reinterpret_cast<float2*>(c.partial_o + c.parts * c.rows * c.dim);
+        c.partial_rounded = reinterpret_cast<float*>(c.partial_stat + c.parts * c.rows);
     }
     return launch_window(c, static_cast<hipStream_t>(stream));
 }

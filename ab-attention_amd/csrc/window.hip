@@ -17,7 +17,9 @@
 // next tile beside this tile's exponentials, this tile's second product beside the
 // next one's logits. The reference of a row moves only where a logit (base 2) passes
 // it by more than 8. P is rounded to the input type for the second product, the output
-// once at the end; sums are float32.
+// once at the end; sums are float32. For a backward pass the output is known better:
+// out + out_rest is the sum before its rounding, over the sum of the rounded P, whose
+// weights add up to one again (a row that one key carries owes nothing to P's rounding).
 //
 // What bounds it: with many keys the matrix cores at the board's power limit, with
 // the LDS (16 KiB read by each wave of a step) and the vector units (118
@@ -130,8 +132,8 @@ struct WindowTile {
     static constexpr int kLdsBytes = kVotes + 16;
 };
 
-// What rounding two values to `rounded` took from them, rounded itself (nothing of
-// values that are not finite).
+// What `rounded` lacks of two values, rounded itself (nothing of values that are not
+// finite).
 template <class T>
 __device__ __forceinline__ uint32_t rest_of(float a, float b, uint32_t rounded) {
     const float x = a - T::lo(rounded), y = b - T::hi(rounded);
@@ -393,8 +395,9 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     };
 
     f32x4 o_acc[kBlocks][2];  // dims 16b + 4lg .. + 3 of row 16j + li
-    // Reference and sum of row j; -inf until the row's first finite logit, then kSlack.
-    float m_run[2], l_run[2], slack[2];
+    // Reference of row j, sum of its weights, for out_rest the same of the rounded ones;
+    // -inf until the row's first finite logit, then kSlack.
+    float m_run[2], l_run[2], r_run[2], slack[2];
     auto reset = [&]() {
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b)
@@ -403,7 +406,7 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             m_run[j] = 0.f;
-            l_run[j] = 0.f;
+            l_run[j] = r_run[j] = 0.f;
             slack[j] = -INFINITY;
         }
     };
@@ -447,6 +450,7 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
             slack[j] = grow ? kSlack : slack[j];
             m_run[j] += shift;
             l_run[j] *= alpha;
+            r_run[j] *= alpha;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) o_acc[b][j] *= alpha;
 #pragma unroll
@@ -514,6 +518,10 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
             asm volatile("" : "+v"(psum[0]), "+v"(psum[1]));
             l_run[0] += psum[0];
             l_run[1] += psum[1];
+            if constexpr (!kPaged)
+                if (c.out_rest)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) r_run[i >> 2] = T::add(pw[i >> 2][i & 3], r_run[i >> 2]);
             if (is_masked(t)) {
 #pragma unroll
                 for (int b = 0; b < kBlocks; ++b)
@@ -644,6 +652,7 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
                         const float a = fast_exp2(s[n][r]), b = fast_exp2(s[n][r + 1]);
                         l_run[n & 1] += a + b;
                         pw[n & 1][2 * (n >> 1) + r / 2] = T::pack(a, b);
+                        r_run[n & 1] = T::add(pw[n & 1][2 * (n >> 1) + r / 2], r_run[n & 1]);
                         sees[n & 1][2 * (n >> 1) + r / 2] = (bits >> r & 1 ? T::kOne : 0u) | (bits >> (r + 1) & 1 ? T::kOne << 16 : 0u);
                     }
                 }
@@ -684,22 +693,28 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     if (!active) return;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        const auto s16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(l_run[j]), __float_as_uint(l_run[j]), false, false);
-        const float l16 = __uint_as_float(s16[0]) + __uint_as_float(s16[1]);
-        const auto s32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(l16), __float_as_uint(l16), false, false);
-        const float l = __uint_as_float(s32[0]) + __uint_as_float(s32[1]);
+        auto over_rows = [](float x) {  // the sum over the four lanes of a row
+            const auto s16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+            const float y = __uint_as_float(s16[0]) + __uint_as_float(s16[1]);
+            const auto s32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+            return __uint_as_float(s32[0]) + __uint_as_float(s32[1]);
+        };
+        const float l = over_rows(l_run[j]), rounded = over_rows(r_run[j]);
         int token, head;
         if (!row_of(j, token, head)) continue;
         const int64_t stat_at = u.b * c.row.batch + head * c.row.head + int64_t(u.off + token) * c.row.token;
         if constexpr (kSplit) {
             const int64_t at = blockIdx.y * c.rows + stat_at;
-            if (lg == 0) c.partial_stat[at] = float2{slack[j] == kSlack ? m_run[j] : -INFINITY, l};
+            if (lg == 0) {
+                c.partial_stat[at] = float2{slack[j] == kSlack ? m_run[j] : -INFINITY, l};
+                if (!kPaged && c.out_rest) c.partial_rounded[at] = rounded;
+            }
             if (l == 0.f) continue;
             float* dst = c.partial_o + at * D + 4 * lg;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) *reinterpret_cast<f32x4*>(dst + 16 * b) = o_acc[b][j];
         } else {
-            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            const float inv = l == 0.f ? 0.f : 1.0f / l, better = kPaged || rounded == 0.f ? inv : 1.0f / rounded;
             uint16_t* orow = static_cast<uint16_t*>(c.out) + u.b * c.out_rows.batch + head * c.out_rows.head +
                              int64_t(u.off + token) * c.out_rows.token + 4 * lg;
 #pragma unroll
@@ -707,9 +722,11 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
                 const f32x4 o = o_acc[b][j] * inv;
                 const u32x2 w = {T::pack(o[0], o[1]), T::pack(o[2], o[3])};
                 *reinterpret_cast<u32x2*>(orow + 16 * b) = w;
-                if (c.out_rest)
+                if (c.out_rest) {
+                    const f32x4 before = o_acc[b][j] * better;
                     *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(c.out_rest) + (orow - static_cast<uint16_t*>(c.out)) + 16 * b) =
-                        u32x2{rest_of<T>(o[0], o[1], w[0]), rest_of<T>(o[2], o[3], w[1])};
+                        u32x2{rest_of<T>(before[0], before[1], w[0]), rest_of<T>(before[2], before[3], w[1])};
+                }
             }
             if (c.lse && lg == 0) c.lse[stat_at] = l == 0.f ? -INFINITY : m_run[j] + log2f(l);
         }
@@ -737,15 +754,23 @@ __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
         out_at = b * c.out_rows.batch + head * c.out_rows.head + token * c.out_rows.token;
     }
     float2 stat = {-INFINITY, 0.f};
-    if (lane < c.parts) stat = c.partial_stat[lane * c.rows + row];
+    float rounded = 0.f;
+    if (lane < c.parts) {
+        stat = c.partial_stat[lane * c.rows + row];
+        if (!kPaged && c.out_rest) rounded = c.partial_rounded[lane * c.rows + row];
+    }
     const bool some = stat.y != 0.f;  // a part without a key has written no row
     float m = some ? stat.x : -INFINITY;
 #pragma unroll
     for (int s = 1; s < 64; s *= 2) m = fmaxf(m, __shfl_xor(m, s));
     const float weight = some ? fast_exp2(stat.x - m) : 0.f;
     float l = some ? weight * stat.y : 0.f, o[D / 64] = {};
+    rounded = some ? weight * rounded : 0.f;
 #pragma unroll
-    for (int s = 1; s < 64; s *= 2) l += __shfl_xor(l, s);
+    for (int s = 1; s < 64; s *= 2) {
+        l += __shfl_xor(l, s);
+        rounded += __shfl_xor(rounded, s);
+    }
     constexpr int kAhead = 4;
     for (int p0 = 0; p0 < c.parts; p0 += kAhead) {
         float x[kAhead][D / 64];
@@ -763,10 +788,10 @@ __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
             for (int e = 0; e < D / 64; ++e) o[e] += w != 0.f ? w * x[i][e] : 0.f;
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const float inv = l == 0.f ? 0.f : 1.0f / l, better = kPaged || rounded == 0.f ? inv : 1.0f / rounded;
     const int64_t at = out_at + lane * (D / 64);
-    const float first = o[0] * inv, second = D == 128 ? o[D / 64 - 1] * inv : 0.f;
-    const uint32_t w = T::pack(first, second), rest = rest_of<T>(first, second, w);
+    const float first = o[0], second = D == 128 ? o[D / 64 - 1] : 0.f;
+    const uint32_t w = T::pack(first * inv, second * inv), rest = rest_of<T>(first * better, second * better, w);
     auto store = [&](void* to, uint32_t value) {
         if constexpr (D == 128)
             *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(to) + at) = value;

@@ -45,6 +45,11 @@ struct Bf16 {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16(lo, hi); }
+    // c + both halves.
+    static __device__ __forceinline__ float add(uint32_t w, float c) {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, kOne * 0x10001u), c, false);
+    }
     static __device__ __forceinline__ float lo(uint32_t w) { return bf16_lo(w); }
     static __device__ __forceinline__ float hi(uint32_t w) { return bf16_hi(w); }
     // Exponent bits of both halves, and what turns an exponent of all ones into
@@ -62,6 +67,10 @@ struct F16 {
         typedef float f32x2 __attribute__((ext_vector_type(2)));
         const f32x2 v = {lo, hi};
         return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+    }
+    static __device__ __forceinline__ float add(uint32_t w, float c) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), __builtin_bit_cast(f16x2, kOne * 0x10001u), c, false);
     }
     static __device__ __forceinline__ float lo(uint32_t w) {
         return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w)));
@@ -140,7 +149,7 @@ struct Rows {
 // offsets[b] .. offsets[b + 1]. `row` gives the place of a query's normaliser.
 struct WindowCall {
     const void *q, *k, *v;
-    void *out, *out_rest;  // out_rest: what out's rounding took, or none
+    void *out, *out_rest;  // out_rest: what out lacks of a better one, or none
     float* lse;
     Rows q_rows, k_rows, v_rows, out_rows, row;
     int32_t batch, heads, kv_heads, tokens;  // tokens: of a batch item, or packed rows in all
@@ -154,6 +163,7 @@ struct WindowCall {
     int32_t parts;                           // parts that every tile's keys are split into
     float* partial_o;                        // [parts][rows][dim] with workspace
     float2* partial_stat;                    // [parts][rows]: reference and sum
+    float* partial_rounded;                  // [parts][rows], for a tensor's out_rest: sum of the rounded weights
     int64_t rows;                            // queries times heads
 };
 

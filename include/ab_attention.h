@@ -285,7 +285,8 @@ int ab_rotary(const ab_rotary_args *args, void *stream);
  *   offsets[batch] on are left as they are. lse f32 [tokens, heads].
  *
  * out_rest (NULL, or of out's strides and type) gets what out's rounding took from
- * the result, rounded itself: ab_window_attention_grad makes its delta of the two.
+ * the result, and of a tensor what rounding the weights did to their sum, rounded
+ * itself: ab_window_attention_grad makes its delta of the two.
  * Strides in elements, multiples of 8 (out: of 4); q, k, v 16-byte aligned, out 8.
  * Limits: tokens and positions under 2^30, a head of k or v (of a page) under 4 GiB.
  * Calls that leave CUs idle split their keys over workgroups with a workspace of

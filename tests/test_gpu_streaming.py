@@ -525,6 +525,53 @@ def test_chunk_bounds_of_device_sizes():
     assert (out == 3).all()
 
 
+def test_chunk_and_window_rest_of_the_output():
+    """The C entries with out_rest: the same output, and together with the rest nearer to the definition. A query of
+    one key's weight alone has just that key's value."""
+    from ab_attention import _lib
+    from ab_attention import streaming as st
+
+    tokens, heads, dim = 700, 3, 64
+    q, k, v = (_rand((1, heads, tokens, dim), BF16, s, 2.0 if s == 1 else 1.0) for s in (1, 2, 3))
+    how = (300, 4, 1, dim ** -0.5)
+    rest = torch.empty_like(q)
+    out, _ = st._window_forward(q, k, v, None, *how, False, rest)
+    assert torch.equal(out, window_attention(q, k, v, window=300, sinks=4))
+    assert torch.equal(out, window_attention(q, k, v.clone().requires_grad_(), window=300, sinks=4))
+    at = torch.arange(tokens, device="cuda")
+    o, _, _ = attend(q[0], k[0], v[0], seen_mask(at, at, 300, 4, 1))
+    both = out[0].double() + rest[0].double()
+    assert (both - o).norm() < 0.9 * (out[0].double() - o).norm()
+    assert torch.equal(both[:, 0], v[0, :, 0].double())
+
+    few = [t[:, :1, :140].contiguous() for t in (q, k, v)]  # so few rows that their keys are split
+    rest = torch.empty_like(few[0])
+    packed = st._window_args(*few, rest, rest, None, None, 0, 0, 1, dim ** -0.5)
+    out, _ = st._window_forward(*few, None, 0, 0, 1, dim ** -0.5, False, rest)
+    assert torch.equal(out, window_attention(*few)) and _lib.raw("ab_window_workspace_bytes")(packed) % (dim * 4 + 12) == 0
+    o, _, _ = attend(*(t[0] for t in few), seen_mask(at[:140], at[:140], None, 0, 1))
+    both = out[0].double() + rest[0].double()
+    assert (both - o).norm() < 0.9 * (out[0].double() - o).norm()
+    assert torch.equal(both[:, 0], few[2][0, :, 0].double())
+
+    cache, table, lengths, offsets = _cache([5, 1], [130, 4000], heads, dim, 16, BF16)
+    q = _rand((6, heads, dim), BF16, 5, 2.0)
+    want = chunk_attention(q, cache, table.cuda(), lengths.cuda(), offsets.cuda())
+    dev = [t.cuda() for t in (lengths, offsets, table)]
+    out, rest = torch.empty_like(q), torch.full_like(q, 9.0)
+    for size in (0, 1 << 24):  # whole rows, rows in parts
+        workspace = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
+        packed = st._WINDOW.pack(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), out.data_ptr(), rest.data_ptr(), 0,
+                                 *(t.data_ptr() for t in dev), 2, heads, heads, 6, dim, 0, cache.k.shape[0], 16, table.shape[1],
+                                 0, 0, 1, dim ** -0.5, 0, q.stride(1), q.stride(0), *cache.k.stride()[:3],
+                                 *cache.v.stride()[:3], 0, out.stride(1), out.stride(0), workspace.data_ptr() if size else 0, size)
+        assert _lib.raw("ab_window_workspace_bytes")(packed) <= 1 << 24
+        st._call("ab_chunk_attention", q.device, packed)
+        # What rounding the output took is at most half a step of it, and what is left of that its own rounding.
+        assert (rest.double().abs() <= 2.0 ** -8 * out.double().abs() + 1e-6).all()
+    assert torch.equal(out, want)
+
+
 def test_chunk_and_append_refuse_rows_that_share_memory():
     cache, *where = _cache([4], [40], 2, 64, 16, BF16)
     where = [t.cuda() for t in where]
