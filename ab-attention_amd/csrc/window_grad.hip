@@ -21,8 +21,8 @@
 // calls with too few of them to fill the chip.
 // What bounds it: the matrix cores at the power limit and the LDS, whose operand
 // reads (one 1 KiB fragment for two MFMAs) take as long as they do. 12 heads of
-// 32,760 tokens, window of four frames of 1,560: keys 2,764 us (1,024 TFLOP/s over
-// four products), queries 1,861 (1,140 over three), deltas 40 to 49, sinks 28. One
+// 32,760 tokens, window of four frames of 1,560: keys 2,645 us (1,070 TFLOP/s over
+// four products), queries 1,804 (1,180 over three), deltas 49, sinks 29. One
 // kernel with the five products alone would have to add dQ up with atomics, in an
 // order of its own each time.
 #include <algorithm>
