@@ -254,12 +254,17 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
         bool bad = false;
         auto scan = [&](int from, int to) {
             const int page = static_cast<int>(c.page.d);
-            for (int i = from / page + tid; i <= (to - 1) / page; i += kWindowThreads)
+            for (int i = from / page + tid; from < to && i <= (to - 1) / page; i += kWindowThreads)
                 bad |= static_cast<uint32_t>(table[i]) >= static_cast<uint32_t>(c.pages);
         };
         if (tiles > 0) {
             const int last = tile0 + tiles - 1;
-            if (tile0 < range.sink_tiles) scan(range.key(tile0), min(mask.sinks, end));
+            if (tile0 < range.sink_tiles) {
+                // The window may begin in the sinks' last tile.
+                const int from = range.key(tile0), to = min(kWindowKeys * min(last + 1, range.sink_tiles), end);
+                scan(from, min(mask.sinks, to));
+                scan(max(mask.low(p_first), from), to);
+            }
             if (last >= range.sink_tiles) scan(range.key(max(tile0, range.sink_tiles)), min(range.key(last) + kWindowKeys, end));
         }
         uint32_t* votes = reinterpret_cast<uint32_t*>(smem + Tile::kVotes);
