@@ -39,7 +39,17 @@ namespace ab {
 namespace {
 
 constexpr int kRing = 4;         // stages of K and of V in LDS
-constexpr float kSlack = 8.0f;  // largest logit (base 2) above a row's reference: P stays within 2^8
+// Base 2: how far a row's reference is below its largest logit when it is moved, and
+// the largest logit above it, so how large P is. Thousands of weights far below the
+// largest one (a sink that takes nearly all of it) add up, and below 2^-14 fp16 has
+// fewer bits: there P reaches up to 2^15.9, which keeps all bits of weights down to
+// 2^-22 of the largest and takes at most 2^-33 of it from any. The reference moves
+// about as often as with bf16's slack of 8 (fp16 480p case 1,515 to 1,517 us; 11 below
+// and a slack of 4 are 1,571).
+template <class T>
+constexpr float kBelow = T::kLift > 0 ? 8.0f : 0.0f;
+template <class T>
+constexpr float kSlack = T::kLift > 0 ? 15.9f : 8.0f;
 
 // What a workgroup works on. The same in all its lanes.
 struct WindowUnit {
@@ -440,8 +450,8 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
                 }
             }
     };
-    // Moves the reference of the rows whose maximum has risen by more than kSlack
-    // above it (or that have none yet): their sums, and the logits at hand, follow.
+    // Moves the reference of the rows whose maximum has risen more than kSlack above
+    // it (or that have none yet): their sums, and the logits at hand, follow.
     auto move_reference = [&](f32x4 (&s)[4], float (&mx)[2]) {
         // A lane's own keys show it: no exchange while nothing grows.
         if (!__any(mx[0] > slack[0] || mx[1] > slack[1])) return;
@@ -450,9 +460,9 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const bool grow = j ? grow1 : grow0;
-            const float shift = grow ? mx[j] : 0.f;
-            const float alpha = slack[j] == kSlack ? fast_exp2(-shift) : 1.f;  // the sums are 0 before
-            slack[j] = grow ? kSlack : slack[j];
+            const float shift = grow ? mx[j] - kBelow<T> : 0.f;
+            const float alpha = slack[j] == kSlack<T> ? fast_exp2(-shift) : 1.f;  // the sums are 0 before
+            slack[j] = grow ? kSlack<T> : slack[j];
             m_run[j] += shift;
             l_run[j] *= alpha;
             r_run[j] *= alpha;
@@ -711,7 +721,7 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
         if constexpr (kSplit) {
             const int64_t at = blockIdx.y * c.rows + stat_at;
             if (lg == 0) {
-                c.partial_stat[at] = float2{slack[j] == kSlack ? m_run[j] : -INFINITY, l};
+                c.partial_stat[at] = float2{slack[j] == kSlack<T> ? m_run[j] : -INFINITY, l};
                 if (!kPaged && c.out_rest) c.partial_rounded[at] = rounded;
             }
             if (l == 0.f) continue;

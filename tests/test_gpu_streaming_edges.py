@@ -1,13 +1,16 @@
 """Streaming operators on the GPU where tables, offsets and values are at the edge of what the interface allows."""
+import math
+
 import pytest
 import torch
 
-from ab_attention.streaming import chunk_attention
+from ab_attention.streaming import PagedCache, chunk_attention, window_attention
+from streaming_reference import attend, check_output, seen_mask
 from test_gpu_streaming import _cache, _check_chunk, _rand
 
 pytestmark = pytest.mark.gpu
 
-BF16 = torch.bfloat16
+BF16, F16 = torch.bfloat16, torch.float16
 
 
 @pytest.mark.parametrize("page,window,sinks,frame,length", [(8, 10, 4, 1, 20), (16, 40, 4, 1, 60), (8, 20, 33, 1, 64), (8, 2, 1, 7, 28),
@@ -25,3 +28,35 @@ def test_chunk_holes_in_the_last_tile_of_sinks(page, window, sinks, frame, lengt
         out, lse = chunk_attention(q, cache, table.cuda(), lengths.cuda(), offsets.cuda(), window=window, sinks=sinks, frame=frame,
                                    return_lse=True)
         _check_chunk(out, lse, q, cache, table, lengths, offsets, window, sinks, frame, BF16)
+
+
+def _under_a_sink(n, heads, drop, spread, seed=0):
+    """q, k, v [1, heads, n, 64] in fp16 of a first key that is `drop` (base 2) above the others and has no value."""
+    q, k, v = (_rand((1, heads, n, 64), F16, seed + s) for s in (1, 2, 3))
+    k *= spread
+    q[..., 0], k[..., 0] = 4, 0
+    k[:, :, 0] = 0
+    k[:, :, 0, 0] = drop * 8 / (4 * math.log2(math.e))
+    v[:, :, 0] = 0
+    return q, k, v
+
+
+@pytest.mark.parametrize("drop,spread", [(12, 1.0), (18, 0.0), (18, 1.0), (21.6, 0.0), (21.6, 1.0), (24, 0.0), (24, 1.0)])
+def test_fp16_output_of_small_probabilities(drop, spread):
+    """A sink that takes nearly all the weight and gives nothing: the output is the sum of thousands of weights that are
+    each rounded relative to their own size. Whole and split rows, tensors and caches."""
+    for n, heads in ((4000, 17), (1300, 1)):
+        q, k, v = _under_a_sink(n, heads, drop, spread)
+        at = torch.arange(n, device="cuda")
+        o, _, size = attend(q[0], k[0], v[0], seen_mask(at, at, None, 0, 1))
+        check_output(window_attention(q, k, v)[0], o, size, F16)
+        check_output(window_attention(q.clone().requires_grad_(), k, v)[0].detach(), o, size, F16)
+    width = 4000 // 16
+    cache = PagedCache(*(t[0, :1].reshape(1, width, 16, 64).transpose(0, 1).contiguous() for t in _under_a_sink(4000, 1, drop, spread)[1:]))
+    dev = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    table = torch.arange(width, dtype=torch.int32, device="cuda")[None]
+    for new, group in ((1, 8), (3000, 16)):
+        q = _rand((new, group, 64), F16, 9)
+        q[..., 0] = 4
+        out, lse = chunk_attention(q, cache, table, dev(4000), dev(0, new), return_lse=True)
+        _check_chunk(out, lse, q, cache, table.cpu(), dev(4000), dev(0, new), None, 0, 1, F16)
