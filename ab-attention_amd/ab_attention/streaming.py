@@ -352,9 +352,10 @@ def append_cache(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table
     """Writes the new keys and values k, v [T, heads, D] into the cache, in place.
 
     Sequence b's new tokens are the rows offsets[b] .. offsets[b + 1] - 1 (int32
-    [B + 1], ascending); ``lengths`` int32 [B] are the tokens of each sequence with
-    the new ones, so that its last row goes to position lengths[b] - 1. Rows whose
-    entry in the page table is no page are dropped. Returns the cache.
+    [B + 1], ascending, bounded to 0 .. T); ``lengths`` int32 [B] are the tokens of
+    each sequence with the new ones, so that its last row goes to position
+    lengths[b] - 1. Rows whose entry in the page table is no page are dropped.
+    Returns the cache.
     """
     if k.shape != v.shape or v.dtype != k.dtype:
         raise ValueError("K and V must be packed tokens [T,H,D] of one shape and type")

@@ -20,7 +20,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendCall c) {
     }
     const int b = __builtin_amdgcn_readfirstlane(before) - 1;
     if (b < 0) return;
-    const int next = c.offsets[b + 1];
+    const int next = min(c.offsets[b + 1], c.tokens);  // as the attention bounds it, so that both see the same positions
     if (row >= next) return;
     const int64_t position = int64_t(c.lengths[b]) - next + row;
     if (position < 0 || position >= int64_t(c.table_width) * c.page.d) return;

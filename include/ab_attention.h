@@ -278,7 +278,8 @@ int ab_rotary(const ab_rotary_args *args, void *stream);
  * ab_chunk_attention: the packed new tokens of `batch` sequences over a paged
  *   cache. q and out [tokens, heads, dim] (their batch stride is not used);
  *   sequence b has the rows offsets[b] .. offsets[b + 1] - 1 (int32
- *   [batch + 1], ascending), the last of which is at position lengths[b] - 1. k, v
+ *   [batch + 1], ascending; what exceeds 0 .. tokens counts as that bound), the
+ *   last of which is at position lengths[b] - 1. k, v
  *   [pages, kv_heads, page_tokens, dim] (strides page, head, token), page_tokens a
  *   multiple of 8; page_table int32 [batch, table_width]. An entry outside
  *   [0, pages) is no page: its keys are not seen. Rows before offsets[0] and from

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from ab_attention.streaming import PagedCache, chunk_attention, window_attention
+from ab_attention.streaming import PagedCache, append_cache, chunk_attention, window_attention
 from streaming_reference import attend, check_output, seen_mask
 from test_gpu_streaming import _cache, _check_chunk, _rand
 
@@ -60,3 +60,22 @@ def test_fp16_output_of_small_probabilities(drop, spread):
         q[..., 0] = 4
         out, lse = chunk_attention(q, cache, table, dev(4000), dev(0, new), return_lse=True)
         _check_chunk(out, lse, q, cache, table.cpu(), dev(4000), dev(0, new), None, 0, 1, F16)
+
+
+def test_append_and_chunk_agree_on_offsets_beyond_the_rows():
+    """Offsets past the packed rows count as their end, those below 0 as 0: append_cache and chunk_attention place the
+    rows alike, and write nothing else."""
+    cache, table, lengths, offsets = _cache([3, 4], [50, 70], 2, 64, 16, BF16)
+    k, v, q = (_rand((7, h, 64), BF16, s, 2.0) for s, h in ((1, 2), (2, 2), (3, 4)))
+    dev = [table.cuda(), lengths.cuda()]
+    want = append_cache(PagedCache(*(t.clone() for t in cache)), k, v, *dev, offsets.cuda())
+    o, lse = chunk_attention(q, want, *dev, offsets.cuda(), return_lse=True)
+    for first, last in ((0, 9), (0, 2 ** 31 - 1), (-2, 7), (-2 ** 31, 40)):
+        far = torch.tensor([first, 3, last], dtype=torch.int32, device="cuda")
+        got = append_cache(PagedCache(*(t.clone() for t in cache)), k, v, *dev, far)
+        assert torch.equal(got.k, want.k) and torch.equal(got.v, want.v), (first, last)
+        guard = torch.full((20, 4, 64), 3.0, dtype=BF16, device="cuda")
+        out, l = chunk_attention(q, got, *dev, far, return_lse=True, out=guard[6:13])
+        assert torch.equal(out, o) and torch.equal(l, lse), (first, last)
+        assert (guard[:6] == 3).all() and (guard[13:] == 3).all()
+    _check_chunk(o, lse, q, want, table, lengths, offsets, None, 0, 1, BF16)
