@@ -775,6 +775,7 @@ __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
         if (!kPaged && c.out_rest) rounded = c.partial_rounded[lane * c.rows + row];
     }
     const bool some = stat.y != 0.f;  // a part without a key has written no row
+    const uint64_t written = __ballot(some);
     float m = some ? stat.x : -INFINITY;
 #pragma unroll
     for (int s = 1; s < 64; s *= 2) m = fmaxf(m, __shfl_xor(m, s));
@@ -798,9 +799,11 @@ __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             if (p0 + i >= c.parts) break;
+            if (!(written >> (p0 + i) & 1)) continue;
             const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), p0 + i));
+            // An infinite value is seen however small its part's weight is.
 #pragma unroll
-            for (int e = 0; e < D / 64; ++e) o[e] += w != 0.f ? w * x[i][e] : 0.f;
+            for (int e = 0; e < D / 64; ++e) o[e] += w == 0.f && !(fabsf(x[i][e]) < INFINITY) ? x[i][e] : w * x[i][e];
         }
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l, better = kPaged || rounded == 0.f ? inv : 1.0f / rounded;

@@ -79,3 +79,25 @@ def test_append_and_chunk_agree_on_offsets_beyond_the_rows():
         assert torch.equal(out, o) and torch.equal(l, lse), (first, last)
         assert (guard[:6] == 3).all() and (guard[13:] == 3).all()
     _check_chunk(o, lse, q, want, table, lengths, offsets, None, 0, 1, BF16)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_chunk_values_that_are_not_finite_whatever_the_split(value):
+    """A key whose weight is far below float32's smallest, with a value that is not finite: the query sees it, alone in
+    the call (its keys split over workgroups) and beside 600 others (not split)."""
+    n, width = 8000, 125
+    table = torch.full((601, width), -1, dtype=torch.int32)
+    table[0] = torch.arange(width, dtype=torch.int32)
+    table[1:, 0] = torch.arange(width, width + 600, dtype=torch.int32)
+    cache = PagedCache(*(_rand((width + 600, 1, 64, 128), BF16, s) for s in (1, 2)))
+    q = _rand((601, 1, 128), BF16, 3)
+    q[0, 0, 0], cache.k[..., 0] = 16, 0
+    cache.k[100, 0, 7, 0] = 160  # position 6407: 16 * 160 / sqrt(128) * log2(e), some 326 above the others
+    cache.v[3, 0, 9, 5] = value  # position 201
+    dev = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    whole = chunk_attention(q, cache, table.cuda(), dev(n, *[33] * 600), dev(*range(602)))
+    split = chunk_attention(q[:1], cache, table[:1].cuda(), dev(n), dev(0, 1))
+    for out in (whole, split):
+        assert not out[0, 0, 5].isfinite()
+        rest = [i for i in range(128) if i != 5]
+        assert torch.equal(out[0, 0, rest], cache.v[100, 0, 7, rest])
