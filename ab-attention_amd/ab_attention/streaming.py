@@ -30,6 +30,7 @@ import struct
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -61,6 +62,13 @@ def _gpu(name: str, first, *others):
         if t is not None and t.device != device:
             raise ValueError(f"{name} requires tensors on one CUDA device")
     return device
+
+
+def _no_tangent(name: str, *tensors):
+    """Refuses tensors with a forward-mode tangent, which the kernels would drop."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise ValueError(f"{name} has no forward-mode derivative")
 
 
 def _call(entry: str, device, packed: bytes):
@@ -108,6 +116,7 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
+        _no_tangent("the gradient of rotary", dq, dk)
         (positions,) = ctx.saved_tensors
         if dq is None:  # only K's result was used
             dq, dk = dk, None
@@ -146,7 +155,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
     behind the axes' stay as they are. D is a multiple of 8; bf16, fp16 or float32.
 
     Returns (q, k) as new tensors (k None if it was), in the memory order of the
-    inputs. Differentiable in q and k (the gradient is the opposite rotation).
+    inputs. Differentiable in q and k (the gradient is the opposite rotation), in
+    reverse mode only.
     """
     if q.ndim != 4 or (k is not None and (k.ndim != 4 or k.shape[::2] != q.shape[::2] or k.shape[3] != q.shape[3])):
         raise ValueError("rotary requires Q [B,H,N,D] and K [B,Hk,N,D] of the same batch, tokens and dim")
@@ -164,6 +174,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
     shape = positions.shape
     if shape != (tokens, len(axes)) and shape != (batch, tokens, len(axes)):
         raise ValueError(f"positions must be [{tokens}, {len(axes)}] or [{batch}, {tokens}, {len(axes)}]")
+    _no_tangent("rotary", q, k, positions)
     _gpu("rotary", q, k, positions)
     if q.shape[1] == 0 or (k is not None and k.shape[1] == 0):
         raise ValueError("rotary requires at least one head")
@@ -240,6 +251,7 @@ class _Window(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dlse):
+        _no_tangent("the gradient of window attention", dout, dlse)
         q, k, v, out, rest, lse, lengths = ctx.saved_tensors
         if dout is None and dlse is None:
             return (None,) * (4 + len(ctx.how))
@@ -268,7 +280,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
 
     Returns o in q's type and memory order, and with ``return_lse`` the base-2
     softmax normaliser as float32 [B, H, N]. Differentiable in q, k and v, through
-    both; the same inputs give the same gradients bit for bit. In fp16 the logits'
+    both, in reverse mode only; the same inputs give the same gradients bit for bit. In fp16 the logits'
     gradients are rounded to fp16 on their way, so the losses of small gradients
     want the scaling that is usual in fp16. Values that are not
     finite reach the results of the queries that see them only, but may reach any
@@ -291,6 +303,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     window, sinks, frame = _mask(window, sinks, frame)
     if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != q.shape[:1] or not lengths.is_contiguous()):
         raise ValueError("lengths must be int32 [B]")
+    _no_tangent("window attention", q, k, v)
     _gpu("window attention", q, k, v, lengths)
     how = (window, sinks, frame, scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
@@ -343,6 +356,7 @@ def _check_cache(name, x, cache, page_table, lengths, offsets):
     for t in (page_table, lengths, offsets):
         if t.dtype != torch.int32 or not t.is_contiguous():
             raise ValueError("page_table, lengths and offsets must be contiguous int32")
+    _no_tangent(name, x, k, v)
     _gpu(name, x, k, v, page_table, lengths, offsets)
     return kv_heads
 
@@ -363,6 +377,7 @@ def append_cache(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table
         raise ValueError("K and V must have the cache's heads")
     if any(not t.is_contiguous() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())) for t in cache):
         raise ValueError("append_cache cannot write to an expanded cache")
+    _no_tangent("append_cache", v)
     device = _gpu("append_cache", k, v)
     k, v = _strided(k), _strided(v)
     pages, heads, page, dim = cache.k.shape
