@@ -31,6 +31,7 @@ from typing import NamedTuple
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -69,6 +70,15 @@ def _no_tangent(name: str, *tensors):
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
                                               for t in tensors):
         raise ValueError(f"{name} has no forward-mode derivative")
+
+
+def _writes(name: str, *tensors):
+    """Tells autograd of writes that go past it, as torch's in-place operations do, so
+    that a gradient which still needs the old values raises."""
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} cannot write to a tensor that requires a gradient")
+    increment_version([t for t in tensors if not t.is_inference()])
 
 
 def _call(entry: str, device, packed: bytes):
@@ -369,7 +379,7 @@ def append_cache(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table
     [B + 1], ascending, bounded to 0 .. T); ``lengths`` int32 [B] are the tokens of
     each sequence with the new ones, so that its last row goes to position
     lengths[b] - 1. Rows whose entry in the page table is no page are dropped.
-    Returns the cache.
+    Returns the cache. Not differentiable: no gradient reaches k and v by it.
     """
     if k.shape != v.shape or v.dtype != k.dtype:
         raise ValueError("K and V must be packed tokens [T,H,D] of one shape and type")
@@ -380,6 +390,7 @@ def append_cache(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table
     _no_tangent("append_cache", v)
     device = _gpu("append_cache", k, v)
     k, v = _strided(k), _strided(v)
+    _writes("append_cache", *cache)
     pages, heads, page, dim = cache.k.shape
     _call("ab_append_cache", device, _APPEND.pack(
         k.data_ptr(), v.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), lengths.data_ptr(), offsets.data_ptr(),
@@ -397,7 +408,8 @@ def chunk_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
     of n is at position lengths[b] - n + i of the mask above. Keys in places that
     the page table gives no page are not seen, and nothing outside of the pages'
     visible tokens is read. D is 64 or 128, bf16 or fp16; H is a multiple of the
-    cache's heads.
+    cache's heads. Not differentiable: the result never requires a gradient, also
+    where q or the cache does (train with ``window_attention``).
 
     Returns o [T, H, D] and with ``return_lse`` the base-2 normaliser float32
     [T, H]. Rows outside of offsets[0] .. offsets[B] - 1 are not written (with
@@ -414,6 +426,8 @@ def chunk_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
     elif (out.shape != q.shape or out.dtype != q.dtype or out.device != device or out.data_ptr() % 8 or out.stride(2) != 1
           or any(n > 1 and (s % 4 or s == 0) for n, s in zip(out.shape[:2], out.stride()))):
         raise ValueError("out must be of Q's shape, type and device, with contiguous rows that start on 8 bytes, each its own")
+    else:
+        _writes("chunk attention", out)
     lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
     if tokens and page_table.shape[0]:
         pages, kv_heads, page, _ = cache.k.shape

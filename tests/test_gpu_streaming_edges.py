@@ -101,3 +101,24 @@ def test_chunk_values_that_are_not_finite_whatever_the_split(value):
         assert not out[0, 0, 5].isfinite()
         rest = [i for i in range(128) if i != 5]
         assert torch.equal(out[0, 0, rest], cache.v[100, 0, 7, rest])
+
+
+def test_saved_tensors_that_are_written_again_are_refused():
+    """Keys that a gradient still needs, then written as a cache by append_cache or as chunk_attention's out."""
+    cache, *where = _cache([4], [10], 2, 64, 16, BF16)
+    where = [t.cuda() for t in where]
+    where[0].zero_()
+    x = _rand((4, 2, 64), BF16, 1)
+
+    def used():
+        q, kept = _rand((1, 2, 16, 64), BF16, 3).requires_grad_(), _rand((1, 2, 16, 64), BF16, 2)
+        return window_attention(q, kept, kept), kept
+
+    out, kept = used()
+    append_cache(PagedCache(kept, kept.clone()), x, x, *where)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    out, kept = used()
+    chunk_attention(x, cache, *where, out=kept[0, :, :4].transpose(0, 1))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()

@@ -64,3 +64,36 @@ def test_forward_mode_over_a_gradient_is_refused(no_launch, op):
         weight = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
         with pytest.raises(ValueError, match="forward-mode"):
             torch.autograd.grad((out * weight).sum(), x)
+
+
+def test_writes_are_counted(no_launch):
+    """The caches' and out's versions, those of their bases and views with them; tensors of inference mode have none."""
+    base = _x(2, 2, 3, 8, 64)
+    cache, x, out = PagedCache(base[:, 0], base[:, 1]), _x(3, 3, 64), _x(3, 3, 64)
+    versions = lambda *tensors: [t._version for t in tensors]  # noqa: E731
+    before = versions(base, cache.k, cache.v)
+    append_cache(cache, x, x, *_where())
+    assert all(a > b for a, b in zip(versions(base, cache.k, cache.v), before))
+    before = versions(base, x)
+    chunk_attention(x, cache, *_where())
+    assert versions(base, x, out) == [*before, 0]
+    assert chunk_attention(x, cache, *_where(), out=out) is out and out._version == 1 and versions(base, x) == before
+    with torch.inference_mode():
+        cache, out = PagedCache(_x(2, 3, 8, 64), _x(2, 3, 8, 64)), _x(3, 3, 64)
+        append_cache(cache, x, x, *_where())
+    with torch.no_grad():
+        append_cache(cache, x, x, *_where())
+        chunk_attention(x, cache, *_where(), out=out)
+
+
+def test_tensors_that_require_a_gradient_are_not_written(no_launch):
+    x, cache = _x(3, 3, 64), PagedCache(_x(2, 3, 8, 64), _x(2, 3, 8, 64))
+    for out in (_x(3, 3, 64).requires_grad_(), _x(3, 3, 64).requires_grad_() * 2):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            chunk_attention(x, cache, *_where(), out=out)
+    learned = PagedCache(cache.k, _x(2, 3, 8, 64).requires_grad_())
+    with pytest.raises(ValueError, match="requires a gradient"):
+        append_cache(learned, x, x, *_where())
+    with torch.no_grad():
+        append_cache(learned, x, x, *_where())
+    assert not chunk_attention(x.clone().requires_grad_(), learned, *_where()).requires_grad
