@@ -72,6 +72,19 @@ def _no_tangent(name: str, *tensors):
         raise ValueError(f"{name} has no forward-mode derivative")
 
 
+def _own_rows(t: torch.Tensor) -> bool:
+    """Whether no two rows of t (its last dim contiguous) share memory: from the smallest
+    stride up, each reaches past all that the smaller ones span."""
+    if t.is_contiguous():
+        return True
+    span = t.shape[-1]
+    for stride, n in sorted((s, n) for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
+        if stride < span:
+            return False
+        span += stride * (n - 1)
+    return True
+
+
 def _writes(name: str, *tensors):
     """Tells autograd of writes that go past it, as torch's in-place operations do, so
     that a gradient which still needs the old values raises."""
@@ -379,16 +392,19 @@ def append_cache(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table
     [B + 1], ascending, bounded to 0 .. T); ``lengths`` int32 [B] are the tokens of
     each sequence with the new ones, so that its last row goes to position
     lengths[b] - 1. Rows whose entry in the page table is no page are dropped.
-    Returns the cache. Not differentiable: no gradient reaches k and v by it.
+    Returns the cache; k and v share no memory with it. Not differentiable: no
+    gradient reaches k and v by it.
     """
     if k.shape != v.shape or v.dtype != k.dtype:
         raise ValueError("K and V must be packed tokens [T,H,D] of one shape and type")
     if _check_cache("append_cache", k, cache, page_table, lengths, offsets) != k.shape[1]:
         raise ValueError("K and V must have the cache's heads")
-    if any(not t.is_contiguous() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())) for t in cache):
-        raise ValueError("append_cache cannot write to an expanded cache")
+    if not (_own_rows(cache.k) and _own_rows(cache.v)):
+        raise ValueError("append_cache cannot write to an expanded cache or one whose rows overlap")
     _no_tangent("append_cache", v)
-    device = _gpu("append_cache", k, v)
+    device = k.device
+    if v.device != device:
+        raise ValueError("append_cache requires tensors on one CUDA device")
     k, v = _strided(k), _strided(v)
     _writes("append_cache", *cache)
     pages, heads, page, dim = cache.k.shape
@@ -414,6 +430,7 @@ def chunk_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
     Returns o [T, H, D] and with ``return_lse`` the base-2 normaliser float32
     [T, H]. Rows outside of offsets[0] .. offsets[B] - 1 are not written (with
     ``out``, a tensor of q's shape and type to write to, they stay as they are).
+    ``out`` may be q itself; it shares no memory with anything else that is read.
     """
     _check_cache("chunk attention", q, cache, page_table, lengths, offsets)
     device = q.device
@@ -424,7 +441,7 @@ def chunk_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
     if out is None:
         out = q.new_empty((tokens, heads, dim))
     elif (out.shape != q.shape or out.dtype != q.dtype or out.device != device or out.data_ptr() % 8 or out.stride(2) != 1
-          or any(n > 1 and (s % 4 or s == 0) for n, s in zip(out.shape[:2], out.stride()))):
+          or any(n > 1 and s % 4 for n, s in zip(out.shape[:2], out.stride())) or not _own_rows(out)):
         raise ValueError("out must be of Q's shape, type and device, with contiguous rows that start on 8 bytes, each its own")
     else:
         _writes("chunk attention", out)

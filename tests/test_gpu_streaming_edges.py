@@ -122,3 +122,14 @@ def test_saved_tensors_that_are_written_again_are_refused():
     chunk_attention(x, cache, *where, out=kept[0, :, :4].transpose(0, 1))
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.sum().backward()
+
+
+@pytest.mark.parametrize("new,total", [([1, 1], [6000, 130]), ([1, 900, 77], [300, 1100, 4000])])
+def test_chunk_out_over_its_queries(new, total):
+    """out may be q itself: whole rows and split ones."""
+    cache, *where = _cache(new, total, 2, 64, 16, BF16)
+    where = [t.cuda() for t in where]
+    q = _rand((sum(new), 8, 64), BF16, 3, 2.0)
+    want = chunk_attention(q, cache, *where, window=3000, sinks=4)
+    assert chunk_attention(q, cache, *where, window=3000, sinks=4, out=q) is q
+    assert torch.equal(q, want)
