@@ -469,6 +469,10 @@ class StreamingAttention:
 
     ``axes`` (with theta, pairing and joint) turns Q and K by ``rotary``; without it
     they are used as they come.
+
+    A step cannot be captured into a graph: ``begin`` makes a new page table each
+    time, which a replay would not follow. Programs that capture steps keep a page
+    table of their own and call ``append_cache`` and ``chunk_attention``.
     """
 
     def __init__(self, layers: int, sequences: int, heads: int, pages: int, page_tokens: int, *, dim: int = 128,
@@ -504,8 +508,13 @@ class StreamingAttention:
         sinks = min(self.sinks * self.frame, low)
         return range(-(-sinks // self.page_tokens), low // self.page_tokens)
 
+    def _refuse_capture(self) -> None:
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise ValueError("steps of StreamingAttention cannot be captured: the next one has another page table")
+
     def begin(self, new) -> None:
         """Starts a step of new[s] more tokens in sequence s."""
+        self._refuse_capture()
         new = [int(n) for n in new]
         if len(new) != len(self.tokens) or min(new) < 0:
             raise ValueError(f"new must give the new tokens of {len(self.tokens)} sequences")
@@ -543,6 +552,7 @@ class StreamingAttention:
         given. Returns o [T, H, D] (and lse [T, H])."""
         if self.offsets is None:
             raise ValueError("attend comes after begin")
+        self._refuse_capture()
         if any(t.ndim != 3 or t.shape[0] != self.step_tokens for t in (q, k, v)):
             raise ValueError(f"Q, K and V must be the step's {self.step_tokens} packed tokens [T,H,D]")
         if self.axes is not None:

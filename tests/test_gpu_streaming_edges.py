@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from ab_attention.streaming import PagedCache, append_cache, chunk_attention, window_attention
+from ab_attention.streaming import PagedCache, StreamingAttention, append_cache, chunk_attention, window_attention
 from streaming_reference import attend, check_output, seen_mask
 from test_gpu_streaming import _cache, _check_chunk, _rand
 
@@ -133,3 +133,19 @@ def test_chunk_out_over_its_queries(new, total):
     want = chunk_attention(q, cache, *where, window=3000, sinks=4)
     assert chunk_attention(q, cache, *where, window=3000, sinks=4, out=q) is q
     assert torch.equal(q, want)
+
+
+def test_streaming_steps_are_not_captured():
+    """A captured attend would go on reading the page table of the step that it was captured in."""
+    stream = StreamingAttention(1, 1, 2, 4, 16, dim=64)
+    stream.begin([5])
+    x = _rand((5, 2, 64), BF16, 1)
+    want = stream.attend(0, x, x, x)
+    graph, y = torch.cuda.CUDAGraph(), torch.zeros(3, device="cuda")
+    with torch.cuda.graph(graph):
+        for call in (lambda: stream.begin([5]), lambda: stream.attend(0, x, x, x)):
+            with pytest.raises(ValueError, match="captured"):
+                call()
+        y.add_(1)
+    graph.replay()
+    assert (y == 1).all() and torch.equal(stream.attend(0, x, x, x), want)
