@@ -43,7 +43,7 @@ def test_rows_of_out(no_launch, stride, own):
 
 
 @pytest.mark.parametrize("stride,own", [
-    ((1536, 512, 64, 1), True), ((1536, 64, 192, 1), True), ((64, 4096, 512, 1), True), ((3072, 1024, 128, 1), True),
+    ((1536, 512, 64, 1), True), ((1536, 64, 192, 1), True), ((64, 4096, 512, 1), True), ((4096, 1280, 128, 1), True),
     ((1024, 512, 64, 1), False), ((1536, 512, 32, 1), False), ((0, 512, 64, 1), False), ((1536, 0, 64, 1), False)])
 def test_rows_of_a_cache(no_launch, stride, own):
     """A cache [2, 3, 8, 64] that is written: views of any order, none whose rows overlap (it may be read)."""
