@@ -16,20 +16,23 @@
 // zeros and is never read. The step is software-pipelined: the first product of the
 // next tile beside this tile's exponentials, this tile's second product beside the
 // next one's logits. The reference of a row moves only where a logit (base 2) passes
-// it by more than 8. P is rounded to the input type for the second product, the output
-// once at the end; sums are float32. For a backward pass the output is known better:
-// out + out_rest is the sum before its rounding, over the sum of the rounded P, whose
-// weights add up to one again (a row that one key carries owes nothing to P's rounding).
+// it by more than 8. P is rounded to the input type for the second product, which the
+// matrix cores multiply in (the output is 2.3e-3 off in bf16 where its own rounding
+// leaves 1.7e-3, in fp16 2.7e-4 and 2.1e-4; what the rounding takes would be a third
+// product), the output once at the end; sums are float32. For a backward pass the
+// output is known better: out + out_rest is the sum before its rounding, over the sum
+// of the rounded P, whose weights add up to one again (a row that one key carries owes
+// nothing to P's rounding).
 //
 // What bounds it: with many keys the matrix cores at the board's power limit, with
 // the LDS (16 KiB read by each wave of a step) and the vector units (118
 // instructions beside 32 MFMAs) close behind: 12 heads of 32,760 tokens that all see
 // each other 1,130 TFLOP/s, causal over frames with a window of four 946 (rows that
-// straddle frames, 16 us a workgroup to fill and empty the pipeline). The
-// straightforward form of this kernel (two stages, one tile at a time) did 605. With
-// single tokens over long caches it is memory: 4.6 TB/s of the 4.9 that a copy
-// reaches, the keys split over workgroups. 9 tiles of a short call take 14 us, half
-// of them the pipeline's filling.
+// straddle frames; filling and emptying the pipelines, 9 us of each of four rounds of
+// 512 workgroups, 21 us of a lone one with its launch). The straightforward form of
+// this kernel (two stages, one tile at a time) did 605. With single tokens over long
+// caches it is memory: 4.7 TB/s of the 4.9 that a copy reaches, the keys split over
+// workgroups. 9 tiles of a short call take 14 us, half of them the pipeline's filling.
 #include <algorithm>
 #include <initializer_list>
 
@@ -104,7 +107,10 @@ __device__ __forceinline__ bool window_unit(const WindowCall& c, const WindowGri
             u.tile = __builtin_amdgcn_readlane(start + tiles - 1, u.b) - slot;
         } else {
             // Sequence b's tiles take the slots from offsets[b] * group / 128 + b on:
-            // never fewer than it needs, so no sum over the sequences is wanted.
+            // never fewer than it needs, so no sum over the sequences is wanted, nor a
+            // lane for each of them. Not the longest first: 64 sequences of 1 to 400 new
+            // tokens over up to 8,000 take 535 us as above, 601 with an empty 65th; single
+            // tokens over up to 16,000 457 and 451.
             grid.place(id, head, slot);
             int before = 0;
             for (int at = 0; at < c.batch; at += 64) {
@@ -846,11 +852,12 @@ int64_t window_tiles(const WindowCall& c) {
 // Parts that the keys of every tile of rows are split into: those that cost least.
 // A workgroup's time is its steps and about 6 us to fill and empty its pipeline; a step
 // takes 0.80 us where each CU has a workgroup and 0.95 where it has two (D = 64: 0.6 of
-// that), and more than 512 workgroups go in rounds. Splitting adds a second kernel
+// that), and more than 512 workgroups go in rounds: a fit to whole calls, masked tiles
+// among them (calls without masks: 0.64 and 0.93 us a step). Splitting adds a second kernel
 // of 6 us and the partial results' traffic. Over 150 calls of 1 to 400 GFLOP drawn from
 // the range of sizes this took 5.7 % less time than as many parts as give each CU two
 // workgroups; lone steps of 0.55 us (the dense kernel's) took 2.6 % less, of 0.90 and
-// 0.95 the same. One token of 8 heads over 16,384 keys: 38 us.
+// 0.95 the same. One token of 8 heads over 16,384 keys: 31 us.
 int window_parts(const WindowCall& c, int64_t most_keys) {
     const double units = double(window_tiles(c)) * (c.paged ? c.kv_heads : int64_t(c.batch) * c.heads);
     const int64_t steps = (most_keys + kWindowKeys - 1) / kWindowKeys;

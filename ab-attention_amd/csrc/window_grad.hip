@@ -11,10 +11,11 @@
 //            share them, one after the other), dK += Y1^T dS, dV += Y2^T P,
 // each with S^T = Y1 X1^T and dP^T = Y2 X2^T on 16x16x32 MFMAs whose lanes hold
 // one owned row and four streamed ones, which is the form the second products
-// take P and dS in. P and dS are rounded to 16 bits there (the matrix cores'
-// input type); all sums are float32. Below 2^-14, a probability among 16,384 equal
-// ones, fp16 has fewer bits: P is 2^10 P there until dV is stored. dS is as large as
-// dO makes it and stays as it is.
+// take P and dS in. P and dS are rounded to 16 bits there (the matrix cores' input
+// type; with it gradients are 2.4e-3 off in bf16 where their own rounding leaves
+// 1.7e-3), and so is out_rest, at most 2^-8 of the output; all sums are float32.
+// Below 2^-14, a probability among 16,384 equal ones, fp16 has fewer bits: P is 2^10 P
+// there until dV is stored. dS is as large as dO makes it and stays as it is.
 // The first keys (sinks) are seen by every later query. Their tiles would run
 // many times longer than the others, so their queries are split into parts whose
 // float32 sums a third kernel adds up, always in the same order; so are all tiles of

@@ -285,6 +285,9 @@ int ab_rotary(const ab_rotary_args *args, void *stream);
  *   [0, pages) is no page: its keys are not seen. Rows before offsets[0] and from
  *   offsets[batch] on are left as they are. lse f32 [tokens, heads].
  *
+ * No two rows of out share memory. out may be q at the very same places, else it
+ * shares none with what is read.
+ *
  * out_rest (NULL, or of out's strides and type) gets what out's rounding took from
  * the result, and of a tensor what rounding the weights did to their sum, rounded
  * itself: ab_window_attention_grad makes its delta of the two.
@@ -332,7 +335,8 @@ int ab_window_attention_grad(const ab_window_grad_args *args, void *stream);
 /* New keys and values k, v [tokens, kv_heads, dim] (16-bit elements) of `batch`
  * sequences into a paged cache (offsets, lengths, page_table and the cache as in
  * ab_chunk_attention; lengths count the new tokens). Rows whose entry is no page
- * are dropped. Strides in elements, multiples of 8 (token, head of k and v in
+ * are dropped. No two rows of the cache share memory, nor k and v with it. Strides
+ * in elements, multiples of 8 (token, head of k and v in
  * k_stride[2], [1]; page, head, token of the cache). */
 typedef struct ab_append_args {
     const void *k, *v;
