@@ -89,6 +89,45 @@ class AppendArgs(ctypes.Structure):
                 ("k_cache_stride", _I64 * 3), ("v_cache_stride", _I64 * 3)]
 
 
+class DraftTreeArgs(ctypes.Structure):
+    """ab_draft_tree_args of include/ab_attention.h."""
+
+    _fields_ = [("parents", _P), ("lengths", _P), ("offsets", _P), ("positions", _P), ("near", _P), ("above", _P),
+                ("batch", _I64), ("tokens", _I64)]
+
+
+class TreeArgs(ctypes.Structure):
+    """ab_tree_args of include/ab_attention.h."""
+
+    _fields_ = [("chunk", WindowArgs), ("positions", _P), ("near", _P), ("above", _P)]
+
+
+class VerifyArgs(ctypes.Structure):
+    """ab_verify_args of include/ab_attention.h."""
+
+    _fields_ = [("target", _P), ("draft", _P), ("tokens", _P), ("parents", _P), ("offsets", _P), ("uniforms", _P),
+                ("path", _P), ("counts", _P), ("next", _P), ("batch", _I64), ("rows", _I64), ("vocab", _I64), ("dtype", _I64),
+                ("wide_tokens", _I64), ("target_stride", _I64), ("draft_stride", _I64), ("workspace", _P),
+                ("workspace_bytes", _SZ)]
+
+
+class KeepArgs(ctypes.Structure):
+    """ab_keep_args of include/ab_attention.h."""
+
+    _fields_ = [("k_cache", _P), ("v_cache", _P), ("lengths", _P), ("offsets", _P), ("page_table", _P), ("path", _P),
+                ("counts", _P), ("layers", _I64), ("batch", _I64), ("kv_heads", _I64), ("tokens", _I64), ("dim", _I64),
+                ("pages", _I64), ("page_tokens", _I64), ("table_width", _I64), ("k_layer", _I64), ("v_layer", _I64),
+                ("k_stride", _I64 * 3), ("v_stride", _I64 * 3)]
+
+
+class CopyArgs(ctypes.Structure):
+    """ab_copy_args of include/ab_attention.h."""
+
+    _fields_ = [("k_cache", _P), ("v_cache", _P), ("moves", _P), ("count", _I64), ("layers", _I64), ("kv_heads", _I64),
+                ("dim", _I64), ("pages", _I64), ("page_tokens", _I64), ("k_layer", _I64), ("v_layer", _I64),
+                ("k_stride", _I64 * 3), ("v_stride", _I64 * 3)]
+
+
 def packer(args_type) -> struct.Struct:
     """The bytes of an argument structure (8-byte fields, arrays and structures of
     them) from its values one after the other: making them so takes a quarter of
@@ -137,6 +176,12 @@ SIGNATURES = {
     "ab_window_grad_workspace_bytes": (_SZ, [ctypes.POINTER(WindowGradArgs)]),
     "ab_window_attention_grad": (ctypes.c_int, [ctypes.POINTER(WindowGradArgs), _P]),
     "ab_append_cache": (ctypes.c_int, [ctypes.POINTER(AppendArgs), _P]),
+    "ab_draft_tree": (ctypes.c_int, [ctypes.POINTER(DraftTreeArgs), _P]),
+    "ab_tree_attention": (ctypes.c_int, [ctypes.POINTER(TreeArgs), _P]),
+    "ab_verify_workspace_bytes": (_SZ, [ctypes.POINTER(VerifyArgs)]),
+    "ab_verify_drafts": (ctypes.c_int, [ctypes.POINTER(VerifyArgs), _P]),
+    "ab_keep_drafts": (ctypes.c_int, [ctypes.POINTER(KeepArgs), _P]),
+    "ab_copy_pages": (ctypes.c_int, [ctypes.POINTER(CopyArgs), _P]),
 }
 
 # name -> (restype, argtypes); mirrors include/ab_attention_static.h
@@ -144,7 +189,7 @@ STATIC_SIGNATURES = {
     "ab_ibcs_sip_static": (ctypes.c_int, [_P, _P, _P, _I64, _I64, _P, _I64, _P, _P, _P]),
 }
 
-ABI_VERSION = 8
+ABI_VERSION = 9
 _lib = None
 _static = None
 

@@ -18,12 +18,18 @@ Serving: ``rotary`` of the new tokens' Q and K, ``append_cache``, then
 keeps the page table. Training: ``rotary`` and ``window_attention``. The
 reference has no counterpart: its attention sees a whole clip at once.
 
+A step that checks several drafted tokens at once: ``draft_tree`` (for ``rotary`` the
+positions), in every layer ``append_cache`` and ``tree_attention``, then
+``verify_drafts`` on the model's probabilities and ``keep_drafts``. ``copy_pages`` is
+for sequences that are continued in several ways from a common beginning.
+
 Everything runs on the current stream of the tensors' device and synchronises
 nothing; sizes that are on the device (lengths, offsets, page tables) are
 bounded by the kernels and never read on the host.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 import math
 import struct
@@ -94,6 +100,11 @@ def _writes(name: str, *tensors):
     increment_version([t for t in tensors if not t.is_inference()])
 
 
+def _bytes_at(data: bytes) -> int:
+    """The address of the bytes, which live as long as ``data``."""
+    return ctypes.cast(data, ctypes.c_void_p).value
+
+
 def _call(entry: str, device, packed: bytes):
     with _lib.on(device):
         status = _lib.raw(entry)(packed, _lib.raw_stream(device))
@@ -102,6 +113,8 @@ def _call(entry: str, device, packed: bytes):
 
 
 _ROTARY, _WINDOW, _APPEND = map(_lib.packer, (_lib.RotaryArgs, _lib.WindowArgs, _lib.AppendArgs))
+_TREE, _VERIFY, _KEEP, _COPY = map(_lib.packer, (_lib.DraftTreeArgs, _lib.VerifyArgs, _lib.KeepArgs, _lib.CopyArgs))
+_TREE_REST = struct.Struct("=3Q")     # ab_tree_args behind its chunk
 _GRAD_REST = struct.Struct("=5Q12q")  # ab_window_grad_args behind its forward part
 _WORKSPACE = struct.Struct("=2Q")     # the last fields of ab_window_args
 _ZERO = (0, 0, 0)
@@ -231,14 +244,14 @@ def _check_window(window, scale, dim):
     return scale
 
 
-def _run(entry, device, packed):
-    """One call with the workspace that it asks for, which lives for the call only."""
+def _run(entry, device, packed, behind=b""):
+    """One call with the workspace that it asks for, which lives for the call only; ``behind``: fields after ab_window_args."""
     with _lib.on(device):
         size = _lib.raw("ab_window_workspace_bytes")(packed)
         if size:
             workspace = torch.empty(size, dtype=torch.uint8, device=device)
             packed = packed[:-_WORKSPACE.size] + _WORKSPACE.pack(workspace.data_ptr(), size)
-        status = _lib.raw(entry)(packed, _lib.raw_stream(device))
+        status = _lib.raw(entry)(packed + behind, _lib.raw_stream(device))
     if status:
         _lib.check(status)
 
@@ -432,7 +445,12 @@ def chunk_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
     ``out``, a tensor of q's shape and type to write to, they stay as they are).
     ``out`` may be q itself; it shares no memory with anything else that is read.
     """
-    _check_cache("chunk attention", q, cache, page_table, lengths, offsets)
+    return _over_cache("chunk attention", "ab_chunk_attention", q, cache, page_table, lengths, offsets, b"", window, sinks, frame,
+                       scale, return_lse, out)
+
+
+def _over_cache(name, entry, q, cache, page_table, lengths, offsets, behind, window, sinks, frame, scale, return_lse, out):
+    _check_cache(name, q, cache, page_table, lengths, offsets)
     device = q.device
     scale = _check_window(window, scale, q.shape[-1])
     window, sinks, frame = _mask(window, sinks, frame)
@@ -444,16 +462,233 @@ def chunk_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
           or any(n > 1 and s % 4 for n, s in zip(out.shape[:2], out.stride())) or not _own_rows(out)):
         raise ValueError("out must be of Q's shape, type and device, with contiguous rows that start on 8 bytes, each its own")
     else:
-        _writes("chunk attention", out)
+        _writes(name, out)
     lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
     if tokens and page_table.shape[0]:
-        pages, kv_heads, page, _ = cache.k.shape
-        _run("ab_chunk_attention", device, _WINDOW.pack(
-            q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), out.data_ptr(), 0, 0 if lse is None else lse.data_ptr(),
+        pages, kv_heads, page, _ = cache[0].shape
+        k, v = cache
+        _run(entry, device, _WINDOW.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0, 0 if lse is None else lse.data_ptr(),
             lengths.data_ptr(), offsets.data_ptr(), page_table.data_ptr(), page_table.shape[0], heads, kv_heads, tokens, dim,
             _DTYPES[q.dtype], pages, page, page_table.shape[1], window, sinks, frame, scale, 0, q.stride(1), q.stride(0),
-            *cache.k.stride()[:3], *cache.v.stride()[:3], 0, out.stride(1), out.stride(0), 0, 0))
+            *k.stride()[:3], *v.stride()[:3], 0, out.stride(1), out.stride(0), 0, 0), behind)
     return (out, lse) if return_lse else out
+
+
+# ---- drafted tokens -----------------------------------------------------------
+
+
+def _ints(name, **tensors):
+    for what, t in tensors.items():
+        if t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous():
+            raise ValueError(f"{name} requires {what} as a contiguous int32 tensor of one dim")
+
+
+class DraftTree(NamedTuple):
+    """``draft_tree``'s results, int32, int64 and int32 [T]. ``positions`` are the new
+    tokens'. Which tokens are on the line down to each, itself too, is said by the places
+    of ``near``'s bits (bit j: 64 (i // 64) + j for the token at place i) and by
+    ``above``, the last place of the line before those 64, or -1."""
+
+    positions: torch.Tensor
+    near: torch.Tensor
+    above: torch.Tensor
+
+
+def draft_tree(parents: torch.Tensor, lengths: torch.Tensor, offsets: torch.Tensor) -> DraftTree:
+    """The tree that the sequences' new tokens are, for all layers of a step.
+
+    Sequence b's n new tokens are the rows offsets[b] .. offsets[b + 1] - 1 (int32
+    [B + 1]), of lengths[b] (int32 [B]) in all. ``parents`` int32 [T] gives for each
+    the place, 0 .. n - 1, of the new token that it follows, which comes before it; any
+    other number is none: the token follows the cached ones. A token with d others
+    above it is at position lengths[b] - n + d, though its keys and values are in the
+    cache's place lengths[b] - n + i, as ``append_cache`` puts them. Rows of no
+    sequence get position 0.
+    """
+    _ints("draft_tree", parents=parents, lengths=lengths, offsets=offsets)
+    if lengths.shape[0] != offsets.shape[0] - 1:
+        raise ValueError("lengths [B] and offsets [B+1] must be of one batch")
+    device = _gpu("draft_tree", parents, lengths, offsets)
+    tokens, batch = parents.shape[0], lengths.shape[0]
+    if batch == 0:
+        return DraftTree(torch.zeros_like(parents), parents.new_zeros(tokens, dtype=torch.int64), torch.full_like(parents, -1))
+    tree = DraftTree(torch.empty_like(parents), parents.new_empty(tokens, dtype=torch.int64), torch.empty_like(parents))
+    if tokens:
+        _call("ab_draft_tree", device, _TREE.pack(parents.data_ptr(), lengths.data_ptr(), offsets.data_ptr(),
+                                                  *(t.data_ptr() for t in tree), batch, tokens))
+    return tree
+
+
+def tree_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tensor,
+                   offsets: torch.Tensor, tree: DraftTree, *, window: int | None = None, sinks: int = 0, frame: int = 1,
+                   scale: float | None = None, return_lse: bool = False, out: torch.Tensor | None = None):
+    """``chunk_attention`` of new tokens that are a tree (``draft_tree`` of the same
+    ``lengths`` and ``offsets``; other values in it give other results, but reach no
+    other memory): every token sees the cached ones that the mask gives its position,
+    and of the new ones those above it and itself, as far as the mask gives it their
+    positions. With ``frame`` above 1 a token sees no later ones of its frame, as
+    those are drafts.
+    """
+    positions, near, above = tree
+    _ints("tree attention", positions=positions, above=above)
+    if near.dtype != torch.int64 or not near.is_contiguous() or not positions.shape == near.shape == above.shape == q.shape[:1]:
+        raise ValueError("tree attention requires the tree of Q's packed tokens")
+    _gpu("tree attention", q, *tree)
+    return _over_cache("tree attention", "ab_tree_attention", q, cache, page_table, lengths, offsets,
+                       _TREE_REST.pack(positions.data_ptr(), near.data_ptr(), above.data_ptr()), window, sinks, frame, scale,
+                       return_lse, out)
+
+
+class Kept(NamedTuple):
+    """``verify_drafts``' results: ``path`` int32 [T], from offsets[b] on the places of
+    sequence b's kept tokens, then -1; ``counts`` int32 [B], how many; ``next`` [B], the
+    token behind them, of the drafts' type."""
+
+    path: torch.Tensor
+    counts: torch.Tensor
+    next: torch.Tensor
+
+
+def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torch.Tensor, parents: torch.Tensor,
+                  offsets: torch.Tensor, uniforms: torch.Tensor) -> Kept:
+    """Which drafted tokens stay, and the token behind them, so that what is written is
+    distributed as the target's probabilities say.
+
+    The new tokens ``tokens`` [T] (int32 or int64), ``parents`` and ``offsets`` are as in
+    ``draft_tree``; the first of each sequence is the one that was written last and is
+    kept, the others hang below it. ``target`` [T, V] are the probabilities of what comes
+    behind each (bf16, fp16 or float32; the values are taken as they are, rows need not
+    add up to one exactly), ``draft`` of the same shape and type the ones that its
+    children were drawn from, or None for children that were chosen without chance, such
+    as the likeliest ones. ``uniforms`` float32 [T] are random numbers in [0, 1).
+
+    From the last kept token on its children j are looked at in the order of their
+    places. With w = target's row and S = 1 at first, j is kept where
+    uniforms[j] * draft[tokens[j]] * S < w[tokens[j]] (None: draft = 1), and the walk goes
+    on from it. Else w becomes max(w - S * draft, 0) and S its sum (where that is 0
+    both stay as they are), or, chosen, S loses w[tokens[j]], which becomes 0. Where no
+    child is left the next token is the first with w > 0 whose running sum of w passes
+    uniforms[offsets[b]] times the whole sum (-1 where all w are 0). Sums are in 64
+    bits. Values that are not positive and finite count as 0, tokens outside of
+    0 .. V - 1 are never kept. A sequence without new tokens has counts 0 and next -1.
+    """
+    if target.ndim != 2 or (draft is not None and draft.shape != target.shape):
+        raise ValueError("target and draft must be [T,V] probabilities of one shape")
+    if target.dtype not in _DTYPES or (draft is not None and draft.dtype != target.dtype):
+        raise ValueError("verify_drafts requires BF16, FP16 or FP32 probabilities of one type")
+    rows, vocab = target.shape
+    if vocab == 0:
+        raise ValueError("verify_drafts requires at least one token in the vocabulary")
+    _ints("verify_drafts", parents=parents, offsets=offsets)
+    if tokens.dtype not in (torch.int32, torch.int64) or uniforms.dtype != torch.float32:
+        raise ValueError("tokens must be int32 or int64, uniforms float32")
+    if not tokens.shape == parents.shape == uniforms.shape == target.shape[:1]:
+        raise ValueError(f"tokens, parents and uniforms must be [{rows}], as target has rows")
+    if offsets.shape[0] == 0:
+        raise ValueError("offsets must be [B+1]")
+    _no_tangent("verify_drafts", target, draft, uniforms)
+    device = _gpu("verify_drafts", target, draft, tokens, parents, offsets, uniforms)
+    tokens, uniforms = tokens.contiguous(), uniforms.contiguous()
+    target, draft = (t if t is None or t.stride(1) == 1 or vocab == 1 else t.contiguous() for t in (target, draft))
+    batch = offsets.shape[0] - 1
+    kept = Kept(torch.empty_like(parents), parents.new_empty(batch), tokens.new_empty(batch))
+    if batch == 0:
+        kept.path.fill_(-1)
+        return kept
+    args = (target.data_ptr(), 0 if draft is None else draft.data_ptr(), tokens.data_ptr(), parents.data_ptr(), offsets.data_ptr(),
+            uniforms.data_ptr(), *(t.data_ptr() for t in kept), batch, rows, vocab, _DTYPES[target.dtype],
+            tokens.dtype == torch.int64, target.stride(0), 0 if draft is None else draft.stride(0))
+    with _lib.on(device):
+        size = _lib.raw("ab_verify_workspace_bytes")(_VERIFY.pack(*args, 0, 0))
+        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        status = _lib.raw("ab_verify_drafts")(_VERIFY.pack(*args, workspace.data_ptr(), size), _lib.raw_stream(device))
+    if status:
+        _lib.check(status)
+    return kept
+
+
+def _check_layers(name, cache):
+    """(layers, strides of a layer in k and v, strides in a layer) of a cache of one layer, or of several, [layers, ..]."""
+    k, v = cache
+    if k.ndim not in (4, 5) or k.shape != v.shape:
+        raise ValueError("the cache must be two [pages,heads,page tokens,D] or [layers,pages,heads,page tokens,D] tensors")
+    dim, page = k.shape[-1], k.shape[-2]
+    if dim != 128 and dim != 64:
+        raise ValueError(f"{name} requires head_dim 64 or 128")
+    if k.dtype not in (torch.bfloat16, torch.float16) or v.dtype != k.dtype:
+        raise ValueError(f"{name} requires a BF16 or FP16 cache")
+    if page == 0 or page % 8:
+        raise ValueError("pages must hold a positive multiple of 8 tokens")
+    if k.shape[-3] == 0:
+        raise ValueError("the cache must have at least one head")
+    for t in cache:
+        if t.data_ptr() % 16 or not (t.is_contiguous() or (
+                t.stride(-1) == 1 and not any(n > 1 and s % 8 for n, s in zip(t.shape, t.stride()[:-1])))):
+            raise ValueError("the cache's rows must be contiguous and start on 16 bytes")
+        if not _own_rows(t):
+            raise ValueError(f"{name} cannot write to an expanded cache or one whose rows overlap")
+    if k.ndim == 4:
+        return 1, (0, 0), k.stride()[:3], v.stride()[:3]
+    return k.shape[0], (k.stride(0), v.stride(0)), k.stride()[1:4], v.stride()[1:4]
+
+
+def keep_drafts(cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tensor, offsets: torch.Tensor,
+                path: torch.Tensor, counts: torch.Tensor) -> PagedCache:
+    """Moves the kept tokens' keys and values next to each other, in place.
+
+    ``path`` int32 [T] and ``counts`` int32 [B] are ``verify_drafts``', the others those
+    that the drafts were appended by: in sequence b, with n new tokens, the cache's
+    position lengths[b] - n + path[offsets[b] + j] is copied to lengths[b] - n + j, for
+    j < counts[b], so that the sequence goes on with lengths[b] - n + counts[b] tokens.
+    Places outside of j .. n - 1 and ones on no page move nothing. The cache may be that of one
+    layer or, as tensors [layers, pages, heads, page tokens, D], of all layers, which one
+    call then takes. No page is in two places of the table. Returns the cache.
+    """
+    layers, layer_strides, k_stride, v_stride = _check_layers("keep_drafts", cache)
+    if page_table.ndim != 2 or page_table.dtype != torch.int32 or not page_table.is_contiguous():
+        raise ValueError("page_table must be contiguous int32 [B,width]")
+    _ints("keep_drafts", lengths=lengths, offsets=offsets, path=path, counts=counts)
+    batch = lengths.shape[0]
+    if not page_table.shape[0] == offsets.shape[0] - 1 == counts.shape[0] == batch:
+        raise ValueError("page_table [B,width], lengths [B], offsets [B+1] and counts [B] must be of one batch")
+    k, v = cache
+    _no_tangent("keep_drafts", k, v)
+    device = _gpu("keep_drafts", k, v, page_table, lengths, offsets, path, counts)
+    _writes("keep_drafts", k, v)
+    pages, heads, page, dim = k.shape[-4:]
+    if layers:
+        _call("ab_keep_drafts", device, _KEEP.pack(
+            k.data_ptr(), v.data_ptr(), lengths.data_ptr(), offsets.data_ptr(), page_table.data_ptr(), path.data_ptr(),
+            counts.data_ptr(), layers, batch, heads, path.shape[0], dim, pages, page, page_table.shape[1], *layer_strides,
+            *k_stride, *v_stride))
+    return cache
+
+
+def copy_pages(cache: PagedCache, moves) -> PagedCache:
+    """Copies pages to pages, in place: ``moves`` are pairs (from, to) of page numbers, on
+    the host. A page that is copied to is named only once. The cache may be that of one
+    layer or of all, as in ``keep_drafts``. Returns the cache. A call captured into a
+    graph repeats the moves that it was captured with.
+    """
+    layers, layer_strides, k_stride, v_stride = _check_layers("copy_pages", cache)
+    k, v = cache
+    pages, heads, page, dim = k.shape[-4:]
+    flat = [int(p) for source, target in moves for p in (source, target)]
+    if flat and not (0 <= min(flat) and max(flat) < pages):
+        raise ValueError(f"moves must name pages from 0 to {pages - 1}")
+    to = set(flat[1::2])
+    if 2 * len(to) != len(flat) or not to.isdisjoint(flat[::2]):
+        raise ValueError("a page that is copied to must be named only once")
+    _no_tangent("copy_pages", k, v)
+    device = _gpu("copy_pages", k, v)
+    _writes("copy_pages", k, v)
+    if flat and layers:
+        host = struct.pack(f"={len(flat)}i", *flat)  # read by the call itself
+        _call("ab_copy_pages", device, _COPY.pack(
+            k.data_ptr(), v.data_ptr(), _bytes_at(host), len(to), layers, heads, dim, pages, page, *layer_strides,
+            *k_stride, *v_stride))
+    return cache
 
 
 class StreamingAttention:
@@ -466,6 +701,11 @@ class StreamingAttention:
     any of their tokens (behind the window, not among the sinks), and by
     ``finish(sequence)``. ``pages`` is how many there are in each layer's cache;
     ``begin`` raises ValueError, and changes nothing, when they do not suffice.
+
+    A step that checks drafted tokens is ``begin(new, parents)``, ``attend`` in every
+    layer, with the positions of ``tree.positions``, and after ``verify_drafts``
+    ``keep(path, counts)``. ``fork(sequence, into)`` continues a sequence in two ways: the
+    pages stay one until either of them writes to one, which ``begin`` copies first.
 
     ``axes`` (with theta, pairing and joint) turns Q and K by ``rotary``; without it
     they are used as they come.
@@ -490,15 +730,18 @@ class StreamingAttention:
         self.window = window
         self.axes, self.turn = axes, dict(theta=theta, pairing=pairing, joint=joint)
         self.page_tokens, self.device = page_tokens, torch.device(device)
-        shape = (pages, heads, page_tokens, dim)
-        self.caches = [PagedCache(*(torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(2)))
-                       for _ in range(layers)]
-        self.device = self.caches[0].k.device  # with its index: other devices may become the current one
+        # All layers' caches, and each layer's part of them.
+        shape = (layers, pages, heads, page_tokens, dim)
+        self.cache = PagedCache(*(torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(2)))
+        self.caches = [PagedCache(self.cache.k[layer], self.cache.v[layer]) for layer in range(layers)]
+        self.device = self.cache.k.device  # with its index: other devices may become the current one
         self.free = list(range(pages - 1, -1, -1))
+        self.owners = [0] * pages        # of each page: the sequences that hold it
         self.tokens = [0] * sequences    # of each sequence, with those of the step that began last
+        self.new = [0] * sequences       # of each sequence: those of that step
         self.held = [{} for _ in range(sequences)]  # of each sequence: place in its table -> page
         self.step_tokens = 0
-        self.page_table = self.lengths = self.offsets = None
+        self.page_table = self.lengths = self.offsets = self.tree = None
 
     def _behind(self, first: int) -> range:
         """The places of a sequence's table that queries from position ``first`` on do not see."""
@@ -512,27 +755,59 @@ class StreamingAttention:
         if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise ValueError("steps of StreamingAttention cannot be captured: the next one has another page table")
 
-    def begin(self, new) -> None:
-        """Starts a step of new[s] more tokens in sequence s."""
+    def _release(self, page: int) -> None:
+        self.owners[page] -= 1
+        if not self.owners[page]:
+            self.free.append(page)
+
+    def begin(self, new, parents=None) -> None:
+        """Starts a step of new[s] more tokens in sequence s. ``parents``, of a step of drafts: for each sequence the
+        places that its tokens follow, as in ``draft_tree``; ``keep`` ends such a step."""
         self._refuse_capture()
+        if self.tree is not None:
+            raise ValueError("keep comes before the step after drafts")
         new = [int(n) for n in new]
         if len(new) != len(self.tokens) or min(new) < 0:
             raise ValueError(f"new must give the new tokens of {len(self.tokens)} sequences")
+        if parents is not None:
+            parents = [[int(p) for p in its] for its in parents]
+            if [len(its) for its in parents] != new:
+                raise ValueError("parents must give a place for each of the sequences' new tokens")
+            if any(not -1 <= p < i for its in parents for i, p in enumerate(its)):
+                raise ValueError("a parent must come before the token that follows it, or be -1")
         total = [t + n for t, n in zip(self.tokens, new)]
-        gone, wanted = [], []
-        for s, (n, length) in enumerate(zip(new, total)):
+        gone, wanted, owners = [], [], {}  # owners: of pages that lose some
+        steps = [(s, n, length) for s, (n, length) in enumerate(zip(new, total)) if n]
+        for s, n, length in steps:
             behind = self._behind(length - n)
-            if n:
-                gone += [(s, i) for i in self.held[s] if i in behind]
-                wanted += [(s, i) for i in range((length - n) // self.page_tokens, -(-length // self.page_tokens))
-                           if i not in self.held[s]]
-        if len(wanted) > len(self.free) + len(gone):
-            raise ValueError(f"{len(wanted)} more pages are needed, {len(self.free) + len(gone)} are free")
+            for i, page in self.held[s].items():
+                if i in behind:
+                    gone.append((s, i))
+                    owners[page] = owners.get(page, self.owners[page]) - 1
+        for s, n, length in steps:
+            for i in range((length - n) // self.page_tokens, -(-length // self.page_tokens)):
+                page = self.held[s].get(i)
+                if page is None:
+                    wanted.append((s, i))
+                elif owners.get(page, self.owners[page]) > 1:  # another sequence's too: this one gets a copy
+                    wanted.append((s, i))
+                    owners[page] = owners.get(page, self.owners[page]) - 1
+        free = len(self.free) + sum(not left for left in owners.values())
+        if len(wanted) > free:
+            raise ValueError(f"{len(wanted)} more pages are needed, {free} are free")
         for s, i in gone:
-            self.free.append(self.held[s].pop(i))
+            self._release(self.held[s].pop(i))
+        moves = []
         for s, i in wanted:
-            self.held[s][i] = self.free.pop()
-        self.tokens, self.step_tokens = total, sum(new)
+            page = self.free.pop()
+            if i in self.held[s]:
+                moves.append((self.held[s][i], page))
+                self._release(self.held[s][i])
+            self.held[s][i] = page
+            self.owners[page] = 1
+        if moves:
+            copy_pages(self.cache, moves)
+        self.tokens, self.new, self.step_tokens = total, new, sum(new)
         width = max(1, max(-(-length // self.page_tokens) for length in total))
         table = [[-1] * width for _ in total]
         for row, held in zip(table, self.held):
@@ -541,9 +816,13 @@ class StreamingAttention:
         offsets = [0]
         for n in new:
             offsets.append(offsets[-1] + n)
-        self.page_table, self.lengths, self.offsets = (
-            torch.tensor(values, dtype=torch.int32, pin_memory=True).to(self.device, non_blocking=True)
-            for values in (table, total, offsets))
+        values = [table, total, offsets]
+        if parents is not None:
+            values.append([p for its in parents for p in its])
+        self.page_table, self.lengths, self.offsets, *rest = (
+            torch.tensor(value, dtype=torch.int32, pin_memory=True).to(self.device, non_blocking=True) for value in values)
+        if rest:
+            self.tree = draft_tree(*rest, self.lengths, self.offsets)
 
     def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor | None = None, *,
                return_lse: bool = False):
@@ -560,11 +839,48 @@ class StreamingAttention:
                 raise ValueError("positions are needed to turn Q and K")
             q, k = (t[0].transpose(0, 1) for t in rotary(*(t.transpose(0, 1)[None] for t in (q, k)), positions, self.axes, **self.turn))
         cache = append_cache(self.caches[layer], k, v, self.page_table, self.lengths, self.offsets)
-        return chunk_attention(q, cache, self.page_table, self.lengths, self.offsets, window=self.window, sinks=self.sinks,
-                               frame=self.frame, scale=self.scale, return_lse=return_lse)
+        how = dict(window=self.window, sinks=self.sinks, frame=self.frame, scale=self.scale, return_lse=return_lse)
+        where = (q, cache, self.page_table, self.lengths, self.offsets)
+        return chunk_attention(*where, **how) if self.tree is None else tree_attention(*where, self.tree, **how)
+
+    def keep(self, path: torch.Tensor, counts: torch.Tensor) -> list:
+        """Ends a step whose tokens were drafts: of sequence s only the counts[s] at the places path says stay
+        (``verify_drafts``' path and counts). Returns the counts as a list, for which it waits for the device."""
+        if self.offsets is None:
+            raise ValueError("keep comes after begin")
+        self._refuse_capture()
+        if counts.shape != (len(self.new),) or path.shape != (self.step_tokens,):
+            raise ValueError(f"path [{self.step_tokens}] and counts [{len(self.new)}] must be of the step's tokens")
+        kept = counts.tolist()
+        if any(n and not 0 <= count <= n for count, n in zip(kept, self.new)):
+            raise ValueError("counts must be from 0 to the sequences' new tokens")
+        keep_drafts(self.cache, self.page_table, self.lengths, self.offsets, path, counts)
+        for s, (count, n) in enumerate(zip(kept, self.new)):
+            if n:
+                self.tokens[s] += count - n
+                last = -(-self.tokens[s] // self.page_tokens)
+                for i in [i for i in self.held[s] if i >= last]:
+                    self._release(self.held[s].pop(i))
+        self.new = [0] * len(self.new)
+        self.page_table = self.lengths = self.offsets = self.tree = None
+        return kept
+
+    def fork(self, sequence: int, into: int) -> None:
+        """Continues a sequence in a second way: ``into``, which must be one that has no tokens, gets all that
+        ``sequence`` has. No page is copied before one of them writes to it. Between steps: the next call is ``begin``."""
+        if self.tree is not None:
+            raise ValueError("keep comes before fork")
+        if self.tokens[into] or self.held[into]:
+            raise ValueError("into must be a sequence without tokens")
+        for page in self.held[sequence].values():
+            self.owners[page] += 1
+        self.held[into] = dict(self.held[sequence])
+        self.tokens[into] = self.tokens[sequence]
+        self.page_table = self.lengths = self.offsets = None
 
     def finish(self, sequence: int) -> None:
-        """Gives a sequence's pages back; it starts again at position 0."""
-        self.free += self.held[sequence].values()
+        """Gives a sequence's pages back, as far as no other one has them; it starts again at position 0."""
+        for page in self.held[sequence].values():
+            self._release(page)
         self.held[sequence] = {}
-        self.tokens[sequence] = 0
+        self.tokens[sequence] = self.new[sequence] = 0

@@ -6,6 +6,7 @@
 
 #include "../../include/ab_attention.h"
 #include "cache.hpp"
+#include "drafts.hpp"
 #include "rotary.hpp"
 #include "window.hpp"
 
@@ -59,6 +60,14 @@ int check_cache(const char* what, int64_t batch, int64_t kv_heads, int64_t pages
         return set_error(AB_ERR_INVALID, "%s: one head of a page must be under 4 GiB", what);
     if (batch > 0 && (!lengths || !offsets || (width > 0 && !table)))
         return set_error(AB_ERR_INVALID, "%s: null pointer", what);
+    return AB_OK;
+}
+
+int check_layers(const char* what, int64_t layers, int64_t k_layer, int64_t v_layer) {
+    if (layers <= 0 || layers > 32767) return set_error(AB_ERR_INVALID, "%s: 1 to 32,767 layers", what);
+    for (int64_t stride : {k_layer, v_layer})
+        if (layers > 1 && (stride < 0 || stride % 8 || stride >= (int64_t(1) << 40)))
+            return set_error(AB_ERR_INVALID, "%s: strides must be multiples of 8 elements from 0 to 2^40", what);
     return AB_OK;
 }
 
@@ -134,10 +143,17 @@ size_t workspace_bytes(const WindowCall& c) {
     return c.parts == 1 ? 0 : size_t(c.parts) * size_t(c.rows) * (size_t(c.dim) * sizeof(float) + sizeof(float2) + rounded);
 }
 
-int window_launch(const char* what, const ab_window_args* a, bool paged, void* stream) {
+int window_launch(const char* what, const ab_window_args* a, bool paged, void* stream, const ab_tree_args* tree = nullptr) {
     if (!a) return set_error(AB_ERR_INVALID, "%s: null pointer", what);
     WindowCall c;
     if (int rc = window_call(what, *a, paged, c)) return rc;
+    if (tree) {
+        if (a->tokens > 0 && a->batch > 0 && (!tree->positions || !tree->near || !tree->above))
+            return set_error(AB_ERR_INVALID, "%s: null pointer", what);
+        c.positions = tree->positions;
+        c.near = tree->near;
+        c.above = tree->above;
+    }
     if (a->batch == 0 || a->tokens == 0) return AB_OK;
     const bool no_cache = paged && (a->pages == 0 || a->table_width == 0);
     if (!a->q || !a->out || (!no_cache && (!a->k || !a->v))) return set_error(AB_ERR_INVALID, "%s: null pointer", what);
@@ -341,6 +357,162 @@ int ab_append_cache(const ab_append_args* a, void* stream) {
     c.pages = static_cast<int32_t>(a->pages);
     c.page = divisor(static_cast<uint32_t>(a->page_tokens));
     return launch_append(c, static_cast<hipStream_t>(stream));
+}
+
+int ab_draft_tree(const ab_draft_tree_args* a, void* stream) {
+    if (!a) return set_error(AB_ERR_INVALID, "draft_tree: null pointer");
+    if (a->batch < 0 || a->tokens < 0 || a->tokens >= kMostTokens || a->batch > 65535)
+        return set_error(AB_ERR_INVALID, "draft_tree: too many tokens or sequences");
+    if (a->batch == 0 || a->tokens == 0) return AB_OK;
+    if (!a->parents || !a->lengths || !a->offsets || !a->positions || !a->near || !a->above)
+        return set_error(AB_ERR_INVALID, "draft_tree: null pointer");
+    const TreeCall c{a->parents, a->lengths, a->offsets, a->positions, a->near, a->above, static_cast<int32_t>(a->batch),
+                     static_cast<int32_t>(a->tokens)};
+    return launch_tree(c, static_cast<hipStream_t>(stream));
+}
+
+int ab_tree_attention(const ab_tree_args* a, void* stream) {
+    if (!a) return set_error(AB_ERR_INVALID, "tree_attention: null pointer");
+    return window_launch("tree_attention", &a->chunk, true, stream, a);
+}
+
+}  // extern "C"
+
+namespace {
+int verify_call(const ab_verify_args& a, VerifyCall& c, size_t& bytes) {
+    const char* what = "verify_drafts";
+    if (a.batch < 0 || a.rows < 0 || a.vocab <= 0) return set_error(AB_ERR_INVALID, "%s: sizes must be positive", what);
+    if (a.batch > 65535 || a.rows >= kMostTokens || a.vocab >= kMostTokens)
+        return set_error(AB_ERR_INVALID, "%s: too many tokens or sequences, or too large a vocabulary", what);
+    if (a.dtype < AB_BF16 || a.dtype > AB_F32) return set_error(AB_ERR_INVALID, "%s: unknown dtype", what);
+    for (int64_t stride : {a.target_stride, a.draft_stride})
+        if (stride < 0 || stride >= (int64_t(1) << 40)) return set_error(AB_ERR_INVALID, "%s: strides must be from 0 to 2^40", what);
+    c = VerifyCall{};
+    c.target = a.target;
+    c.draft = a.draft;
+    c.target_row = a.target_stride;
+    c.draft_row = a.draft_stride;
+    c.tokens = a.tokens;
+    c.wide = a.wide_tokens != 0;
+    c.parents = a.parents;
+    c.offsets = a.offsets;
+    c.uniforms = a.uniforms;
+    c.path = a.path;
+    c.counts = a.counts;
+    c.next = a.next;
+    c.batch = static_cast<int32_t>(a.batch);
+    c.rows = static_cast<int32_t>(a.rows);
+    c.vocab = static_cast<int32_t>(a.vocab);
+    c.parts = static_cast<int32_t>((a.vocab + kVerifyPart - 1) / kVerifyPart);
+    c.type = static_cast<int32_t>(a.dtype);
+    bytes = size_t(a.batch) * sizeof(VerifyState) + (size_t(a.batch) * c.parts + size_t(a.rows)) * sizeof(double);
+    c.state = static_cast<VerifyState*>(a.workspace);
+    c.sums = reinterpret_cast<double*>(c.state + a.batch);
+    c.totals = c.sums + a.batch * c.parts;
+    return AB_OK;
+}
+}  // namespace
+
+extern "C" {
+
+size_t ab_verify_workspace_bytes(const ab_verify_args* a) {
+    VerifyCall c;
+    size_t bytes;
+    return !a || verify_call(*a, c, bytes) ? 0 : bytes;
+}
+
+int ab_verify_drafts(const ab_verify_args* a, void* stream) {
+    const char* what = "verify_drafts";
+    if (!a) return set_error(AB_ERR_INVALID, "%s: null pointer", what);
+    VerifyCall c;
+    size_t bytes;
+    if (int rc = verify_call(*a, c, bytes)) return rc;
+    if (a->batch == 0) return AB_OK;
+    if (!a->offsets || !a->counts || !a->next || !a->workspace ||
+        (a->rows > 0 && (!a->target || !a->tokens || !a->parents || !a->uniforms || !a->path)))
+        return set_error(AB_ERR_INVALID, "%s: null pointer", what);
+    if (a->workspace_bytes < bytes)
+        return set_error(AB_ERR_INVALID, "%s: workspace of %zu bytes is smaller than the %zu required", what, a->workspace_bytes, bytes);
+    const uintptr_t element = a->dtype == AB_F32 ? 4 : 2;
+    if (!aligned(a->workspace, 16) || !aligned(a->target, element) || !aligned(a->draft, element))
+        return set_error(AB_ERR_INVALID, "%s: misaligned pointer", what);
+    return launch_verify(c, static_cast<hipStream_t>(stream));
+}
+
+int ab_keep_drafts(const ab_keep_args* a, void* stream) {
+    const char* what = "keep_drafts";
+    if (!a) return set_error(AB_ERR_INVALID, "%s: null pointer", what);
+    if (int rc = check_heads(what, a->batch, a->kv_heads, a->kv_heads, a->tokens, a->dim)) return rc;
+    KeepCall c{};
+    if (int rc = check_cache(what, a->batch, a->kv_heads, a->pages, a->page_tokens, a->table_width, a->k_stride, a->v_stride,
+                             a->page_table, a->lengths, a->offsets, c.k_rows, c.v_rows))
+        return rc;
+    if (a->table_width * a->page_tokens >= kMostTokens)
+        return set_error(AB_ERR_INVALID, "%s: a page table covers fewer than 2^30 tokens", what);
+    if (int rc = check_layers(what, a->layers, a->k_layer, a->v_layer)) return rc;
+    if (a->batch == 0 || a->tokens == 0 || a->pages == 0 || a->table_width == 0) return AB_OK;
+    if (!a->k_cache || !a->v_cache || !a->path || !a->counts) return set_error(AB_ERR_INVALID, "%s: null pointer", what);
+    if (!aligned(a->k_cache, 16) || !aligned(a->v_cache, 16))
+        return set_error(AB_ERR_INVALID, "%s: tensors must be 16-byte aligned", what);
+    c.k_cache = a->k_cache;
+    c.v_cache = a->v_cache;
+    c.k_layer = a->k_layer;
+    c.v_layer = a->v_layer;
+    c.table = a->page_table;
+    c.lengths = a->lengths;
+    c.offsets = a->offsets;
+    c.path = a->path;
+    c.counts = a->counts;
+    c.layers = static_cast<int32_t>(a->layers);
+    c.batch = static_cast<int32_t>(a->batch);
+    c.kv_heads = static_cast<int32_t>(a->kv_heads);
+    c.dim = static_cast<int32_t>(a->dim);
+    c.tokens = static_cast<int32_t>(a->tokens);
+    c.table_width = static_cast<int32_t>(a->table_width);
+    c.pages = static_cast<int32_t>(a->pages);
+    c.page = divisor(static_cast<uint32_t>(a->page_tokens));
+    return launch_keep(c, static_cast<hipStream_t>(stream));
+}
+
+int ab_copy_pages(const ab_copy_args* a, void* stream) {
+    const char* what = "copy_pages";
+    if (!a) return set_error(AB_ERR_INVALID, "%s: null pointer", what);
+    if (int rc = check_heads(what, 1, a->kv_heads, a->kv_heads, 1, a->dim)) return rc;
+    Rows k, v;
+    if (int rc = check_cache(what, 0, a->kv_heads, a->pages, a->page_tokens, 0, a->k_stride, a->v_stride, nullptr, nullptr, nullptr, k, v))
+        return rc;
+    if (int rc = check_layers(what, a->layers, a->k_layer, a->v_layer)) return rc;
+    if (a->count < 0 || a->kv_heads * a->page_tokens * a->dim / 8 >= (int64_t(1) << 31))
+        return set_error(AB_ERR_INVALID, "%s: too large a page", what);
+    if (a->count == 0) return AB_OK;
+    if (!a->k_cache || !a->v_cache || !a->moves) return set_error(AB_ERR_INVALID, "%s: null pointer", what);
+    if (!aligned(a->k_cache, 16) || !aligned(a->v_cache, 16))
+        return set_error(AB_ERR_INVALID, "%s: tensors must be 16-byte aligned", what);
+    for (int64_t i = 0; i < 2 * a->count; ++i)
+        if (a->moves[i] < 0 || a->moves[i] >= a->pages) return set_error(AB_ERR_INVALID, "%s: there is no page %d", what, a->moves[i]);
+    CopyCall c{};
+    c.k_cache = a->k_cache;
+    c.v_cache = a->v_cache;
+    c.k_layer = a->k_layer;
+    c.v_layer = a->v_layer;
+    c.k_page = k.batch;
+    c.v_page = v.batch;
+    // Both tensors' rows in the order that the keys have in memory.
+    const bool heads_outside = k.head >= k.token;
+    c.k_outer = heads_outside ? k.head : k.token;
+    c.k_inner = heads_outside ? k.token : k.head;
+    c.v_outer = heads_outside ? v.head : v.token;
+    c.v_inner = heads_outside ? v.token : v.head;
+    c.inner = divisor(static_cast<uint32_t>(heads_outside ? a->page_tokens : a->kv_heads));
+    c.pieces = static_cast<uint32_t>(a->kv_heads * a->page_tokens * a->dim / 8);
+    c.dim = static_cast<int32_t>(a->dim);
+    c.layers = static_cast<int32_t>(a->layers);
+    for (int64_t at = 0; at < a->count; at += kMovesAtOnce) {
+        c.count = static_cast<int32_t>(std::min<int64_t>(kMovesAtOnce, a->count - at));
+        std::copy(a->moves + 2 * at, a->moves + 2 * (at + c.count), &c.moves[0][0]);
+        if (int rc = launch_copy(c, static_cast<hipStream_t>(stream))) return rc;
+    }
+    return AB_OK;
 }
 
 }  // extern "C"

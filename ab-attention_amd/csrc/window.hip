@@ -177,7 +177,7 @@ __device__ __forceinline__ void max_over_rows(float& a, float& b) {
     b = __uint_as_float(u[1]);
 }
 
-template <class T, int D, bool kPaged, bool kSplit>
+template <class T, int D, bool kPaged, bool kSplit, bool kTree>
 __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c, WindowGrid places) {
     using Tile = WindowTile<T, D>;
     constexpr int kSteps = Tile::kSteps, kBlocks = Tile::kBlocks, kOps = Tile::kOps;
@@ -196,7 +196,8 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     const WindowMask mask = c.mask;
     const int row0 = u.tile * kWindowRows, rows = min(kWindowRows, u.n * group - row0);
     auto token_at = [&](int r) { return kPaged ? (row0 + r) / group : row0 + r; };
-    const int p_first = max(u.first + token_at(0), 0), p_last = min(u.first + token_at(rows - 1), u.length - 1);
+    // A tree's tokens are at positions from u.first on, and see nothing in the cache behind their own place.
+    const int p_first = max(u.first + (kTree ? 0 : token_at(0)), 0), p_last = min(u.first + token_at(rows - 1), u.length - 1);
     TileRange range;
     range.set(mask, p_first, p_last, u.length);
     const int end = range.end;
@@ -229,17 +230,22 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
         }
     };
     int low[2], seen[2], sink[2];  // keys low .. low + seen - 1 and 0 .. sink - 1
+    int line[2];                   // of a tree: the token whose line is seen too, or -1
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         int token, head;
         const bool stored = row_of(j, token, head);
-        const int p = u.first + token;
-        const bool sees = stored && p >= 0 && p < u.length;
-        const int high = mask.high(max(p, 0), u.length);
+        const int p = kTree ? c.positions[u.off + token] : u.first + token;
+        const bool sees = stored && p >= 0 && (kTree || p < u.length);
+        // Of a tree the bounds are those of the keys before it.
+        const int high = kTree ? max(u.first, 0) : mask.high(max(p, 0), u.length);
         low[j] = mask.low(max(p, 0));
-        seen[j] = sees ? high - low[j] : 0;
+        seen[j] = sees ? max(high - low[j], 0) : 0;
         sink[j] = sees ? min(mask.sinks, high) : 0;
+        if constexpr (kTree) line[j] = sees ? token : -1;
     }
+    // Whether the window of some token can end between drafts: then their positions count too.
+    const bool cut = kTree && mask.low(max(p_last, 0)) > u.first;
     // Tiles that every row of this wave sees need no mask: keys from full_low to
     // full_high, and those before full_sink. A wave with a row that exists but
     // sees nothing masks every tile.
@@ -247,10 +253,10 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     const int wave_rows = min(32, rows - wave * 32);
     const bool active = wave_rows > 0;
     if (active) {
-        const int pf = u.first + token_at(wave * 32), pl = u.first + token_at(wave * 32 + wave_rows - 1);
+        const int pf = u.first + (kTree ? 0 : token_at(wave * 32)), pl = u.first + token_at(wave * 32 + wave_rows - 1);
         if (pf >= 0 && pl < u.length) {
             full_low = mask.low(pl);
-            full_high = mask.high(pf, u.length);
+            full_high = kTree ? pf : mask.high(pf, u.length);
             full_sink = min(mask.sinks, full_high);
         }
     }
@@ -412,6 +418,31 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 bits |= static_cast<uint32_t>(key + r - low[j]) < static_cast<uint32_t>(seen[j]) || key + r < sink[j] ? 1u << r : 0u;
+        if constexpr (kTree)
+            if (t < tiles && key + 3 >= u.first && key < end && line[j] >= 0 && (!holes || on_page(key))) {
+                // Places among the new tokens; the line's word of 64 of them, walked up to.
+                const int place = key - u.first;
+                auto word_of = [&](int block) -> uint64_t {
+                    int i = line[j];
+                    while (i >= 0 && i >> 6 > block) {
+                        const int up = c.above[u.off + i];
+                        i = up < (i & ~63) ? up : -1;
+                    }
+                    return i >= 0 && i >> 6 == block ? c.near[u.off + i] : 0;
+                };
+                const int block = max(place, 0) >> 6;
+                const uint64_t word = word_of(block), next = (place + 3) >> 6 > block ? word_of(block + 1) : 0;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = place + r;
+                    bool on = i >= 0 && i <= line[j] && ((i >> 6 > block ? next : word) >> (i & 63) & 1);
+                    if (on && cut) {
+                        const int p = c.positions[u.off + i];
+                        on = p >= low[j] || p < mask.sinks;
+                    }
+                    bits |= on ? 1u << r : 0u;
+                }
+            }
         return bits;
     };
 
@@ -827,12 +858,12 @@ __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
     if (c.lse && lane == 0) c.lse[row] = l == 0.f ? -INFINITY : m + log2f(l);
 }
 
-template <class T, int D, bool kPaged>
+template <class T, int D, bool kPaged, bool kTree = false>
 int launch_as(const WindowCall& c, hipStream_t stream) {
     const int64_t tiles = window_tiles(c), heads = kPaged ? c.kv_heads : int64_t(c.batch) * c.heads;
     const WindowGrid places = window_grid(heads, tiles);
     const dim3 grid(places.size(), static_cast<unsigned>(c.parts));
-    const auto kernel = c.parts == 1 ? window_kernel<T, D, kPaged, false> : window_kernel<T, D, kPaged, true>;
+    const auto kernel = c.parts == 1 ? window_kernel<T, D, kPaged, false, kTree> : window_kernel<T, D, kPaged, true, kTree>;
     constexpr int kLds = WindowTile<T, D>::kLdsBytes;
     if (int rc = ensure_lds_limit(reinterpret_cast<const void*>(kernel), kLds)) return rc;
     hipLaunchKernelGGL(kernel, grid, dim3(kWindowThreads), kLds, stream, c, places);
@@ -881,6 +912,7 @@ int window_parts(const WindowCall& c, int64_t most_keys) {
 int launch_window(const WindowCall& c, hipStream_t stream) {
     auto typed = [&](auto t) {
         using T = decltype(t);
+        if (c.near) return c.dim == 128 ? launch_as<T, 128, true, true>(c, stream) : launch_as<T, 64, true, true>(c, stream);
         if (c.dim == 128) return c.paged ? launch_as<T, 128, true>(c, stream) : launch_as<T, 128, false>(c, stream);
         return c.paged ? launch_as<T, 64, true>(c, stream) : launch_as<T, 64, false>(c, stream);
     };

@@ -156,6 +156,9 @@ struct WindowCall {
     int32_t dim, half;                       // half: 0 bf16, 1 fp16
     bool paged;
     const int32_t *lengths, *offsets, *table;
+    // New tokens that are a tree (TreeCall's results), or none.
+    const int32_t *positions, *above;
+    const uint64_t* near;
     int32_t table_width, pages;
     Divisor page, group;                     // tokens of a page; query heads of a K/V head
     WindowMask mask;

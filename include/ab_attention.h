@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define AB_ABI_VERSION 8
+#define AB_ABI_VERSION 9
 
 enum ab_status {
     AB_OK = 0,
@@ -347,6 +347,92 @@ typedef struct ab_append_args {
     int64_t k_stride[3], v_stride[3], k_cache_stride[3], v_cache_stride[3];
 } ab_append_args;
 int ab_append_cache(const ab_append_args *args, void *stream);
+
+/* ---- Drafted tokens: a step that checks several at once ----------------------
+ * No counterpart in the reference. A sequence's new tokens (offsets, lengths as in
+ * ab_chunk_attention) are a tree: parents int32 [tokens] gives the place, among its
+ * sequence's new tokens, of the one that each follows; a number that is no earlier
+ * place (-1) is none, and the token follows the cached ones. Token i is at position
+ * lengths[b] - n + (tokens above it), though in the cache at lengths[b] - n + i.
+ *
+ * ab_draft_tree: positions int32 [tokens]; the tokens on the line down to each, itself
+ *   too, in words of 64 places: near uint64 [tokens] the word of its own 64, above
+ *   int32 [tokens] the last place of the line before those, or -1. Rows of no sequence
+ *   get 0, 0, -1. No output shares memory with anything else. */
+typedef struct ab_draft_tree_args {
+    const int32_t *parents, *lengths, *offsets;
+    int32_t *positions;
+    uint64_t *near;
+    int32_t *above;
+    int64_t batch, tokens;
+} ab_draft_tree_args;
+int ab_draft_tree(const ab_draft_tree_args *args, void *stream);
+
+/* ab_chunk_attention of new tokens that are a tree: the query at position p sees the
+ * cached keys that the mask gives it, and of the new ones those of its line, itself too,
+ * whose positions the mask gives it. positions, near and above are ab_draft_tree's for
+ * the same lengths and offsets. Workspace: ab_window_workspace_bytes(&args->chunk). */
+typedef struct ab_tree_args {
+    ab_window_args chunk;
+    const int32_t *positions;
+    const uint64_t *near;
+    const int32_t *above;
+} ab_tree_args;
+int ab_tree_attention(const ab_tree_args *args, void *stream);
+
+/* Which drafts stay. A sequence's first new token is kept; then, from the last kept one
+ * on, the tokens j that follow it are looked at in the order of their places. With target
+ * [tokens, vocab] (row i: probabilities behind token i), w the row of the last kept
+ * token and S = 1 at first, j is kept, and becomes the last kept one, where
+ *   uniforms[j] * q * S < w[tokens[j]],   q = draft[last kept][tokens[j]], or 1,
+ * and else w <- max(w - S draft[last kept], 0), S <- sum of w (both stay where that is
+ * 0), or without `draft` S <- S - w[tokens[j]], w[tokens[j]] <- 0. Where none is left
+ * next[b] is the first entry with w > 0 whose running sum of w passes uniforms[first] times
+ * the sum of w (or the last with w > 0; -1 if there is none). Sums are in 64 bits;
+ * entries that are not positive and finite count as 0, and so do tokens outside
+ * 0 .. vocab - 1. path int32 [tokens]: from offsets[b] on the counts[b] kept places, then
+ * -1; a sequence without new tokens has counts 0, next -1. target and draft of one type,
+ * rows contiguous, strides in elements; tokens and next int32, or with wide_tokens int64.
+ * workspace: ab_verify_workspace_bytes(args) bytes, 16-byte aligned. */
+typedef struct ab_verify_args {
+    const void *target, *draft;
+    const void *tokens;
+    const int32_t *parents, *offsets;
+    const float *uniforms;
+    int32_t *path, *counts;
+    void *next;
+    int64_t batch, rows, vocab, dtype, wide_tokens;
+    int64_t target_stride, draft_stride;
+    void *workspace;
+    size_t workspace_bytes;
+} ab_verify_args;
+size_t ab_verify_workspace_bytes(const ab_verify_args *args);
+int ab_verify_drafts(const ab_verify_args *args, void *stream);
+
+/* The kept tokens' keys and values next to each other: in each of `layers` caches
+ * [pages, kv_heads, page_tokens, dim] (16-bit elements; k_layer, v_layer from one to the
+ * next) position lengths[b] - n + path[offsets[b] + j] is copied to lengths[b] - n + j, for
+ * j < counts[b], all as they were before. A place outside j .. n - 1, or on no page, moves
+ * nothing. No two rows of the caches share memory, no page is in two places of the table. */
+typedef struct ab_keep_args {
+    void *k_cache, *v_cache;
+    const int32_t *lengths, *offsets, *page_table, *path, *counts;
+    int64_t layers, batch, kv_heads, tokens, dim;
+    int64_t pages, page_tokens, table_width;
+    int64_t k_layer, v_layer, k_stride[3], v_stride[3];
+} ab_keep_args;
+int ab_keep_drafts(const ab_keep_args *args, void *stream);
+
+/* Pages copied to pages, in each of `layers` caches: moves int32 [count][2] in host
+ * memory, read before the call returns, from and to. Pages that are copied to are named
+ * once. */
+typedef struct ab_copy_args {
+    void *k_cache, *v_cache;
+    const int32_t *moves;
+    int64_t count, layers, kv_heads, dim, pages, page_tokens;
+    int64_t k_layer, v_layer, k_stride[3], v_stride[3];
+} ab_copy_args;
+int ab_copy_pages(const ab_copy_args *args, void *stream);
 
 #ifdef __cplusplus
 }
