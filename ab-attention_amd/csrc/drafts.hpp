@@ -18,10 +18,11 @@ struct TreeCall {
 
 // Where a sequence's verification stands between its two kernels.
 struct VerifyState {
+    double less;     // drawn drafts: what is left of p is max(p - less q, 0)
     int32_t last;    // the last kept token's place
     int32_t next;    // the first place that has not been looked at
     int32_t counts;  // kept tokens
-    int32_t less;    // drafts turned down behind the last kept token, as far as the sums take them in
+    int32_t gone;    // drafts turned down behind the last kept token
 };
 
 struct VerifyCall {
@@ -37,11 +38,12 @@ struct VerifyCall {
     int32_t type;  // 0 bf16, 1 fp16, 2 fp32
     VerifyState* state;  // [batch]
     double* sums;        // [batch][parts]
-    double* totals;      // [rows]: of a sequence, at less: sum of what was left before that draft was turned down
+    int32_t times;       // a part is so many times kVerifyStep tokens of the vocabulary
 };
 
 int launch_tree(const TreeCall& call, hipStream_t stream);
 int launch_verify(const VerifyCall& call, hipStream_t stream);
-constexpr int kVerifyPart = 1024;  // tokens of the vocabulary in a part
+constexpr int kVerifyStep = 1024;   // tokens of the vocabulary that a wave takes at a time
+constexpr int kVerifyParts = 256;   // of a vocabulary, at most
 
 }  // namespace ab

@@ -403,12 +403,13 @@ int verify_call(const ab_verify_args& a, VerifyCall& c, size_t& bytes) {
     c.batch = static_cast<int32_t>(a.batch);
     c.rows = static_cast<int32_t>(a.rows);
     c.vocab = static_cast<int32_t>(a.vocab);
-    c.parts = static_cast<int32_t>((a.vocab + kVerifyPart - 1) / kVerifyPart);
+    const int64_t steps = (a.vocab + kVerifyStep - 1) / kVerifyStep;
+    c.times = static_cast<int32_t>((steps + kVerifyParts - 1) / kVerifyParts);
+    c.parts = static_cast<int32_t>((steps + c.times - 1) / c.times);
     c.type = static_cast<int32_t>(a.dtype);
-    bytes = size_t(a.batch) * sizeof(VerifyState) + (size_t(a.batch) * c.parts + size_t(a.rows)) * sizeof(double);
+    bytes = size_t(a.batch) * sizeof(VerifyState) + size_t(a.batch) * c.parts * sizeof(double);
     c.state = static_cast<VerifyState*>(a.workspace);
     c.sums = reinterpret_cast<double*>(c.state + a.batch);
-    c.totals = c.sums + a.batch * c.parts;
     return AB_OK;
 }
 }  // namespace
