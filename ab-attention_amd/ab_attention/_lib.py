@@ -177,6 +177,7 @@ SIGNATURES = {
     "ab_window_attention_grad": (ctypes.c_int, [ctypes.POINTER(WindowGradArgs), _P]),
     "ab_append_cache": (ctypes.c_int, [ctypes.POINTER(AppendArgs), _P]),
     "ab_draft_tree": (ctypes.c_int, [ctypes.POINTER(DraftTreeArgs), _P]),
+    "ab_tree_workspace_bytes": (_SZ, [ctypes.POINTER(TreeArgs)]),
     "ab_tree_attention": (ctypes.c_int, [ctypes.POINTER(TreeArgs), _P]),
     "ab_verify_workspace_bytes": (_SZ, [ctypes.POINTER(VerifyArgs)]),
     "ab_verify_drafts": (ctypes.c_int, [ctypes.POINTER(VerifyArgs), _P]),

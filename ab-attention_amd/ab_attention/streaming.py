@@ -244,10 +244,11 @@ def _check_window(window, scale, dim):
     return scale
 
 
-def _run(entry, device, packed, behind=b""):
-    """One call with the workspace that it asks for, which lives for the call only; ``behind``: fields after ab_window_args."""
+def _run(entry, device, packed, behind=b"", asks="ab_window_workspace_bytes"):
+    """One call with the workspace that it ``asks`` for, which lives for the call only; ``behind``: fields after
+    ab_window_args."""
     with _lib.on(device):
-        size = _lib.raw("ab_window_workspace_bytes")(packed)
+        size = _lib.raw(asks)(packed + behind)
         if size:
             workspace = torch.empty(size, dtype=torch.uint8, device=device)
             packed = packed[:-_WORKSPACE.size] + _WORKSPACE.pack(workspace.data_ptr(), size)
@@ -445,11 +446,13 @@ def chunk_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
     ``out``, a tensor of q's shape and type to write to, they stay as they are).
     ``out`` may be q itself; it shares no memory with anything else that is read.
     """
-    return _over_cache("chunk attention", "ab_chunk_attention", q, cache, page_table, lengths, offsets, b"", window, sinks, frame,
+    return _over_cache("chunk attention", ("ab_chunk_attention",), q, cache, page_table, lengths, offsets, window, sinks, frame,
                        scale, return_lse, out)
 
 
-def _over_cache(name, entry, q, cache, page_table, lengths, offsets, behind, window, sinks, frame, scale, return_lse, out):
+def _over_cache(name, entry, q, cache, page_table, lengths, offsets, window, sinks, frame, scale, return_lse, out, *behind):
+    """``entry``: the library's, and the one that says its workspace's size if it is another; ``behind``: bytes of its
+    arguments after ab_window_args."""
     _check_cache(name, q, cache, page_table, lengths, offsets)
     device = q.device
     scale = _check_window(window, scale, q.shape[-1])
@@ -467,11 +470,11 @@ def _over_cache(name, entry, q, cache, page_table, lengths, offsets, behind, win
     if tokens and page_table.shape[0]:
         pages, kv_heads, page, _ = cache[0].shape
         k, v = cache
-        _run(entry, device, _WINDOW.pack(
+        _run(entry[0], device, _WINDOW.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0, 0 if lse is None else lse.data_ptr(),
             lengths.data_ptr(), offsets.data_ptr(), page_table.data_ptr(), page_table.shape[0], heads, kv_heads, tokens, dim,
             _DTYPES[q.dtype], pages, page, page_table.shape[1], window, sinks, frame, scale, 0, q.stride(1), q.stride(0),
-            *k.stride()[:3], *v.stride()[:3], 0, out.stride(1), out.stride(0), 0, 0), behind)
+            *k.stride()[:3], *v.stride()[:3], 0, out.stride(1), out.stride(0), 0, 0), *behind, *entry[1:])
     return (out, lse) if return_lse else out
 
 
@@ -535,9 +538,9 @@ def tree_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor,
     if near.dtype != torch.int64 or not near.is_contiguous() or not positions.shape == near.shape == above.shape == q.shape[:1]:
         raise ValueError("tree attention requires the tree of Q's packed tokens")
     _gpu("tree attention", q, *tree)
-    return _over_cache("tree attention", "ab_tree_attention", q, cache, page_table, lengths, offsets,
-                       _TREE_REST.pack(positions.data_ptr(), near.data_ptr(), above.data_ptr()), window, sinks, frame, scale,
-                       return_lse, out)
+    return _over_cache("tree attention", ("ab_tree_attention", "ab_tree_workspace_bytes"), q, cache, page_table, lengths, offsets,
+                       window, sinks, frame, scale, return_lse, out,
+                       _TREE_REST.pack(positions.data_ptr(), near.data_ptr(), above.data_ptr()))
 
 
 class Kept(NamedTuple):

@@ -143,6 +143,17 @@ size_t workspace_bytes(const WindowCall& c) {
     return c.parts == 1 ? 0 : size_t(c.parts) * size_t(c.rows) * (size_t(c.dim) * sizeof(float) + sizeof(float2) + rounded);
 }
 
+// A tree's parts. All of its tiles of rows look at what its first token's window shows, and
+// at the drafts.
+void plan_tree_call(const ab_window_args& a, WindowCall& c) {
+    const int64_t length = a.table_width * a.page_tokens;
+    plan_tree(c, std::min(length, most_keys(a, length) + a.tokens));
+}
+
+size_t tree_workspace_bytes(const WindowCall& c) {
+    return size_t(c.rows) * sizeof(int4) + size_t(c.slots) * kWindowRows * (size_t(c.dim) * sizeof(float) + sizeof(float2));
+}
+
 int window_launch(const char* what, const ab_window_args* a, bool paged, void* stream, const ab_tree_args* tree = nullptr) {
     if (!a) return set_error(AB_ERR_INVALID, "%s: null pointer", what);
     WindowCall c;
@@ -150,6 +161,7 @@ int window_launch(const char* what, const ab_window_args* a, bool paged, void* s
     if (tree) {
         if (a->tokens > 0 && a->batch > 0 && (!tree->positions || !tree->near || !tree->above))
             return set_error(AB_ERR_INVALID, "%s: null pointer", what);
+        plan_tree_call(*a, c);
         c.positions = tree->positions;
         c.near = tree->near;
         c.above = tree->above;
@@ -160,7 +172,16 @@ int window_launch(const char* what, const ab_window_args* a, bool paged, void* s
     if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->out, 8) || !aligned(a->out_rest, 8))
         return set_error(AB_ERR_INVALID, "%s: q/k/v must be 16-byte and out 8-byte aligned", what);
     if (!a->workspace) c.parts = 1;
-    if (c.parts > 1) {
+    if (tree) {
+        if (!a->workspace) return set_error(AB_ERR_INVALID, "%s: null pointer", what);
+        if (a->workspace_bytes < tree_workspace_bytes(c))
+            return set_error(AB_ERR_INVALID, "%s: workspace of %zu bytes is smaller than the %zu required", what,
+                             a->workspace_bytes, tree_workspace_bytes(c));
+        if (!aligned(a->workspace, 16)) return set_error(AB_ERR_INVALID, "%s: workspace must be 16-byte aligned", what);
+        c.row_parts = static_cast<int4*>(a->workspace);
+        c.partial_o = reinterpret_cast<float*>(c.row_parts + c.rows);
+        c.partial_stat = reinterpret_cast<float2*>(c.partial_o + int64_t(c.slots) * kWindowRows * c.dim);
+    } else if (!tree && c.parts > 1) {
         if (a->workspace_bytes < workspace_bytes(c))
             return set_error(AB_ERR_INVALID, "%s: workspace of %zu bytes is smaller than the %zu required", what,
                              a->workspace_bytes, workspace_bytes(c));
@@ -369,6 +390,13 @@ int ab_draft_tree(const ab_draft_tree_args* a, void* stream) {
     const TreeCall c{a->parents, a->lengths, a->offsets, a->positions, a->near, a->above, static_cast<int32_t>(a->batch),
                      static_cast<int32_t>(a->tokens)};
     return launch_tree(c, static_cast<hipStream_t>(stream));
+}
+
+size_t ab_tree_workspace_bytes(const ab_tree_args* a) {
+    WindowCall c;
+    if (!a || a->chunk.batch <= 0 || a->chunk.tokens <= 0 || window_call("tree_attention", a->chunk, true, c)) return 0;
+    plan_tree_call(a->chunk, c);
+    return tree_workspace_bytes(c);
 }
 
 int ab_tree_attention(const ab_tree_args* a, void* stream) {

@@ -62,6 +62,10 @@ struct WindowUnit {
     int off;               // their first row in the packed tensor (0 without offsets)
     int first;             // position of its first new token
     int length;            // keys of it
+    // Of a tree: which of the tile's steps these are, whether that is all of them, and else
+    // where the rows' sums go, and, of the first part, how many parts there are.
+    int from, to, slot, parts;
+    bool whole;
 };
 
 template <bool kPaged>
@@ -135,6 +139,125 @@ __device__ __forceinline__ bool window_unit(const WindowCall& c, const WindowGri
     }
 }
 
+// x of the lane that a DPP control names, 0 where there is none.
+template <int kControl>
+__device__ __forceinline__ int lane_moved(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, kControl, 15, 15, true);
+}
+template <int kControl>
+__device__ __forceinline__ double lane_moved(double x) {
+    const int2 halves = __builtin_bit_cast(int2, x);
+    return __builtin_bit_cast(double, int2{lane_moved<kControl>(halves.x), lane_moved<kControl>(halves.y)});
+}
+__device__ __forceinline__ double lane_value(double x, int lane) {
+    const int2 halves = __builtin_bit_cast(int2, x);
+    return __builtin_bit_cast(double, int2{__builtin_amdgcn_readlane(halves.x, lane), __builtin_amdgcn_readlane(halves.y, lane)});
+}
+// x and those of the lanes before.
+__device__ __forceinline__ double running_sum(double x, int lane) {
+    x += lane_moved<0x111>(x);  // row_shr 1, 2, 4, 8
+    x += lane_moved<0x112>(x);
+    x += lane_moved<0x114>(x);
+    x += lane_moved<0x118>(x);
+    const double one = lane_value(x, 15), two = one + lane_value(x, 31), three = two + lane_value(x, 47);
+    return x + (lane < 16 ? 0.0 : lane < 32 ? one : lane < 48 ? two : three);
+}
+__device__ __forceinline__ int most_of_lanes(int x) {  // of numbers that are not negative
+    x = max(x, lane_moved<0x111>(x));
+    x = max(x, lane_moved<0x112>(x));
+    x = max(x, lane_moved<0x114>(x));
+    x = max(x, lane_moved<0x118>(x));
+    return max(max(__builtin_amdgcn_readlane(x, 15), __builtin_amdgcn_readlane(x, 31)),
+               max(__builtin_amdgcn_readlane(x, 47), __builtin_amdgcn_readlane(x, 63)));
+}
+
+// A tree's work, which its workgroups deal out among themselves: how many sequences there
+// are, and how long they are, is on the device. For a head all steps (tiles of keys) of all
+// tiles of rows of all sequences stand in a row, sequence by sequence, and workgroup w of the
+// head's c.wanted takes the `each` steps from w each on, at least kTreeSteps: all do the
+// same, whatever the lengths. What it has is the end of one tile of rows, perhaps some
+// whole ones, and the beginning of another. Counts are whole numbers in 64-bit floats.
+struct TreeWork {
+    double at, end;  // this workgroup's steps that are left
+    double each;
+    int w, kv_head;
+    bool first;      // none has been done
+
+    struct Sequence {
+        int off, n, length, tiles, steps;
+    };
+    static __device__ __forceinline__ Sequence look_at(const WindowCall& c, int b) {
+        Sequence s;
+        const bool there = b < c.batch;
+        b = min(b, c.batch - 1);
+        s.off = min(max(c.offsets[b], 0), c.tokens);
+        s.n = there ? min(max(c.offsets[b + 1], 0), c.tokens) - s.off : 0;
+        s.length = static_cast<int>(min(int64_t(max(c.lengths[b], 0)), int64_t(c.table_width) * c.page.d));
+        s.tiles = s.n > 0 ? static_cast<int>((int64_t(s.n) * c.group.d + kWindowRows - 1) / kWindowRows) : 0;
+        TileRange range;
+        range.set(c.mask, max(s.length - s.n, 0), s.length - 1, s.length);
+        s.steps = max(range.tiles, 1);  // rows that see nothing are written too
+        return s;
+    }
+
+    __device__ __forceinline__ TreeWork(const WindowCall& c, int id) : first(true) {
+        const int lane = threadIdx.x & 63;
+        double steps = 0.0;
+        int longest = 0;
+        for (int b = 0; b < c.batch; b += 64) {
+            const Sequence s = look_at(c, b + lane);
+            steps += static_cast<double>(s.tiles) * s.steps;
+            longest = max(longest, s.tiles > 0 ? s.steps : 0);
+        }
+        const double all = lane_value(running_sum(steps, lane), 63);
+        // A tile of rows has at most kMostParts parts, the two at its ends among them.
+        const int least = max(kTreeSteps, most_of_lanes(longest) / (kMostParts - 2) + 1);
+        each = lane_value(fmax(floor(all * c.share) + 1.0, static_cast<double>(least)), 0);
+        w = id / c.kv_heads;
+        kv_head = __builtin_amdgcn_readfirstlane(id - w * c.kv_heads);
+        w = __builtin_amdgcn_readfirstlane(w);
+        at = lane_value(each * w, 0);
+        end = lane_value(fmin(at + each, all), 0);
+    }
+
+    // The next tile of rows and its steps; false if there is none.
+    __device__ __forceinline__ bool next(const WindowCall& c, WindowUnit& u) {
+        if (!(__builtin_amdgcn_readfirstlane(at < end))) return false;
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        double before = 0.0;
+        for (int b = 0; b < c.batch; b += 64) {
+            const Sequence s = look_at(c, b + lane);
+            const double its = static_cast<double>(s.tiles) * s.steps, until = before + running_sum(its, lane);
+            const uint64_t here = __ballot(until > at && until - its <= at);
+            before = lane_value(until, 63);
+            if (here == 0) continue;
+            const int l = __builtin_ctzll(here);
+            auto uniform = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+            u.b = b + l;
+            u.off = uniform(s.off);
+            u.n = uniform(s.n);
+            u.length = uniform(s.length);
+            u.first = u.length - u.n;
+            u.kv_head = kv_head;
+            u.head = kv_head * static_cast<int>(c.group.d);
+            const int steps = uniform(s.steps);
+            const double start = lane_value(until - its, l), tile = floor((at - start + 0.5) / steps), here_from = at - start - tile * steps;
+            const double until_here = fmin(static_cast<double>(steps), here_from + (end - at));
+            u.tile = __builtin_amdgcn_readfirstlane(static_cast<int>(tile));
+            u.from = __builtin_amdgcn_readfirstlane(static_cast<int>(here_from));
+            u.to = __builtin_amdgcn_readfirstlane(static_cast<int>(until_here));
+            u.whole = u.from == 0 && u.to == steps;
+            u.slot = 2 * (w * c.kv_heads + kv_head) + (first ? 0 : 1);
+            u.parts = __builtin_amdgcn_readfirstlane(static_cast<int>(floor((start + (tile + 1) * steps - 0.5) / each))) - w + 1;
+            first = false;
+            at = lane_value(at + until_here - here_from, 0);
+            return true;
+        }
+        return false;
+    }
+};
+
 template <class T, int D>
 struct WindowTile {
     static constexpr int kSteps = D / 32;                  // MFMA k-steps of S
@@ -146,6 +269,9 @@ struct WindowTile {
     static constexpr int kVRing = kRing * kBytes;
     static constexpr int kVotes = 2 * kRing * kBytes;
     static constexpr int kLdsBytes = kVotes + 16;
+    static constexpr int kMasks = kLdsBytes;  // a tree's masks, behind the others
+    static constexpr int kMaskWords = 3968;   // two workgroups fit a CU
+    static constexpr int kTreeLdsBytes = kMasks + 4 * kMaskWords;
 };
 
 // What `rounded` lacks of two values, rounded itself (nothing of values that are not
@@ -166,6 +292,17 @@ __device__ __forceinline__ float vmax(float a, float b) {
 }
 #pragma clang diagnostic pop
 
+// Of a word of a line, whose tokens' depths go up to `depth` (moved to the next word's),
+// those of at least `from` or below `sinks`.
+__device__ __forceinline__ uint64_t within(uint64_t word, int& depth, int from, int sinks) {
+    const int count = __popcll(word), first = depth - count + 1;
+    depth = first - 1;
+    uint64_t late = word, rest = word;
+    for (int i = min(from - first, count); i > 0; --i) late &= late - 1;
+    for (int i = min(sinks - first, count); i > 0; --i) rest &= rest - 1;
+    return late | (word & ~rest);
+}
+
 // The maxima of a and b over the four lanes l, 16 + l, 32 + l, 48 + l.
 __device__ __forceinline__ void max_over_rows(float& a, float& b) {
     const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
@@ -177,17 +314,17 @@ __device__ __forceinline__ void max_over_rows(float& a, float& b) {
     b = __uint_as_float(u[1]);
 }
 
+extern __shared__ __align__(16) unsigned char smem[];
+
 template <class T, int D, bool kPaged, bool kSplit, bool kTree>
-__global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c, WindowGrid places) {
+__device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUnit& u) {
     using Tile = WindowTile<T, D>;
     constexpr int kSteps = Tile::kSteps, kBlocks = Tile::kBlocks, kOps = Tile::kOps;
-    extern __shared__ __align__(16) unsigned char smem[];
-    touch(c.q, c.k_rows.batch, c.row.batch, c.lengths, c.rows, places.heads);
-
-    WindowUnit u;
-    if (!window_unit<kPaged>(c, places, blockIdx.x, u)) return;
+    const bool split = kSplit && (!kTree || !u.whole);
     const int group = kPaged ? c.group.d : 1;
-    const int tid = threadIdx.x, lane = tid & 63;
+    int tid = threadIdx.x;
+    if constexpr (kTree) asm volatile("" : "+v"(tid));  // made anew for every tile of rows, not kept beside the passes
+    const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4;
 
@@ -202,7 +339,10 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     range.set(mask, p_first, p_last, u.length);
     const int end = range.end;
     int tile0 = 0, tiles = range.tiles;
-    if constexpr (kSplit) {
+    if constexpr (kTree) {
+        tile0 = min(u.from, tiles);
+        tiles = min(u.to, tiles) - tile0;
+    } else if constexpr (kSplit) {
         const int part = blockIdx.y;
         tile0 = static_cast<int>(int64_t(tiles) * part / c.parts);
         tiles = static_cast<int>(int64_t(tiles) * (part + 1) / c.parts) - tile0;
@@ -229,31 +369,30 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
             for (int s = 0; s < kSteps; ++s) bq[j][s] = *reinterpret_cast<const u32x4*>(qrow + 32 * s);
         }
     };
+    // Of a tree: where the masks of the row's token are in LDS.
     int low[2], seen[2], sink[2];  // keys low .. low + seen - 1 and 0 .. sink - 1
-    int line[2];                   // of a tree: the token whose line is seen too, or -1
+    int masks[2];
+    if constexpr (!kTree) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        int token, head;
-        const bool stored = row_of(j, token, head);
-        const int p = kTree ? c.positions[u.off + token] : u.first + token;
-        const bool sees = stored && p >= 0 && (kTree || p < u.length);
-        // Of a tree the bounds are those of the keys before it.
-        const int high = kTree ? max(u.first, 0) : mask.high(max(p, 0), u.length);
-        low[j] = mask.low(max(p, 0));
-        seen[j] = sees ? max(high - low[j], 0) : 0;
-        sink[j] = sees ? min(mask.sinks, high) : 0;
-        if constexpr (kTree) line[j] = sees ? token : -1;
+        for (int j = 0; j < 2; ++j) {
+            int token, head;
+            const bool stored = row_of(j, token, head);
+            const int p = u.first + token;
+            const bool sees = stored && p >= 0 && p < u.length;
+            const int high = mask.high(max(p, 0), u.length);
+            low[j] = mask.low(max(p, 0));
+            seen[j] = sees ? high - low[j] : 0;
+            sink[j] = sees ? min(mask.sinks, high) : 0;
+        }
     }
-    // Whether the window of some token can end between drafts: then their positions count too.
-    const bool cut = kTree && mask.low(max(p_last, 0)) > u.first;
-    // Tiles that every row of this wave sees need no mask: keys from full_low to
-    // full_high, and those before full_sink. A wave with a row that exists but
-    // sees nothing masks every tile.
+    // Tiles that every row of this wave (of a tree: of the workgroup) sees need no mask: keys
+    // from full_low to full_high, and those before full_sink. A wave with a row that exists
+    // but sees nothing masks every tile.
     int full_low = 0, full_high = 0, full_sink = 0;
     const int wave_rows = min(32, rows - wave * 32);
     const bool active = wave_rows > 0;
-    if (active) {
-        const int pf = u.first + (kTree ? 0 : token_at(wave * 32)), pl = u.first + token_at(wave * 32 + wave_rows - 1);
+    if (kTree || active) {
+        const int pf = u.first + (kTree ? 0 : token_at(wave * 32)), pl = u.first + token_at(kTree ? rows - 1 : wave * 32 + wave_rows - 1);
         if (pf >= 0 && pl < u.length) {
             full_low = mask.low(pl);
             full_high = kTree ? pf : mask.high(pf, u.length);
@@ -410,40 +549,24 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     auto is_masked = [&](int t) {
         return static_cast<uint32_t>(t - clear_from) >= static_cast<uint32_t>(clear) && t >= clear_sink;
     };
+    // Of a masked tile of a tree: which one it is.
+    auto mask_of = [&](int t) { return t - clear_sink - (t >= clear_from ? clear : 0); };
     // Bit r of the result: key 16h + 4lg + r of tile t is seen by row 16j + li.
     auto seen_keys = [&](int t, int h, int j) {
-        const int key = range.key(tile0 + t) + 16 * h + 4 * lg;
-        uint32_t bits = 0;
-        if (t < tiles && (!kPaged || !holes || on_page(key)))
+        if constexpr (kTree) {
+            if (t >= tiles) return 0u;
+            if (!is_masked(t)) return 15u;
+            const uint32_t* its = reinterpret_cast<const uint32_t*>(smem + Tile::kMasks) + masks[j];
+            return its[mask_of(t)] >> (16 * h + 4 * lg) & 15u;
+        } else {
+            const int key = range.key(tile0 + t) + 16 * h + 4 * lg;
+            uint32_t bits = 0;
+            if (t < tiles && (!kPaged || !holes || on_page(key)))
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                bits |= static_cast<uint32_t>(key + r - low[j]) < static_cast<uint32_t>(seen[j]) || key + r < sink[j] ? 1u << r : 0u;
-        if constexpr (kTree)
-            if (t < tiles && key + 3 >= u.first && key < end && line[j] >= 0 && (!holes || on_page(key))) {
-                // Places among the new tokens; the line's word of 64 of them, walked up to.
-                const int place = key - u.first;
-                auto word_of = [&](int block) -> uint64_t {
-                    int i = line[j];
-                    while (i >= 0 && i >> 6 > block) {
-                        const int up = c.above[u.off + i];
-                        i = up < (i & ~63) ? up : -1;
-                    }
-                    return i >= 0 && i >> 6 == block ? c.near[u.off + i] : 0;
-                };
-                const int block = max(place, 0) >> 6;
-                const uint64_t word = word_of(block), next = (place + 3) >> 6 > block ? word_of(block + 1) : 0;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = place + r;
-                    bool on = i >= 0 && i <= line[j] && ((i >> 6 > block ? next : word) >> (i & 63) & 1);
-                    if (on && cut) {
-                        const int p = c.positions[u.off + i];
-                        on = p >= low[j] || p < mask.sinks;
-                    }
-                    bits |= on ? 1u << r : 0u;
-                }
-            }
-        return bits;
+                for (int r = 0; r < 4; ++r)
+                    bits |= static_cast<uint32_t>(key + r - low[j]) < static_cast<uint32_t>(seen[j]) || key + r < sink[j] ? 1u << r : 0u;
+            return bits;
+        }
     };
 
     f32x4 o_acc[kBlocks][2];  // dims 16b + 4lg .. + 3 of row 16j + li
@@ -639,7 +762,7 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
             for (int n = 0; n < 4; ++n)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    s0[n][r] *= c.scale_log2;
+                    s0[n][r] = kTree ? __builtin_fmaf(s0[n][r], c.scale_log2, -m_run[n & 1]) : s0[n][r] * c.scale_log2;
                     mx[n & 1] = fmaxf(mx[n & 1], s0[n][r]);
                 }
             if (is_masked(0)) mask_logits(0, s0, mx);
@@ -674,7 +797,6 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     // rows that do not see them: V without them, and where a row sees one, an
     // infinity of its sign (or, for NaN, of both).
     auto careful_pass = [&]() {
-        reset();
         landed_and_barrier<0>();
         first_place();
         for (int t = 0; t < tiles; ++t) {
@@ -740,7 +862,112 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     };
     // Without a key there may be no page table either: nothing is asked for.
     reset();
-    if (tiles > 0 && fast_pass()) careful_pass();
+    if constexpr (kTree) {
+        // A tree's masks lie in LDS: for each of the tile's tokens a word for each masked tile of
+        // keys. Where they do not all fit (128 tokens and more than 31 masked tiles) the tiles
+        // are taken in segments.
+        const int base = u.first, token0 = token_at(0), tokens = token_at(rows - 1) - token0 + 1, fit = Tile::kMaskWords / tokens;
+        const int part0 = tile0, part_tiles = tiles;
+        // In tiles of the part: clear ones are 0 .. sinks_end - 1 and window .. window_end - 1.
+        const int sinks_end = max(clear_sink, 0), window = max(clear_from, sinks_end), window_end = max(clear_from + clear, window);
+        const bool cut = mask.low(max(p_last, 0)) > base;
+        // What p sees of the cached keys from key0 on.
+        auto cached = [&](int p, int low_of, int key0) {
+            auto below = [&](int key) {  // keys of the tile before it
+                const int n = min(max(key - key0, 0), kWindowKeys);
+                return n == kWindowKeys ? ~0u : (1u << n) - 1;
+            };
+            uint32_t bits = p < 0 ? 0u : (below(base) & ~below(low_of)) | below(min(mask.sinks, max(base, 0)));
+            return bits;
+        };
+        auto paged = [&](int key0) {
+            uint32_t bits = ~0u;
+            if (holes)
+                for (int g = 0; g < 4; ++g)
+                    if (!on_page(key0 + 8 * g)) bits &= ~(0xffu << (8 * g));
+            return bits;
+        };
+        auto each_segment = [&](auto pass) {
+            bool odd = false;
+            for (int from = 0, to = 0; from < part_tiles; from = to) {
+                // As many tiles as have `fit` masked ones.
+                int left = fit, at = max(from, sinks_end);
+                if (at < window) {
+                    const int run = min(window - at, left);
+                    left -= run;
+                    at += run;
+                }
+                if (at >= window) at = max(at, window_end) + left;
+                to = min(part_tiles, at);
+                tile0 = part0 + from;
+                tiles = to - from;
+                clear_sink = max(sinks_end - from, 0);
+                clear_from = max(window - from, clear_sink);
+                clear = max(window_end - from - clear_from, 0);
+                const int masked = max(0, min(tiles, clear_from) - clear_sink) + max(0, tiles - clear_from - clear);
+                auto tile_of = [&](int w) { return w + clear_sink + (w + clear_sink >= clear_from ? clear : 0); };
+                uint32_t* words = reinterpret_cast<uint32_t*>(smem + Tile::kMasks);
+                // The last `drafts` of the masked tiles have drafts among their keys.
+                int drafts = 0;
+                while (drafts < masked && range.key(tile0 + tile_of(masked - 1 - drafts)) + kWindowKeys > base) ++drafts;
+                int thread = tid;
+                asm volatile("" : "+v"(thread));  // nothing made of it is kept in registers beside the passes
+                for (int t = thread & (kWindowRows - 1); t < tokens; t += kWindowRows) {
+                    const int p = c.positions[u.off + token0 + t], low_of = mask.low(max(p, 0));
+                    for (int w = thread / kWindowRows; w < masked - drafts; w += kWindowThreads / kWindowRows) {
+                        const int key0 = range.key(tile0 + tile_of(w));
+                        words[t * masked + w] = cached(p, low_of, key0) & paged(key0);
+                    }
+                    if (thread >= kWindowRows || drafts == 0) continue;
+                    // Up the token's line, in words of 64 places, as the tiles of drafts go down.
+                    int i = token0 + t, depth = p - base;  // the last token of the line that has not been looked at
+                    int block = -1;
+                    uint64_t word = 0;
+                    auto half = [&](int h) {  // places 32h .. 32h + 31
+                        if (h < 0) return 0u;
+                        if (h >> 1 != block) {
+                            block = h >> 1;
+                            word = 0;
+                            while (i >= 64 * block && i >= 0) {
+                                const int place = i & ~63, up = c.above[u.off + i];
+                                uint64_t its = c.near[u.off + i];
+                                if (cut) its = within(its, depth, low_of - base, mask.sinks - base);
+                                if (place == 64 * block) word = its;
+                                i = up < place ? up : -1;
+                            }
+                        }
+                        return static_cast<uint32_t>(word >> (32 * (h & 1)));
+                    };
+                    uint32_t upper = 0;
+                    for (int w = masked - 1; w >= masked - drafts; --w) {
+                        const int key0 = range.key(tile0 + tile_of(w)), place = key0 - base;
+                        if (w == masked - 1) upper = half((place >> 5) + 1);
+                        const uint32_t lower = half(place >> 5);
+                        const uint32_t line = __builtin_amdgcn_alignbit(upper, lower, place & 31);
+                        upper = lower;
+                        words[t * masked + w] = (cached(p, low_of, key0) | (p < 0 ? 0u : line)) & paged(key0);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int row = row0 + min((thread >> 6) * 32 + 16 * j + (thread & 15), rows - 1);
+                    masks[j] = (row / group - token0) * masked;
+                }
+                odd |= pass();
+            }
+            return odd;
+        };
+        if (each_segment(fast_pass)) {
+            reset();
+            each_segment([&]() {
+                careful_pass();
+                return false;
+            });
+        }
+    } else if (tiles > 0 && fast_pass()) {
+        reset();
+        careful_pass();
+    }
 
     if (!active) return;
 #pragma unroll
@@ -755,8 +982,10 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
         int token, head;
         if (!row_of(j, token, head)) continue;
         const int64_t stat_at = u.b * c.row.batch + head * c.row.head + int64_t(u.off + token) * c.row.token;
-        if constexpr (kSplit) {
-            const int64_t at = blockIdx.y * c.rows + stat_at;
+        const int place = wave * 32 + 16 * j + li;
+        if (kTree && u.from == 0 && lg == 0) c.row_parts[stat_at] = make_int4(u.slot, u.whole ? 1 : u.parts, place, 0);
+        if (split) {
+            const int64_t at = kTree ? int64_t(u.slot) * kWindowRows + place : blockIdx.y * c.rows + stat_at;
             if (lg == 0) {
                 c.partial_stat[at] = float2{slack[j] == kSlack<T> ? m_run[j] : -INFINITY, l};
                 if (!kPaged && c.out_rest) c.partial_rounded[at] = rounded;
@@ -785,12 +1014,30 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     }
 }
 
+template <class T, int D, bool kPaged, bool kSplit>
+__global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c, WindowGrid places) {
+    touch(c.q, c.k_rows.batch, c.row.batch, c.lengths, c.rows, places.heads);
+    WindowUnit u;
+    if (window_unit<kPaged>(c, places, blockIdx.x, u)) window_rows<T, D, kPaged, kSplit, false>(c, u);
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(kWindowThreads, D == 64 ? 3 : 2) void tree_attention_kernel(WindowCall c) {
+    touch(c.q, c.k_rows.batch, c.row.batch, c.lengths, c.rows, c.near);
+    TreeWork work(c, blockIdx.x);
+    WindowUnit u;
+    while (work.next(c, u)) {
+        window_rows<T, D, true, true, true>(c, u);
+        landed_and_barrier<0>();  // every wave is done with the LDS
+    }
+}
+
 // A split row: m = max over its parts, w = 2^(m_part - m), o = sum w o_part /
 // sum w l_part. One wave per row: lane p looks at part p (of at most 64), then all
 // lanes add up the parts' rows, four loads ahead. Bound by reading the partial
 // results or, for few rows, by two loads after one another (part after part, 52 parts
-// took 50 us).
-template <class T, int D, bool kPaged>
+// took 50 us). A tree's rows say how many parts they have, and where.
+template <class T, int D, bool kPaged, bool kTree>
 __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
     const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (row >= c.rows) return;
@@ -805,11 +1052,26 @@ __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
         const int64_t bh = row / c.tokens, token = row - bh * c.tokens, b = bh / c.heads, head = bh - b * c.heads;
         out_at = b * c.out_rows.batch + head * c.out_rows.head + token * c.out_rows.token;
     }
+    int parts = c.parts;
+    int64_t first_part = row, to_next = c.rows, begin = 0;
+    if constexpr (kTree) {
+        const int4 its = c.row_parts[row];
+        parts = __builtin_amdgcn_readfirstlane(its.y);
+        // One part has been written whole; a row that offsets which do not ascend leave out may hold anything.
+        // The first part may be the last thing that its workgroup did, the others are the first.
+        if (parts < 2 || parts > kMostParts || its.x < 0 || its.z < 0 || its.z >= kWindowRows ||
+            its.x + int64_t(2) * c.kv_heads * (parts - 1) >= c.slots)
+            return;
+        first_part = int64_t(its.x & ~1) * kWindowRows + its.z;
+        to_next = int64_t(2) * c.kv_heads * kWindowRows;
+        begin = (its.x & 1) * kWindowRows;
+    }
+    auto part_at = [&](int p) { return first_part + p * to_next + (p == 0 ? begin : 0); };
     float2 stat = {-INFINITY, 0.f};
     float rounded = 0.f;
-    if (lane < c.parts) {
-        stat = c.partial_stat[lane * c.rows + row];
-        if (!kPaged && c.out_rest) rounded = c.partial_rounded[lane * c.rows + row];
+    if (lane < parts) {
+        stat = c.partial_stat[part_at(lane)];
+        if (!kPaged && c.out_rest) rounded = c.partial_rounded[part_at(lane)];
     }
     const bool some = stat.y != 0.f;  // a part without a key has written no row
     const uint64_t written = __ballot(some);
@@ -825,17 +1087,17 @@ __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
         rounded += __shfl_xor(rounded, s);
     }
     constexpr int kAhead = 4;
-    for (int p0 = 0; p0 < c.parts; p0 += kAhead) {
+    for (int p0 = 0; p0 < parts; p0 += kAhead) {
         float x[kAhead][D / 64];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const float* src = c.partial_o + (min(p0 + i, c.parts - 1) * c.rows + row) * D + lane * (D / 64);
+            const float* src = c.partial_o + part_at(min(p0 + i, parts - 1)) * D + lane * (D / 64);
 #pragma unroll
             for (int e = 0; e < D / 64; ++e) x[i][e] = src[e];
         }
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            if (p0 + i >= c.parts) break;
+            if (p0 + i >= parts) break;
             if (!(written >> (p0 + i) & 1)) continue;
             const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), p0 + i));
             // An infinite value is seen however small its part's weight is.
@@ -858,18 +1120,29 @@ __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
     if (c.lse && lane == 0) c.lse[row] = l == 0.f ? -INFINITY : m + log2f(l);
 }
 
-template <class T, int D, bool kPaged, bool kTree = false>
+template <class T, int D, bool kPaged>
 int launch_as(const WindowCall& c, hipStream_t stream) {
     const int64_t tiles = window_tiles(c), heads = kPaged ? c.kv_heads : int64_t(c.batch) * c.heads;
     const WindowGrid places = window_grid(heads, tiles);
     const dim3 grid(places.size(), static_cast<unsigned>(c.parts));
-    const auto kernel = c.parts == 1 ? window_kernel<T, D, kPaged, false, kTree> : window_kernel<T, D, kPaged, true, kTree>;
+    const auto kernel = c.parts == 1 ? window_kernel<T, D, kPaged, false> : window_kernel<T, D, kPaged, true>;
     constexpr int kLds = WindowTile<T, D>::kLdsBytes;
     if (int rc = ensure_lds_limit(reinterpret_cast<const void*>(kernel), kLds)) return rc;
     hipLaunchKernelGGL(kernel, grid, dim3(kWindowThreads), kLds, stream, c, places);
     if (int rc = check_launch("window_kernel")) return rc;
     if (c.parts == 1) return 0;
-    hipLaunchKernelGGL((window_combine_kernel<T, D, kPaged>), dim3(static_cast<unsigned>((c.rows + 3) / 4)), dim3(256), 0, stream, c);
+    hipLaunchKernelGGL((window_combine_kernel<T, D, kPaged, false>), dim3(static_cast<unsigned>((c.rows + 3) / 4)), dim3(256), 0, stream, c);
+    return check_launch("window_combine_kernel");
+}
+
+template <class T, int D>
+int launch_tree_as(const WindowCall& c, hipStream_t stream) {
+    const auto kernel = tree_attention_kernel<T, D>;
+    constexpr int kLds = WindowTile<T, D>::kTreeLdsBytes;
+    if (int rc = ensure_lds_limit(reinterpret_cast<const void*>(kernel), kLds)) return rc;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(c.groups)), dim3(kWindowThreads), kLds, stream, c);
+    if (int rc = check_launch("tree_attention_kernel")) return rc;
+    hipLaunchKernelGGL((window_combine_kernel<T, D, true, true>), dim3(static_cast<unsigned>((c.rows + 3) / 4)), dim3(256), 0, stream, c);
     return check_launch("window_combine_kernel");
 }
 }  // namespace
@@ -909,10 +1182,24 @@ int window_parts(const WindowCall& c, int64_t most_keys) {
     return best;
 }
 
+// As many workgroups as the chip takes at once (two to a CU, with D = 64 three), or as there
+// are parts; the parts themselves are TreeWork's.
+void plan_tree(WindowCall& c, int64_t most_keys) {
+    // A sequence of x rows has at most (x - 1) / 128 + 1 tiles of rows.
+    const int64_t packed = int64_t(c.tokens) * c.group.d;
+    const int64_t units = packed <= c.batch ? packed : (packed - c.batch) / kWindowRows + c.batch;
+    const int64_t steps = (most_keys + 2 * kWindowKeys - 1) / kWindowKeys + 1;
+    const int64_t groups = (c.dim == 128 ? 512 : 768) / c.kv_heads;
+    const int64_t wanted = std::max<int64_t>(1, std::min(groups, (units * steps + kTreeSteps - 1) / kTreeSteps));
+    c.share = 1.0 / double(wanted);
+    c.groups = static_cast<int32_t>(wanted * c.kv_heads);
+    c.slots = 2 * c.groups;
+}
+
 int launch_window(const WindowCall& c, hipStream_t stream) {
     auto typed = [&](auto t) {
         using T = decltype(t);
-        if (c.near) return c.dim == 128 ? launch_as<T, 128, true, true>(c, stream) : launch_as<T, 64, true, true>(c, stream);
+        if (c.near) return c.dim == 128 ? launch_tree_as<T, 128>(c, stream) : launch_tree_as<T, 64>(c, stream);
         if (c.dim == 128) return c.paged ? launch_as<T, 128, true>(c, stream) : launch_as<T, 128, false>(c, stream);
         return c.paged ? launch_as<T, 64, true>(c, stream) : launch_as<T, 64, false>(c, stream);
     };

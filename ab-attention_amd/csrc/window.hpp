@@ -168,6 +168,11 @@ struct WindowCall {
     float2* partial_stat;                    // [parts][rows]: reference and sum
     float* partial_rounded;                  // [parts][rows], for a tensor's out_rest: sum of the rounded weights
     int64_t rows;                            // queries times heads
+    // Of a tree, whose parts are chosen by the kernel: workgroups, one by the number of
+    // those of a head, and places for parts' rows, [slots][kWindowRows].
+    int32_t groups, slots;
+    double share;
+    int4* row_parts;                         // [rows]: first place, parts, row in the place
 };
 
 // One call of the backward pass over strided tensors. `stat` holds, for every
@@ -193,6 +198,8 @@ struct WindowGradCall {
 
 constexpr int kWindowThreads = 256;
 constexpr int kWindowRows = 128;  // query rows of a workgroup
+constexpr int kTreeSteps = 4;     // tiles of keys of a part of a tree's, at least
+constexpr int kMostParts = 64;    // of a tile of rows
 constexpr int kWindowKeys = 32;   // keys of a tile
 
 // Keys of a run of tiles: the first `sink_tiles` tiles start at 0, the others at
@@ -253,6 +260,8 @@ inline WindowGrid window_grid(int64_t heads, int64_t tiles) { return {static_cas
 int launch_window(const WindowCall& call, hipStream_t stream);
 int window_parts(const WindowCall& call, int64_t most_keys);
 int64_t window_tiles(const WindowCall& call);
+// Sets groups, share and slots of a tree's call; most_keys as above.
+void plan_tree(WindowCall& call, int64_t most_keys);
 int launch_window_grad(const WindowGradCall& call, hipStream_t stream);
 // Sets the tiles and parts of a split; returns the floats of stat and of partial.
 void plan_window_grad(WindowGradCall& call, int64_t& stat, int64_t& partial);

@@ -45,22 +45,18 @@ def tree_tensors(tree, base):
 def tree_mask(tree, base, length, window, sinks, frame):
     """bool [n, length]: what every new token sees of the cache's places (those below 0 do not exist)."""
     n = len(tree)
-    of_line = lines(tree)
-    slot_position = torch.arange(length)
-    for j in range(n):
-        if base + j >= 0:
-            slot_position[base + j] = base + len(of_line[j]) - 1
-    mask = torch.zeros((n, length), dtype=torch.bool)
-    for i, line in enumerate(of_line):
-        p = base + len(line) - 1
-        if p < 0:
-            continue
-        mask[i, :max(base, 0)] = True
-        for j in line:
-            if base + j >= 0:
-                mask[i, base + j] = True
-        if window is not None:
-            mask[i] &= (p // frame - slot_position // frame < window) | (slot_position // frame < sinks)
+    of_line = torch.zeros((n, n), dtype=torch.bool)
+    for i, parent in enumerate(tree):
+        if 0 <= parent < i:
+            of_line[i] = of_line[parent]
+        of_line[i, i] = True
+    position = base + of_line.sum(1) - 1
+    there = max(0, -base)  # the first new token that has a place
+    key_position = torch.cat([torch.arange(max(base, 0)), position[there:]])
+    mask = torch.cat([torch.ones((n, max(base, 0)), dtype=torch.bool), of_line[:, there:]], 1) & (position >= 0)[:, None]
+    if window is not None:
+        p, t = position[:, None] // frame, key_position[None] // frame
+        mask &= (p - t < window) | (t < sinks)
     return mask
 
 
