@@ -151,7 +151,7 @@ void plan_tree_call(const ab_window_args& a, WindowCall& c) {
 }
 
 size_t tree_workspace_bytes(const WindowCall& c) {
-    return size_t(c.rows) * sizeof(int4) + size_t(c.slots) * kWindowRows * (size_t(c.dim) * sizeof(float) + sizeof(float2));
+    return size_t(c.rows) * sizeof(int4) + size_t(c.slots) * c.tile_rows * (size_t(c.dim) * sizeof(float) + sizeof(float2));
 }
 
 int window_launch(const char* what, const ab_window_args* a, bool paged, void* stream, const ab_tree_args* tree = nullptr) {
@@ -180,7 +180,7 @@ int window_launch(const char* what, const ab_window_args* a, bool paged, void* s
         if (!aligned(a->workspace, 16)) return set_error(AB_ERR_INVALID, "%s: workspace must be 16-byte aligned", what);
         c.row_parts = static_cast<int4*>(a->workspace);
         c.partial_o = reinterpret_cast<float*>(c.row_parts + c.rows);
-        c.partial_stat = reinterpret_cast<float2*>(c.partial_o + int64_t(c.slots) * kWindowRows * c.dim);
+        c.partial_stat = reinterpret_cast<float2*>(c.partial_o + int64_t(c.slots) * c.tile_rows * c.dim);
     } else if (!tree && c.parts > 1) {
         if (a->workspace_bytes < workspace_bytes(c))
             return set_error(AB_ERR_INVALID, "%s: workspace of %zu bytes is smaller than the %zu required", what,

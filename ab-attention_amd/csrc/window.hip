@@ -62,10 +62,9 @@ struct WindowUnit {
     int off;               // their first row in the packed tensor (0 without offsets)
     int first;             // position of its first new token
     int length;            // keys of it
-    // Of a tree: which of the tile's steps these are, whether that is all of them, and else
-    // where the rows' sums go, and, of the first part, how many parts there are.
-    int from, to, slot, parts;
-    bool whole;
+    // Of a tree: which part of how many of the tile's keys, where its rows go if there are
+    // several, and how far the next part's place is.
+    int part, parts, slot, stride;
 };
 
 template <bool kPaged>
@@ -145,22 +144,22 @@ __device__ __forceinline__ int lane_moved(int x) {
     return __builtin_amdgcn_update_dpp(0, x, kControl, 15, 15, true);
 }
 template <int kControl>
-__device__ __forceinline__ double lane_moved(double x) {
-    const int2 halves = __builtin_bit_cast(int2, x);
-    return __builtin_bit_cast(double, int2{lane_moved<kControl>(halves.x), lane_moved<kControl>(halves.y)});
+__device__ __forceinline__ float lane_moved(float x) {
+    return __builtin_bit_cast(float, lane_moved<kControl>(__builtin_bit_cast(int, x)));
 }
-__device__ __forceinline__ double lane_value(double x, int lane) {
-    const int2 halves = __builtin_bit_cast(int2, x);
-    return __builtin_bit_cast(double, int2{__builtin_amdgcn_readlane(halves.x, lane), __builtin_amdgcn_readlane(halves.y, lane)});
+template <class N>
+__device__ __forceinline__ N lane_value(N x, int lane) {
+    return __builtin_bit_cast(N, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
 }
 // x and those of the lanes before.
-__device__ __forceinline__ double running_sum(double x, int lane) {
+template <class N>
+__device__ __forceinline__ N running_sum(N x, int lane) {
     x += lane_moved<0x111>(x);  // row_shr 1, 2, 4, 8
     x += lane_moved<0x112>(x);
     x += lane_moved<0x114>(x);
     x += lane_moved<0x118>(x);
-    const double one = lane_value(x, 15), two = one + lane_value(x, 31), three = two + lane_value(x, 47);
-    return x + (lane < 16 ? 0.0 : lane < 32 ? one : lane < 48 ? two : three);
+    const N one = lane_value(x, 15), two = one + lane_value(x, 31), three = two + lane_value(x, 47);
+    return x + (lane < 16 ? N(0) : lane < 32 ? one : lane < 48 ? two : three);
 }
 __device__ __forceinline__ int most_of_lanes(int x) {  // of numbers that are not negative
     x = max(x, lane_moved<0x111>(x));
@@ -171,92 +170,108 @@ __device__ __forceinline__ int most_of_lanes(int x) {  // of numbers that are no
                max(__builtin_amdgcn_readlane(x, 47), __builtin_amdgcn_readlane(x, 63)));
 }
 
-// A tree's work, which its workgroups deal out among themselves: how many sequences there
-// are, and how long they are, is on the device. For a head all steps (tiles of keys) of all
-// tiles of rows of all sequences stand in a row, sequence by sequence, and workgroup w of the
-// head's c.wanted takes the `each` steps from w each on, at least kTreeSteps: all do the
-// same, whatever the lengths. What it has is the end of one tile of rows, perhaps some
-// whole ones, and the beginning of another. Counts are whole numbers in 64-bit floats.
-struct TreeWork {
-    double at, end;  // this workgroup's steps that are left
-    double each;
-    int w, kv_head;
-    bool first;      // none has been done
+// A kernel's first argument, read anew where it is asked for: else the compiler reads all of
+// it at the start and keeps it in lanes of vector registers, two instructions for every use.
+__device__ __forceinline__ const WindowCall& arguments() {
+    auto at = (const __attribute__((address_space(4))) WindowCall*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    return *(const WindowCall*)at;
+}
 
+// A tree's workgroup: of which sequence, tile of rows, K/V head and part of the keys.
+//
+// How many sequences there are, and how long they are, is on the device, so the kernel
+// itself deals out the work. With `steps` tiles of keys for each of the `tiles` of rows of
+// a sequence, all are cut into parts of at most C steps; lane k looks at C = longest / (k + 1),
+// and the C that costs least is taken: a workgroup's C steps and its filling, in rounds
+// where there are more workgroups than run at once, or what reading all keys takes, if that
+// is more; parts cost a second kernel and the traffic of their sums. (To give every workgroup the same number of steps, of two
+// tiles of rows if need be, costs more than it saves: 8 sequences of 4,026 keys 50 us, in
+// whole parts XX.) The longest sequences come first; within one part, tile of rows, head:
+// with eight heads (or 16, ..) the tiles of rows that share keys are on one XCD.
+template <int kRows>
+__device__ __forceinline__ bool tree_unit(const WindowCall& c, int id, WindowUnit& u) {
+    const int lane = threadIdx.x & 63, group = static_cast<int>(c.group.d), heads = c.kv_heads;
     struct Sequence {
         int off, n, length, tiles, steps;
     };
-    static __device__ __forceinline__ Sequence look_at(const WindowCall& c, int b) {
+    auto look_at = [&](int b) {
         Sequence s;
         const bool there = b < c.batch;
         b = min(b, c.batch - 1);
         s.off = min(max(c.offsets[b], 0), c.tokens);
         s.n = there ? min(max(c.offsets[b + 1], 0), c.tokens) - s.off : 0;
         s.length = static_cast<int>(min(int64_t(max(c.lengths[b], 0)), int64_t(c.table_width) * c.page.d));
-        s.tiles = s.n > 0 ? static_cast<int>((int64_t(s.n) * c.group.d + kWindowRows - 1) / kWindowRows) : 0;
+        s.tiles = s.n > 0 ? (s.n * group + kRows - 1) / kRows : 0;
         TileRange range;
         range.set(c.mask, max(s.length - s.n, 0), s.length - 1, s.length);
-        s.steps = max(range.tiles, 1);  // rows that see nothing are written too
+        s.steps = s.tiles > 0 ? max(range.tiles, 1) : 0;  // rows that see nothing are written too
         return s;
+    };
+    Sequence s = look_at(lane);
+    float work = static_cast<float>(s.tiles) * static_cast<float>(s.steps);
+    int units = s.tiles, longest = s.steps;
+    for (int b = 64; b < c.batch; b += 64) {
+        const Sequence more = look_at(b + lane);
+        work += static_cast<float>(more.tiles) * static_cast<float>(more.steps);
+        units += more.tiles;
+        longest = max(longest, more.steps);
     }
-
-    __device__ __forceinline__ TreeWork(const WindowCall& c, int id) : first(true) {
-        const int lane = threadIdx.x & 63;
-        double steps = 0.0;
-        int longest = 0;
-        for (int b = 0; b < c.batch; b += 64) {
-            const Sequence s = look_at(c, b + lane);
-            steps += static_cast<double>(s.tiles) * s.steps;
-            longest = max(longest, s.tiles > 0 ? s.steps : 0);
+    longest = most_of_lanes(longest);
+    if (longest == 0) return false;
+    work = lane_value(running_sum(work, lane), 63);
+    units = lane_value(running_sum(units, lane), 63);
+    int each;
+    {
+        const float k = lane + 1.f, steps = fmaxf(ceilf(longest / k), 1.f), whole = static_cast<float>(units * heads);
+        // Workgroups, and the most there can be.
+        const float cut = work * heads / steps, most = cut + whole, groups = c.batch == 1 ? whole * ceilf(longest / steps) : cut + 0.5f * whole;
+        float cost = fmaxf(fmaxf(1.f, (lane == 0 ? whole : groups) * c.share) * (steps * c.step_cost + kFilling), work * heads * c.read_cost);
+        if (lane > 0) cost += kJoining + groups * c.sums_cost;
+        if (lane > 0 && (steps < kTreeSteps || most > c.slots)) cost = INFINITY;
+        // The lane of the least cost; costs are positive, so their bits are in their order.
+        const int least = 0x7f800000 - most_of_lanes(0x7f800000 - __builtin_bit_cast(int, cost));
+        const int best = __builtin_ctzll(__ballot(__builtin_bit_cast(int, cost) == least) | (uint64_t(1) << 63));
+        each = __builtin_amdgcn_readlane(static_cast<int>(steps), best);
+        if (best == 0) each = longest;
+    }
+    auto parts_of = [&](int steps) { return (steps + each - 1) / each; };
+    const int mine = id / heads;
+    u.kv_head = __builtin_amdgcn_readfirstlane(id - mine * heads);
+    int before = 0;
+    for (int b = 0; b < c.batch; b += 64) {
+        if (b > 0) s = look_at(b + lane);
+        const int parts = parts_of(s.steps), all = s.tiles * parts;
+        int start = before + running_sum(all, lane) - all;
+        if (c.batch <= 64) {
+            start = 0;
+            for (int j = 0; j < c.batch; ++j) {
+                const int other = __builtin_amdgcn_readlane(s.steps, j), its = __builtin_amdgcn_readlane(all, j);
+                start += other > s.steps || (other == s.steps && j < lane) ? its : 0;
+            }
         }
-        const double all = lane_value(running_sum(steps, lane), 63);
-        // A tile of rows has at most kMostParts parts, the two at its ends among them.
-        const int least = max(kTreeSteps, most_of_lanes(longest) / (kMostParts - 2) + 1);
-        each = lane_value(fmax(floor(all * c.share) + 1.0, static_cast<double>(least)), 0);
-        w = id / c.kv_heads;
-        kv_head = __builtin_amdgcn_readfirstlane(id - w * c.kv_heads);
-        w = __builtin_amdgcn_readfirstlane(w);
-        at = lane_value(each * w, 0);
-        end = lane_value(fmin(at + each, all), 0);
-    }
-
-    // The next tile of rows and its steps; false if there is none.
-    __device__ __forceinline__ bool next(const WindowCall& c, WindowUnit& u) {
-        if (!(__builtin_amdgcn_readfirstlane(at < end))) return false;
-        int lane = threadIdx.x & 63;
-        asm volatile("" : "+v"(lane));
-        double before = 0.0;
-        for (int b = 0; b < c.batch; b += 64) {
-            const Sequence s = look_at(c, b + lane);
-            const double its = static_cast<double>(s.tiles) * s.steps, until = before + running_sum(its, lane);
-            const uint64_t here = __ballot(until > at && until - its <= at);
-            before = lane_value(until, 63);
-            if (here == 0) continue;
-            const int l = __builtin_ctzll(here);
-            auto uniform = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
-            u.b = b + l;
-            u.off = uniform(s.off);
-            u.n = uniform(s.n);
-            u.length = uniform(s.length);
+        const uint64_t here = __ballot(mine >= start && mine < start + all);
+        if (here) {
+            const int at = __builtin_ctzll(here);
+            auto its = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+            u.b = b + at;
+            u.off = its(s.off);
+            u.n = its(s.n);
+            u.length = its(s.length);
+            u.parts = its(parts);
+            const int tiles = its(s.tiles), place = mine - its(start);
+            u.part = __builtin_amdgcn_readfirstlane(place / tiles);
+            u.tile = __builtin_amdgcn_readfirstlane(place - u.part * tiles);
+            u.stride = tiles * heads;
+            u.slot = __builtin_amdgcn_readfirstlane(id);
+            u.head = u.kv_head * group;
             u.first = u.length - u.n;
-            u.kv_head = kv_head;
-            u.head = kv_head * static_cast<int>(c.group.d);
-            const int steps = uniform(s.steps);
-            const double start = lane_value(until - its, l), tile = floor((at - start + 0.5) / steps), here_from = at - start - tile * steps;
-            const double until_here = fmin(static_cast<double>(steps), here_from + (end - at));
-            u.tile = __builtin_amdgcn_readfirstlane(static_cast<int>(tile));
-            u.from = __builtin_amdgcn_readfirstlane(static_cast<int>(here_from));
-            u.to = __builtin_amdgcn_readfirstlane(static_cast<int>(until_here));
-            u.whole = u.from == 0 && u.to == steps;
-            u.slot = 2 * (w * c.kv_heads + kv_head) + (first ? 0 : 1);
-            u.parts = __builtin_amdgcn_readfirstlane(static_cast<int>(floor((start + (tile + 1) * steps - 0.5) / each))) - w + 1;
-            first = false;
-            at = lane_value(at + until_here - here_from, 0);
             return true;
         }
-        return false;
+        before = __builtin_amdgcn_readlane(start + all, 63);
     }
-};
+    return false;
+}
 
 template <class T, int D>
 struct WindowTile {
@@ -269,10 +284,13 @@ struct WindowTile {
     static constexpr int kVRing = kRing * kBytes;
     static constexpr int kVotes = 2 * kRing * kBytes;
     static constexpr int kLdsBytes = kVotes + 16;
-    static constexpr int kMasks = kLdsBytes;  // a tree's masks, behind the others
-    static constexpr int kMaskWords = 3968;   // two workgroups fit a CU
-    static constexpr int kTreeLdsBytes = kMasks + 4 * kMaskWords;
+    static constexpr int kMasks = kVotes + 32;  // a tree's masks, behind the others
 };
+
+// Words of a tree's masks: what fits two workgroups of four waves to a CU, or one of eight.
+template <int kWaves>
+constexpr int kMaskWords = kWaves == 4 ? 3968 : 16384;
+
 
 // What `rounded` lacks of two values, rounded itself (nothing of values that are not
 // finite).
@@ -316,22 +334,27 @@ __device__ __forceinline__ void max_over_rows(float& a, float& b) {
 
 extern __shared__ __align__(16) unsigned char smem[];
 
-template <class T, int D, bool kPaged, bool kSplit, bool kTree>
+template <class T, int D, bool kPaged, bool kSplit, bool kTree, int kWaves = 4>
 __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUnit& u) {
     using Tile = WindowTile<T, D>;
     constexpr int kSteps = Tile::kSteps, kBlocks = Tile::kBlocks, kOps = Tile::kOps;
-    const bool split = kSplit && (!kTree || !u.whole);
+    constexpr int kRows = 32 * kWaves, kThreads = 64 * kWaves;
+    // Of eight waves four transfer K and four V.
+    constexpr bool kApart = kWaves == 8;
+    static_assert(kWaves == 4 || (kApart && kTree));
+    const bool split = kSplit && (!kTree || u.parts > 1);
     const int group = kPaged ? c.group.d : 1;
     int tid = threadIdx.x;
     if constexpr (kTree) asm volatile("" : "+v"(tid));  // made anew for every tile of rows, not kept beside the passes
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4;
+    const int loader = kApart ? wave & 3 : wave;  // transfers keys 8 loader .. + 7 of a tile
 
     // Bounds of the rows r0 .. r1 of the tile that exist: keys that some row
     // sees, and those that every row sees.
     const WindowMask mask = c.mask;
-    const int row0 = u.tile * kWindowRows, rows = min(kWindowRows, u.n * group - row0);
+    const int row0 = u.tile * kRows, rows = min(kRows, u.n * group - row0);
     auto token_at = [&](int r) { return kPaged ? (row0 + r) / group : row0 + r; };
     // A tree's tokens are at positions from u.first on, and see nothing in the cache behind their own place.
     const int p_first = max(u.first + (kTree ? 0 : token_at(0)), 0), p_last = min(u.first + token_at(rows - 1), u.length - 1);
@@ -339,13 +362,10 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
     range.set(mask, p_first, p_last, u.length);
     const int end = range.end;
     int tile0 = 0, tiles = range.tiles;
-    if constexpr (kTree) {
-        tile0 = min(u.from, tiles);
-        tiles = min(u.to, tiles) - tile0;
-    } else if constexpr (kSplit) {
-        const int part = blockIdx.y;
-        tile0 = static_cast<int>(int64_t(tiles) * part / c.parts);
-        tiles = static_cast<int>(int64_t(tiles) * (part + 1) / c.parts) - tile0;
+    if constexpr (kSplit) {
+        const int part = kTree ? u.part : blockIdx.y, parts = kTree ? u.parts : c.parts;
+        tile0 = static_cast<int>(int64_t(tiles) * part / parts);
+        tiles = static_cast<int>(int64_t(tiles) * (part + 1) / parts) - tile0;
     }
     // Row 16j + li of this wave's 32: its token and query head.
     auto row_of = [&](int j, int& token, int& head) {
@@ -407,15 +427,30 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
     const int32_t* table = kPaged ? c.table + int64_t(u.b) * c.table_width : nullptr;
     const int last_entry = c.table_width - 1;
 
+    // What a tree's masks are made of is asked for beside the page table, and read again later.
+    int token_position = 0, token_above = 0;
+    uint64_t token_near = 0;
+    if constexpr (kTree) {
+        const int token = u.off + token_at(min(tid & (kRows - 1), rows - 1));
+        token_position = c.positions[token];
+        token_above = c.above[token];
+        token_near = c.near[token];
+    }
+
     // Whether a key that some row would see lies on no page (then every tile
     // asks the table for its keys). Pages between the sinks and the window, which
     // may have been given back, do not count.
     bool holes = false;
+    auto any_vote = [&](const uint32_t* votes) {
+        u32x4 all = *reinterpret_cast<const u32x4*>(votes);
+        if constexpr (kWaves == 8) all |= *reinterpret_cast<const u32x4*>(votes + 4);
+        return __builtin_amdgcn_readfirstlane(all[0] | all[1] | all[2] | all[3]) != 0;
+    };
     if constexpr (kPaged) {
         bool bad = false;
         auto scan = [&](int from, int to) {
             const int page = static_cast<int>(c.page.d);
-            for (int i = from / page + tid; from < to && i <= (to - 1) / page; i += kWindowThreads)
+            for (int i = from / page + tid; from < to && i <= (to - 1) / page; i += kThreads)
                 bad |= static_cast<uint32_t>(table[i]) >= static_cast<uint32_t>(c.pages);
         };
         if (tiles > 0) {
@@ -432,9 +467,9 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
         const uint32_t vote = __any(bad) ? 1u : 0u;
         if (lane == 0) votes[wave] = vote;
         landed_and_barrier<0>();
-        const u32x4 all = *reinterpret_cast<const u32x4*>(votes);
-        holes = __builtin_amdgcn_readfirstlane(all[0] | all[1] | all[2] | all[3]) != 0;
+        holes = any_vote(votes);
     }
+    if constexpr (kTree) asm volatile("" ::"v"(token_position), "v"(token_above), "v"(token_near));
     auto on_page = [&](int key) {
         const uint32_t q0 = __umulhi(static_cast<uint32_t>(key), c.page.m);
         const uint32_t index = q0 + (static_cast<uint32_t>(key) - q0 * c.page.d >= c.page.d ? 1u : 0u);
@@ -450,7 +485,7 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
 #pragma unroll
     for (int e = 0; e < kOps; ++e) {
         constexpr int kChunks = D / 8;
-        const int key = lane / kChunks, pos = lane % kChunks, in_tile = 8 * wave + Tile::kOpKeys * e + key;
+        const int key = lane / kChunks, pos = lane % kChunks, in_tile = 8 * loader + Tile::kOpKeys * e + key;
         k_src[e] = uint32_t(Tile::kOpKeys * e + key) * k_token + uint32_t(pos ^ (in_tile % kChunks)) * 16u;
         const int quad = D == 128 ? e : lane >> 5, block = (lane >> 3) % kBlocks, r = (lane >> 1) & 3, h = lane & 1;
         v_src[e] = uint32_t(4 * quad + r) * v_token + uint32_t(2 * (block ^ (quad & 1)) + h) * 16u;
@@ -469,7 +504,7 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
     uint32_t next_at = 0;
     auto ask = [&]() {
         if constexpr (kPaged) {
-            const uint32_t key = next_key + 8 * wave;
+            const uint32_t key = next_key + 8 * loader;
             const uint32_t near = __umulhi(key, c.page.m), rest = key - near * c.page.d;
             const uint32_t index = rest >= c.page.d ? near + 1 : near;
             next_at = rest >= c.page.d ? rest - c.page.d : rest;
@@ -482,7 +517,7 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
         next_key = range.key(tile0);
     };
     auto next_place = [&]() {
-        const int key = next_key + 8 * wave;
+        const int key = next_key + 8 * loader;
         const bool there = next_tile < tiles;
         Place p{0, static_cast<uint32_t>(key), there ? static_cast<uint32_t>(end) : 0u};
         if constexpr (kPaged) {
@@ -510,14 +545,16 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
                                        p.there == 0 ? 0 : kPaged ? p.there * token - less : all);
         const uint32_t at = p.at * token;
         if constexpr (kOps == 2)
-            buffer_to_lds(buffer, src[0] + at, src[1] + at, lds + wave * (8 * D * 2));
+            buffer_to_lds(buffer, src[0] + at, src[1] + at, lds + loader * (8 * D * 2));
         else
-            buffer_to_lds(buffer, src[0] + at, lds + wave * (8 * D * 2));
+            buffer_to_lds(buffer, src[0] + at, lds + loader * (8 * D * 2));
     };
     auto move_k = [&](int t, const Place& p) {
+        if (kApart && wave >= 4) return;
         move(kbase, c.k_rows, k_token, k_less, k_all, k_src, p, lds0 + (t & (kRing - 1)) * Tile::kBytes);
     };
     auto move_v = [&](int t, const Place& p) {
+        if (kApart && wave < 4) return;
         move(vbase, c.v_rows, v_token, v_less, v_all, v_src, p, lds0 + Tile::kVRing + (t & (kRing - 1)) * Tile::kBytes);
     };
 
@@ -640,6 +677,7 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
     // adds V(t)^T P(t)^T beside the logits of tile t + 1 and the reads of K(t + 2).
     // Returns whether a tile that some rows see in part held a value that is not
     // finite: 0 times it is no zero, so the tile cannot be computed like that.
+    bool first_pass = true;
     auto fast_pass = [&]() -> bool {
         uint32_t odd = 0;
         // Places of K(t + 5), of tile t + 4 and of V(t + 3) before step t.
@@ -650,7 +688,7 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
             kp = next_place();
         };
         auto step = [&](int t, f32x4 (&sc)[4], f32x4 (&sn)[4], float (&mx)[2], u32x4 (&ka)[2 * kSteps]) {
-            landed_and_barrier<4 * kOps>();
+            landed_and_barrier<(kApart ? 2 : 4) * kOps>();
             ask();
             if (!active) {
                 move_k(t + 5, kp);
@@ -735,8 +773,29 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
         // transfers before step 0 are then K(3), V(1), V(2), K(4), as its wait expects.
         {
             first_place();
-            const Place p0 = ask_place(), p1 = ask_place(), p2 = ask_place();
-            vp = ask_place();
+            Place p0, p1, p2;
+            if constexpr (kTree) {
+                // The page table's entries of six tiles at once, a lane each.
+                const uint32_t key = range.key(tile0 + min(lane, 5)) + 8 * loader, near = __umulhi(key, c.page.m), rest = key - near * c.page.d;
+                const bool more = rest >= c.page.d;
+                const int entry = table[min(more ? near + 1 : near, static_cast<uint32_t>(last_entry))], at = more ? rest - c.page.d : rest;
+                auto place = [&](int t) {
+                    next_entry = __builtin_amdgcn_readlane(entry, t);
+                    next_at = __builtin_amdgcn_readlane(at, t);
+                    return next_place();
+                };
+                p0 = place(0);
+                p1 = place(1);
+                p2 = place(2);
+                vp = place(3);
+                mp = place(4);
+                kp = place(5);
+            } else {
+                p0 = ask_place();
+                p1 = ask_place();
+                p2 = ask_place();
+                vp = ask_place();
+            }
             move_k(0, p0);
             move_k(1, p1);
             move_k(2, p2);
@@ -745,13 +804,17 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
             move_v(1, p1);
             move_v(2, p2);
         }
-        if (active) read_q();  // behind the transfers, not before them
-        mp = ask_place();
-        kp = ask_place();
+        if (!kTree || first_pass) {
+            if (active) read_q();  // behind the transfers, not before them
+        }
+        if constexpr (!kTree) {
+            mp = ask_place();
+            kp = ask_place();
+        }
         f32x4 s0[4], s1[4];
         u32x4 ka[2 * kSteps];
         float mx[2] = {-INFINITY, -INFINITY};
-        landed_and_barrier<5 * kOps>();
+        landed_and_barrier<(kApart ? 2 : 5) * kOps>();
         if (active) {
 #pragma unroll
             for (int f = 0; f < 2 * kSteps; ++f) ka[f] = read_k(0, f);
@@ -789,8 +852,7 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
         landed_and_barrier<0>();
         if (lane == 0) votes[wave] = vote;
         landed_and_barrier<0>();
-        const u32x4 all = *reinterpret_cast<const u32x4*>(votes);
-        return __builtin_amdgcn_readfirstlane(all[0] | all[1] | all[2] | all[3]) != 0;
+        return any_vote(votes);
     };
 
     // The same sums, tile by tile, with values that are not finite kept from the
@@ -864,9 +926,9 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
     reset();
     if constexpr (kTree) {
         // A tree's masks lie in LDS: for each of the tile's tokens a word for each masked tile of
-        // keys. Where they do not all fit (128 tokens and more than 31 masked tiles) the tiles
+        // keys. Where they do not all fit (256 tokens and more than 64 masked tiles) the tiles
         // are taken in segments.
-        const int base = u.first, token0 = token_at(0), tokens = token_at(rows - 1) - token0 + 1, fit = Tile::kMaskWords / tokens;
+        const int base = u.first, token0 = token_at(0), tokens = token_at(rows - 1) - token0 + 1, fit = kMaskWords<kWaves> / tokens;
         const int part0 = tile0, part_tiles = tiles;
         // In tiles of the part: clear ones are 0 .. sinks_end - 1 and window .. window_end - 1.
         const int sinks_end = max(clear_sink, 0), window = max(clear_from, sinks_end), window_end = max(clear_from + clear, window);
@@ -912,16 +974,19 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
                 while (drafts < masked && range.key(tile0 + tile_of(masked - 1 - drafts)) + kWindowKeys > base) ++drafts;
                 int thread = tid;
                 asm volatile("" : "+v"(thread));  // nothing made of it is kept in registers beside the passes
-                for (int t = thread & (kWindowRows - 1); t < tokens; t += kWindowRows) {
-                    const int p = c.positions[u.off + token0 + t], low_of = mask.low(max(p, 0));
-                    for (int w = thread / kWindowRows; w < masked - drafts; w += kWindowThreads / kWindowRows) {
+                for (int t = thread & (kRows - 1); t < tokens; t += kRows) {
+                    int i = token0 + t;  // the last token of its line that has not been looked at
+                    const int p = c.positions[u.off + i];
+                    int up = c.above[u.off + i];
+                    uint64_t its = c.near[u.off + i];
+                    const int low_of = mask.low(max(p, 0));
+                    for (int w = thread / kRows; w < masked - drafts; w += kThreads / kRows) {
                         const int key0 = range.key(tile0 + tile_of(w));
                         words[t * masked + w] = cached(p, low_of, key0) & paged(key0);
                     }
-                    if (thread >= kWindowRows || drafts == 0) continue;
+                    if (thread >= kRows || drafts == 0) continue;
                     // Up the token's line, in words of 64 places, as the tiles of drafts go down.
-                    int i = token0 + t, depth = p - base;  // the last token of the line that has not been looked at
-                    int block = -1;
+                    int depth = p - base, block = -1;
                     uint64_t word = 0;
                     auto half = [&](int h) {  // places 32h .. 32h + 31
                         if (h < 0) return 0u;
@@ -929,11 +994,14 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
                             block = h >> 1;
                             word = 0;
                             while (i >= 64 * block && i >= 0) {
-                                const int place = i & ~63, up = c.above[u.off + i];
-                                uint64_t its = c.near[u.off + i];
+                                const int place = i & ~63;
                                 if (cut) its = within(its, depth, low_of - base, mask.sinks - base);
                                 if (place == 64 * block) word = its;
                                 i = up < place ? up : -1;
+                                if (i >= 0) {
+                                    its = c.near[u.off + i];
+                                    up = c.above[u.off + i];
+                                }
                             }
                         }
                         return static_cast<uint32_t>(word >> (32 * (h & 1)));
@@ -954,6 +1022,7 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
                     masks[j] = (row / group - token0) * masked;
                 }
                 odd |= pass();
+                first_pass = false;
             }
             return odd;
         };
@@ -970,6 +1039,7 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
     }
 
     if (!active) return;
+    const WindowCall& e = kTree ? arguments() : c;  // the rest of the call
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         auto over_rows = [](float x) {  // the sum over the four lanes of a row
@@ -981,35 +1051,35 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
         const float l = over_rows(l_run[j]), rounded = over_rows(r_run[j]);
         int token, head;
         if (!row_of(j, token, head)) continue;
-        const int64_t stat_at = u.b * c.row.batch + head * c.row.head + int64_t(u.off + token) * c.row.token;
+        const int64_t stat_at = u.b * e.row.batch + head * e.row.head + int64_t(u.off + token) * e.row.token;
         const int place = wave * 32 + 16 * j + li;
-        if (kTree && u.from == 0 && lg == 0) c.row_parts[stat_at] = make_int4(u.slot, u.whole ? 1 : u.parts, place, 0);
+        if (kTree && u.part == 0 && lg == 0) e.row_parts[stat_at] = make_int4(u.slot, u.parts, place, u.stride);
         if (split) {
-            const int64_t at = kTree ? int64_t(u.slot) * kWindowRows + place : blockIdx.y * c.rows + stat_at;
+            const int64_t at = kTree ? int64_t(u.slot) * kRows + place : blockIdx.y * e.rows + stat_at;
             if (lg == 0) {
-                c.partial_stat[at] = float2{slack[j] == kSlack<T> ? m_run[j] : -INFINITY, l};
-                if (!kPaged && c.out_rest) c.partial_rounded[at] = rounded;
+                e.partial_stat[at] = float2{slack[j] == kSlack<T> ? m_run[j] : -INFINITY, l};
+                if (!kPaged && e.out_rest) e.partial_rounded[at] = rounded;
             }
             if (l == 0.f) continue;
-            float* dst = c.partial_o + at * D + 4 * lg;
+            float* dst = e.partial_o + at * D + 4 * lg;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) *reinterpret_cast<f32x4*>(dst + 16 * b) = o_acc[b][j];
         } else {
             const float inv = l == 0.f ? 0.f : 1.0f / l, better = kPaged || rounded == 0.f ? inv : 1.0f / rounded;
-            uint16_t* orow = static_cast<uint16_t*>(c.out) + u.b * c.out_rows.batch + head * c.out_rows.head +
-                             int64_t(u.off + token) * c.out_rows.token + 4 * lg;
+            uint16_t* orow = static_cast<uint16_t*>(e.out) + u.b * e.out_rows.batch + head * e.out_rows.head +
+                             int64_t(u.off + token) * e.out_rows.token + 4 * lg;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
                 const f32x4 o = o_acc[b][j] * inv;
                 const u32x2 w = {T::pack(o[0], o[1]), T::pack(o[2], o[3])};
                 *reinterpret_cast<u32x2*>(orow + 16 * b) = w;
-                if (c.out_rest) {
+                if (e.out_rest) {
                     const f32x4 before = o_acc[b][j] * better;
-                    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(c.out_rest) + (orow - static_cast<uint16_t*>(c.out)) + 16 * b) =
+                    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(e.out_rest) + (orow - static_cast<uint16_t*>(e.out)) + 16 * b) =
                         u32x2{rest_of<T>(before[0], before[1], w[0]), rest_of<T>(before[2], before[3], w[1])};
                 }
             }
-            if (c.lse && lg == 0) c.lse[stat_at] = l == 0.f ? -INFINITY : m_run[j] + log2f(l);
+            if (e.lse && lg == 0) e.lse[stat_at] = l == 0.f ? -INFINITY : m_run[j] + log2f(l);
         }
     }
 }
@@ -1021,23 +1091,19 @@ __global__ __launch_bounds__(kWindowThreads, 2) void window_kernel(WindowCall c,
     if (window_unit<kPaged>(c, places, blockIdx.x, u)) window_rows<T, D, kPaged, kSplit, false>(c, u);
 }
 
-template <class T, int D>
-__global__ __launch_bounds__(kWindowThreads, D == 64 ? 3 : 2) void tree_attention_kernel(WindowCall c) {
+template <class T, int D, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, D == 64 && kWaves == 4 ? 3 : 2) void tree_attention_kernel(WindowCall c) {
     touch(c.q, c.k_rows.batch, c.row.batch, c.lengths, c.rows, c.near);
-    TreeWork work(c, blockIdx.x);
     WindowUnit u;
-    while (work.next(c, u)) {
-        window_rows<T, D, true, true, true>(c, u);
-        landed_and_barrier<0>();  // every wave is done with the LDS
-    }
+    if (tree_unit<32 * kWaves>(arguments(), blockIdx.x, u)) window_rows<T, D, true, true, true, kWaves>(arguments(), u);
 }
 
 // A split row: m = max over its parts, w = 2^(m_part - m), o = sum w o_part /
 // sum w l_part. One wave per row: lane p looks at part p (of at most 64), then all
 // lanes add up the parts' rows, four loads ahead. Bound by reading the partial
 // results or, for few rows, by two loads after one another (part after part, 52 parts
-// took 50 us). A tree's rows say how many parts they have, and where.
-template <class T, int D, bool kPaged, bool kTree>
+// took 50 us).
+template <class T, int D, bool kPaged>
 __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
     const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (row >= c.rows) return;
@@ -1052,26 +1118,11 @@ __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
         const int64_t bh = row / c.tokens, token = row - bh * c.tokens, b = bh / c.heads, head = bh - b * c.heads;
         out_at = b * c.out_rows.batch + head * c.out_rows.head + token * c.out_rows.token;
     }
-    int parts = c.parts;
-    int64_t first_part = row, to_next = c.rows, begin = 0;
-    if constexpr (kTree) {
-        const int4 its = c.row_parts[row];
-        parts = __builtin_amdgcn_readfirstlane(its.y);
-        // One part has been written whole; a row that offsets which do not ascend leave out may hold anything.
-        // The first part may be the last thing that its workgroup did, the others are the first.
-        if (parts < 2 || parts > kMostParts || its.x < 0 || its.z < 0 || its.z >= kWindowRows ||
-            its.x + int64_t(2) * c.kv_heads * (parts - 1) >= c.slots)
-            return;
-        first_part = int64_t(its.x & ~1) * kWindowRows + its.z;
-        to_next = int64_t(2) * c.kv_heads * kWindowRows;
-        begin = (its.x & 1) * kWindowRows;
-    }
-    auto part_at = [&](int p) { return first_part + p * to_next + (p == 0 ? begin : 0); };
     float2 stat = {-INFINITY, 0.f};
     float rounded = 0.f;
-    if (lane < parts) {
-        stat = c.partial_stat[part_at(lane)];
-        if (!kPaged && c.out_rest) rounded = c.partial_rounded[part_at(lane)];
+    if (lane < c.parts) {
+        stat = c.partial_stat[lane * c.rows + row];
+        if (!kPaged && c.out_rest) rounded = c.partial_rounded[lane * c.rows + row];
     }
     const bool some = stat.y != 0.f;  // a part without a key has written no row
     const uint64_t written = __ballot(some);
@@ -1087,17 +1138,17 @@ __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
         rounded += __shfl_xor(rounded, s);
     }
     constexpr int kAhead = 4;
-    for (int p0 = 0; p0 < parts; p0 += kAhead) {
+    for (int p0 = 0; p0 < c.parts; p0 += kAhead) {
         float x[kAhead][D / 64];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const float* src = c.partial_o + part_at(min(p0 + i, parts - 1)) * D + lane * (D / 64);
+            const float* src = c.partial_o + (min(p0 + i, c.parts - 1) * c.rows + row) * D + lane * (D / 64);
 #pragma unroll
             for (int e = 0; e < D / 64; ++e) x[i][e] = src[e];
         }
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            if (p0 + i >= parts) break;
+            if (p0 + i >= c.parts) break;
             if (!(written >> (p0 + i) & 1)) continue;
             const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), p0 + i));
             // An infinite value is seen however small its part's weight is.
@@ -1120,6 +1171,86 @@ __global__ __launch_bounds__(256) void window_combine_kernel(WindowCall c) {
     if (c.lse && lane == 0) c.lse[row] = l == 0.f ? -INFINITY : m + log2f(l);
 }
 
+// A tree's split rows, as above: 16 lanes take a row of a part. Few rows: the four groups of
+// a wave take every fourth part of one row; many: a row each. Statistics and values are
+// asked for together, four parts ahead, so a row takes two loads after one another (the
+// first says where the parts are) for up to four parts of a group.
+template <class T, int D, int kGroups>
+__global__ __launch_bounds__(256) void tree_combine_kernel(WindowCall c) {
+    const int lane = threadIdx.x & 63, of16 = lane & 15, group = kGroups == 4 ? lane >> 4 : 0;
+    const int64_t row = int64_t(blockIdx.x) * (16 / kGroups) + (kGroups == 4 ? threadIdx.x >> 6 : threadIdx.x >> 4);
+    if (row >= c.rows) return;
+    const int token = static_cast<int>(static_cast<uint32_t>(row / c.heads)), head = static_cast<int>(row - int64_t(token) * c.heads);
+    const int4 its = c.row_parts[row];
+    // Rows before the first sequence and behind the last stay as they were.
+    if (token < c.offsets[0] || token >= c.offsets[c.batch]) return;
+    const int parts = its.y, slot = its.x, in_tile = its.z;
+    // One part has been written whole; a row that offsets which do not ascend leave out may
+    // hold anything.
+    if (parts < 2 || parts > kMostParts || slot < 0 || its.w < 0 || in_tile < 0 || in_tile >= c.tile_rows ||
+        slot + int64_t(its.w) * (parts - 1) >= c.slots)
+        return;
+    auto place = [&](int p) { return (slot + int64_t(its.w) * p) * c.tile_rows + in_tile; };
+    // An infinite value is seen however small its part's weight is.
+    auto weighted = [](float w, float x) { return w == 0.f && !(fabsf(x) < INFINITY) ? x : w * x; };
+    constexpr int kEach = D / 16, kAhead = 4;
+    float m = -INFINITY, l = 0.f, o[kEach] = {};
+    for (int p0 = 0; p0 < parts; p0 += kGroups * kAhead) {
+        float2 stat[kAhead];
+        f32x4 x[kAhead][kEach / 4];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int p = p0 + kGroups * i + group;
+            stat[i] = float2{-INFINITY, 0.f};
+#pragma unroll
+            for (int e = 0; e < kEach / 4; ++e) x[i][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (p < parts) {
+                const int64_t at = place(p);
+                stat[i] = c.partial_stat[at];
+#pragma unroll
+                for (int e = 0; e < kEach / 4; ++e) x[i][e] = *reinterpret_cast<const f32x4*>(c.partial_o + at * D + of16 * kEach + 4 * e);
+            }
+        }
+        float top = m;  // a part without a key has written no row
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (stat[i].y != 0.f) top = fmaxf(top, stat[i].x);
+        const float before = l == 0.f ? 0.f : fast_exp2(m - top);
+        l *= before;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) o[e] = weighted(before, o[e]);
+        m = top;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (stat[i].y == 0.f) continue;
+            const float w = fast_exp2(stat[i].x - m);
+            l += w * stat[i].y;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) o[e] += weighted(w, x[i][e / 4][e % 4]);
+        }
+    }
+    // The groups.
+#pragma unroll
+    for (int s = 16; s < 16 * kGroups; s *= 2) {
+        const float its_m = __shfl_xor(m, s), its_l = __shfl_xor(l, s), top = fmaxf(m, its_m);
+        const float w = l == 0.f ? 0.f : fast_exp2(m - top), its_w = its_l == 0.f ? 0.f : fast_exp2(its_m - top);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const float mine = weighted(w, o[e]), its = weighted(its_w, __shfl_xor(o[e], s));
+            o[e] = mine + its;
+        }
+        l = w * l + its_w * its_l;
+        m = top;
+    }
+    if (group != 0) return;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    uint16_t* out = static_cast<uint16_t*>(c.out) + head * c.out_rows.head + int64_t(token) * c.out_rows.token + of16 * kEach;
+#pragma unroll
+    for (int e = 0; e < kEach; e += 4)
+        *reinterpret_cast<u32x2*>(out + e) = u32x2{T::pack(o[e] * inv, o[e + 1] * inv), T::pack(o[e + 2] * inv, o[e + 3] * inv)};
+    if (c.lse && of16 == 0) c.lse[row] = l == 0.f ? -INFINITY : m + log2f(l);
+}
+
 template <class T, int D, bool kPaged>
 int launch_as(const WindowCall& c, hipStream_t stream) {
     const int64_t tiles = window_tiles(c), heads = kPaged ? c.kv_heads : int64_t(c.batch) * c.heads;
@@ -1131,19 +1262,24 @@ int launch_as(const WindowCall& c, hipStream_t stream) {
     hipLaunchKernelGGL(kernel, grid, dim3(kWindowThreads), kLds, stream, c, places);
     if (int rc = check_launch("window_kernel")) return rc;
     if (c.parts == 1) return 0;
-    hipLaunchKernelGGL((window_combine_kernel<T, D, kPaged, false>), dim3(static_cast<unsigned>((c.rows + 3) / 4)), dim3(256), 0, stream, c);
+    hipLaunchKernelGGL((window_combine_kernel<T, D, kPaged>), dim3(static_cast<unsigned>((c.rows + 3) / 4)), dim3(256), 0, stream, c);
     return check_launch("window_combine_kernel");
 }
 
-template <class T, int D>
+constexpr int64_t kFewRows = 4096;
+
+template <class T, int D, int kWaves>
 int launch_tree_as(const WindowCall& c, hipStream_t stream) {
-    const auto kernel = tree_attention_kernel<T, D>;
-    constexpr int kLds = WindowTile<T, D>::kTreeLdsBytes;
+    const auto kernel = tree_attention_kernel<T, D, kWaves>;
+    constexpr int kLds = WindowTile<T, D>::kMasks + 4 * kMaskWords<kWaves>;
     if (int rc = ensure_lds_limit(reinterpret_cast<const void*>(kernel), kLds)) return rc;
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(c.groups)), dim3(kWindowThreads), kLds, stream, c);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(c.groups)), dim3(64 * kWaves), kLds, stream, c);
     if (int rc = check_launch("tree_attention_kernel")) return rc;
-    hipLaunchKernelGGL((window_combine_kernel<T, D, true, true>), dim3(static_cast<unsigned>((c.rows + 3) / 4)), dim3(256), 0, stream, c);
-    return check_launch("window_combine_kernel");
+    if (c.rows <= kFewRows)
+        hipLaunchKernelGGL((tree_combine_kernel<T, D, 4>), dim3(static_cast<unsigned>((c.rows + 3) / 4)), dim3(256), 0, stream, c);
+    else
+        hipLaunchKernelGGL((tree_combine_kernel<T, D, 1>), dim3(static_cast<unsigned>((c.rows + 15) / 16)), dim3(256), 0, stream, c);
+    return check_launch("tree_combine_kernel");
 }
 }  // namespace
 
@@ -1182,24 +1318,29 @@ int window_parts(const WindowCall& c, int64_t most_keys) {
     return best;
 }
 
-// As many workgroups as the chip takes at once (two to a CU, with D = 64 three), or as there
-// are parts; the parts themselves are TreeWork's.
+// The parts themselves are tree_unit's, which keeps to the groups and slots given here.
 void plan_tree(WindowCall& c, int64_t most_keys) {
-    // A sequence of x rows has at most (x - 1) / 128 + 1 tiles of rows.
     const int64_t packed = int64_t(c.tokens) * c.group.d;
-    const int64_t units = packed <= c.batch ? packed : (packed - c.batch) / kWindowRows + c.batch;
+    c.tile_rows = c.dim == 128 && packed > int64_t(c.batch) * 128 ? 256 : 128;
+    // A sequence of x rows has at most (x - 1) / tile_rows + 1 tiles of rows.
+    const int64_t units = (packed <= c.batch ? packed : (packed - c.batch) / c.tile_rows + c.batch) * c.kv_heads;
     const int64_t steps = (most_keys + 2 * kWindowKeys - 1) / kWindowKeys + 1;
-    const int64_t groups = (c.dim == 128 ? 512 : 768) / c.kv_heads;
-    const int64_t wanted = std::max<int64_t>(1, std::min(groups, (units * steps + kTreeSteps - 1) / kTreeSteps));
-    c.share = 1.0 / double(wanted);
-    c.groups = static_cast<int32_t>(wanted * c.kv_heads);
-    c.slots = 2 * c.groups;
+    const int64_t parts = std::min<int64_t>(kMostParts, (steps + kTreeSteps - 1) / kTreeSteps);
+    const int64_t at_once = c.tile_rows == 256 ? 256 : c.dim == 128 ? 512 : 768;
+    c.slots = static_cast<int32_t>(std::min(units * parts, 2 * at_once));
+    c.groups = static_cast<int32_t>(std::max<int64_t>(units, c.slots));
+    c.share = 1.f / float(at_once);
+    c.step_cost = c.tile_rows == 256 ? 1.1f : c.dim == 128 ? 0.9f : 0.55f;
+    c.read_cost = float(kWindowKeys * c.dim * 4) / 4.7e6f;
+    const double rows = std::min<double>(c.tile_rows, double(packed) / c.batch);
+    c.sums_cost = static_cast<float>(rows * (c.dim * 4.0 + 8) * 2 / 4.5e6);
 }
 
 int launch_window(const WindowCall& c, hipStream_t stream) {
     auto typed = [&](auto t) {
         using T = decltype(t);
-        if (c.near) return c.dim == 128 ? launch_tree_as<T, 128>(c, stream) : launch_tree_as<T, 64>(c, stream);
+        if (c.near && c.tile_rows == 256) return c.dim == 128 ? launch_tree_as<T, 128, 8>(c, stream) : launch_tree_as<T, 64, 8>(c, stream);
+        if (c.near) return c.dim == 128 ? launch_tree_as<T, 128, 4>(c, stream) : launch_tree_as<T, 64, 4>(c, stream);
         if (c.dim == 128) return c.paged ? launch_as<T, 128, true>(c, stream) : launch_as<T, 128, false>(c, stream);
         return c.paged ? launch_as<T, 64, true>(c, stream) : launch_as<T, 64, false>(c, stream);
     };

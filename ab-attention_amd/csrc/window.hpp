@@ -168,11 +168,12 @@ struct WindowCall {
     float2* partial_stat;                    // [parts][rows]: reference and sum
     float* partial_rounded;                  // [parts][rows], for a tensor's out_rest: sum of the rounded weights
     int64_t rows;                            // queries times heads
-    // Of a tree, whose parts are chosen by the kernel: workgroups, one by the number of
-    // those of a head, and places for parts' rows, [slots][kWindowRows].
-    int32_t groups, slots;
-    double share;
-    int4* row_parts;                         // [rows]: first place, parts, row in the place
+    // Of a tree, whose parts are chosen by the kernel: workgroups, places for parts' rows
+    // [slots][tile_rows], rows of a tile; one by the workgroups that run at once; and in us what
+    // a step costs, the reading of its keys, and writing and reading the sums of a part.
+    int32_t groups, slots, tile_rows;
+    float share, step_cost, read_cost, sums_cost;
+    int4* row_parts;                         // [rows]: first place, parts, row in the place, from place to place
 };
 
 // One call of the backward pass over strided tensors. `stat` holds, for every
@@ -200,6 +201,8 @@ constexpr int kWindowThreads = 256;
 constexpr int kWindowRows = 128;  // query rows of a workgroup
 constexpr int kTreeSteps = 4;     // tiles of keys of a part of a tree's, at least
 constexpr int kMostParts = 64;    // of a tile of rows
+constexpr float kFilling = 9.f;   // us that filling and emptying a workgroup's pipeline takes
+constexpr float kJoining = 6.f;   // and the second kernel of parts
 constexpr int kWindowKeys = 32;   // keys of a tile
 
 // Keys of a run of tiles: the first `sink_tiles` tiles start at 0, the others at
@@ -260,7 +263,7 @@ inline WindowGrid window_grid(int64_t heads, int64_t tiles) { return {static_cas
 int launch_window(const WindowCall& call, hipStream_t stream);
 int window_parts(const WindowCall& call, int64_t most_keys);
 int64_t window_tiles(const WindowCall& call);
-// Sets groups, share and slots of a tree's call; most_keys as above.
+// Sets what is said above of a tree's call.
 void plan_tree(WindowCall& call, int64_t most_keys);
 int launch_window_grad(const WindowGradCall& call, hipStream_t stream);
 // Sets the tiles and parts of a split; returns the floats of stat and of partial.
