@@ -286,8 +286,9 @@ _HERE = contextlib.nullcontext()
 
 
 def on(device: torch.device):
-    """``torch.cuda.device(device)``, free where it is the current device."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    """``torch.cuda.device(device)``, nearly free where it is the current device (asked for
+    without ``torch.cuda.current_device``'s own checks, 0.3 us)."""
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def address(t: torch.Tensor | None) -> int:

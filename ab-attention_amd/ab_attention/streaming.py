@@ -116,7 +116,7 @@ _ROTARY, _WINDOW, _APPEND = map(_lib.packer, (_lib.RotaryArgs, _lib.WindowArgs, 
 _TREE, _VERIFY, _KEEP, _COPY = map(_lib.packer, (_lib.DraftTreeArgs, _lib.VerifyArgs, _lib.KeepArgs, _lib.CopyArgs))
 _TREE_REST = struct.Struct("=3Q")     # ab_tree_args behind its chunk
 _GRAD_REST = struct.Struct("=5Q12q")  # ab_window_grad_args behind its forward part
-_WORKSPACE = struct.Struct("=2Q")     # the last fields of ab_window_args
+_WORKSPACE = struct.Struct("=2Q")     # the last fields of ab_window_args and ab_verify_args
 _ZERO = (0, 0, 0)
 
 
@@ -245,8 +245,8 @@ def _check_window(window, scale, dim):
 
 
 def _run(entry, device, packed, behind=b"", asks="ab_window_workspace_bytes"):
-    """One call with the workspace that it ``asks`` for, which lives for the call only; ``behind``: fields after
-    ab_window_args."""
+    """One call with the workspace that it ``asks`` for, the last two fields of ``packed``, which lives for the call
+    only; ``behind``: fields after those."""
     with _lib.on(device):
         size = _lib.raw(asks)(packed + behind)
         if size:
@@ -599,41 +599,42 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
     if batch == 0:
         kept.path.fill_(-1)
         return kept
-    args = (target.data_ptr(), 0 if draft is None else draft.data_ptr(), tokens.data_ptr(), parents.data_ptr(), offsets.data_ptr(),
-            uniforms.data_ptr(), *(t.data_ptr() for t in kept), batch, rows, vocab, _DTYPES[target.dtype],
-            tokens.dtype == torch.int64, target.stride(0), 0 if draft is None else draft.stride(0))
-    with _lib.on(device):
-        size = _lib.raw("ab_verify_workspace_bytes")(_VERIFY.pack(*args, 0, 0))
-        workspace = torch.empty(size, dtype=torch.uint8, device=device)
-        status = _lib.raw("ab_verify_drafts")(_VERIFY.pack(*args, workspace.data_ptr(), size), _lib.raw_stream(device))
-    if status:
-        _lib.check(status)
+    path, counts, after = kept
+    _run("ab_verify_drafts", device, _VERIFY.pack(
+        target.data_ptr(), 0 if draft is None else draft.data_ptr(), tokens.data_ptr(), parents.data_ptr(), offsets.data_ptr(),
+        uniforms.data_ptr(), path.data_ptr(), counts.data_ptr(), after.data_ptr(), batch, rows, vocab, _DTYPES[target.dtype],
+        tokens.dtype == torch.int64, target.stride(0), 0 if draft is None else draft.stride(0), 0, 0), b"",
+        "ab_verify_workspace_bytes")
     return kept
 
 
 def _check_layers(name, cache):
-    """(layers, strides of a layer in k and v, strides in a layer) of a cache of one layer, or of several, [layers, ..]."""
+    """(layers, sizes of a layer, strides of a layer in k and v, strides in a layer) of a cache of one layer, or of
+    several, [layers, ..]."""
     k, v = cache
-    if k.ndim not in (4, 5) or k.shape != v.shape:
+    shape, dtype = k.shape, k.dtype
+    if not 4 <= len(shape) <= 5 or shape != v.shape:
         raise ValueError("the cache must be two [pages,heads,page tokens,D] or [layers,pages,heads,page tokens,D] tensors")
-    dim, page = k.shape[-1], k.shape[-2]
+    pages, heads, page, dim = shape[-4:]
     if dim != 128 and dim != 64:
         raise ValueError(f"{name} requires head_dim 64 or 128")
-    if k.dtype not in (torch.bfloat16, torch.float16) or v.dtype != k.dtype:
+    if (dtype != torch.bfloat16 and dtype != torch.float16) or v.dtype != dtype:
         raise ValueError(f"{name} requires a BF16 or FP16 cache")
     if page == 0 or page % 8:
         raise ValueError("pages must hold a positive multiple of 8 tokens")
-    if k.shape[-3] == 0:
+    if heads == 0:
         raise ValueError("the cache must have at least one head")
     for t in cache:
-        if t.data_ptr() % 16 or not (t.is_contiguous() or (
-                t.stride(-1) == 1 and not any(n > 1 and s % 8 for n, s in zip(t.shape, t.stride()[:-1])))):
+        whole = t.is_contiguous()
+        if t.data_ptr() % 16 or not (whole or (
+                t.stride(-1) == 1 and not any(n > 1 and s % 8 for n, s in zip(shape, t.stride()[:-1])))):
             raise ValueError("the cache's rows must be contiguous and start on 16 bytes")
-        if not _own_rows(t):
+        if not (whole or _own_rows(t)):
             raise ValueError(f"{name} cannot write to an expanded cache or one whose rows overlap")
-    if k.ndim == 4:
-        return 1, (0, 0), k.stride()[:3], v.stride()[:3]
-    return k.shape[0], (k.stride(0), v.stride(0)), k.stride()[1:4], v.stride()[1:4]
+    if len(shape) == 4:
+        return 1, (pages, heads, page, dim), (0, 0), k.stride()[:3], v.stride()[:3]
+    a, b = k.stride(), v.stride()
+    return shape[0], (pages, heads, page, dim), (a[0], b[0]), a[1:4], b[1:4]
 
 
 def keep_drafts(cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tensor, offsets: torch.Tensor,
@@ -648,7 +649,7 @@ def keep_drafts(cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tens
     layer or, as tensors [layers, pages, heads, page tokens, D], of all layers, which one
     call then takes. No page is in two places of the table. Returns the cache.
     """
-    layers, layer_strides, k_stride, v_stride = _check_layers("keep_drafts", cache)
+    layers, (pages, heads, page, dim), layer_strides, k_stride, v_stride = _check_layers("keep_drafts", cache)
     if page_table.ndim != 2 or page_table.dtype != torch.int32 or not page_table.is_contiguous():
         raise ValueError("page_table must be contiguous int32 [B,width]")
     _ints("keep_drafts", lengths=lengths, offsets=offsets, path=path, counts=counts)
@@ -659,7 +660,6 @@ def keep_drafts(cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tens
     _no_tangent("keep_drafts", k, v)
     device = _gpu("keep_drafts", k, v, page_table, lengths, offsets, path, counts)
     _writes("keep_drafts", k, v)
-    pages, heads, page, dim = k.shape[-4:]
     if layers:
         _call("ab_keep_drafts", device, _KEEP.pack(
             k.data_ptr(), v.data_ptr(), lengths.data_ptr(), offsets.data_ptr(), page_table.data_ptr(), path.data_ptr(),
@@ -674,9 +674,8 @@ def copy_pages(cache: PagedCache, moves) -> PagedCache:
     layer or of all, as in ``keep_drafts``. Returns the cache. A call captured into a
     graph repeats the moves that it was captured with.
     """
-    layers, layer_strides, k_stride, v_stride = _check_layers("copy_pages", cache)
+    layers, (pages, heads, page, dim), layer_strides, k_stride, v_stride = _check_layers("copy_pages", cache)
     k, v = cache
-    pages, heads, page, dim = k.shape[-4:]
     flat = [int(p) for source, target in moves for p in (source, target)]
     if flat and not (0 <= min(flat) and max(flat) < pages):
         raise ValueError(f"moves must name pages from 0 to {pages - 1}")

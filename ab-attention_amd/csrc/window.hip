@@ -33,6 +33,17 @@
 // this kernel (two stages, one tile at a time) did 605. With single tokens over long
 // caches it is memory: 4.7 TB/s of the 4.9 that a copy reaches, the keys split over
 // workgroups. 9 tiles of a short call take 14 us, half of them the pipeline's filling.
+//
+// A tree of drafted tokens (tree_attention_kernel) takes the same passes over tiles of 128 or
+// 256 rows. Its rows are not in the order of their positions: the bounds of clear tiles are
+// those of all a sequence's tokens, and what each token sees of the other tiles (the ends of
+// sinks and window, the drafts, all of them where a page is missing) is made into words of 32
+// keys in LDS before the passes, which then take one LDS read for a masked tile and row, and
+// none of the mask's arithmetic. The first form walked up the tree in every masked tile (4 x
+// 701 drafts 195 us, now 80). Bound like the others: one sequence of 64 drafts, 256 rows over
+// 100,000 keys, 119 us where reading takes 84 and the products 88; of 16 drafts 77 us, 5.3
+// TB/s; a few keys (26 drafts over 1,017) 15 us, all of it one thing after another: which
+// sequence, its page table, its masks, four tiles of keys, 3,000 instructions of one wave.
 #include <algorithm>
 #include <initializer_list>
 
@@ -185,10 +196,11 @@ __device__ __forceinline__ const WindowCall& arguments() {
 // a sequence, all are cut into parts of at most C steps; lane k looks at C = longest / (k + 1),
 // and the C that costs least is taken: a workgroup's C steps and its filling, in rounds
 // where there are more workgroups than run at once, or what reading all keys takes, if that
-// is more; parts cost a second kernel and the traffic of their sums. (To give every workgroup the same number of steps, of two
-// tiles of rows if need be, costs more than it saves: 8 sequences of 4,026 keys 50 us, in
-// whole parts XX.) The longest sequences come first; within one part, tile of rows, head:
-// with eight heads (or 16, ..) the tiles of rows that share keys are on one XCD.
+// is more; parts cost a second kernel and the traffic of their sums. (The same number of
+// steps for every workgroup, of two tiles of rows if need be, is slower, as each tile fills
+// the pipeline anew: 8 sequences of 4,026 keys 50 us, in whole parts 41.) The longest
+// sequences come first; within one part, tile of rows, head: with eight heads (or 16, ..)
+// the tiles of rows that share keys are on one XCD.
 template <int kRows>
 __device__ __forceinline__ bool tree_unit(const WindowCall& c, int id, WindowUnit& u) {
     const int lane = threadIdx.x & 63, group = static_cast<int>(c.group.d), heads = c.kv_heads;
@@ -291,7 +303,6 @@ struct WindowTile {
 template <int kWaves>
 constexpr int kMaskWords = kWaves == 4 ? 3968 : 16384;
 
-
 // What `rounded` lacks of two values, rounded itself (nothing of values that are not
 // finite).
 template <class T>
@@ -345,7 +356,7 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
     const bool split = kSplit && (!kTree || u.parts > 1);
     const int group = kPaged ? c.group.d : 1;
     int tid = threadIdx.x;
-    if constexpr (kTree) asm volatile("" : "+v"(tid));  // made anew for every tile of rows, not kept beside the passes
+    if constexpr (kTree) asm volatile("" : "+v"(tid));  // not known from tree_unit, whose values would be kept for it
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4;
@@ -389,9 +400,8 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
             for (int s = 0; s < kSteps; ++s) bq[j][s] = *reinterpret_cast<const u32x4*>(qrow + 32 * s);
         }
     };
-    // Of a tree: where the masks of the row's token are in LDS.
     int low[2], seen[2], sink[2];  // keys low .. low + seen - 1 and 0 .. sink - 1
-    int masks[2];
+    int masks[2];                  // of a tree instead: where the masks of the row's token are in LDS
     if constexpr (!kTree) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -939,8 +949,7 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
                 const int n = min(max(key - key0, 0), kWindowKeys);
                 return n == kWindowKeys ? ~0u : (1u << n) - 1;
             };
-            uint32_t bits = p < 0 ? 0u : (below(base) & ~below(low_of)) | below(min(mask.sinks, max(base, 0)));
-            return bits;
+            return p < 0 ? 0u : (below(base) & ~below(low_of)) | below(min(mask.sinks, max(base, 0)));
         };
         auto paged = [&](int key0) {
             uint32_t bits = ~0u;
@@ -1266,6 +1275,9 @@ int launch_as(const WindowCall& c, hipStream_t stream) {
     return check_launch("window_combine_kernel");
 }
 
+// Rows of partial results that are added up by a wave each: fewer than fill the chip with
+// four rows to a wave (512 rows of 32 parts: 9.6 us, a wave and four loads at a time 15.3;
+// 19,000 rows of 2 or 3 parts, four to a wave 8.4 us, a wave each 18).
 constexpr int64_t kFewRows = 4096;
 
 template <class T, int D, int kWaves>
@@ -1319,6 +1331,11 @@ int window_parts(const WindowCall& c, int64_t most_keys) {
 }
 
 // The parts themselves are tree_unit's, which keeps to the groups and slots given here.
+//
+// Tiles of 256 rows, for eight waves, where sequences have more than 128 rows on average: keys
+// are then read once for twice the rows (one sequence of 64 drafts, 256 rows of 100,000
+// keys: 119 us, in tiles of 128 rows 150). Not with D = 64, whose four waves take a third of
+// a CU (4 x 701 drafts 80 us, of eight waves 103).
 void plan_tree(WindowCall& c, int64_t most_keys) {
     const int64_t packed = int64_t(c.tokens) * c.group.d;
     c.tile_rows = c.dim == 128 && packed > int64_t(c.batch) * 128 ? 256 : 128;
@@ -1339,8 +1356,9 @@ void plan_tree(WindowCall& c, int64_t most_keys) {
 int launch_window(const WindowCall& c, hipStream_t stream) {
     auto typed = [&](auto t) {
         using T = decltype(t);
-        if (c.near && c.tile_rows == 256) return c.dim == 128 ? launch_tree_as<T, 128, 8>(c, stream) : launch_tree_as<T, 64, 8>(c, stream);
-        if (c.near) return c.dim == 128 ? launch_tree_as<T, 128, 4>(c, stream) : launch_tree_as<T, 64, 4>(c, stream);
+        if (c.near)
+            return c.dim == 64 ? launch_tree_as<T, 64, 4>(c, stream)
+                               : c.tile_rows == 128 ? launch_tree_as<T, 128, 4>(c, stream) : launch_tree_as<T, 128, 8>(c, stream);
         if (c.dim == 128) return c.paged ? launch_as<T, 128, true>(c, stream) : launch_as<T, 128, false>(c, stream);
         return c.paged ? launch_as<T, 64, true>(c, stream) : launch_as<T, 64, false>(c, stream);
     };

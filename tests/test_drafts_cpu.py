@@ -154,10 +154,12 @@ def test_library_draft_tree(change, msg):
 
 
 @pytest.mark.parametrize("change,msg", [({"near": 0}, b"null"), ({"positions": 0}, b"null"), ({"chunk.dim": 96}, b"64 or 128"),
-                                        ({"chunk.lengths": 0}, b"null"), ({"chunk.page_tokens": 12}, b"multiple of 8")])
+                                        ({"chunk.lengths": 0}, b"null"), ({"chunk.page_tokens": 12}, b"multiple of 8"),
+                                        ({"chunk.workspace": 0}, b"null"), ({"chunk.workspace_bytes": 8}, b"smaller"),
+                                        ({"chunk.workspace": _A + 8}, b"aligned")])
 def test_library_tree_attention(change, msg):
     fields = {"positions": _A, "near": _A, "above": _A}
-    chunk = dict(q=_A, k=_A, v=_A, out=_A, lengths=_A, offsets=_A, page_table=_A, batch=1, heads=2, kv_heads=1, tokens=5, dim=64,
+    chunk = dict(q=_A, k=_A, v=_A, out=_A, workspace=_A, workspace_bytes=1 << 30, lengths=_A, offsets=_A, page_table=_A, batch=1, heads=2, kv_heads=1, tokens=5, dim=64,
                  pages=3, page_tokens=8, table_width=2, frame=1, scale=0.1, q_stride=(0, 64, 128), k_stride=(512, 512, 64),
                  v_stride=(512, 512, 64), out_stride=(0, 64, 128))
     _check("ab_tree_attention", _lib.TreeArgs, {**{f"chunk.{k}": v for k, v in chunk.items()}, **fields}, change, msg)

@@ -113,7 +113,8 @@ class _Call:
 @pytest.mark.parametrize("dim,heads,kv_heads", [(128, 8, 2), (64, 3, 3), (128, 1, 1), (64, 16, 1)])
 @pytest.mark.parametrize("new,cached,page,branch", [
     ((1,), (0,), 8, 1), ((5,), (0,), 16, 2), ((26,), (101,), 16, 3), ((64, 1, 33), (0, 250, 63), 64, -1),
-    ((65, 0, 130), (31, 5, 2), 32, 0), ((300,), (77,), 8, -1), ((17,) * 67, tuple(range(67)), 24, 2)])
+    ((65, 0, 130), (31, 5, 2), 32, 0), ((300,), (77,), 8, -1), ((17,) * 67, tuple(range(67)), 24, 2),
+    ((1, 2, 0) * 110, (3, 700, 9) * 110, 32, 1)])
 def test_tree_attention(dtype, dim, heads, kv_heads, new, cached, page, branch):
     call = _Call(new, cached, heads, kv_heads, dim, page, dtype, 11, branch)
     o, lse = call.run()
@@ -129,6 +130,19 @@ def test_tree_attention_windows(window, sinks, frame, new, cached, branch):
     how = dict(window=window, sinks=sinks, frame=frame)
     o, lse = call.run(**how)
     call.check(o, lse, **how)
+
+
+@pytest.mark.parametrize("window,sinks,frame", [(None, 0, 1), (4, 0, 1), (40, 130, 1), (5, 1, 7)])
+@pytest.mark.parametrize("heads,new,cached,branch", [(8, (26, 80), (1500, 3), 2), (8, (17,), (41,), 0), (5, (33, 0, 128), (70, 5, 0), -1),
+                                                     (1, (2200,), (21,), 3)])
+def test_tree_attention_many_rows(heads, new, cached, branch, window, sinks, frame):
+    """Sequences of more than 128 rows: token and query head of the group."""
+    call = _Call(new, cached, heads, 1, 128, 16, BF16, 17, branch)
+    how = dict(window=window, sinks=sinks, frame=frame)
+    call.check(*call.run(**how), **how)
+    call.table[0, 1] = -1
+    call.table[0, (cached[0] + new[0] // 2) // 16] = 10 ** 9  # a page of drafts
+    call.check(*call.run(**how), **how)
 
 
 @pytest.mark.parametrize("cached", [3000, 9001])
@@ -186,9 +200,10 @@ def test_missing_pages_and_strides():
     call.check(o, lse)
 
 
-def test_drafts_that_are_not_seen_may_hold_anything():
+@pytest.mark.parametrize("heads", [4, 14])
+def test_drafts_that_are_not_seen_may_hold_anything(heads):
     """Infinities and NaN in another line's keys and values reach no token that does not follow them."""
-    call = _Call((40,), (21,), 4, 2, 128, 16, BF16, 4, 2)
+    call = _Call((40,), (21,), heads, 2, 128, 16, BF16, 4, 2)
     ref_o, ref_lse, spread = tree_attend(call.q, call.cache, call.table[0], 61, call.trees[0])
     size = logit_size(call.q, call.cache.k)
     bad = 17
