@@ -16,16 +16,20 @@ constexpr int kWave = 64;
 // goes on. A walk up a line takes a step for every 64 places, and every layer's
 // attention reads 16 bytes a token.
 //
-// One wave per sequence, 64 tokens at a time, a lane each: six rounds of pointer
-// doubling (word, steps and end of a line twice as long each time) by lane exchanges. Bound by
-// launch and the latency of two loads.
-__global__ __launch_bounds__(kWave) void tree_kernel(TreeCall c) {
-    const int b = blockIdx.x, lane = threadIdx.x;
+// One workgroup per sequence, 256 tokens at a time, a lane each: every wave follows the lines
+// inside its 64 by six rounds of pointer doubling (word, steps and end of a line twice as
+// long each time) by lane exchanges; then the waves take the positions above theirs one after
+// the other. Bound by launch and latency: 26 drafts 2.1 us, 4 x 701 4.3 (one wave for all of a
+// sequence 7.6).
+constexpr int kTreeWaves = 4;
+__global__ __launch_bounds__(kWave * kTreeWaves) void tree_kernel(TreeCall c) {
+    constexpr int kTokens = kWave * kTreeWaves;
+    const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int off = min(max(c.offsets[b], 0), c.tokens), n = min(max(c.offsets[b + 1], 0), c.tokens) - off;
     const int first = c.lengths[b] - n;
     // Rows of no sequence.
     auto clear = [&](int from, int to) {
-        for (int i = from + lane; i < to; i += kWave) {
+        for (int i = from + static_cast<int>(threadIdx.x); i < to; i += kTokens) {
             c.positions[i] = 0;
             c.near[i] = 0;
             c.above[i] = -1;
@@ -33,8 +37,11 @@ __global__ __launch_bounds__(kWave) void tree_kernel(TreeCall c) {
     };
     if (b == 0) clear(0, off);
     if (b == c.batch - 1) clear(off + max(n, 0), c.tokens);
-    for (int block = 0; block < n; block += kWave) {
-        const int i = block + lane;
+    // Positions of earlier tokens; of those past what fits, what was written.
+    constexpr int kNear = 4096;
+    __shared__ int positions[kNear];
+    for (int block0 = 0; block0 < n; block0 += kTokens) {
+        const int block = block0 + wave * kWave, i = block + lane;
         int parent = i < n ? c.parents[off + i] : -1;
         if (parent >= i) parent = -1;
         const bool inside = parent >= block;
@@ -50,12 +57,20 @@ __global__ __launch_bounds__(kWave) void tree_kernel(TreeCall c) {
         }
         const int above = max(__shfl(parent, end), -1);
         if (i < n) {
-            // Positions of earlier tokens are this wave's own writes.
-            c.positions[off + i] = above >= 0 ? c.positions[off + above] + 1 + steps : first + steps;
             c.near[off + i] = word;
             c.above[off + i] = above;
         }
-        __threadfence_block();
+        for (int w = 0; w < kTreeWaves && block0 + w * kWave < n; ++w) {
+            if (wave == w && i < n) {
+                int position = first + steps;
+                if (above >= kNear) position = c.positions[off + above] + 1 + steps;
+                else if (above >= 0) position = positions[above] + 1 + steps;
+                if (i < kNear) positions[i] = position;
+                c.positions[off + i] = position;
+            }
+            __threadfence_block();
+            __syncthreads();
+        }
     }
 }
 
@@ -82,6 +97,13 @@ __global__ __launch_bounds__(kWave) void tree_kernel(TreeCall c) {
 // are fetched together before the first is looked at; then each of its waves adds up a
 // part of what is left. sample_kernel, one workgroup per sequence, goes on from there:
 // where more drawn drafts are turned down it adds up the whole vocabulary by itself.
+//
+// A chain of 7 drafts over 32,000 tokens takes 4.6 + 4.8 us, 48 chosen trees over 128,000
+// 10.0 + 5.2, bound by latency: the walk, a reading, the choice among a few values. What
+// one CU adds up by itself takes 2.3 us over 1,000 tokens, 4.1 over 32,000 and 8.9 over
+// 100,000, as much 64-bit arithmetic as loading (16 drawn trees with four drafts behind a
+// token, four or five such sums after one another: 5 + 40 us). A kernel for every further
+// sum would spread them over the chip, and cost those that have none 2 us and a launch each.
 
 // The value of an element, and its weight: of what is negative, infinite or no number 0.
 // As unsigned numbers the bits of positive finite ones are those up to the largest one's.
@@ -494,7 +516,7 @@ int launch_verify_as(const VerifyCall& c, hipStream_t stream) {
 }  // namespace
 
 int launch_tree(const TreeCall& c, hipStream_t stream) {
-    hipLaunchKernelGGL(tree_kernel, dim3(static_cast<unsigned>(c.batch)), dim3(kWave), 0, stream, c);
+    hipLaunchKernelGGL(tree_kernel, dim3(static_cast<unsigned>(c.batch)), dim3(kWave * kTreeWaves), 0, stream, c);
     return check_launch("tree_kernel");
 }
 

@@ -256,11 +256,16 @@ __device__ __forceinline__ bool tree_unit(const WindowCall& c, int id, WindowUni
         const int parts = parts_of(s.steps), all = s.tiles * parts;
         int start = before + running_sum(all, lane) - all;
         if (c.batch <= 64) {
+            // In the order of the keys; there are at most 2^25 steps.
+            const uint32_t key = static_cast<uint32_t>(s.steps) * 64 + 63 - lane;
             start = 0;
-            for (int j = 0; j < c.batch; ++j) {
-                const int other = __builtin_amdgcn_readlane(s.steps, j), its = __builtin_amdgcn_readlane(all, j);
-                start += other > s.steps || (other == s.steps && j < lane) ? its : 0;
-            }
+            for (int j0 = 0; j0 < c.batch; j0 += 8)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t other = __builtin_amdgcn_readlane(key, j0 + j);
+                    const int its = __builtin_amdgcn_readlane(all, j0 + j);
+                    start += other > key ? its : 0;
+                }
         }
         const uint64_t here = __ballot(mine >= start && mine < start + all);
         if (here) {

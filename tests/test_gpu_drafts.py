@@ -39,7 +39,7 @@ def _packed(trees, before=0, behind=0):
 
 
 @pytest.mark.parametrize("branch", [-1, 0, 1, 2, 3])
-@pytest.mark.parametrize("sizes", [(1,), (2, 0, 3), (63, 64, 65), (26,) * 70, (300, 1, 129), (1025,)])
+@pytest.mark.parametrize("sizes", [(1,), (2, 0, 3), (63, 64, 65), (26,) * 70, (300, 1, 129), (1025,), (5, 4500)])
 def test_draft_tree(sizes, branch):
     trees = [make_tree(n, branch, s) for s, n in enumerate(sizes)]
     lengths = [n + 7 * s - 3 for s, n in enumerate(sizes)]  # the first sequence lacks three tokens
