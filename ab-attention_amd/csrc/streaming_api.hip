@@ -151,7 +151,8 @@ void plan_tree_call(const ab_window_args& a, WindowCall& c) {
 }
 
 size_t tree_workspace_bytes(const WindowCall& c) {
-    return size_t(c.rows) * sizeof(int4) + size_t(c.slots) * c.tile_rows * (size_t(c.dim) * sizeof(float) + sizeof(float2));
+    const size_t starts = c.batch > 64 ? size_t(c.batch + 2) * sizeof(int32_t) : 0;
+    return size_t(c.rows) * sizeof(int4) + size_t(c.slots) * c.tile_rows * (size_t(c.dim) * sizeof(float) + sizeof(float2)) + starts;
 }
 
 int window_launch(const char* what, const ab_window_args* a, bool paged, void* stream, const ab_tree_args* tree = nullptr) {
@@ -181,6 +182,7 @@ int window_launch(const char* what, const ab_window_args* a, bool paged, void* s
         c.row_parts = static_cast<int4*>(a->workspace);
         c.partial_o = reinterpret_cast<float*>(c.row_parts + c.rows);
         c.partial_stat = reinterpret_cast<float2*>(c.partial_o + int64_t(c.slots) * c.tile_rows * c.dim);
+        c.starts = c.batch > 64 ? reinterpret_cast<int32_t*>(c.partial_stat + int64_t(c.slots) * c.tile_rows) : nullptr;
     } else if (!tree && c.parts > 1) {
         if (a->workspace_bytes < workspace_bytes(c))
             return set_error(AB_ERR_INVALID, "%s: workspace of %zu bytes is smaller than the %zu required", what,

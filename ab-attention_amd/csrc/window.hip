@@ -189,7 +189,27 @@ __device__ __forceinline__ const WindowCall& arguments() {
     return *(const WindowCall*)at;
 }
 
-// A tree's workgroup: of which sequence, tile of rows, K/V head and part of the keys.
+// A sequence of a tree's call: its rows' tiles, and the tiles of keys that they take.
+struct TreeSequence {
+    int off, n, length, tiles, steps;
+};
+template <int kRows>
+__device__ __forceinline__ TreeSequence tree_sequence(const WindowCall& c, int b) {
+    TreeSequence s;
+    const bool there = b < c.batch;
+    b = min(b, c.batch - 1);
+    s.off = min(max(c.offsets[b], 0), c.tokens);
+    s.n = there ? min(max(c.offsets[b + 1], 0), c.tokens) - s.off : 0;
+    s.length = static_cast<int>(min(int64_t(max(c.lengths[b], 0)), int64_t(c.table_width) * c.page.d));
+    s.tiles = s.n > 0 ? (s.n * static_cast<int>(c.group.d) + kRows - 1) / kRows : 0;
+    TileRange range;
+    range.set(c.mask, max(s.length - s.n, 0), s.length - 1, s.length);
+    s.steps = s.tiles > 0 ? max(range.tiles, 1) : 0;  // rows that see nothing are written too
+    return s;
+}
+
+// How many steps a part has at most, by what the call's sequences have: steps of all tiles of
+// rows, those tiles, the longest's steps.
 //
 // How many sequences there are, and how long they are, is on the device, so the kernel
 // itself deals out the work. With `steps` tiles of keys for each of the `tiles` of rows of
@@ -198,96 +218,132 @@ __device__ __forceinline__ const WindowCall& arguments() {
 // where there are more workgroups than run at once, or what reading all keys takes, if that
 // is more; parts cost a second kernel and the traffic of their sums. (The same number of
 // steps for every workgroup, of two tiles of rows if need be, is slower, as each tile fills
-// the pipeline anew: 8 sequences of 4,026 keys 50 us, in whole parts 41.) The longest
-// sequences come first; within one part, tile of rows, head: with eight heads (or 16, ..)
-// the tiles of rows that share keys are on one XCD.
+// the pipeline anew: 8 sequences of 4,026 keys 50 us, in whole parts 41.)
+__device__ __forceinline__ int tree_part(const WindowCall& c, float work, int units, int longest) {
+    const int lane = threadIdx.x & 63, heads = c.kv_heads;
+    const float k = lane + 1.f, steps = fmaxf(ceilf(longest / k), 1.f), whole = static_cast<float>(units) * heads;
+    // Workgroups, and the most there can be.
+    const float cut = work * heads / steps, most = cut + whole, groups = c.batch == 1 ? whole * ceilf(longest / steps) : cut + 0.5f * whole;
+    float cost = fmaxf(fmaxf(1.f, (lane == 0 ? whole : groups) * c.share) * (steps * c.step_cost + kFilling), work * heads * c.read_cost);
+    if (lane > 0) cost += kJoining + groups * c.sums_cost;
+    if (lane > 0 && (steps < kTreeSteps || most > c.slots)) cost = INFINITY;
+    // The lane of the least cost; costs are positive, so their bits are in their order.
+    const int least = 0x7f800000 - most_of_lanes(0x7f800000 - __builtin_bit_cast(int, cost));
+    const int best = __builtin_ctzll(__ballot(__builtin_bit_cast(int, cost) == least) | (uint64_t(1) << 63));
+    return best == 0 ? longest : __builtin_amdgcn_readlane(static_cast<int>(steps), best);
+}
+
+// A tree's workgroup: of which sequence, tile of rows, K/V head and part of the keys.
+//
+// Of at most 64 sequences every wave looks at them all, a lane each, and the longest come
+// first. Of more a kernel before this one says where each one's workgroups begin (1,024
+// sequences of a token over 200 keys 283 us, by every workgroup itself 454). Within a sequence
+// part, tile of rows, head: with eight heads (or 16, ..) the tiles of rows that share keys
+// are on one XCD.
 template <int kRows>
 __device__ __forceinline__ bool tree_unit(const WindowCall& c, int id, WindowUnit& u) {
     const int lane = threadIdx.x & 63, group = static_cast<int>(c.group.d), heads = c.kv_heads;
-    struct Sequence {
-        int off, n, length, tiles, steps;
-    };
-    auto look_at = [&](int b) {
-        Sequence s;
-        const bool there = b < c.batch;
-        b = min(b, c.batch - 1);
-        s.off = min(max(c.offsets[b], 0), c.tokens);
-        s.n = there ? min(max(c.offsets[b + 1], 0), c.tokens) - s.off : 0;
-        s.length = static_cast<int>(min(int64_t(max(c.lengths[b], 0)), int64_t(c.table_width) * c.page.d));
-        s.tiles = s.n > 0 ? (s.n * group + kRows - 1) / kRows : 0;
-        TileRange range;
-        range.set(c.mask, max(s.length - s.n, 0), s.length - 1, s.length);
-        s.steps = s.tiles > 0 ? max(range.tiles, 1) : 0;  // rows that see nothing are written too
-        return s;
-    };
-    Sequence s = look_at(lane);
-    float work = static_cast<float>(s.tiles) * static_cast<float>(s.steps);
-    int units = s.tiles, longest = s.steps;
-    for (int b = 64; b < c.batch; b += 64) {
-        const Sequence more = look_at(b + lane);
-        work += static_cast<float>(more.tiles) * static_cast<float>(more.steps);
-        units += more.tiles;
-        longest = max(longest, more.steps);
-    }
-    longest = most_of_lanes(longest);
-    if (longest == 0) return false;
-    work = lane_value(running_sum(work, lane), 63);
-    units = lane_value(running_sum(units, lane), 63);
-    int each;
-    {
-        const float k = lane + 1.f, steps = fmaxf(ceilf(longest / k), 1.f), whole = static_cast<float>(units * heads);
-        // Workgroups, and the most there can be.
-        const float cut = work * heads / steps, most = cut + whole, groups = c.batch == 1 ? whole * ceilf(longest / steps) : cut + 0.5f * whole;
-        float cost = fmaxf(fmaxf(1.f, (lane == 0 ? whole : groups) * c.share) * (steps * c.step_cost + kFilling), work * heads * c.read_cost);
-        if (lane > 0) cost += kJoining + groups * c.sums_cost;
-        if (lane > 0 && (steps < kTreeSteps || most > c.slots)) cost = INFINITY;
-        // The lane of the least cost; costs are positive, so their bits are in their order.
-        const int least = 0x7f800000 - most_of_lanes(0x7f800000 - __builtin_bit_cast(int, cost));
-        const int best = __builtin_ctzll(__ballot(__builtin_bit_cast(int, cost) == least) | (uint64_t(1) << 63));
-        each = __builtin_amdgcn_readlane(static_cast<int>(steps), best);
-        if (best == 0) each = longest;
-    }
-    auto parts_of = [&](int steps) { return (steps + each - 1) / each; };
     const int mine = id / heads;
-    u.kv_head = __builtin_amdgcn_readfirstlane(id - mine * heads);
-    int before = 0;
-    for (int b = 0; b < c.batch; b += 64) {
-        if (b > 0) s = look_at(b + lane);
-        const int parts = parts_of(s.steps), all = s.tiles * parts;
-        int start = before + running_sum(all, lane) - all;
-        if (c.batch <= 64) {
-            // In the order of the keys; there are at most 2^25 steps.
-            const uint32_t key = static_cast<uint32_t>(s.steps) * 64 + 63 - lane;
-            start = 0;
-            for (int j0 = 0; j0 < c.batch; j0 += 8)
+    TreeSequence s;
+    int each, start = 0;
+    auto parts_of = [&](int steps) { return (steps + each - 1) / each; };
+    if (c.starts) {
+        each = c.starts[c.batch + 1];
+        if (mine >= c.starts[c.batch]) return false;
+        // The last sequence that begins at `mine` or before, a 64th of the range at a time.
+        int first = 0;
+        for (int range = c.batch; range > 1;) {
+            const int step = (range + 63) / 64, at = lane * step;
+            const int places = max(__popcll(__ballot(at < range && c.starts[min(first + at, c.batch)] <= mine)), 1) - 1;
+            first += places * step;
+            range = min(step, range - places * step);
+        }
+        u.b = __builtin_amdgcn_readfirstlane(first);
+        s = tree_sequence<kRows>(c, u.b);
+        start = c.starts[u.b];
+    } else {
+        s = tree_sequence<kRows>(c, lane);
+        const int longest = most_of_lanes(s.steps);
+        if (longest == 0) return false;
+        const float work = static_cast<float>(s.tiles) * static_cast<float>(s.steps);
+        each = tree_part(c, lane_value(running_sum(work, lane), 63), lane_value(running_sum(s.tiles, lane), 63), longest);
+        // In the order of the keys; there are at most 2^25 steps.
+        const uint32_t key = static_cast<uint32_t>(s.steps) * 64 + 63 - lane;
+        const int all = s.tiles * parts_of(s.steps);
+        for (int j0 = 0; j0 < c.batch; j0 += 8)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t other = __builtin_amdgcn_readlane(key, j0 + j);
-                    const int its = __builtin_amdgcn_readlane(all, j0 + j);
-                    start += other > key ? its : 0;
-                }
-        }
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t other = __builtin_amdgcn_readlane(key, j0 + j);
+                const int its = __builtin_amdgcn_readlane(all, j0 + j);
+                start += other > key ? its : 0;
+            }
         const uint64_t here = __ballot(mine >= start && mine < start + all);
-        if (here) {
-            const int at = __builtin_ctzll(here);
-            auto its = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
-            u.b = b + at;
-            u.off = its(s.off);
-            u.n = its(s.n);
-            u.length = its(s.length);
-            u.parts = its(parts);
-            const int tiles = its(s.tiles), place = mine - its(start);
-            u.part = __builtin_amdgcn_readfirstlane(place / tiles);
-            u.tile = __builtin_amdgcn_readfirstlane(place - u.part * tiles);
-            u.stride = tiles * heads;
-            u.slot = __builtin_amdgcn_readfirstlane(id);
-            u.head = u.kv_head * group;
-            u.first = u.length - u.n;
-            return true;
-        }
-        before = __builtin_amdgcn_readlane(start + all, 63);
+        if (!here) return false;
+        u.b = __builtin_ctzll(here);
+        for (int* x : {&s.off, &s.n, &s.length, &s.tiles, &s.steps, &start}) *x = __builtin_amdgcn_readlane(*x, u.b);
     }
-    return false;
+    for (int* x : {&each, &s.off, &s.n, &s.length, &s.tiles, &s.steps, &start}) *x = __builtin_amdgcn_readfirstlane(*x);
+    u.parts = parts_of(s.steps);
+    const int place = mine - start;
+    // Offsets that do not ascend may give a sequence more tiles than were counted.
+    if (place < 0 || place >= s.tiles * u.parts || (u.parts > 1 && id >= c.slots)) return false;
+    u.part = __builtin_amdgcn_readfirstlane(place / s.tiles);
+    u.tile = __builtin_amdgcn_readfirstlane(place - u.part * s.tiles);
+    u.kv_head = __builtin_amdgcn_readfirstlane(id - mine * heads);
+    u.stride = s.tiles * heads;
+    u.slot = __builtin_amdgcn_readfirstlane(id);
+    u.head = u.kv_head * group;
+    u.off = s.off;
+    u.n = s.n;
+    u.length = s.length;
+    u.first = u.length - u.n;
+    return true;
+}
+
+constexpr int kPlanThreads = 1024;
+
+// Of more than 64 sequences: the first workgroup of each (over all heads), how many
+// there are, and the steps of a part. One workgroup, a thread for each sequence.
+template <int kRows>
+__global__ __launch_bounds__(kPlanThreads) void tree_plan_kernel(WindowCall c) {
+    constexpr int kWaves = kPlanThreads / 64;
+    __shared__ float works[kWaves];
+    __shared__ int counts[kWaves], longests[kWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    float work = 0.f;
+    int units = 0, longest = 0;
+    for (int b = tid; b < c.batch; b += kPlanThreads) {
+        const TreeSequence s = tree_sequence<kRows>(c, b);
+        work += static_cast<float>(s.tiles) * static_cast<float>(s.steps);
+        units += s.tiles;
+        longest = max(longest, s.steps);
+    }
+    works[wave] = lane_value(running_sum(work, lane), 63);
+    counts[wave] = lane_value(running_sum(units, lane), 63);
+    longests[wave] = most_of_lanes(longest);
+    __syncthreads();
+    work = 0.f, units = 0, longest = 1;
+    for (int w = 0; w < kWaves; ++w) {
+        work += works[w];
+        units += counts[w];
+        longest = max(longest, longests[w]);
+    }
+    const int each = tree_part(c, work, units, longest);
+    int before = 0;
+    for (int b0 = 0; b0 < c.batch; b0 += kPlanThreads) {
+        const TreeSequence s = tree_sequence<kRows>(c, b0 + tid);
+        const int all = s.tiles * ((s.steps + each - 1) / each), sum = running_sum(all, lane);
+        __syncthreads();
+        counts[wave] = lane_value(sum, 63);
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) before += counts[w];
+        if (b0 + tid < c.batch) c.starts[b0 + tid] = before + sum - all;
+        for (int w = wave; w < kWaves; ++w) before += counts[w];
+    }
+    if (tid == 0) {
+        c.starts[c.batch] = before;
+        c.starts[c.batch + 1] = each;
+    }
 }
 
 template <class T, int D>
@@ -1290,6 +1346,10 @@ int launch_tree_as(const WindowCall& c, hipStream_t stream) {
     const auto kernel = tree_attention_kernel<T, D, kWaves>;
     constexpr int kLds = WindowTile<T, D>::kMasks + 4 * kMaskWords<kWaves>;
     if (int rc = ensure_lds_limit(reinterpret_cast<const void*>(kernel), kLds)) return rc;
+    if (c.starts) {
+        hipLaunchKernelGGL(tree_plan_kernel<32 * kWaves>, dim3(1), dim3(kPlanThreads), 0, stream, c);
+        if (int rc = check_launch("tree_plan_kernel")) return rc;
+    }
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(c.groups)), dim3(64 * kWaves), kLds, stream, c);
     if (int rc = check_launch("tree_attention_kernel")) return rc;
     if (c.rows <= kFewRows)

@@ -174,6 +174,7 @@ struct WindowCall {
     int32_t groups, slots, tile_rows;
     float share, step_cost, read_cost, sums_cost;
     int4* row_parts;                         // [rows]: first place, parts, row in the place, from place to place
+    int32_t* starts;                         // of more than 64 sequences [batch + 2]: tree_plan_kernel's
 };
 
 // One call of the backward pass over strided tensors. `stat` holds, for every

@@ -155,6 +155,17 @@ def test_tree_attention_split(cached, n, branch):
     call.check(*call.run(window=2500, sinks=5), window=2500, sinks=5)
 
 
+@pytest.mark.parametrize("new,cached", [((3, 0, 7, 1) * 25, (9000, 5, 40, 2500) * 25), ((0,) * 70 + (40,) + (0,) * 60, (1,) * 70 + (20000,) + (3,) * 60),
+                                        ((1, 0, 2) * 500, (0, 9, 30) * 500), ((2, 0, 0, 1) * 1050 + (0,), (5, 1, 2, 0) * 1050 + (4,))])
+def test_tree_attention_many_sequences(new, cached):
+    """Sequences that share one K/V head, more than a wave, a workgroup and 64 waves have lanes; a few of them long."""
+    call = _Call(new, cached, 4, 1, 128, 64, BF16, 23, 2, before=2, behind=1)
+    out = torch.full_like(call.q, 7.0)
+    o, lse = call.run(out=out)
+    assert (o[:2] == 7).all() and (o[-1:] == 7).all()
+    call.check(o, lse)
+
+
 @pytest.mark.parametrize("heads,kv_heads,n,branch", [(1, 1, 1100, 0), (2, 2, 1500, -1), (8, 1, 4300, 1), (3, 1, 3100, 0)])
 @pytest.mark.parametrize("cached", [0, 21, 70])
 def test_tree_attention_long_drafts(heads, kv_heads, n, branch, cached):
@@ -261,6 +272,24 @@ def test_a_tree_of_other_values_stays_inside():
         for how in ({}, dict(window=5, sinks=1)):
             o = tree_attention(call.q, call.cache, call.table, call.lengths, call.offsets, DraftTree(positions, near, above), **how)
             assert torch.isfinite(o).all()
+
+
+@pytest.mark.parametrize("batch", [3, 90])
+def test_offsets_of_other_values_stay_inside(batch):
+    """Offsets that do not ascend, lengths past the table: nothing outside is reached, and every call ends."""
+    call = _Call((7,) * batch, (30,) * batch, 4, 2, 64, 16, BF16, 19, 2)
+    gen = torch.Generator("cuda").manual_seed(2)
+    for low, high in ((-5, 7 * batch + 5), (-2 ** 31, 2 ** 31 - 1)):
+        offsets = torch.randint(low, high, (batch + 1,), generator=gen, device="cuda", dtype=torch.int32)
+        lengths = torch.randint(low, high, (batch,), generator=gen, device="cuda", dtype=torch.int32)
+        tree = draft_tree(call.parents, lengths, offsets)
+        out = torch.zeros_like(call.q)
+        tree_attention(call.q, call.cache, call.table, lengths, offsets, tree, out=out)
+        uniforms = torch.rand(7 * batch, generator=gen, device="cuda")
+        target = torch.rand((7 * batch, 50), generator=gen, device="cuda")
+        kept = verify_drafts(target, None, torch.zeros_like(call.parents), call.parents, offsets, uniforms)
+        keep_drafts(call.cache, call.table, lengths, offsets, kept.path, kept.counts)
+        assert torch.isfinite(out).all() and all(torch.isfinite(t).all() for t in call.cache)
 
 
 # ---- verification -------------------------------------------------------------
