@@ -647,7 +647,8 @@ def keep_drafts(cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tens
     j < counts[b], so that the sequence goes on with lengths[b] - n + counts[b] tokens.
     Places outside of j .. n - 1 and ones on no page move nothing. The cache may be that of one
     layer or, as tensors [layers, pages, heads, page tokens, D], of all layers, which one
-    call then takes. No page is in two places of the table. Returns the cache.
+    call then takes. No page that has new tokens is in two places of the table. Returns
+    the cache.
     """
     layers, (pages, heads, page, dim), layer_strides, k_stride, v_stride = _check_layers("keep_drafts", cache)
     if page_table.ndim != 2 or page_table.dtype != torch.int32 or not page_table.is_contiguous():

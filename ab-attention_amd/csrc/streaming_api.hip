@@ -183,7 +183,7 @@ int window_launch(const char* what, const ab_window_args* a, bool paged, void* s
         c.partial_o = reinterpret_cast<float*>(c.row_parts + c.rows);
         c.partial_stat = reinterpret_cast<float2*>(c.partial_o + int64_t(c.slots) * c.tile_rows * c.dim);
         c.starts = c.batch > 64 ? reinterpret_cast<int32_t*>(c.partial_stat + int64_t(c.slots) * c.tile_rows) : nullptr;
-    } else if (!tree && c.parts > 1) {
+    } else if (c.parts > 1) {
         if (a->workspace_bytes < workspace_bytes(c))
             return set_error(AB_ERR_INVALID, "%s: workspace of %zu bytes is smaller than the %zu required", what,
                              a->workspace_bytes, workspace_bytes(c));

@@ -415,7 +415,8 @@ int ab_verify_drafts(const ab_verify_args *args, void *stream);
  * [pages, kv_heads, page_tokens, dim] (16-bit elements; k_layer, v_layer from one to the
  * next) position lengths[b] - n + path[offsets[b] + j] is copied to lengths[b] - n + j, for
  * j < counts[b], all as they were before. A place outside j .. n - 1, or on no page, moves
- * nothing. No two rows of the caches share memory, no page is in two places of the table. */
+ * nothing. No two rows of the caches share memory, no page that has new tokens is in two
+ * places of the table. */
 typedef struct ab_keep_args {
     void *k_cache, *v_cache;
     const int32_t *lengths, *offsets, *page_table, *path, *counts;

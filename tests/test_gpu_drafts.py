@@ -187,6 +187,21 @@ def test_a_chain_is_a_chunk(dim, new, cached):
         call.check(o2, lse2, **how)
 
 
+@pytest.mark.parametrize("pages,width", [(0, 4), (3, 0), (0, 0)])
+@pytest.mark.parametrize("batch", [2, 70])
+def test_a_cache_without_keys(pages, width, batch):
+    cache = PagedCache(*(torch.zeros((pages, 2, 16, 128), dtype=BF16, device="cuda") for _ in range(2)))
+    new = (3, 50) * (batch // 2)
+    lengths, offsets = _ints([20] * batch), _offsets(new)
+    tree = draft_tree(_packed([make_tree(n, 2, 1) for n in new]), lengths, offsets)
+    q = _rand((sum(new), 4, 128), BF16, 1)
+    o, lse = tree_attention(q, cache, torch.zeros((batch, width), dtype=torch.int32, device="cuda"), lengths, offsets, tree, return_lse=True)
+    assert not o.any() and (lse == -math.inf).all()
+    kept = keep_drafts(cache, torch.zeros((batch, width), dtype=torch.int32, device="cuda"), lengths, offsets,
+                       torch.full_like(tree.above, 1), _ints([2] * batch))
+    assert kept is cache and not any(t.any() for t in cache)
+
+
 def test_rows_of_no_sequence_stay():
     call = _Call((9, 0, 20), (30, 4, 0), 4, 2, 64, 8, F16, 8, 2, before=3, behind=5)
     out = torch.full_like(call.q, 7.0)
