@@ -156,6 +156,7 @@ def test_tree_attention_split(cached, n, branch):
 
 
 @pytest.mark.parametrize("new,cached", [((3, 0, 7, 1) * 25, (9000, 5, 40, 2500) * 25), ((0,) * 70 + (40,) + (0,) * 60, (1,) * 70 + (20000,) + (3,) * 60),
+                                        ((40, 33) * 40, (700, 9) * 40), ((90, 1, 0) * 50, (5000, 3, 1) * 50),
                                         ((1, 0, 2) * 500, (0, 9, 30) * 500), ((2, 0, 0, 1) * 1050 + (0,), (5, 1, 2, 0) * 1050 + (4,))])
 def test_tree_attention_many_sequences(new, cached):
     """Sequences that share one K/V head, more than a wave, a workgroup and 64 waves have lanes; a few of them long."""
