@@ -162,6 +162,7 @@ int window_launch(const char* what, const ab_window_args* a, bool paged, void* s
     if (tree) {
         if (a->tokens > 0 && a->batch > 0 && (!tree->positions || !tree->near || !tree->above))
             return set_error(AB_ERR_INVALID, "%s: null pointer", what);
+        if (a->out_rest) return set_error(AB_ERR_INVALID, "%s: out_rest must be null", what);
         plan_tree_call(*a, c);
         c.positions = tree->positions;
         c.near = tree->near;
@@ -396,7 +397,7 @@ int ab_draft_tree(const ab_draft_tree_args* a, void* stream) {
 
 size_t ab_tree_workspace_bytes(const ab_tree_args* a) {
     WindowCall c;
-    if (!a || a->chunk.batch <= 0 || a->chunk.tokens <= 0 || window_call("tree_attention", a->chunk, true, c)) return 0;
+    if (!a || a->chunk.batch <= 0 || a->chunk.tokens <= 0 || a->chunk.out_rest || window_call("tree_attention", a->chunk, true, c)) return 0;
     plan_tree_call(a->chunk, c);
     return tree_workspace_bytes(c);
 }

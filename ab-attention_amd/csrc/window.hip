@@ -1163,7 +1163,7 @@ __device__ __forceinline__ void window_rows(const WindowCall& c, const WindowUni
                 const f32x4 o = o_acc[b][j] * inv;
                 const u32x2 w = {T::pack(o[0], o[1]), T::pack(o[2], o[3])};
                 *reinterpret_cast<u32x2*>(orow + 16 * b) = w;
-                if (e.out_rest) {
+                if (!kTree && e.out_rest) {
                     const f32x4 before = o_acc[b][j] * better;
                     *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(e.out_rest) + (orow - static_cast<uint16_t*>(e.out)) + 16 * b) =
                         u32x2{rest_of<T>(before[0], before[1], w[0]), rest_of<T>(before[2], before[3], w[1])};

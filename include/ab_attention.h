@@ -371,8 +371,9 @@ int ab_draft_tree(const ab_draft_tree_args *args, void *stream);
 /* ab_chunk_attention of new tokens that are a tree: the query at position p sees the
  * cached keys that the mask gives it, and of the new ones those of its line, itself too,
  * whose positions the mask gives it. positions, near and above are ab_draft_tree's for
- * the same lengths and offsets. The chunk's workspace fields are this call's, of
- * ab_tree_workspace_bytes(args) bytes, 16-byte aligned, never 0 where there are tokens. */
+ * the same lengths and offsets. The chunk's out_rest is NULL; its workspace fields are
+ * this call's, of ab_tree_workspace_bytes(args) bytes, 16-byte aligned, never 0 where
+ * there are tokens. */
 typedef struct ab_tree_args {
     ab_window_args chunk;
     const int32_t *positions;
