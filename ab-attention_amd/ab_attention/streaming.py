@@ -733,11 +733,12 @@ class StreamingAttention:
         self.window = window
         self.axes, self.turn = axes, dict(theta=theta, pairing=pairing, joint=joint)
         self.page_tokens, self.device = page_tokens, torch.device(device)
-        # All layers' caches, and each layer's part of them.
+        # All layers' caches, for the operators that take them at once, and each layer's part. To autograd
+        # a part is a tensor of its own (.data), which writes to other layers leave as it was.
         shape = (layers, pages, heads, page_tokens, dim)
-        self.cache = PagedCache(*(torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(2)))
-        self.caches = [PagedCache(self.cache.k[layer], self.cache.v[layer]) for layer in range(layers)]
-        self.device = self.cache.k.device  # with its index: other devices may become the current one
+        self._all = PagedCache(*(torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(2)))
+        self.caches = [PagedCache(self._all.k[layer].data, self._all.v[layer].data) for layer in range(layers)]
+        self.device = self._all.k.device  # with its index: other devices may become the current one
         self.free = list(range(pages - 1, -1, -1))
         self.owners = [0] * pages        # of each page: the sequences that hold it
         self.tokens = [0] * sequences    # of each sequence, with those of the step that began last
@@ -757,6 +758,10 @@ class StreamingAttention:
     def _refuse_capture(self) -> None:
         if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise ValueError("steps of StreamingAttention cannot be captured: the next one has another page table")
+
+    def _writes_all(self) -> None:
+        """Tells autograd of a write to all layers."""
+        _writes("StreamingAttention", *(t for cache in self.caches for t in cache))
 
     def _release(self, page: int) -> None:
         self.owners[page] -= 1
@@ -798,6 +803,8 @@ class StreamingAttention:
         free = len(self.free) + sum(not left for left in owners.values())
         if len(wanted) > free:
             raise ValueError(f"{len(wanted)} more pages are needed, {free} are free")
+        if any(i in self.held[s] for s, i in wanted):  # copied below
+            self._writes_all()
         for s, i in gone:
             self._release(self.held[s].pop(i))
         moves = []
@@ -809,7 +816,7 @@ class StreamingAttention:
             self.held[s][i] = page
             self.owners[page] = 1
         if moves:
-            copy_pages(self.cache, moves)
+            copy_pages(self._all, moves)
         self.tokens, self.new, self.step_tokens = total, new, sum(new)
         width = max(1, max(-(-length // self.page_tokens) for length in total))
         table = [[-1] * width for _ in total]
@@ -857,7 +864,10 @@ class StreamingAttention:
         kept = counts.tolist()
         if any(n and not 0 <= count <= n for count, n in zip(kept, self.new)):
             raise ValueError("counts must be from 0 to the sequences' new tokens")
-        keep_drafts(self.cache, self.page_table, self.lengths, self.offsets, path, counts)
+        _ints("keep", path=path, counts=counts)
+        _gpu("keep", self._all.k, path, counts)
+        self._writes_all()
+        keep_drafts(self._all, self.page_table, self.lengths, self.offsets, path, counts)
         for s, (count, n) in enumerate(zip(kept, self.new)):
             if n:
                 self.tokens[s] += count - n
