@@ -241,7 +241,8 @@ __device__ __forceinline__ int tree_part(const WindowCall& c, float work, int un
     // The lane of the least cost; costs are positive, so their bits are in their order.
     const int least = 0x7f800000 - most_of_lanes(0x7f800000 - __builtin_bit_cast(int, cost));
     const int best = __builtin_ctzll(__ballot(__builtin_bit_cast(int, cost) == least) | (uint64_t(1) << 63));
-    return best == 0 ? longest : __builtin_amdgcn_readlane(static_cast<int>(steps), best);
+    // Float32 steps may be one short of kMostParts parts where there are more than 2^23.
+    return best == 0 ? longest : max(__builtin_amdgcn_readlane(static_cast<int>(steps), best), (longest + kMostParts - 1) / kMostParts);
 }
 
 // A tree's workgroup: of which sequence, tile of rows, K/V head and part of the keys.
