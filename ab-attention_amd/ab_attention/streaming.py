@@ -647,8 +647,8 @@ def keep_drafts(cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tens
     j < counts[b], so that the sequence goes on with lengths[b] - n + counts[b] tokens.
     Places outside of j .. n - 1 and ones on no page move nothing. The cache may be that of one
     layer or, as tensors [layers, pages, heads, page tokens, D], of all layers, which one
-    call then takes. No page that has new tokens is in two places of the table. Returns
-    the cache.
+    call then takes. Its keys and values share no memory, and no page that has new tokens
+    is in two places of the table. Returns the cache.
     """
     layers, (pages, heads, page, dim), layer_strides, k_stride, v_stride = _check_layers("keep_drafts", cache)
     if page_table.ndim != 2 or page_table.dtype != torch.int32 or not page_table.is_contiguous():
@@ -658,6 +658,8 @@ def keep_drafts(cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tens
     if not page_table.shape[0] == offsets.shape[0] - 1 == counts.shape[0] == batch:
         raise ValueError("page_table [B,width], lengths [B], offsets [B+1] and counts [B] must be of one batch")
     k, v = cache
+    if k.data_ptr() == v.data_ptr() and k.numel():
+        raise ValueError("keep_drafts requires keys and values that share no memory")
     _no_tangent("keep_drafts", k, v)
     device = _gpu("keep_drafts", k, v, page_table, lengths, offsets, path, counts)
     _writes("keep_drafts", k, v)

@@ -1,7 +1,11 @@
 """Drafted tokens: calls at the edge of what is allowed, without a launch (CPU only)."""
 import ctypes
 
+import pytest
+import torch
+
 from ab_attention import _lib
+from ab_attention.streaming import PagedCache, keep_drafts
 
 _A = 4096  # a 16-byte aligned stand-in address: every case is rejected before any runtime call
 
@@ -24,3 +28,11 @@ def test_a_tree_has_no_out_rest():
     assert lib.ab_tree_attention(ctypes.byref(args), None) == 1
     assert b"out_rest" in lib.ab_last_error(), lib.ab_last_error()
     assert lib.ab_tree_workspace_bytes(ctypes.byref(args)) == 0
+
+
+@pytest.mark.parametrize("shape", [(3, 2, 8, 64), (2, 3, 2, 8, 64)])
+def test_keys_and_values_in_one_place_are_not_moved(shape):
+    """Each would move rows that the other one reads."""
+    x, ints = torch.zeros(shape, dtype=torch.bfloat16), torch.zeros(5, dtype=torch.int32)
+    with pytest.raises(ValueError, match="share no memory"):
+        keep_drafts(PagedCache(x, x), ints[:2][None], ints[:1], ints[:2], ints, ints[:1])
