@@ -19,8 +19,8 @@ constexpr int kWave = 64;
 // One workgroup per sequence, 256 tokens at a time, a lane each: every wave follows the lines
 // inside its 64 by six rounds of pointer doubling (word, steps and end of a line twice as
 // long each time) by lane exchanges; then the waves take the positions above theirs one after
-// the other. Bound by launch and latency: 26 drafts 2.1 us, 4 x 701 4.3 (one wave for all of a
-// sequence 7.6).
+// the other. Bound by launch and latency: in calls in a row 26 drafts 2.1 us, 4 x 701 4.2 (one
+// wave for all of a sequence 7.6).
 constexpr int kTreeWaves = 4;
 __global__ __launch_bounds__(kWave * kTreeWaves) void tree_kernel(TreeCall c) {
     constexpr int kTokens = kWave * kTreeWaves;
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(kWave * kTreeWaves) void tree_kernel(TreeCall c) {
 // where more drawn drafts are turned down it adds up the whole vocabulary by itself.
 //
 // A chain of 7 drafts over 32,000 tokens takes 4.6 + 4.8 us, 48 chosen trees over 128,000
-// 10.0 + 5.2, bound by latency: the walk, a reading, the choice among a few values. What
+// 10.4 + 5.2, bound by latency: the walk, a reading, the choice among a few values. What
 // one CU adds up by itself takes 2.3 us over 1,000 tokens, 4.1 over 32,000 and 8.9 over
 // 100,000, as much 64-bit arithmetic as loading (16 drawn trees with four drafts behind a
 // token, four or five such sums after one another: 5 + 40 us). A kernel for every further

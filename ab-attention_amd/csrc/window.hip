@@ -40,10 +40,11 @@
 // sinks and window, the drafts, all of them where a page is missing) is made into words of 32
 // keys in LDS before the passes, which then take one LDS read for a masked tile and row, and
 // none of the mask's arithmetic. The first form walked up the tree in every masked tile (4 x
-// 701 drafts 195 us, now 80). Bound like the others: one sequence of 64 drafts, 256 rows over
-// 100,000 keys, 119 us where reading takes 84 and the products 88; of 16 drafts 77 us, 5.3
-// TB/s; a few keys (26 drafts over 1,017) 15 us, all of it one thing after another: which
-// sequence, its page table, its masks, four tiles of keys, 3,000 instructions of one wave.
+// 701 drafts 195 us, now 82). Bound like the others: one sequence of 64 drafts, 256 rows over
+// 100,000 keys, 132 to 136 us where reading takes 84 and the products 81; of 16 drafts 98, 4.2
+// TB/s, of one 91; a few keys (26 drafts over 1,017) 18 us, all of it one thing after another:
+// which sequence, its page table, its masks, four tiles of keys, 3,000 instructions of one wave.
+// (Calls in a row, with the kernel that joins parts: 9 us of the first, 8, 4 of the last.)
 #include <algorithm>
 #include <initializer_list>
 
@@ -1420,8 +1421,8 @@ int window_parts(const WindowCall& c, int64_t most_keys) {
 //
 // Tiles of 256 rows, for eight waves, where sequences have more than 128 rows on average: keys
 // are then read once for twice the rows (one sequence of 64 drafts, 256 rows of 100,000
-// keys: 119 us, in tiles of 128 rows 150). Not with D = 64, whose four waves take a third of
-// a CU (4 x 701 drafts 80 us, of eight waves 103).
+// keys, with the joining of parts: 136 us, in tiles of 128 rows 193). Not with D = 64, whose
+// four waves take a third of a CU (4 x 701 drafts 82 us, of eight waves a quarter more).
 void plan_tree(WindowCall& c, int64_t most_keys) {
     const int64_t packed = int64_t(c.tokens) * c.group.d;
     c.tile_rows = c.dim == 128 && packed > int64_t(c.batch) * 128 ? 256 : 128;
